@@ -408,6 +408,169 @@ int sf_qk_norm_rope(const void *q, int64_t q_stride_token, const void *k,
                     const void *sin, void *q_out, void *k_out,
                     sf_stream_t stream);
 
+/*
+ * K8: the block cache.  Keys and values of a sequence whose complete blocks
+ * of SF_KV_BLOCK tokens are held in 8 bits, with one scale per block, head and
+ * K or V, and whose last tokens are held in bf16 in a ring of blocks until
+ * they are folded.  No counterpart in the reference, whose target keeps a bf16
+ * DynamicCache; the calls take the places of its update and of
+ * _compact_tree_cache (eagle3_tree.py:833-858).
+ *   x^ = code * 2^e,  e the least integer >= SF_KV_MIN_EXPONENT with
+ *                     max |x| over the block's finite values <= q 2^e,
+ *   code = x / 2^e to the nearest (ties to even) int8 (q = 127) or e4m3
+ *   (q = 448); a value that is not finite is held as NaN (int8: code -128).
+ * Powers of two make x / 2^e and x^ exact, so the codes do not depend on how
+ * they are computed and x^ is a bf16 number.
+ *   k8, v8       [heads, capacity_blocks, 64 * head_dim] codes
+ *   k_scale, v_scale  fp32 [heads, capacity_blocks]
+ *   flags        int32 [heads, capacity_blocks]: bit 0 (1): the values (keys)
+ *                hold a NaN code
+ *   k_tail, v_tail  bf16 [heads, ring_blocks, 64 * head_dim]: block j of the
+ *                sequence at j % ring_blocks
+ *   tail_flags   int32 [heads, ring_blocks]: the values of the block may hold
+ *                infinity or NaN
+ * heads = batch * kv_heads (times the layers for sf_kv_compact and sf_kv_fold,
+ * whose arrays then hold the layers one after another).  All buffers 16-byte
+ * aligned; the ring starts zeroed.  Blocks below folded_blocks are read from
+ * the 8-bit arrays, the others from the ring.  The order of values inside a
+ * block is the library's own (csrc/kv_blocks.h).
+ * head_dim 64 or 128.
+ */
+#define SF_KV_BLOCK 64
+#define SF_KV_E4M3 0
+#define SF_KV_INT8 1
+#define SF_KV_MIN_EXPONENT (-60)
+/* Positions that one sf_kv_compact call takes. */
+#define SF_KV_MAX_MOVES 256
+typedef struct sf_kv_cache {
+  void *k8, *v8;
+  float *k_scale, *v_scale;
+  int32_t *flags;
+  void *k_tail, *v_tail;
+  int32_t *tail_flags;
+  int32_t heads, head_dim, held;
+  int32_t capacity_blocks, ring_blocks;
+  int32_t folded_blocks;
+} sf_kv_cache;
+
+/*
+ * Writes tokens [start, start + tokens) of every (sequence, head): element
+ * (b, h, t, d) of k and v is read at b * stride_batch + h * stride_head +
+ * t * stride_token + d.  Rows of the last block behind them become zeros.
+ * The blocks touched must be at or above folded_blocks and fit the ring and
+ * the capacity (SF_ERR_INVALID_ARGUMENT).
+ */
+int sf_kv_append(const sf_kv_cache *cache, int kv_heads, const void *k,
+                 int64_t k_stride_batch, int64_t k_stride_head,
+                 int64_t k_stride_token, const void *v, int64_t v_stride_batch,
+                 int64_t v_stride_head, int64_t v_stride_token, int64_t start,
+                 int tokens, sf_stream_t stream);
+
+/*
+ * Moves the rows of tokens base + positions[i] to base + first + i, i < count
+ * (the accepted path of a draft tree): positions is a host array, strictly
+ * ascending, with positions[i] >= first + i, and end is the number of tokens
+ * the ring holds rows of.  count <= SF_KV_MAX_MOVES.
+ */
+int sf_kv_compact(const sf_kv_cache *cache, int64_t base, int first,
+                  const int32_t *positions, int count, int64_t end,
+                  sf_stream_t stream);
+
+/*
+ * Folds the ring's blocks [folded_blocks, folded_blocks + blocks), which are
+ * complete, into the 8-bit arrays.  The ring keeps them.
+ */
+int sf_kv_fold(const sf_kv_cache *cache, int blocks, sf_stream_t stream);
+
+/*
+ * x^ of tokens [start, start + tokens) as bf16 [heads, tokens, head_dim],
+ * contiguous, 16-byte aligned (the ring's rows as they are).
+ */
+int sf_kv_read(const sf_kv_cache *cache, int64_t start, int tokens, void *k,
+               void *v, sf_stream_t stream);
+
+/*
+ * K9: grouped-query attention over a block cache of `keys` tokens:
+ *   out[b, qi, qh, :] = sum_s p_s * v^[b, h, s, :],
+ *   p = softmax over admitted keys s of scale * (q[b, qi, qh, :] . k^[b, h, s, :])
+ * h = qh / (q_heads / kv_heads), scores and sums in fp32, p rounded to bf16
+ * for the product with v^, the result rounded to bf16 once.  The mask
+ * covers the last mask_keys keys; a key before them is admitted by every row.
+ * With mask == NULL key s is admitted when s <= keys - queries + qi.  A row that
+ * admits no key gets zeros; what a key that is not admitted holds has no effect.
+ *   q     bf16, element (b, qi, qh, d) at b * q_stride_batch +
+ *         qi * q_stride_token + qh * q_stride_head + d, 16-byte aligned rows
+ *   mask  uint8/bool, element (b, qi, s) at b * mask_stride_batch +
+ *         qi * mask_stride_query + (s - (keys - mask_keys))
+ *   out   bf16 [batch, queries, q_heads, head_dim], contiguous
+ *   workspace  16-byte aligned device memory of at least
+ *         sf_block_attention_workspace bytes, in use until the call's kernels
+ *         have run; with less (or NULL) the keys of a call are not split.
+ */
+int64_t sf_block_attention_workspace(int batch, int queries, int keys,
+                                     int q_heads, int kv_heads, int head_dim);
+int sf_block_attention(const sf_kv_cache *cache, int batch, int kv_heads,
+                       int keys, const void *q, int64_t q_stride_batch,
+                       int64_t q_stride_head, int64_t q_stride_token,
+                       int queries, int q_heads, const uint8_t *mask,
+                       int64_t mask_stride_batch, int64_t mask_stride_query,
+                       int mask_keys, float scale, void *out, void *workspace,
+                       int64_t workspace_bytes, sf_stream_t stream);
+
+/*
+ * K10: rotary positions of queries and keys.  For pair i of a head's first
+ * rotary_dim elements, (a, b) = elements (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) if interleaved:
+ *   angle = position * turns[i]  (in turns, fp64, reduced before its rounding)
+ *   (a, b) -> factor * (a cos - b sin, b cos + a sin)
+ * in fp32 with one rounding; the other elements are copied.
+ *   x (q and k)  dtype [batch, tokens, heads, head_dim], element (b, t, h, d)
+ *                at b * stride_batch + t * stride_token + h * stride_head + d
+ *   positions    int64, (b, t) at b * position_stride + t (0: one row for all)
+ *   turns        fp64 [rotary_dim / 2], |position * turns| < 2^51
+ *   out          dtype [batch, heads, tokens, head_dim], contiguous
+ * dtype: SF_BF16, SF_F16 or SF_F32; rotary_dim even, <= head_dim <= 1024.
+ */
+#define SF_BF16 0
+#define SF_F16 1
+#define SF_F32 2
+int sf_rotary(int dtype, const void *q, int64_t q_stride_batch,
+              int64_t q_stride_token, int64_t q_stride_head, int q_heads,
+              const void *k, int64_t k_stride_batch, int64_t k_stride_token,
+              int64_t k_stride_head, int k_heads, const int64_t *positions,
+              int64_t position_stride, const double *turns, float factor,
+              int batch, int tokens, int head_dim, int rotary_dim,
+              int interleaved, void *q_out, void *k_out, sf_stream_t stream);
+
+/*
+ * K11: rules on logits.  With n = counts[v] + occurrences of v in paths[r]
+ * (entries outside [0, vocab) count for nothing), each step rounded to fp32:
+ *   y = x                                        if n == 0
+ *   y = (x < 0 ? x * repetition : x / repetition)
+ *       - ((frequency * n) + presence)           otherwise
+ *   y = y + bias[v]                              with a bias
+ *   y = -inf                                     where allowed has a 0 bit
+ *   x        dtype [rows, vocab], row stride logits_stride
+ *   counts   int32 [vocab] or NULL
+ *   paths    int32 [rows, path_length], contiguous, or NULL
+ *   bias     fp32, element (r, v) at r * bias_stride + v, or NULL
+ *   allowed  int32 words, bit v % 32 of word r * allowed_stride + v / 32, or NULL
+ *   out      dtype [rows, vocab], row stride out_stride: y rounded to dtype
+ *            (may equal logits), or NULL
+ *   tokens   int64 [rows]: the lowest v of the largest y (fp32, a NaN above all;
+ *            -1 where no y is above -inf), or NULL
+ *   workspace  device memory of sf_logit_rules_workspace bytes (with tokens)
+ */
+int64_t sf_logit_rules_workspace(int rows, int vocab);
+int sf_logit_rules(int dtype, const void *logits, int64_t logits_stride,
+                   int rows, int vocab, const int32_t *counts,
+                   const int32_t *paths, int path_length, float repetition,
+                   float presence, float frequency, const float *bias,
+                   int64_t bias_stride, const int32_t *allowed,
+                   int64_t allowed_stride, void *out, int64_t out_stride,
+                   int64_t *tokens, void *workspace, int64_t workspace_bytes,
+                   sf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,18 @@ _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 
+class KVCacheStruct(ctypes.Structure):
+    """sf_kv_cache."""
+
+    _fields_ = [("k8", _p), ("v8", _p), ("k_scale", _p), ("v_scale", _p), ("flags", _p),
+                ("k_tail", _p), ("v_tail", _p), ("tail_flags", _p),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("held", ctypes.c_int32),
+                ("capacity_blocks", ctypes.c_int32), ("ring_blocks", ctypes.c_int32),
+                ("folded_blocks", ctypes.c_int32)]
+
+
+_f = ctypes.c_float
+
 # name -> (argtypes, restype); mirrors include/specfit_amd.h.
 SIGNATURES = {
     "sf_abi_version": ([], _i),
@@ -47,6 +59,18 @@ SIGNATURES = {
     "sf_rms_norm": ([_p, _i64, _i, _i, _p, ctypes.c_float, _p, _i64, _p], _i),
     "sf_qk_norm_rope": ([_p, _i64, _p, _i64, _i, _i, _i, _i, _p, _p, ctypes.c_float, _p, _p, _p,
                          _p, _p], _i),
+    "sf_kv_append": ([_p, _i, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i, _p], _i),
+    "sf_kv_compact": ([_p, _i64, _i, _p, _i, _i64, _p], _i),
+    "sf_kv_fold": ([_p, _i, _p], _i),
+    "sf_kv_read": ([_p, _i64, _i, _p, _p, _p], _i),
+    "sf_block_attention_workspace": ([_i, _i, _i, _i, _i, _i], _i64),
+    "sf_block_attention": ([_p, _i, _i, _i, _p, _i64, _i64, _i64, _i, _i, _p, _i64, _i64, _i, _f,
+                            _p, _p, _i64, _p], _i),
+    "sf_rotary": ([_i, _p, _i64, _i64, _i64, _i, _p, _i64, _i64, _i64, _i, _p, _i64, _p, _f, _i,
+                   _i, _i, _i, _i, _p, _p, _p], _i),
+    "sf_logit_rules_workspace": ([_i, _i], _i64),
+    "sf_logit_rules": ([_i, _p, _i64, _i, _i, _p, _p, _i, _f, _f, _f, _p, _i64, _p, _i64, _p, _i64,
+                        _p, _p, _i64, _p], _i),
 }
 
 

@@ -21,7 +21,8 @@ OBJ_DIR = os.path.join(PKG_DIR, "_build")
 OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ("abi.hip", "router.hip", "dispatch.hip", "swiglu.hip", "combine.hip",
-           "attention.hip", "norm.hip", "codec.hip")
+           "attention.hip", "norm.hip", "codec.hip", "kv_blocks.hip", "block_attention.hip",
+           "rotary.hip", "logits.hip")
 
 HIPCC_FLAGS = (
     f"--offload-arch={OFFLOAD_ARCH}",

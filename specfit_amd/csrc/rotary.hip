@@ -1,0 +1,200 @@
+// K10: rotary positions of queries and keys.
+//
+// For token (b, t) and pair i the angle in turns is position * turns[i], taken
+// in fp64 and reduced to half a turn before it is rounded to fp32: at position
+// 10^6 an fp32 product would be off by a sixteenth of a radian.  The sines are
+// the same for every head, so a workgroup computes those of its tokens once
+// into LDS; (a, b) -> (a cos - b sin, b cos + a sin) then runs over its heads
+// in 16-byte pieces.  Bound by the bytes of q and k, in and out.
+#include <algorithm>
+
+#include "sf_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 8;  // of a workgroup
+
+struct RotaryArgs {
+  const void* x[2];  // q, k
+  int64_t batch[2], tok[2], head[2];
+  int heads[2];
+  void* out[2];
+  const int64_t* positions;
+  int64_t position_stride;
+  const double* turns;
+  float factor;
+  int B, T, D, R;
+  int tokens;  // of a workgroup
+};
+
+template <int DTYPE>
+struct Type;
+template <>
+struct Type<SF_BF16> {
+  typedef uint16_t Elem;
+  static __device__ __forceinline__ float load(uint16_t v) { return sf_bf16_to_f32(v); }
+  static __device__ __forceinline__ uint16_t store(float v) { return sf_f32_to_bf16(v); }
+};
+template <>
+struct Type<SF_F16> {
+  typedef uint16_t Elem;
+  static __device__ __forceinline__ float load(uint16_t v) {
+    return static_cast<float>(__builtin_bit_cast(_Float16, v));
+  }
+  static __device__ __forceinline__ uint16_t store(float v) {
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+  }
+};
+template <>
+struct Type<SF_F32> {
+  typedef float Elem;
+  static __device__ __forceinline__ float load(float v) { return v; }
+  static __device__ __forceinline__ float store(float v) { return v; }
+};
+
+// VEC elements per access: those of 16 bytes, or 1.
+template <int DTYPE, int VEC, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
+  using Ty = Type<DTYPE>;
+  using Elem = typename Ty::Elem;
+  struct __attribute__((aligned(VEC * sizeof(Elem)))) Piece {
+    Elem e[VEC];
+  };
+  extern __shared__ float2 turn[];  // (cos, sin) times the factor, [tokens][R / 2]
+  const int half = a.R / 2;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * a.tokens;
+  const int64_t all = static_cast<int64_t>(a.B) * a.T;
+  const int count = static_cast<int>(min(static_cast<int64_t>(a.tokens), all - first));
+  for (int n = threadIdx.x; n < count * half; n += kThreads) {
+    const int64_t token = first + n / half;
+    const int64_t b = token / a.T;
+    const double p = static_cast<double>(a.positions[b * a.position_stride + (token - b * a.T)]) *
+                     a.turns[n % half];
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (p - __builtin_rint(p))), &s, &c);
+    turn[n] = make_float2(c * a.factor, s * a.factor);
+  }
+  __syncthreads();
+
+  // A unit of work: two pieces of VEC pairs apart (half layout), one piece of
+  // VEC / 2 pairs (interleaved; VEC 1: a pair), or a piece that is copied.
+  constexpr int kStep = INTERLEAVED ? (VEC > 1 ? VEC : 2) : VEC;
+  const int turned = (INTERLEAVED ? a.R : half) / kStep;
+  const int units = turned + (a.D - a.R) / VEC;
+  const int heads = a.heads[0] + a.heads[1];
+  for (int n = blockIdx.y * kThreads + threadIdx.x; n < count * heads * units;
+       n += gridDim.y * kThreads) {
+    const int u = n % units;
+    int h = (n / units) % heads;
+    const int i = n / units / heads;
+    const int64_t token = first + i;
+    const int64_t b = token / a.T, t = token - b * a.T;
+    const int w = h >= a.heads[0];
+    if (w) h -= a.heads[0];
+    const Elem* x = static_cast<const Elem*>(a.x[w]) + b * a.batch[w] + t * a.tok[w] + h * a.head[w];
+    Elem* y = static_cast<Elem*>(a.out[w]) + ((b * a.heads[w] + h) * a.T + t) * a.D;
+    const float2* cs = turn + i * half;
+    if (u >= turned) {
+      const int d = a.R + (u - turned) * VEC;
+      *reinterpret_cast<Piece*>(y + d) = *reinterpret_cast<const Piece*>(x + d);
+    } else if (!INTERLEAVED) {
+      const int d = u * VEC;
+      const Piece p = *reinterpret_cast<const Piece*>(x + d);
+      const Piece q = *reinterpret_cast<const Piece*>(x + d + half);
+      Piece r, s;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float2 f = cs[d + e];
+        const float u0 = Ty::load(p.e[e]), u1 = Ty::load(q.e[e]);
+        r.e[e] = Ty::store(__builtin_fmaf(u0, f.x, -(u1 * f.y)));
+        s.e[e] = Ty::store(__builtin_fmaf(u1, f.x, u0 * f.y));
+      }
+      *reinterpret_cast<Piece*>(y + d) = r;
+      *reinterpret_cast<Piece*>(y + d + half) = s;
+    } else {
+      const int d = u * kStep;
+      Elem in[kStep], out[kStep];
+#pragma unroll
+      for (int e = 0; e < kStep; e += VEC) {
+        const Piece p = *reinterpret_cast<const Piece*>(x + d + e);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) in[e + j] = p.e[j];
+      }
+#pragma unroll
+      for (int e = 0; e < kStep; e += 2) {
+        const float2 f = cs[(d + e) / 2];
+        const float u0 = Ty::load(in[e]), u1 = Ty::load(in[e + 1]);
+        out[e] = Ty::store(__builtin_fmaf(u0, f.x, -(u1 * f.y)));
+        out[e + 1] = Ty::store(__builtin_fmaf(u1, f.x, u0 * f.y));
+      }
+#pragma unroll
+      for (int e = 0; e < kStep; e += VEC) {
+        Piece p;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.e[j] = out[e + j];
+        *reinterpret_cast<Piece*>(y + d + e) = p;
+      }
+    }
+  }
+}
+
+template <int DTYPE, int VEC>
+void launch(const RotaryArgs& a, bool interleaved, dim3 grid, hipStream_t s) {
+  const size_t lds = static_cast<size_t>(a.tokens) * (a.R / 2) * sizeof(float2);
+  if (interleaved)
+    rotary_kernel<DTYPE, VEC, true><<<grid, kThreads, lds, s>>>(a);
+  else
+    rotary_kernel<DTYPE, VEC, false><<<grid, kThreads, lds, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" int sf_rotary(int dtype, const void* q, int64_t q_stride_batch, int64_t q_stride_token,
+                         int64_t q_stride_head, int q_heads, const void* k, int64_t k_stride_batch,
+                         int64_t k_stride_token, int64_t k_stride_head, int k_heads,
+                         const int64_t* positions, int64_t position_stride, const double* turns,
+                         float factor, int batch, int tokens, int head_dim, int rotary_dim,
+                         int interleaved, void* q_out, void* k_out, sf_stream_t stream) {
+  if ((dtype != SF_BF16 && dtype != SF_F16 && dtype != SF_F32) || batch < 0 || tokens < 0 ||
+      q_heads < 0 || k_heads < 0)
+    return SF_ERR_INVALID_ARGUMENT;
+  if (head_dim < 2 || head_dim > 1024 || rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 ||
+      q_heads > 4096 || k_heads > 4096)
+    return SF_ERR_UNSUPPORTED_SHAPE;
+  const int64_t all = static_cast<int64_t>(batch) * tokens;
+  if (all == 0 || q_heads + k_heads == 0) return SF_OK;
+  if (all >= (int64_t{1} << 31)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (!positions || !turns || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)))
+    return SF_ERR_INVALID_ARGUMENT;
+  RotaryArgs a = {{q, k}, {q_stride_batch, k_stride_batch}, {q_stride_token, k_stride_token},
+                  {q_stride_head, k_stride_head}, {q_heads, k_heads}, {q_out, k_out},
+                  positions, position_stride, turns, factor, batch, tokens, head_dim, rotary_dim, 1};
+  const int size = dtype == SF_F32 ? 4 : 2;
+  const int vec = 16 / size;
+  // 16-byte accesses where every row, and both halves of the turned part,
+  // begin on 16 bytes.
+  bool wide = head_dim % vec == 0 && rotary_dim % (interleaved ? vec : 2 * vec) == 0;
+  for (int w = 0; w < 2; ++w)
+    if (a.heads[w])
+      wide = wide && reinterpret_cast<uintptr_t>(a.x[w]) % 16 == 0 &&
+             reinterpret_cast<uintptr_t>(a.out[w]) % 16 == 0 && a.batch[w] % vec == 0 &&
+             a.tok[w] % vec == 0 && a.head[w] % vec == 0;
+  const int units = wide ? (head_dim - rotary_dim / (interleaved ? 1 : 2)) / vec : head_dim;
+  const int per_token = (q_heads + k_heads) * units;
+  a.tokens = static_cast<int>(std::min<int64_t>(kMaxTokens, std::max<int64_t>(1, all / 2048)));
+  // A lone token's heads are dealt over workgroups.
+  const int shares = a.tokens > 1 ? 1 : std::min(16, std::max(1, per_token / (4 * kThreads)));
+  const dim3 grid(static_cast<uint32_t>((all + a.tokens - 1) / a.tokens), shares);
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const bool il = interleaved != 0;
+  if (dtype == SF_BF16) {
+    wide ? launch<SF_BF16, 8>(a, il, grid, s) : launch<SF_BF16, 1>(a, il, grid, s);
+  } else if (dtype == SF_F16) {
+    wide ? launch<SF_F16, 8>(a, il, grid, s) : launch<SF_F16, 1>(a, il, grid, s);
+  } else {
+    wide ? launch<SF_F32, 4>(a, il, grid, s) : launch<SF_F32, 1>(a, il, grid, s);
+  }
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}

@@ -1,4 +1,4 @@
-"""PyTorch-facing wrappers of the C-ABI kernels (K1-K4 and the H2D copy).
+"""PyTorch-facing wrappers of the C-ABI kernels (K1-K11 and the H2D copy).
 
 Tensors are plumbing: each wrapper checks dtype, device, shape and
 contiguity on the host, allocates outputs with the caching allocator and
@@ -834,3 +834,424 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
                                        k_out.data_ptr(), _stream_handle(stream, q.device))
     _native.check(rc, "sf_qk_norm_rope")
     return q_out, k_out
+
+
+# ------------------------------------------------------------------ K8 ----
+KV_BLOCK = 64                       # tokens of a cache block (SF_KV_BLOCK)
+KV_HELD = {"e4m3": 0, "int8": 1}    # how complete blocks are held
+_KV_MAX_MOVES = 256                 # positions of one sf_kv_compact call
+
+
+class _on_device:
+    """Makes ``device`` current for a launch on it."""
+
+    __slots__ = ("_index", "_previous")
+
+    def __init__(self, device: torch.device) -> None:
+        self._index = device.index
+
+    def __enter__(self) -> None:
+        current = torch._C._cuda_getDevice()
+        self._previous = None if self._index in (None, current) else current
+        if self._previous is not None:
+            torch.cuda.set_device(self._index)
+
+    def __exit__(self, *exc) -> None:
+        if self._previous is not None:
+            torch.cuda.set_device(self._previous)
+
+
+def _scratch(nbytes: int, device: torch.device, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """Scratch memory from the pool of the stream that uses it: a block of
+    another stream's pool may still be read there by kernels queued before it
+    was given back."""
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+class KVBlocks:
+    """Device storage of a block cache (K8): for every layer, sequence and
+    key/value head, ``capacity_blocks`` blocks of 64 tokens in 8 bits with a
+    power-of-two scale each for keys and values, and a ring of ``ring_blocks``
+    bf16 blocks for the tokens that are not folded yet.  Which tokens are there
+    and which blocks are folded is the caller's knowledge
+    (``specfit_amd.runtime.BlockKVCache`` keeps it); ``folded`` is the number
+    of blocks, from the first, that are read from the 8-bit arrays."""
+
+    def __init__(self, *, layers: int, batch: int, kv_heads: int, head_dim: int,
+                 capacity_blocks: int, ring_blocks: int, held: str,
+                 device: torch.device | str) -> None:
+        if min(layers, batch, kv_heads, capacity_blocks, ring_blocks) < 1:
+            raise ValueError("layers, batch, kv_heads and block counts must be positive")
+        if head_dim not in (64, 128):
+            raise ValueError("block caches hold head dims 64 and 128")
+        if held not in KV_HELD:
+            raise ValueError(f"held must be one of {sorted(KV_HELD)}")
+        if layers * batch * kv_heads > 65535:
+            raise ValueError("a block cache holds at most 65535 heads over its layers and batch")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("block caches live on a HIP device")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.layers, self.batch, self.kv_heads, self.head_dim = layers, batch, kv_heads, head_dim
+        self.capacity_blocks, self.ring_blocks = capacity_blocks, ring_blocks
+        self.held, self.device = held, device
+        heads, width = batch * kv_heads, KV_BLOCK * head_dim
+        shape, ring = (layers, heads, capacity_blocks), (layers, heads, ring_blocks)
+        self.keys = torch.empty((*shape, width), dtype=torch.uint8, device=device)
+        self.values = torch.empty((*shape, width), dtype=torch.uint8, device=device)
+        self.scales = torch.ones((2, *shape), dtype=torch.float32, device=device)
+        self.flags = torch.zeros(shape, dtype=torch.int32, device=device)
+        # Zeroed once: what a ring block holds behind its tokens has to be finite.
+        self.tail_keys = torch.zeros((*ring, width), dtype=_BF16, device=device)
+        self.tail_values = torch.zeros((*ring, width), dtype=_BF16, device=device)
+        self.tail_flags = torch.zeros(ring, dtype=torch.int32, device=device)
+        self._folded = 0
+        self._structs = [self._struct(layer, heads) for layer in range(layers)]
+        self._whole = self._struct(0, layers * heads)
+        self._refs = [ctypes.addressof(s) for s in self._structs]
+        self._whole_ref = ctypes.addressof(self._whole)
+
+    def _struct(self, layer: int, heads: int) -> _native.KVCacheStruct:
+        return _native.KVCacheStruct(
+            self.keys[layer].data_ptr(), self.values[layer].data_ptr(),
+            self.scales[0, layer].data_ptr(), self.scales[1, layer].data_ptr(),
+            self.flags[layer].data_ptr(), self.tail_keys[layer].data_ptr(),
+            self.tail_values[layer].data_ptr(), self.tail_flags[layer].data_ptr(), heads,
+            self.head_dim, KV_HELD[self.held], self.capacity_blocks, self.ring_blocks, 0)
+
+    @property
+    def folded(self) -> int:
+        return self._folded
+
+    @folded.setter
+    def folded(self, blocks: int) -> None:
+        if not 0 <= blocks <= self.capacity_blocks:
+            raise ValueError("folded blocks out of range")
+        self._folded = blocks
+        self._whole.folded_blocks = blocks
+        for s in self._structs:
+            s.folded_blocks = blocks
+
+    def _check_layer(self, layer: int) -> int:
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"layer {layer} of a block cache of {self.layers} layers")
+        return self._refs[layer]
+
+    def _check_rows(self, name: str, t: torch.Tensor) -> None:
+        _require_cuda(name, t, _BF16)
+        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[3] != self.head_dim:
+            raise ValueError(f"{name} must be [{self.batch}, heads, tokens, {self.head_dim}]")
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on the cache's device")
+
+
+def kv_append(blocks: KVBlocks, layer: int, key: torch.Tensor, value: torch.Tensor, start: int, *,
+              stream: torch.cuda.Stream | None = None) -> None:
+    """Writes key and value [batch, kv_heads, T, head_dim] (bf16, any strides
+    with a unit last one) as tokens start .. start + T - 1 of ``layer``."""
+    ref = blocks._check_layer(layer)
+    for name, t in (("key", key), ("value", value)):
+        blocks._check_rows(name, t)
+        if t.shape[1] != blocks.kv_heads:
+            raise ValueError(f"{name} must have {blocks.kv_heads} heads")
+    if key.shape != value.shape:
+        raise ValueError("key and value differ in shape")
+    if key.stride(3) != 1:
+        key = key.contiguous()
+    if value.stride(3) != 1:
+        value = value.contiguous()
+    (kb, kh, kt, _), (vb, vh, vt, _) = key.stride(), value.stride()
+    with _on_device(blocks.device):
+        rc = _native.lib().sf_kv_append(ref, blocks.kv_heads, key.data_ptr(), kb, kh, kt,
+                                        value.data_ptr(), vb, vh, vt, int(start), key.shape[2],
+                                        _stream_handle(stream, blocks.device))
+    _native.check(rc, "sf_kv_append")
+
+
+def kv_compact(blocks: KVBlocks, base: int, positions: Sequence[int], end: int, *,
+               stream: torch.cuda.Stream | None = None) -> None:
+    """Moves the rows of tokens base + positions[i] to base + i in every
+    layer; ``positions`` ascend strictly and ``end`` is the number of tokens
+    the layers hold."""
+    positions = [int(p) for p in positions]
+    if any(p < 0 or base + p >= end for p in positions) or \
+            any(b <= a for a, b in zip(positions, positions[1:])):
+        raise ValueError("positions must ascend strictly and name tokens of the cache")
+    first = 0
+    while first < len(positions) and positions[first] == first:
+        first += 1  # these rows stay where they are
+    with _on_device(blocks.device):
+        for at in range(first, len(positions), _KV_MAX_MOVES):
+            part = positions[at:at + _KV_MAX_MOVES]
+            rc = _native.lib().sf_kv_compact(
+                blocks._whole_ref, int(base), at,
+                ctypes.cast((ctypes.c_int32 * len(part))(*part), ctypes.c_void_p), len(part),
+                int(end), _stream_handle(stream, blocks.device))
+            _native.check(rc, "sf_kv_compact")
+
+
+def kv_fold(blocks: KVBlocks, count: int, *, stream: torch.cuda.Stream | None = None) -> None:
+    """Folds the next ``count`` blocks of every layer, complete in the ring,
+    into 8 bits; later calls read them from there."""
+    with _on_device(blocks.device):
+        rc = _native.lib().sf_kv_fold(blocks._whole_ref, int(count),
+                                      _stream_handle(stream, blocks.device))
+    _native.check(rc, "sf_kv_fold")
+    blocks.folded += int(count)
+
+
+def kv_read(blocks: KVBlocks, layer: int, start: int, stop: int, *,
+            stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of tokens start .. stop - 1 as the attention sees them,
+    bf16 [batch, kv_heads, tokens, head_dim]."""
+    ref = blocks._check_layer(layer)
+    if not 0 <= start <= stop:
+        raise ValueError("tokens out of range")
+    shape = (blocks.batch, blocks.kv_heads, stop - start, blocks.head_dim)
+    keys = torch.empty(shape, dtype=_BF16, device=blocks.device)
+    values = torch.empty(shape, dtype=_BF16, device=blocks.device)
+    if stop > start:
+        with _on_device(blocks.device):
+            rc = _native.lib().sf_kv_read(ref, int(start), stop - start, keys.data_ptr(),
+                                          values.data_ptr(), _stream_handle(stream, blocks.device))
+        _native.check(rc, "sf_kv_read")
+    return keys, values
+
+
+# ------------------------------------------------------------------ K9 ----
+@functools.lru_cache(maxsize=256)
+def _block_attention_workspace(batch: int, queries: int, keys: int, q_heads: int, kv_heads: int,
+                               head_dim: int) -> int:
+    return _native.lib().sf_block_attention_workspace(batch, queries, keys, q_heads, kv_heads,
+                                                      head_dim)
+
+
+def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int,
+                    mask: torch.Tensor | None, scale: float, *,
+                    stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Grouped-query attention over the first ``keys`` tokens of a block
+    cache's layer (K9).
+
+    query [batch, Hq, Q, head_dim] bf16, Hq a multiple of the cache's heads;
+    mask bool [batch or 1, 1, Q, M] (True = attend) over the last M <= keys
+    keys, those before them admitted, or None for causal attention aligned to
+    the end of the keys.  A row that admits no key gives zeros.  Returns
+    [batch, Q, Hq, head_dim] bf16.  With ``stream``, the inputs and the output
+    (memory of the current stream) are the caller's to order between the two
+    streams."""
+    ref = blocks._check_layer(layer)
+    blocks._check_rows("query", query)
+    B, Hq, Q, D = query.shape
+    if Hq < 1 or Hq % blocks.kv_heads:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    if keys < 0:
+        raise ValueError("keys must not be negative")
+    device = blocks.device
+    mask_ptr, mask_batch, mask_q, mask_keys = None, 0, 0, 0
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError("block attention takes a bool mask (True = attend)")
+        if mask.device != device or mask.dim() != 4 or mask.shape[0] not in (1, B) \
+                or mask.shape[1] != 1 or mask.shape[2] != Q or mask.shape[3] > keys:
+            raise ValueError(f"mask must be bool [1 or {B}, 1, {Q}, up to {keys} keys]")
+        if mask.stride(3) != 1:
+            mask = mask.contiguous()
+        mask_batch, _, mask_q, _ = mask.stride()
+        if mask.shape[0] == 1:
+            mask_batch = 0
+        mask_keys = mask.shape[3]
+    out = torch.empty((B, Q, Hq, D), dtype=_BF16, device=device)
+    if Q == 0:
+        return out
+    if keys == 0:
+        return out.zero_()
+    if mask is not None:
+        # A mask of no keys admits them all: any address but null.
+        mask_ptr = mask.data_ptr() if mask_keys else out.data_ptr()
+    qb, qh, qt, qd = query.stride()
+    if qd != 1 or (qb | qh | qt) % 8 or query.data_ptr() % 16:
+        query = query.clone(memory_format=torch.contiguous_format)
+        qb, qh, qt, _ = query.stride()
+    need = _block_attention_workspace(B, Q, keys, Hq, blocks.kv_heads, D)
+    work_ptr = None
+    if need:
+        try:
+            work = _scratch(need, device, stream)
+            work_ptr = work.data_ptr()
+        except torch.OutOfMemoryError:
+            need = 0  # the keys are not split then
+    with _on_device(device):
+        rc = _native.lib().sf_block_attention(
+            ref, B, blocks.kv_heads, keys, query.data_ptr(), qb, qh, qt, Q, Hq, mask_ptr,
+            mask_batch, mask_q, mask_keys, float(scale), out.data_ptr(), work_ptr, need,
+            _stream_handle(stream, device))
+    _native.check(rc, "sf_block_attention")
+    return out
+
+
+# ----------------------------------------------------------------- K10 ----
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table, *,
+                 stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary positions of queries and keys (K10).
+
+    q [B, T, Hq, D] and k [B, T, Hk, D], bf16, fp16 or fp32 (one type, any
+    strides with a unit last one); positions int64 [B, T], [1, T] or [T];
+    ``table`` a ``specfit_amd.rotary.RotaryTable`` on the same device.  Returns
+    (q, k) as [B, H, T, D] contiguous.  Angles are taken in fp64, so far
+    positions keep them; each output is rounded once."""
+    if q.dtype not in _DTYPES:
+        raise ValueError("q must be bf16, fp16 or fp32")
+    _require_cuda("q", q)
+    _require_cuda("k", k, q.dtype)
+    _require_cuda("positions", positions, torch.int64)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError("q and k must be [batch, tokens, heads, head_dim] of the same tokens")
+    B, T, Hq, D = q.shape
+    Hk = k.shape[2]
+    if D != table.head_dim:
+        raise ValueError(f"the table is for head dim {table.head_dim}, not {D}")
+    turns = table.turns
+    if k.device != q.device or positions.device != q.device or turns.device != q.device:
+        raise ValueError("q, k, positions and the table must share a device")
+    if positions.dim() == 1:
+        positions = positions[None]
+    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] not in (1, B):
+        raise ValueError(f"positions must be [{B} or 1, {T}]")
+    if positions.stride(1) != 1:
+        positions = positions.contiguous()
+    step = positions.stride(0) if positions.shape[0] == B and B > 1 else 0
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    q_out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=q.device)
+    k_out = torch.empty((B, Hk, T, D), dtype=q.dtype, device=q.device)
+    (qb, qt, qh, _), (kb, kt, kh, _) = q.stride(), k.stride()
+    with _on_device(q.device):
+        rc = _native.lib().sf_rotary(
+            _DTYPES[q.dtype], q.data_ptr(), qb, qt, qh, Hq, k.data_ptr(), kb, kt, kh, Hk,
+            positions.data_ptr(), step, turns.data_ptr(), table.factor, B, T, D, table.rotary_dim,
+            table.interleaved, q_out.data_ptr(), k_out.data_ptr(), _stream_handle(stream, q.device))
+    _native.check(rc, "sf_rotary")
+    return q_out, k_out
+
+
+# ----------------------------------------------------------------- K11 ----
+@functools.lru_cache(maxsize=256)
+def _logit_rules_workspace(rows: int, vocab: int) -> int:
+    return _native.lib().sf_logit_rules_workspace(rows, vocab)
+
+
+def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, out,
+                 want_tokens, stream):
+    if logits.dtype not in _DTYPES:
+        raise ValueError("logits must be bf16, fp16 or fp32")
+    _require_cuda("logits", logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    N, V = logits.shape
+    if V == 0:
+        raise ValueError("logits must have a vocabulary")
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    device = logits.device
+    if not repetition > 0:
+        raise ValueError("the repetition penalty must be positive")
+    counts_ptr = paths_ptr = bias_ptr = allowed_ptr = None
+    length = bias_stride = allowed_stride = 0
+    if counts is not None:
+        _require_cuda("counts", counts, torch.int32)
+        if counts.shape != (V,) or counts.device != device or not counts.is_contiguous():
+            raise ValueError(f"counts must be contiguous int32 [{V}]")
+        counts_ptr = counts.data_ptr()
+    if paths is not None:
+        _require_cuda("paths", paths, torch.int32)
+        if paths.dim() != 2 or paths.shape[0] != N or paths.device != device:
+            raise ValueError(f"paths must be int32 [{N}, length]")
+        paths = paths.contiguous()
+        length, paths_ptr = paths.shape[1], paths.data_ptr()
+    if bias is not None:
+        _require_cuda("bias", bias, torch.float32)
+        if bias.device != device or bias.shape not in ((V,), (1, V), (N, V)):
+            raise ValueError(f"bias must be fp32 [{V}] or [{N}, {V}]")
+        if bias.stride(-1) != 1:
+            bias = bias.contiguous()
+        bias_stride = bias.stride(0) if bias.dim() == 2 and bias.shape[0] > 1 else 0
+        if bias.dim() == 2 and bias.shape[0] > 1 and bias_stride == 0:
+            bias = bias[0]  # one row expanded
+        bias_ptr = bias.data_ptr()
+    if allowed is not None:
+        words = (V + 31) // 32
+        _require_cuda("allowed", allowed, torch.int32)
+        if allowed.device != device or allowed.shape not in ((words,), (1, words), (N, words)):
+            raise ValueError(f"allowed must be int32 [{words}] or [{N}, {words}]")
+        if allowed.stride(-1) != 1:
+            allowed = allowed.contiguous()
+        allowed_stride = allowed.stride(0) if allowed.dim() == 2 and allowed.shape[0] > 1 else 0
+        allowed_ptr = allowed.data_ptr()
+    tokens = work = None
+    need = 0
+    if want_tokens:
+        tokens = torch.empty(N, dtype=torch.int64, device=device)
+    if N == 0:
+        return tokens
+    if want_tokens:
+        need = _logit_rules_workspace(N, V)
+        work = _scratch(need, device, stream)
+    out_ptr, out_stride = (None, 0) if out is None else (out.data_ptr(), out.stride(0))
+    with _on_device(device):
+        rc = _native.lib().sf_logit_rules(
+            _DTYPES[logits.dtype], logits.data_ptr(), logits.stride(0), N, V, counts_ptr, paths_ptr,
+            length, float(repetition), float(presence), float(frequency), bias_ptr, bias_stride,
+            allowed_ptr, allowed_stride, out_ptr, out_stride, _ptr(tokens), _ptr(work), need,
+            _stream_handle(stream, device))
+    _native.check(rc, "sf_logit_rules")
+    return tokens
+
+
+def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
+                  paths: torch.Tensor | None = None, repetition: float = 1.0,
+                  presence: float = 0.0, frequency: float = 0.0,
+                  bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Repetition penalties, a bias and an allowed set on rows of logits (K11).
+
+    logits [N, V] bf16, fp16 or fp32.  n = counts[v] (int32 [V]) + the
+    occurrences of v in the row of paths (int32 [N, P]; entries outside the
+    vocabulary, such as a padding of -1, count for nothing).  A token with
+    n > 0 has x -> (x * repetition if x < 0 else x / repetition) -
+    (frequency * n + presence); then bias (fp32 [V] or [N, V]) is added, and a
+    token whose bit v % 32 of word v // 32 of allowed (int32 [V / 32 up] or
+    [N, V / 32 up]) is 0 becomes -inf.  Each step is rounded to fp32, the result
+    once more to the logits' type.  ``out`` may be ``logits``."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
+            or out.dim() != 2 or out.stride(1) != 1:
+        raise ValueError("out must be like logits, with a unit last stride")
+    elif out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("the rows of out must not overlap")
+    _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, out, False,
+                 stream)
+    return out
+
+
+def greedy_tokens(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
+                  paths: torch.Tensor | None = None, repetition: float = 1.0,
+                  presence: float = 0.0, frequency: float = 0.0,
+                  bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                  stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """int64 [N]: each row's token with the largest adjusted logit (in fp32,
+    before adjust_logits' last rounding), the lowest of equals; a NaN counts as
+    the largest, and a row in which nothing is above -inf gives -1.  Arguments
+    as adjust_logits."""
+    return _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, None,
+                        True, stream)

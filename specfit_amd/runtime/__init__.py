@@ -1,11 +1,13 @@
 """Drop-in runtime of the offloaded Qwen3-MoE verification path
 (mirrors the public names of the reference's ``specfit.runtime``)."""
+from .block_kv_cache import BlockKVCache
 from .cache_observer import (CacheTransition, CacheTransitionCounters, CacheTransitionObserver,
                              RecordingCacheTransitionObserver,
                              aggregate_cache_transition_counters)
 from .cache_snapshot import CacheSlotSnapshot, GpuExpertCacheSnapshot, PendingTransferSnapshot
 from .gpu_expert_cache import GpuExpertCache
 from .lease import ExpertCacheStats, ExpertLease, NoEvictableSlotError
+from .logit_rules import LogitRules
 from .qwen3_offloaded_experts import (ExpertExecutionPolicy, Qwen3OffloadedExperts,
                                       ReductionMode)
 from .qwen3_expert_prefetch import Qwen3ExpertPrefetch
@@ -24,6 +26,7 @@ from .tree_verify import (Eagle3DraftTree, TreeVerification, compact_tree_cache,
                           verify_draft_tree)
 
 __all__ = [
+    "BlockKVCache", "LogitRules",
     "CacheSlotSnapshot", "CacheTransition", "CacheTransitionCounters",
     "CacheTransitionObserver", "ExpertCacheStats", "ExpertExecutionPolicy", "ExpertKey",
     "ExpertLease", "GpuExpertCache", "GpuExpertCacheSnapshot", "NoEvictableSlotError",

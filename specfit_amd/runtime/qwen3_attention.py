@@ -14,6 +14,13 @@ becomes a view of its rows) and the forward runs one GEMM over it instead of
 three; K7 reads the query and key heads straight out of the fused rows.  A
 projection whose weight was replaced afterwards (``module.to``, a new
 Parameter) turns the fused GEMM off for that layer.
+
+With a ``BlockKVCache`` as ``past_key_values`` the new keys and values go
+into it and the attention runs over its 8-bit blocks (K9), whatever the
+config's attention implementation.  With a rotary table
+(``install_hip_attention(model, rotary=...)``) the rotary embedding takes its
+angles from the position ids (K10), for any batch and head dim, instead of
+from the model's bf16 cosines.
 """
 from __future__ import annotations
 
@@ -22,11 +29,14 @@ import torch.nn.functional as F
 from torch import nn
 
 from .. import ops
+from ..rotary import RotaryTable
+from .block_kv_cache import BlockKVCache
 
 
 class Qwen3AttentionHip(nn.Module):
-    def __init__(self, attention: nn.Module) -> None:
+    def __init__(self, attention: nn.Module, rotary: RotaryTable | None = None) -> None:
         super().__init__()
+        self.rotary = rotary
         for name in ("config", "layer_idx", "head_dim", "num_key_value_groups", "scaling",
                      "attention_dropout", "is_causal", "sliding_window"):
             setattr(self, name, getattr(attention, name))
@@ -58,9 +68,10 @@ class Qwen3AttentionHip(nn.Module):
                                            self.v_proj.weight.data_ptr()) == self._qkv_ptrs)
 
     @classmethod
-    def from_module(cls, attention: nn.Module) -> "Qwen3AttentionHip":
+    def from_module(cls, attention: nn.Module,
+                    rotary: RotaryTable | None = None) -> "Qwen3AttentionHip":
         """Wrap an HF ``Qwen3MoeAttention`` (shares its submodules)."""
-        return cls(attention)
+        return cls(attention, rotary)
 
     def _fused(self, hidden_states: torch.Tensor, cos: torch.Tensor) -> bool:
         return (hidden_states.dim() == 3 and hidden_states.shape[0] == 1
@@ -88,7 +99,13 @@ class Qwen3AttentionHip(nn.Module):
         else:
             q = self.q_proj(hidden_states).view(hidden_shape)
             k = self.k_proj(hidden_states).view(hidden_shape)
-        if self._fused(hidden_states, cos):
+        if self.rotary is not None:
+            positions = kwargs.get("position_ids")
+            if positions is None:
+                raise ValueError("a rotary table needs the position ids")
+            query_states, key_states = ops.rotary_embed(self.q_norm(q), self.k_norm(k), positions,
+                                                        self.rotary)
+        elif self._fused(hidden_states, cos):
             query_states, key_states = ops.qk_norm_rope(
                 q, k, self.q_norm.weight, self.k_norm.weight, self.q_norm.variance_epsilon,
                 cos.contiguous(), sin.contiguous())
@@ -100,6 +117,15 @@ class Qwen3AttentionHip(nn.Module):
             value_states = qkv[..., nq + nk:].view(hidden_shape).transpose(1, 2)
         else:
             value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
+        if isinstance(past_key_values, BlockKVCache):
+            if self.training and self.attention_dropout:
+                raise ValueError("a block cache is for inference (no dropout)")
+            if self.sliding_window is not None:
+                raise ValueError("a block cache has no sliding window")
+            past_key_values.append(self.layer_idx, key_states, value_states)
+            attn_output = past_key_values.attend(self.layer_idx, query_states, attention_mask,
+                                                 self.scaling)
+            return self.o_proj(attn_output.reshape(*input_shape, -1)), None
         if past_key_values is not None:
             key_states, value_states = past_key_values.update(key_states, value_states,
                                                               self.layer_idx)
@@ -113,14 +139,18 @@ class Qwen3AttentionHip(nn.Module):
         return self.o_proj(attn_output), attn_weights
 
 
-def install_hip_attention(model: nn.Module) -> int:
+def install_hip_attention(model: nn.Module, rotary: RotaryTable | None = None) -> int:
     """Replace every ``Qwen3MoeAttention`` of ``model`` with a
-    ``Qwen3AttentionHip`` sharing its submodules; returns how many."""
+    ``Qwen3AttentionHip`` sharing its submodules; returns how many.  With
+    ``rotary`` (``RotaryTable.from_config(model.config, device=...)``) these,
+    and those already there, take their rotary embedding from it."""
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeAttention
 
     count = 0
     for layer in model.model.layers:
         if isinstance(layer.self_attn, Qwen3MoeAttention):
-            layer.self_attn = Qwen3AttentionHip.from_module(layer.self_attn)
+            layer.self_attn = Qwen3AttentionHip.from_module(layer.self_attn, rotary)
             count += 1
+        elif rotary is not None and isinstance(layer.self_attn, Qwen3AttentionHip):
+            layer.self_attn.rotary = rotary
     return count

@@ -25,6 +25,10 @@ from math import isclose, isfinite, log
 import numpy as np
 import torch
 
+from .block_kv_cache import BlockKVCache
+from .logit_rules import LogitRules
+from .qwen3_attention import Qwen3AttentionHip
+
 
 @dataclass(frozen=True, slots=True)
 class Eagle3DraftTree:
@@ -128,6 +132,15 @@ class Eagle3DraftTree:
         host[:, base_kv_length:] = self.ancestor_matrix()
         return torch.from_numpy(host).to(device).view(1, 1, q, base_kv_length + q)
 
+    def path_indices(self) -> np.ndarray:
+        """int64 [1 + N, 1 + depth]: the rows of the verification input on
+        each row's path, from the seed to itself, padded with -1."""
+        rows = [(0,)]
+        for node, parent in enumerate(self.parent_ids, start=1):
+            rows.append(rows[parent] + (node,))
+        width = max(len(r) for r in rows)
+        return np.array([r + (-1,) * (width - len(r)) for r in rows], dtype=np.int64)
+
     def accepted_path(self, verifier_token_ids: torch.Tensor) -> tuple[int, ...]:
         """Greedy acceptance: from the seed, follow the child whose token is
         the verifier's prediction at its parent (eagle3_types.py:475-502)."""
@@ -179,8 +192,15 @@ def _first_eos_position(committed: torch.Tensor, eos_token_ids) -> int | None:
 def compact_tree_cache(cache, *, base_kv_length: int, verification_positions: tuple[int, ...],
                        verification_node_count: int) -> None:
     """Keep the prefix and the verified positions of every cache layer
-    (eagle3_tree.py:833-858)."""
+    (eagle3_tree.py:833-858).  A BlockKVCache also folds the blocks that
+    this completes."""
     expected = base_kv_length + verification_node_count
+    if isinstance(cache, BlockKVCache):
+        if any(cache.get_seq_length(l) != expected for l in range(cache.blocks.layers)):
+            raise RuntimeError("target cache layer has an unexpected length")
+        cache.compact(base_kv_length, verification_positions)
+        cache.commit()
+        return
     index = None
     dest = slice(base_kv_length, base_kv_length + len(verification_positions))
     for layer in cache.layers:
@@ -196,22 +216,46 @@ def compact_tree_cache(cache, *, base_kv_length: int, verification_positions: tu
     cache.crop(base_kv_length + len(verification_positions))
 
 
+def _attends_in_blocks(target, cache) -> bool:
+    """Whether every attention layer runs over the block cache itself."""
+    return isinstance(cache, BlockKVCache) and all(
+        isinstance(layer.self_attn, Qwen3AttentionHip) for layer in target.model.layers)
+
+
 def verify_draft_tree(target, tree: Eagle3DraftTree, pending_seed: torch.Tensor, cache, *,
-                      eos_token_ids=(), commit: bool = True) -> TreeVerification:
+                      eos_token_ids=(), commit: bool = True, rules: LogitRules | None = None,
+                      allowed: torch.Tensor | None = None) -> TreeVerification:
     """One verification forward of ``tree`` against ``cache`` (a HF
     DynamicCache holding the committed prefix), as eagle3_tree.py:1202-1290:
     target(input_ids=[seed, drafts], attention_mask=tree mask,
     position_ids=base + depth, past_key_values=cache, use_cache=True,
     logits_to_keep=0); greedy verifier tokens; accepted path; EOS cut; and,
-    when ``commit``, the KV compaction to the verified positions."""
+    when ``commit``, the KV compaction to the verified positions.
+
+    ``cache`` may be a BlockKVCache; layers that attend over its blocks get the
+    tree's own part of the mask only.  With ``rules`` the verifier tokens are
+    the greedy ones of the adjusted logits: rules.counts is the histogram of
+    the committed prefix (the seed and each row's path come on top), ``allowed``
+    int32 [1 + N, vocab / 32 up] a grammar's set per row (without rules, the
+    set alone).  ``commit`` then counts the committed tokens.  A row in which
+    nothing is allowed has the verifier token -1, which no draft matches; if
+    the last committed row is one, the pending seed is -1."""
     verify_ids = tree.verification_token_ids(pending_seed)
     base = cache.get_seq_length()
     device = verify_ids.device
-    mask = tree.verification_attention_mask(base_kv_length=base, device=device)
+    mask = tree.verification_attention_mask(
+        base_kv_length=0 if _attends_in_blocks(target, cache) else base, device=device)
     positions = tree.verification_position_ids(base_kv_length=base, device=device)
     outputs = target(input_ids=verify_ids, attention_mask=mask, position_ids=positions,
                      past_key_values=cache, use_cache=True, logits_to_keep=0)
-    verifier = outputs.logits.argmax(dim=-1)
+    if rules is None and allowed is None:
+        verifier = outputs.logits.argmax(dim=-1)
+    else:
+        if rules is None:
+            rules = LogitRules()
+        paths = torch.from_numpy(tree.path_indices()).to(device)
+        paths = torch.where(paths < 0, -1, verify_ids[0][paths.clamp_min(0)]).to(torch.int32)
+        verifier = rules.greedy(outputs.logits[0], paths, allowed=allowed)[None]
     accepted = tree.accepted_path(verifier)
     vpos = (0,) + accepted
     committed = verify_ids[:, vpos]
@@ -225,6 +269,8 @@ def verify_draft_tree(target, tree: Eagle3DraftTree, pending_seed: torch.Tensor,
     if commit:
         compact_tree_cache(cache, base_kv_length=base, verification_positions=vpos,
                            verification_node_count=verify_ids.shape[1])
+        if rules is not None and rules.counts is not None:
+            rules.count(committed)
     last = vpos[-1]
     return TreeVerification(verify_ids=verify_ids, logits=outputs.logits,
                             verifier_tokens=verifier, accepted_node_ids=accepted,
