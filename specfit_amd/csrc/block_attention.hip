@@ -12,10 +12,9 @@
 // so neither costs an instruction per value.  M, a row's maximum in log2
 // units, is a reference only: every weight of a row has the same one.
 //
-// direct form: a wavefront owns 16 or 32 rows and takes its operands straight
-// from the cache into registers, whose order is that of the matrix
-// instructions (no LDS, no barrier); the four wavefronts of a workgroup take
-// every fourth tile and merge their states at the end.
+// Two forms, and a kernel that merges splits of the keys: few rows per KV head go
+// straight from the cache to registers (direct_kernel), many share tiles in LDS
+// (staged_kernel); plan_of chooses.
 #include <algorithm>
 
 #include "kv_blocks.h"
@@ -26,9 +25,28 @@ namespace {
 
 typedef float sf_f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * SF_WAVE;
+// Where a value is made in a branch that is rarely taken: keeps the compiler
+// from running the branch always and selecting.  After a computation that is
+// meant to overlap with what stands beside it: keeps it from being moved down to
+// its use.
+template <typename T>
+__device__ __forceinline__ void pin(T& x) {
+  asm volatile("" : "+v"(x));
+}
+
+// Loads and stores through pointers of the argument structs, explicitly global.
+template <typename T>
+__device__ __forceinline__ T ld(const T* p) {
+  return *(const __attribute__((address_space(1))) T*)(p);
+}
+
+constexpr int kDirectRows = 16;
+constexpr int kDirectWaves = 8;
+constexpr int kDirectThreads = kDirectWaves * SF_WAVE;
 constexpr int kMaxSplits = 128;
+constexpr int kStagedWaves = 8;
+constexpr int kStagedThreads = kStagedWaves * SF_WAVE;
+constexpr int kStagedRows = 32 * kStagedWaves;
 
 struct Args {
   sf_kv_cache c;
@@ -57,6 +75,13 @@ __device__ __forceinline__ float max_raw(float x, float y) {
   return __builtin_amdgcn_fmed3f(x, y, INFINITY);  // one instruction; a NaN gives the other
 }
 
+// The largest of three (fmaxf of matrix results would canonicalise each first).
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
+
 __device__ __forceinline__ float swap32_max(float x) {
   const int v = __float_as_int(x);
   const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
@@ -81,18 +106,27 @@ __device__ __forceinline__ float swap16_sum(float x) {
   return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
 
-// Whether a row admits keys key .. key + 3, a byte each.
+// Whether a row admits keys key .. key + 3, a byte each: one load, at the
+// nearest place within the mask's keys, shifted.  Keys before the mask are
+// admitted, keys past the end are not.
 __device__ __forceinline__ uint32_t admitted(const uint8_t* row, int key, int mask_begin, int S) {
-  uint32_t w = 0;
-  if (key >= mask_begin && key + 4 <= S) {
-    __builtin_memcpy(&w, row + (key - mask_begin), 4);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (key + i < S)
-        w |= (key + i < mask_begin ? 1u : static_cast<uint32_t>(row[key + i - mask_begin]))
-             << (8 * i);
+  const int off = key - mask_begin, count = S - mask_begin;
+  if (count >= 4) {  // uniform
+    const int at = min(max(off, 0), count - 4);
+    uint32_t w;
+    __builtin_memcpy(&w, row + at, 4);
+    const int past = min(off - at, 4), before = min(at - off, 4);
+    if (past > 0) w = static_cast<uint32_t>(static_cast<uint64_t>(w) >> (8 * past));
+    if (before > 0)
+      w = static_cast<uint32_t>(static_cast<uint64_t>(w) << (8 * before)) |
+          0x01010101u >> (32 - 8 * before);
+    return w;
   }
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (key + i < S)
+      w |= (key + i < mask_begin ? 1u : static_cast<uint32_t>(row[key + i - mask_begin])) << (8 * i);
   return w;
 }
 
@@ -224,16 +258,25 @@ struct Rows {
       for (int i = 0; i < kN; ++i) acc[t][i] = 0.f;
   }
 
-  // Scores (in s) to weights as bf16 (in w, the B operands of the values'
-  // product); factor: of the scores, to log2 units.
-  __device__ __forceinline__ void softmax(Acc (&s)[Sh::kScoreTiles], float factor, float v_scale,
-                                          sf_u32x4 (&w)[Sh::kPSteps]) {
-    float mx[2] = {s[0][0], s[1][0]};
+  // The largest of the lane's scores.
+  static __device__ __forceinline__ float top(const Acc (&s)[Sh::kScoreTiles]) {
+    float mx[2] = {s[0][0], s[0][1]};
 #pragma unroll
     for (int t = 0; t < Sh::kScoreTiles; ++t)
 #pragma unroll
-      for (int i = 0; i < kN; ++i) mx[t & 1] = max_raw(mx[t & 1], s[t][i]);
-    const float mnew = fmaxf(m, Sh::row_max(max_raw(mx[0], mx[1])) * factor);
+      for (int i = 0; i < kN; i += 4) {
+        mx[0] = max3(mx[0], s[t][i], s[t][i + 1]);
+        mx[1] = max3(mx[1], s[t][i + 2], s[t][i + 3]);
+      }
+    return max_raw(mx[0], mx[1]);
+  }
+
+  // Brings the state to the maximum over a tile whose largest score of the lane
+  // is `most`; factor: of the scores, to log2 units.  mul and base: a score's
+  // weight times the value scale is 2^(s mul + base).
+  __device__ __forceinline__ void raise(Acc (&s)[Sh::kScoreTiles], float most, float factor,
+                                        float v_scale, float& mul, float& base) {
+    const float mnew = fmaxf(m, Sh::row_max(most) * factor);
     if (__any(mnew > m)) {
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mnew);
       l *= alpha;
@@ -244,36 +287,55 @@ struct Rows {
       m = mnew;
     }
     const float shift = static_cast<float>(static_cast<int>(__float_as_uint(v_scale) >> 23) - 127);
-    float base = m == -INFINITY ? 0.f : shift - m;
-    float mul = factor;
+    base = m == -INFINITY ? 0.f : shift - m;
+    mul = factor;
     const bool large = fabsf(m) > kFusedMax && m != -INFINITY;
     if (__any(large)) {
-      const float top = large ? m : 0.f;
+      const float off = large ? m : 0.f;
 #pragma unroll
-      for (int t = 0; t < Sh::kScoreTiles; ++t)
+      for (int t = 0; t < Sh::kScoreTiles; ++t) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) s[t][i] = s[t][i] * factor - top;
+        for (int i = 0; i < kN; ++i) s[t][i] = s[t][i] * factor - off;
+        pin(s[t]);
+      }
       if (large) base = shift;
       mul = 1.f;
     }
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int t = 0; t < Sh::kScoreTiles; ++t)
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], mul, base));
-        sum[i & 1] += s[t][i];
-      }
+  }
+
+  // The n-th pair of scores to weights times the value scale, as bf16 into w (the
+  // B operands of the values' product, in the order of the lane's scores), and
+  // added to sum.
+  static constexpr int kPairs = Sh::kScoreTiles * kN / 2;
+  static __device__ __forceinline__ void weigh_pair(const Acc (&s)[Sh::kScoreTiles], int n,
+                                                    float mul, float base, float (&sum)[2],
+                                                    sf_u32x4 (&w)[Sh::kPSteps]) {
+    const float p0 =
+        __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n / kN][2 * n % kN], mul, base));
+    const float p1 =
+        __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n / kN][2 * n % kN + 1], mul, base));
+    sum[0] += p0;
+    sum[1] += p1;
+    w[n / 4][n % 4] = sf_pack_bf16(p0, p1);
+  }
+  __device__ __forceinline__ void add_sum(const float (&sum)[2], float v_scale) {
     // 1 / v_scale, a power of two.
     l = __builtin_fmaf(sum[0] + sum[1],
                        __uint_as_float((254u << 23) - __float_as_uint(v_scale)), l);
+  }
+  __device__ __forceinline__ void weigh(const Acc (&s)[Sh::kScoreTiles], float mul, float base,
+                                        float v_scale, sf_u32x4 (&w)[Sh::kPSteps]) {
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < Sh::kPSteps; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = 8 * k + 2 * j;  // in the order of the lane's scores
-        w[k][j] = sf_pack_bf16(s[n / kN][n % kN], s[n / kN][n % kN + 1]);
-      }
+    for (int n = 0; n < kPairs; ++n) weigh_pair(s, n, mul, base, sum, w);
+    add_sum(sum, v_scale);
+  }
+
+  __device__ __forceinline__ void softmax(Acc (&s)[Sh::kScoreTiles], float factor, float v_scale,
+                                          sf_u32x4 (&w)[Sh::kPSteps]) {
+    float mul, base;
+    raise(s, top(s), factor, v_scale, mul, base);
+    weigh(s, mul, base, v_scale, w);
   }
 };
 
@@ -299,76 +361,452 @@ __device__ __forceinline__ sf_u32x4 entries(const sf_u32x4& v, int kind) {
   return r;
 }
 
-// 1 where a weight is not 0.
-__device__ __forceinline__ sf_u32x4 present(const sf_u32x4& w) {
-  sf_u32x4 r;
+// What a lane needs to restrict the scores of a tile: its mask's bytes, loaded
+// with the tile's keys, or the keys that its row sees without a mask.
+template <typename Sh, bool MASK>
+struct Admit {
+  const uint8_t* row;  // the mask of the lane's row
+  int mask_begin, S, lane_end;
+  int full;            // keys below it are admitted by all of the wavefront's rows
+  uint32_t words[Sh::kWords];
+
+  __device__ __forceinline__ void load(int lane, int key0) {
+    if (!MASK || key0 + kBlockTokens <= full) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    r[j] = (w[j] & 0x7fffu ? 0x3f80u : 0u) | (w[j] & 0x7fff0000u ? 0x3f800000u : 0u);
-  return r;
+    for (int g = 0; g < Sh::kWords; ++g) {
+      words[g] = admitted(row, key0 + Sh::key(lane, g), mask_begin, S);
+      pin(words[g]);
+    }
+  }
+  // Scores of keys that the row does not admit: -inf.
+  __device__ __forceinline__ void restrict_scores(typename Sh::Acc (&s)[Sh::kScoreTiles], int lane,
+                                                  int key0) const {
+    constexpr int kN = acc_size<typename Sh::Acc>();
+    if (key0 + kBlockTokens <= full) return;
+#pragma unroll
+    for (int g = 0; g < Sh::kWords; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool ok = MASK ? ((words[g] >> (8 * i)) & 0xffu) != 0
+                             : key0 + Sh::key(lane, g) + i < lane_end;
+        if (!ok) s[4 * g / kN][4 * g % kN + i] = -INFINITY;
+      }
+#pragma unroll
+    for (int t = 0; t < Sh::kScoreTiles; ++t) pin(s[t]);
+  }
+};
+
+// Where a call's row of the output, or of its partial results, lies.
+__device__ __forceinline__ int64_t out_row_at(const Args& a, int head, int row) {
+  const int b = head / a.kv_heads, h = head - b * a.kv_heads;
+  const int t = row / a.G;
+  return (static_cast<int64_t>(b) * a.Q + t) * (static_cast<int64_t>(a.kv_heads) * a.G) + h * a.G +
+         (row - t * a.G);
 }
 
-// acc += V^T P^T for a tile whose values hold infinities or NaN: they reach the
-// rows that give their key a weight and no others (0 times them in the product
-// would).  operand(t, k): the values' operand of output tile t, step k.  Rare,
-// so it is written for few registers: one kind after the other.
-template <typename Sh, bool CODE, typename Operand>
-__device__ __forceinline__ void add_special(Operand operand, const sf_u32x4 (&w)[Sh::kPSteps],
-                                            typename Sh::Acc (&acc)[Sh::kOutTiles]) {
+// A tile's operands of the two products, for the rare paths.
+template <int D, int ROWS, int HELD>
+struct TileOperands {
+  using Sh = Shape<D, ROWS>;
+  const char *k, *v;  // of the lane's first piece
+  bool coded;
+
+  __device__ __forceinline__ TileOperands(const Args& a, int head, int tile, int lane) {
+    coded = tile < a.c.folded_blocks;
+    if (coded) {
+      const int64_t at =
+          (static_cast<int64_t>(head) * a.c.capacity_blocks + tile) * (kBlockTokens * D);
+      k = static_cast<const char*>(a.c.k8) + at + 16 * Sh::key_lane(lane);
+      v = static_cast<const char*>(a.c.v8) + at + 16 * Sh::value_lane(lane);
+    } else {
+      const int64_t at = (static_cast<int64_t>(head) * a.c.ring_blocks + tile % a.c.ring_blocks) *
+                         (2 * kBlockTokens * D);
+      k = static_cast<const char*>(a.c.k_tail) + at + 16 * Sh::key_lane16(lane);
+      v = static_cast<const char*>(a.c.v_tail) + at + 16 * Sh::value_lane16(lane);
+    }
+  }
+  static __device__ __forceinline__ sf_u32x4 code_operand(const char* p, int step) {
+    sf_u32x4 x, y;
+    sf_codes_frags<HELD>(sf_ld16(p), x, y);
+    return step & 1 ? y : x;
+  }
+  __device__ __forceinline__ sf_u32x4 key(int t, int s) const {
+    return coded ? code_operand(k + 16 * Sh::key_piece(t, s >> 1), s)
+                 : sf_ld16(k + 16 * Sh::key_piece16(t, s));
+  }
+  __device__ __forceinline__ sf_u32x4 value(int t, int s) const {
+    return coded ? code_operand(v + 16 * Sh::value_piece(t, s >> 1), s)
+                 : sf_ld16(v + 16 * Sh::value_piece16(t, s));
+  }
+  // The operand's entries of a kind (see entries).
+  __device__ __forceinline__ sf_u32x4 of_kind(const sf_u32x4& x, int kind) const {
+    return HELD == SF_KV_INT8 && coded ? entries<true>(x, kind) : entries<false>(x, kind);
+  }
+};
+
+// What the tiles' values hold that is not finite (the loops take zeros in its
+// place, as 0 times it would reach the rows that do not admit its key): an
+// infinity or NaN is added to its element of the rows that admit the key.  An
+// int8 key with a NaN code (which the loops take for -128) makes the rows that
+// admit it NaN.  After the loops, so that their registers are free for it.
+template <int D, int ROWS, int HELD, bool MASK>
+__device__ __forceinline__ void add_special(Rows<D, ROWS>& r, const Args& a, int head, int lane,
+                                            int begin, int end, int step,
+                                            Admit<Shape<D, ROWS>, MASK>& admit) {
+  using Sh = Shape<D, ROWS>;
   using Acc = typename Sh::Acc;
   constexpr int kN = acc_size<Acc>();
 #pragma unroll 1
-  for (int t = 0; t < Sh::kOutTiles; ++t) {
-    Acc o;
+  for (int tile = begin; tile < end; tile += step) {
+    const TileOperands<D, ROWS, HELD> x(a, head, tile, lane);
+    const int flag =
+        x.coded ? a.c.flags[static_cast<int64_t>(head) * a.c.capacity_blocks + tile]
+                : a.c.tail_flags[static_cast<int64_t>(head) * a.c.ring_blocks +
+                                 tile % a.c.ring_blocks];
+    if (!flag) continue;
+    Acc s[Sh::kScoreTiles];  // 0 where the row admits the key
 #pragma unroll
-    for (int u = 0; u < Sh::kOutTiles; ++u)
-      if (u == t) o = acc[u];
+    for (int t = 0; t < Sh::kScoreTiles; ++t)
 #pragma unroll
-    for (int k = 0; k < Sh::kPSteps; ++k) o = Sh::mma(entries<CODE>(operand(t, k), 3), w[k], o);
-#pragma unroll 1
-    for (int kind = 0; kind < 3; ++kind) {
-      Acc has;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) has[i] = 0.f;
+      for (int i = 0; i < kN; ++i) s[t][i] = 0.f;
+    admit.load(lane, tile * kBlockTokens);
+    admit.restrict_scores(s, lane, tile * kBlockTokens);
+    if (flag & kFlagValue) {
+      sf_u32x4 w[Sh::kPSteps];
 #pragma unroll
       for (int k = 0; k < Sh::kPSteps; ++k)
-        has = Sh::mma(entries<CODE>(operand(t, k), kind), present(w[k]), has);
-      const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
 #pragma unroll
-      for (int i = 0; i < kN; ++i)
-        if (has[i] > 0.f) o[i] += add;
+        for (int j = 0; j < 4; ++j) {
+          const int n = 8 * k + 2 * j;
+          w[k][j] = (s[n / kN][n % kN] == 0.f ? 0x3f80u : 0u) |
+                    (s[n / kN][n % kN + 1] == 0.f ? 0x3f800000u : 0u);
+        }
+#pragma unroll 1
+      for (int kind = 0; kind < 3; ++kind) {
+        const float add = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+        for (int t = 0; t < Sh::kOutTiles; ++t) {
+          Acc has;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) has[i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < Sh::kPSteps; ++k)
+            has = Sh::mma(x.of_kind(x.value(t, k), kind), w[k], has);
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (has[i] > 0.f) r.acc[t][i] += add;
+        }
+      }
     }
+    if (HELD == SF_KV_INT8 && x.coded && (flag & kFlagKey)) {
+      const sf_u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+      bool bad = false;
 #pragma unroll
-    for (int u = 0; u < Sh::kOutTiles; ++u)
-      if (u == t) acc[u] = o;
+      for (int t = 0; t < Sh::kScoreTiles; ++t) {
+        Acc has;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) has[i] = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < Sh::kSteps; ++k) has = Sh::mma(entries<true>(x.key(t, k), 2), ones, has);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) bad |= has[i] > 0.f && s[t][i] == 0.f;
+      }
+      if (bad) r.l = __builtin_nanf("");  // a part of the row's sum
+    }
   }
 }
 
-// Scores of int8 keys that hold a NaN code: NaN.  operand(t, p): the keys'
-// operand of score tile t, step p.
-template <typename Sh, typename Operand>
-__device__ __forceinline__ void mark_nan_keys(Operand operand,
-                                              typename Sh::Acc (&s)[Sh::kScoreTiles]) {
+// The form of many rows: 32 rows per wavefront, 256 per workgroup, which share
+// each tile.  A tile is staged in LDS as bf16 in the cache's own order, codes
+// converted once for the eight wavefronts, so every operand is read as 64
+// consecutive 16-byte pieces.
+//
+// A wavefront's own matrix and vector work overlap: while the weights of tile
+// i are computed, the matrix unit forms the scores of tile i + 1, and while it
+// adds the values of tile i, the maximum of those scores is taken.  So in
+// iteration i the keys of i + 1 and the values of i are read, and one barrier
+// is enough with two buffers of keys and three of values (what a wavefront
+// writes before the barrier of iteration i, others last read before that of
+// i - 1).
+template <int D, int HELD, bool MASK>
+__global__ __launch_bounds__(kStagedThreads, 1) void staged_kernel(const Args a) {
+  using Sh = Shape<D, 32>;
   using Acc = typename Sh::Acc;
-  constexpr int kN = acc_size<Acc>();
-  const sf_u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  constexpr int kPieces = kBlockTokens * D / 8;             // of a tile's keys or values, bf16
+  constexpr int kLoads = 2 * kPieces / kStagedThreads;      // of both per thread, bf16
+  constexpr int kCodes = kPieces / 2;                       // of keys or values in 8 bits
+  __shared__ __attribute__((aligned(16))) sf_u32x4 k_lds[2][kPieces];
+  __shared__ __attribute__((aligned(16))) sf_u32x4 v_lds[3][kPieces];
+  const int lane = threadIdx.x & (SF_WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / SF_WAVE);
+  const int head = blockIdx.x % a.c.heads;
+  const int rest = blockIdx.x / a.c.heads;
+  const int split = rest % a.splits;
+  const int block_row = (a.row_tiles - 1 - rest / a.splits) * (kStagedRows);
+  const int wave_row = block_row + 32 * wave;
+  const int b = head / a.kv_heads;
+  const int h = head - b * a.kv_heads;
+  const int row = wave_row + Sh::row(lane);
+  const int row_c = min(row, a.rows - 1);
+  const int tok = row_c / a.G;
+  const int q_head = h * a.G + (row_c - tok * a.G);
+
+  const int diag = a.S - a.Q + 1;  // keys that token 0 sees
+  const int last = min(block_row + kStagedRows, a.rows) - 1;
+  const int keys_end = MASK ? a.S : min(a.S, diag + last / a.G);
+  const int begin = split * a.split_tiles;
+  const int end = min(begin + a.split_tiles, (keys_end + kBlockTokens - 1) / kBlockTokens);
+  Admit<Sh, MASK> admit;
+  admit.row = MASK ? a.mask + b * a.mask_batch + tok * a.mask_q : nullptr;
+  admit.mask_begin = a.mask_begin;
+  admit.S = a.S;
+  admit.lane_end = diag + tok;
+  admit.full = MASK ? min(a.S, a.mask_begin) : max(0, diag + min(wave_row, a.rows - 1) / a.G);
+
+  const int64_t cap = static_cast<int64_t>(head) * a.c.capacity_blocks;
+  const int64_t ring = static_cast<int64_t>(head) * a.c.ring_blocks;
+  const char* k8 = static_cast<const char*>(a.c.k8) + cap * (kBlockTokens * D);
+  const char* v8 = static_cast<const char*>(a.c.v8) + cap * (kBlockTokens * D);
+  const float* k_scale = a.c.k_scale + cap;
+  const float* v_scale = a.c.v_scale + cap;
+  const int32_t* flags8 = a.c.flags + cap;
+  const char* kt = static_cast<const char*>(a.c.k_tail) + ring * (2 * kBlockTokens * D);
+  const char* vt = static_cast<const char*>(a.c.v_tail) + ring * (2 * kBlockTokens * D);
+  const int32_t* tail_flags = a.c.tail_flags + ring;
+
+  // A tile on its way: into registers, and from there (bf16) into LDS.
+  // Its pieces are dealt out keys first, then values.
+  sf_u32x4 raw[kLoads];
+  int special = 0;
+  // First piece of the wavefront's j-th 64: of the keys, or (- count) the values.
+  auto first_piece = [&](int j) { return j * kStagedThreads + wave * SF_WAVE; };
+  auto load_tile = [&](int t) {
+    if (t < a.c.folded_blocks) {
+      const int64_t at = static_cast<int64_t>(t) * (kBlockTokens * D);
+#pragma unroll
+      for (int j = 0; j < kLoads / 2; ++j) {
+        const int n = first_piece(j);
+        raw[j] = sf_ld16((n < kCodes ? k8 + 16 * n : v8 + 16 * (n - kCodes)) + at, 16 * lane);
+      }
+    } else {
+      const int64_t at = static_cast<int64_t>(t % a.c.ring_blocks) * (2 * kBlockTokens * D);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int n = first_piece(j);
+        raw[j] = sf_ld16((n < kPieces ? kt + 16 * n : vt + 16 * (n - kPieces)) + at, 16 * lane);
+      }
+    }
+  };
+  auto stage_tile = [&](int t, sf_u32x4* kl, sf_u32x4* vl) {
+    int flag;
+    if (t < a.c.folded_blocks) {
+      flag = ld(flags8 + t);
+#pragma unroll
+      for (int j = 0; j < kLoads / 2; ++j) {
+        const int n = first_piece(j);
+        const bool values = n >= kCodes;
+        sf_u32x4 x, y;
+        sf_codes_frags<HELD>(raw[j], x, y);
+        if (values && (flag & kFlagValue)) {
+          x = entries<HELD == SF_KV_INT8>(x, 3);
+          y = entries<HELD == SF_KV_INT8>(y, 3);
+          pin(x);
+          pin(y);
+        }
+        sf_u32x4* to = (values ? vl + 2 * (n - kCodes) : kl + 2 * n) + lane;
+        to[0] = x;
+        to[SF_WAVE] = y;
+      }
+    } else {
+      flag = ld(tail_flags + t % a.c.ring_blocks);
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int n = first_piece(j);
+        if (n >= kPieces && flag) {
+          raw[j] = entries<false>(raw[j], 3);
+          pin(raw[j]);
+        }
+        ((n < kPieces ? kl + n : vl + (n - kPieces)) + lane)[0] = raw[j];
+      }
+    }
+    special |= flag;
+  };
+
+  using R = Rows<D, 32>;
+  R r;
+  r.clear();
+  sf_u32x4 qf[Sh::kSteps];
+  auto scores = [&](const sf_u32x4* kl, Acc(&s)[Sh::kScoreTiles]) {
+#pragma unroll
+    for (int t = 0; t < Sh::kScoreTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
+#pragma unroll
+    for (int st = 0; st < Sh::kSteps; ++st)
+#pragma unroll
+      for (int t = 0; t < Sh::kScoreTiles; ++t)
+        s[t] = Sh::mma(kl[Sh::key_piece16(t, st) + lane], qf[st], s[t]);
+  };
+
+  float most = -INFINITY;  // of the lane's scores of the tile at hand
+  Acc s0[Sh::kScoreTiles], s1[Sh::kScoreTiles];
+  int v_slot = 0;          // of the tile at hand
+  if (begin < end) {
+    load_tile(begin);
+    {
+      const uint16_t* q = a.q + b * a.q_batch + q_head * a.q_head + tok * a.q_tok;
+#pragma unroll
+      for (int s = 0; s < Sh::kSteps; ++s)
+        qf[s] = (sf_ld16(q + Sh::query_d(lane, s)) & a.keep) ^ a.flip;
+    }
+    admit.load(lane, begin * kBlockTokens);
+    stage_tile(begin, k_lds[begin & 1], v_lds[0]);
+    if (begin + 1 < end) load_tile(begin + 1);
+    __syncthreads();
+    scores(k_lds[begin & 1], s0);
+    admit.restrict_scores(s0, lane, begin * kBlockTokens);
+    most = R::top(s0);
+  }
+
+  auto add_values = [&](const sf_u32x4* vl, const sf_u32x4(&w)[Sh::kPSteps]) {
+#pragma unroll
+    for (int k = 0; k < Sh::kPSteps; ++k)
+#pragma unroll
+      for (int t = 0; t < Sh::kOutTiles; ++t)
+        r.acc[t] = Sh::mma(vl[Sh::value_piece16(t, k) + lane], w[k], r.acc[t]);
+  };
+  auto tile_scales = [&](int tile, float& factor, float& scale_v) {
+    factor = a.scale_log2;
+    scale_v = 1.f;
+    if (tile < a.c.folded_blocks) {
+      factor *= ld(k_scale + tile);
+      scale_v = ld(v_scale + tile);
+    }
+  };
+  // Tile `tile`, whose scores are in s and which is not the last; `next` takes
+  // the scores of the one after.
+  auto step = [&](int tile, Acc(&s)[Sh::kScoreTiles], Acc(&next)[Sh::kScoreTiles]) {
+    const sf_u32x4* vl = v_lds[v_slot];
+    v_slot = v_slot == 2 ? 0 : v_slot + 1;
+    float factor, scale_v, mul, base;
+    tile_scales(tile, factor, scale_v);
+    stage_tile(tile + 1, k_lds[(tile + 1) & 1], v_lds[v_slot]);
+    if (tile + 2 < end) load_tile(tile + 2);
+    admit.load(lane, (tile + 1) * kBlockTokens);
+    r.raise(s, most, factor, scale_v, mul, base);
+    __syncthreads();  // tile + 1 is complete
+    // Both blocks are written in the order in which they are to run: an operand's
+    // read kAhead products ahead of its use, a product, and vector work for the
+    // time it takes.
+    constexpr int kAhead = 3;
+    sf_u32x4 w[Sh::kPSteps];
+    {
+      constexpr int kProducts = 2 * Sh::kSteps;
+      const sf_u32x4* kl = k_lds[(tile + 1) & 1] + lane;
+      auto read = [&](int i) { return kl[Sh::key_piece16(i & 1, i >> 1)]; };
+      sf_u32x4 x[kProducts];
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < Sh::kScoreTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) next[t][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = read(i);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        if (i + kAhead < kProducts) x[i + kAhead] = read(i + kAhead);
+        next[i & 1] = Sh::mma(x[i], qf[i >> 1], next[i & 1]);
+#pragma unroll
+        for (int n = i * R::kPairs / kProducts; n < (i + 1) * R::kPairs / kProducts; ++n) {
+          R::weigh_pair(s, n, mul, base, sum, w);
+          uint32_t pair = w[n / 4][n % 4];
+          pin(pair);
+          w[n / 4][n % 4] = pair;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      r.add_sum(sum, scale_v);
+    }
+    admit.restrict_scores(next, lane, (tile + 1) * kBlockTokens);
+    {
+      constexpr int kProducts = Sh::kPSteps * Sh::kOutTiles;
+      auto read = [&](int i) {
+        return vl[Sh::value_piece16(i % Sh::kOutTiles, i / Sh::kOutTiles) + lane];
+      };
+      sf_u32x4 x[kProducts];
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = read(i);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        if (i + kAhead < kProducts) x[i + kAhead] = read(i + kAhead);
+        Acc& o = r.acc[i % Sh::kOutTiles];
+        o = Sh::mma(x[i], w[i / Sh::kOutTiles], o);
+#pragma unroll
+        for (int n = i * R::kPairs / kProducts; n < (i + 1) * R::kPairs / kProducts; ++n)
+          mx[n & 1] = max3(mx[n & 1], next[2 * n / 16][2 * n % 16], next[2 * n / 16][2 * n % 16 + 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      most = max_raw(mx[0], mx[1]);
+    }
+  };
+  int tile = begin;
 #pragma unroll 1
-  for (int t = 0; t < Sh::kScoreTiles; ++t) {
-    Acc has;
+  for (; tile + 2 < end; tile += 2) {
+    step(tile, s0, s1);
+    step(tile + 1, s1, s0);
+  }
+  if (tile + 1 < end) {
+    step(tile, s0, s1);
+    ++tile;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) has[i] = 0.f;
-#pragma unroll 1
-    for (int p = 0; p < Sh::kSteps; ++p) has = Sh::mma(entries<true>(operand(t, p), 2), ones, has);
+    for (int t = 0; t < Sh::kScoreTiles; ++t) s0[t] = s1[t];
+  }
+  if (tile < end) {
+    float factor, scale_v, mul, base;
+    sf_u32x4 w[Sh::kPSteps];
+    tile_scales(tile, factor, scale_v);
+    r.raise(s0, most, factor, scale_v, mul, base);
+    r.weigh(s0, mul, base, scale_v, w);
+    add_values(v_lds[v_slot], w);
+  }
+  if (special)
+    add_special<D, 32, HELD, MASK>(r, a, head, lane, begin, end, 1, admit);
+  r.l = Sh::row_sum(r.l);
+  if (row >= a.rows) return;
+  if (a.splits > 1) {
+    const int64_t at = (static_cast<int64_t>(split) * a.c.heads + head) * a.rows + row;
+    if (Sh::group(lane) == 0) a.part_ml[at] = make_float2(r.m, r.l);
 #pragma unroll
-    for (int u = 0; u < Sh::kScoreTiles; ++u)
+    for (int t = 0; t < Sh::kOutTiles; ++t)
 #pragma unroll
-      for (int i = 0; i < kN; ++i)
-        if (u == t && has[i] > 0.f) s[u][i] = __builtin_nanf("");
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(a.part_acc + at * D + Sh::out_d(lane, t, j)) =
+            make_float4(r.acc[t][4 * j], r.acc[t][4 * j + 1], r.acc[t][4 * j + 2],
+                        r.acc[t][4 * j + 3]);
+  } else {
+    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+    uint16_t* out = a.out + out_row_at(a, head, row) * D;
+#pragma unroll
+    for (int t = 0; t < Sh::kOutTiles; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint2*>(out + Sh::out_d(lane, t, j)) =
+            make_uint2(sf_pack_bf16(r.acc[t][4 * j] * inv, r.acc[t][4 * j + 1] * inv),
+                       sf_pack_bf16(r.acc[t][4 * j + 2] * inv, r.acc[t][4 * j + 3] * inv));
   }
 }
 
-template <int D, int ROWS, int HELD, bool MASK>
-__global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(const Args a) {
+// The form of few rows: 16 rows per workgroup, whose eight wavefronts take every
+// eighth tile and merge their states in LDS.  Operands go straight from the
+// cache into registers, whose order is that of the matrix instructions (no
+// LDS, no barrier).  Decoding long contexts is bound by the cache's bytes
+// (131072 int8 keys of 4 heads of 128: 24 us, 5.6 TB/s), short calls by
+// latency (5 us for one tile per wavefront), trees by the conversions of codes
+// and the softmax (0.23 us per tile and CU).
+template <int D, int HELD, bool MASK>
+__global__ __launch_bounds__(kDirectThreads, 1) void direct_kernel(const Args a) {
+  constexpr int ROWS = kDirectRows;
   using Sh = Shape<D, ROWS>;
   using Acc = typename Sh::Acc;
   constexpr int kN = acc_size<Acc>();
@@ -388,24 +826,18 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
   const int tok = row / a.G;
   const int q_head = h * a.G + (row - tok * a.G);
 
-  sf_u32x4 qf[Sh::kSteps];
-  {
-    const uint16_t* q = a.q + b * a.q_batch + q_head * a.q_head + tok * a.q_tok;
-#pragma unroll
-    for (int s = 0; s < Sh::kSteps; ++s)
-      qf[s] = (sf_ld16(q + Sh::query_d(lane, s)) & a.keep) ^ a.flip;
-  }
-
-  // Tiles [begin, end) of the workgroup; keys below `full` need no look at the
-  // causal rule, the mask or the end.
+  // Tiles [begin, end) of the workgroup.
   const int last_tok = (min(first_row + ROWS, a.rows) - 1) / a.G;
   const int diag = a.S - a.Q + 1;  // keys that token 0 sees
   const int keys_end = MASK ? a.S : min(a.S, diag + last_tok);
   const int begin = split * a.split_tiles;
   const int end = min(begin + a.split_tiles, (keys_end + kBlockTokens - 1) / kBlockTokens);
-  const int full = MASK ? min(a.S, a.mask_begin) : max(0, diag + first_row / a.G);
-  const int lane_end = MASK ? a.S : diag + tok;  // keys of this lane's row (no mask)
-  const uint8_t* mask = MASK ? a.mask + b * a.mask_batch + tok * a.mask_q : nullptr;
+  Admit<Sh, MASK> admit;
+  admit.row = MASK ? a.mask + b * a.mask_batch + tok * a.mask_q : nullptr;
+  admit.mask_begin = a.mask_begin;
+  admit.S = a.S;
+  admit.lane_end = diag + tok;
+  admit.full = MASK ? min(a.S, a.mask_begin) : max(0, diag + first_row / a.G);
 
   const int64_t cap = static_cast<int64_t>(head) * a.c.capacity_blocks;
   const int64_t ring = static_cast<int64_t>(head) * a.c.ring_blocks;
@@ -422,34 +854,17 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
                    16 * Sh::value_lane16(lane);
   const int32_t* tail_flags = a.c.tail_flags + ring;
 
-  Rows<D, ROWS> r;
-  r.clear();
-
-  auto restrict_scores = [&](int tile, Acc(&s)[Sh::kScoreTiles]) {
-    const int key0 = tile * kBlockTokens;
-    if (key0 + kBlockTokens <= full) return;
-#pragma unroll
-    for (int g = 0; g < Sh::kWords; ++g) {
-      const int key = key0 + Sh::key(lane, g);
-      const uint32_t w = MASK ? admitted(mask, key, a.mask_begin, a.S) : 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool ok = MASK ? ((w >> (8 * i)) & 0xffu) != 0 : key + i < lane_end;
-        if (!ok) s[4 * g / kN][4 * g % kN + i] = -INFINITY;
-      }
-    }
-  };
-
-  int tile = begin + wave;
+  int tile = begin + wave, special = 0;
   const int end8 = min(end, a.c.folded_blocks);
-  // Blocks in 8 bits.  The registers of a tile's keys (values) are filled again
-  // as soon as its products are done with them.
-  sf_u32x4 kr[kPieces], vr[kPieces];
-  auto load_keys = [&](int t) {
+  // Blocks in 8 bits.  A tile's keys are loaded while the one before is worked
+  // on; the registers of its values are filled again as soon as the products
+  // are done with them.
+  sf_u32x4 kr[kPieces], kn[kPieces], vr[kPieces];
+  auto load_keys = [&](int t, sf_u32x4(&to)[kPieces]) {
     const char* p = k8 + static_cast<int64_t>(t) * (kBlockTokens * D);
 #pragma unroll
     for (int n = 0; n < kPieces; ++n)
-      kr[n] = sf_ld16(p + 16 * Sh::key_piece(n / kKeyPairs, n % kKeyPairs));
+      to[n] = sf_ld16(p + 16 * Sh::key_piece(n / kKeyPairs, n % kKeyPairs));
   };
   auto load_values = [&](int t) {
     const char* p = v8 + static_cast<int64_t>(t) * (kBlockTokens * D);
@@ -458,14 +873,27 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
       vr[n] = sf_ld16(p + 16 * Sh::value_piece(n / kValuePairs, n % kValuePairs));
   };
   if (tile < end8) {
-    load_keys(tile);
+    load_keys(tile, kn);
     load_values(tile);
   }
+  sf_u32x4 qf[Sh::kSteps];
+  {
+    const uint16_t* q = a.q + b * a.q_batch + q_head * a.q_head + tok * a.q_tok;
+#pragma unroll
+    for (int s = 0; s < Sh::kSteps; ++s)
+      qf[s] = (sf_ld16(q + Sh::query_d(lane, s)) & a.keep) ^ a.flip;
+  }
+  Rows<D, ROWS> r;
+  r.clear();
 #pragma unroll 1
-  for (; tile < end8; tile += kWaves) {
-    const int flag = flags8[tile];
-    const float factor = a.scale_log2 * k_scale[tile];
-    const float scale_v = v_scale[tile];
+  for (; tile < end8; tile += kDirectWaves) {
+    const int flag = ld(flags8 + tile);
+    const float factor = a.scale_log2 * ld(k_scale + tile);
+    const float scale_v = ld(v_scale + tile);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) kr[n] = kn[n];
+    if (tile + kDirectWaves < end8) load_keys(tile + kDirectWaves, kn);
+    admit.load(lane, tile * kBlockTokens);
     Acc s[Sh::kScoreTiles];
 #pragma unroll
     for (int t = 0; t < Sh::kScoreTiles; ++t) {
@@ -480,50 +908,36 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // keep conversions next to their products
-    if (tile + kWaves < end8) load_keys(tile + kWaves);
-    if (HELD == SF_KV_INT8 && (flag & kFlagKey)) {
-      const char* p8 = k8 + static_cast<int64_t>(tile) * (kBlockTokens * D);
-      mark_nan_keys<Sh>(
-          [&](int t, int p) {
-            sf_u32x4 x, y;
-            sf_codes_frags<HELD>(sf_ld16(p8 + 16 * Sh::key_piece(t, p >> 1)), x, y);
-            return p & 1 ? y : x;
-          },
-          s);
-    }
-    restrict_scores(tile, s);
+    admit.restrict_scores(s, lane, tile * kBlockTokens);
     sf_u32x4 w[Sh::kPSteps];
     r.softmax(s, factor, scale_v, w);
     __builtin_amdgcn_sched_barrier(0);
-    if (flag & kFlagValue) {
-      const char* p8 = v8 + static_cast<int64_t>(tile) * (kBlockTokens * D);
-      add_special<Sh, HELD == SF_KV_INT8>(
-          [&](int t, int k) {
-            sf_u32x4 x, y;
-            sf_codes_frags<HELD>(sf_ld16(p8 + 16 * Sh::value_piece(t, k >> 1)), x, y);
-            return k & 1 ? y : x;
-          },
-          w, r.acc);
-    } else {
+    auto add_values = [&](auto finite) {
 #pragma unroll
       for (int t = 0; t < Sh::kOutTiles; ++t)
 #pragma unroll
         for (int p = 0; p < kValuePairs; ++p) {
           sf_u32x4 x, y;
           sf_codes_frags<HELD>(vr[t * kValuePairs + p], x, y);
-          r.acc[t] = Sh::mma(x, w[2 * p], r.acc[t]);
-          r.acc[t] = Sh::mma(y, w[2 * p + 1], r.acc[t]);
+          r.acc[t] = Sh::mma(finite(x), w[2 * p], r.acc[t]);
+          r.acc[t] = Sh::mma(finite(y), w[2 * p + 1], r.acc[t]);
         }
-    }
-    if (tile + kWaves < end8) load_values(tile + kWaves);
+    };
+    if (flag & kFlagValue)
+      add_values([](const sf_u32x4& x) { return entries<HELD == SF_KV_INT8>(x, 3); });
+    else
+      add_values([](const sf_u32x4& x) { return x; });
+    special |= flag;
+    if (tile + kDirectWaves < end8) load_values(tile + kDirectWaves);
   }
   // Blocks of the ring.
 #pragma unroll 1
-  for (; tile < end; tile += kWaves) {
+  for (; tile < end; tile += kDirectWaves) {
     const int slot = tile % a.c.ring_blocks;
     const char* kp = kt + static_cast<int64_t>(slot) * (2 * kBlockTokens * D);
     const char* vp = vt + static_cast<int64_t>(slot) * (2 * kBlockTokens * D);
-    const int flag = tail_flags[slot];
+    const int flag = ld(tail_flags + slot);
+    admit.load(lane, tile * kBlockTokens);
     Acc s[Sh::kScoreTiles];
 #pragma unroll
     for (int t = 0; t < Sh::kScoreTiles; ++t) {
@@ -533,26 +947,36 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
       for (int st = 0; st < Sh::kSteps; ++st)
         s[t] = Sh::mma(sf_ld16(kp + 16 * Sh::key_piece16(t, st)), qf[st], s[t]);
     }
-    restrict_scores(tile, s);
+    // The values too, so that both are on their way together.
+    sf_u32x4 v16[Sh::kOutTiles][Sh::kPSteps];
+#pragma unroll
+    for (int t = 0; t < Sh::kOutTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < Sh::kPSteps; ++k) v16[t][k] = sf_ld16(vp + 16 * Sh::value_piece16(t, k));
+    admit.restrict_scores(s, lane, tile * kBlockTokens);
     sf_u32x4 w[Sh::kPSteps];
     r.softmax(s, a.scale_log2, 1.f, w);
-    if (flag) {
-      add_special<Sh, false>([&](int t, int k) { return sf_ld16(vp + 16 * Sh::value_piece16(t, k)); },
-                             w, r.acc);
-    } else {
+    auto add_values = [&](auto finite) {
 #pragma unroll
       for (int t = 0; t < Sh::kOutTiles; ++t)
 #pragma unroll
         for (int k = 0; k < Sh::kPSteps; ++k)
-          r.acc[t] = Sh::mma(sf_ld16(vp + 16 * Sh::value_piece16(t, k)), w[k], r.acc[t]);
-    }
+          r.acc[t] = Sh::mma(finite(v16[t][k]), w[k], r.acc[t]);
+    };
+    if (flag)
+      add_values([](const sf_u32x4& x) { return entries<false>(x, 3); });
+    else
+      add_values([](const sf_u32x4& x) { return x; });
+    special |= flag;
   }
+  if (special)
+    add_special<D, ROWS, HELD, MASK>(r, a, head, lane, begin + wave, end, kDirectWaves, admit);
   r.l = Sh::row_sum(r.l);
 
   // Merge the wavefronts' states in their order.
   constexpr int kRow = D + 4;
-  __shared__ __attribute__((aligned(16))) float acc_lds[kWaves][ROWS * kRow];
-  __shared__ float2 ml_lds[kWaves][ROWS];
+  __shared__ __attribute__((aligned(16))) float acc_lds[kDirectWaves][ROWS * kRow];
+  __shared__ float2 ml_lds[kDirectWaves][ROWS];
   if (Sh::group(lane) == 0) ml_lds[wave][Sh::row(lane)] = make_float2(r.m, r.l);
 #pragma unroll
   for (int t = 0; t < Sh::kOutTiles; ++t)
@@ -562,18 +986,18 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
           make_float4(r.acc[t][4 * j], r.acc[t][4 * j + 1], r.acc[t][4 * j + 2],
                       r.acc[t][4 * j + 3]);
   __syncthreads();
-  for (int n = threadIdx.x; n < ROWS * D / 4; n += kThreads) {
+  for (int n = threadIdx.x; n < ROWS * D / 4; n += kDirectThreads) {
     const int rr = n / (D / 4);
     const int d = 4 * (n % (D / 4));
     const int out_row = first_row + rr;
     if (out_row >= a.rows) continue;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) M = fmaxf(M, ml_lds[w][rr].x);
+    for (int w = 0; w < kDirectWaves; ++w) M = fmaxf(M, ml_lds[w][rr].x);
     float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
     if (M != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
+      for (int w = 0; w < kDirectWaves; ++w) {
         const float2 ml = ml_lds[w][rr];
         if (ml.x == -INFINITY) continue;
         const float f = __builtin_amdgcn_exp2f(ml.x - M);
@@ -590,9 +1014,7 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
       *reinterpret_cast<float4*>(a.part_acc + at * D + d) = make_float4(o[0], o[1], o[2], o[3]);
       if (d == 0) a.part_ml[at] = make_float2(M, l);
     } else {
-      const int t = out_row / a.G;
-      const int64_t to = (static_cast<int64_t>(b) * a.Q + t) * (static_cast<int64_t>(a.kv_heads) * a.G) +
-                         h * a.G + (out_row - t * a.G);
+      const int64_t to = out_row_at(a, head, out_row);
       const float inv = l == 0.f ? 0.f : 1.f / l;
       *reinterpret_cast<uint2*>(a.out + to * D + d) =
           make_uint2(sf_pack_bf16(o[0] * inv, o[1] * inv), sf_pack_bf16(o[2] * inv, o[3] * inv));
@@ -600,51 +1022,65 @@ __global__ __launch_bounds__(kThreads, ROWS == 16 ? 2 : 1) void direct_kernel(co
   }
 }
 
-// Merges the splits of a row in their order: eight groups of them per row,
-// D / 4 lanes each.
+// Merges the splits of a row.  A thread looks at one split's (maximum, sum);
+// groups of D / 4 lanes then add every kGroups-th accumulator, with their loads
+// issued ahead of the weights, and the groups' sums are added in their order.
+// (One after the other, the 128 splits of 8 rows took 16.9 us.)
+constexpr int kMergeWaves = 4;
+constexpr int kMergeThreads = kMergeWaves * SF_WAVE;
+
 template <int D>
-__global__ __launch_bounds__(kThreads) void merge_kernel(const Args a) {
-  constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Args a) {
+  constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+  constexpr int kLoads = kMaxSplits / kGroups;
+  static_assert(kMaxSplits <= kMergeThreads, "a thread per split");
   __shared__ float4 acc_lds[kGroups][kLanes];
-  __shared__ float2 ml_lds[kGroups];
+  __shared__ float weight[kMaxSplits];
+  __shared__ float top_lds[kMergeWaves], sum_lds[kMergeWaves];
   const int row = blockIdx.x;
   const int head = blockIdx.y;
   const int g = threadIdx.x / kLanes, d = 4 * (threadIdx.x % kLanes);
   const int64_t step = static_cast<int64_t>(a.c.heads) * a.rows;
   const int64_t at = static_cast<int64_t>(head) * a.rows + row;
-  const int per = (a.splits + kGroups - 1) / kGroups;
-  const int s0 = g * per, s1 = min(a.splits, s0 + per);
-  float M = -INFINITY;
-  for (int s = s0; s < s1; ++s) M = fmaxf(M, a.part_ml[s * step + at].x);
-  float l = 0.f;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (threadIdx.x < a.splits) ml = a.part_ml[threadIdx.x * step + at];
+  float4 x[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j)
+    if (j * kGroups < a.splits)
+      x[j] = *reinterpret_cast<const float4*>(
+          a.part_acc + (min(j * kGroups + g, a.splits - 1) * step + at) * D + d);
+  const float wave_top = sf_wave_max(ml.x);
+  if (threadIdx.x % SF_WAVE == 0) top_lds[threadIdx.x / SF_WAVE] = wave_top;
+  __syncthreads();
+  float M = top_lds[0];
+#pragma unroll
+  for (int w = 1; w < kMergeWaves; ++w) M = fmaxf(M, top_lds[w]);
+  const float f = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
+  if (threadIdx.x < kMaxSplits) weight[threadIdx.x] = f;
+  const float wave_sum = sf_wave_sum(ml.y * f);
+  if (threadIdx.x % SF_WAVE == 0) sum_lds[threadIdx.x / SF_WAVE] = wave_sum;
+  __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float2 ml, const float4 x, float top) {
-    if (ml.x == -INFINITY) return;
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    l = __builtin_fmaf(ml.y, f, l);
-    o.x = __builtin_fmaf(x.x, f, o.x);
-    o.y = __builtin_fmaf(x.y, f, o.y);
-    o.z = __builtin_fmaf(x.z, f, o.z);
-    o.w = __builtin_fmaf(x.w, f, o.w);
+  auto add = [&](const float4& y, float w) {
+    o.x = __builtin_fmaf(y.x, w, o.x);
+    o.y = __builtin_fmaf(y.y, w, o.y);
+    o.z = __builtin_fmaf(y.z, w, o.z);
+    o.w = __builtin_fmaf(y.w, w, o.w);
   };
-  for (int s = s0; s < s1; ++s)
-    add(a.part_ml[s * step + at],
-        *reinterpret_cast<const float4*>(a.part_acc + (s * step + at) * D + d), M);
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j)
+    if (j * kGroups < a.splits && j * kGroups + g < a.splits) add(x[j], weight[j * kGroups + g]);
   acc_lds[g][threadIdx.x % kLanes] = o;
-  if (d == 0) ml_lds[g] = make_float2(M, l);
   __syncthreads();
   if (g != 0) return;
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kGroups; ++i) top = fmaxf(top, ml_lds[i].x);
-  l = 0.f;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) add(ml_lds[i], acc_lds[i][threadIdx.x], top);
-  const int b = head / a.kv_heads, h = head - b * a.kv_heads;
-  const int t = row / a.G;
-  const int64_t to = (static_cast<int64_t>(b) * a.Q + t) * (static_cast<int64_t>(a.kv_heads) * a.G) +
-                     h * a.G + (row - t * a.G);
+  for (int i = 0; i < kGroups; ++i) add(acc_lds[i][threadIdx.x], 1.f);
+  float l = sum_lds[0];
+#pragma unroll
+  for (int w = 1; w < kMergeWaves; ++w) l += sum_lds[w];
+  const int64_t to = out_row_at(a, head, row);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(a.out + to * D + d) =
       make_uint2(sf_pack_bf16(o.x * inv, o.y * inv), sf_pack_bf16(o.z * inv, o.w * inv));
@@ -652,51 +1088,74 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(const Args a) {
 
 // How a call's rows and keys are dealt out.
 struct Plan {
-  int rows, tile_rows, row_tiles, splits, split_tiles;
+  bool staged;
+  int rows, row_tiles, splits, split_tiles;
 };
 
+// The form and the splits that are expected to take the shortest, in hundredths
+// of a microsecond, of each form unsplit and split over the chip's 256 CUs (one
+// workgroup each).  Measured at 32 / 4 heads of 128: a direct workgroup takes
+// 5 us and 0.25 us per tile of 64 keys, a staged one 6 us and 2.3 us; merging
+// splits is a second kernel of 4.5 us (more with many rows: it moves their fp32
+// states twice).  So the direct form serves decoding and the trees of short
+// contexts (a 61-node tree after 1024 tokens, 488 rows per KV head: 9.4 us direct
+// and unsplit, 17 staged and split, 25 staged), the staged form prompts and
+// large trees (128 nodes and 16 heads after 32777 tokens: 185 us, 1300 direct).
 Plan plan_of(int heads, int group, int queries, int keys) {
-  Plan p;
-  p.rows = queries * group;
-  p.tile_rows = p.rows <= 16 ? 16 : 32;
-  p.row_tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
+  const int rows = queries * group;
   const int tiles = (keys + kBlockTokens - 1) / kBlockTokens;
-  // Two workgroups for each of the 256 CUs, each with a tile per wavefront.
-  const int64_t base = static_cast<int64_t>(heads) * p.row_tiles;
-  int64_t splits = base >= 512 ? 1 : (512 + base - 1) / base;
-  splits = std::min<int64_t>(splits, (tiles + kWaves - 1) / kWaves);
-  splits = std::min<int64_t>(std::max<int64_t>(splits, 1), kMaxSplits);
-  p.split_tiles = static_cast<int>((tiles + splits - 1) / splits);
-  p.split_tiles = (p.split_tiles + kWaves - 1) / kWaves * kWaves;
-  p.splits = (tiles + p.split_tiles - 1) / p.split_tiles;
-  if (p.splits < 1) p.splits = 1;
-  return p;
+  Plan best = {};
+  double best_cost = 0;
+  for (const bool staged : {false, true}) {
+    const int tile_rows = staged ? kStagedRows : kDirectRows;
+    const int row_tiles = (rows + tile_rows - 1) / tile_rows;
+    const int64_t base = static_cast<int64_t>(heads) * row_tiles;
+    for (const bool split : {false, true}) {
+      int splits = 1, split_tiles = tiles;
+      if (split) {
+        splits = static_cast<int>(std::min<int64_t>(kMaxSplits, 256 / base));
+        if (splits < 2) continue;
+        split_tiles = (tiles + splits - 1) / splits;
+        // The direct form's wavefronts take a tile each at a time.
+        if (!staged) split_tiles = (split_tiles + kDirectWaves - 1) / kDirectWaves * kDirectWaves;
+        splits = (tiles + split_tiles - 1) / split_tiles;
+        if (splits < 2) continue;
+      }
+      const double rounds = static_cast<double>((base * splits + 255) / 256);
+      double cost = rounds * (staged ? 600 + 230. * split_tiles : 500 + 25. * split_tiles);
+      if (splits > 1) cost += 450 + 0.002 * heads * static_cast<double>(rows) * splits;
+      if (best.rows == 0 || cost < best_cost) {
+        best = {staged, rows, row_tiles, splits, split_tiles};
+        best_cost = cost;
+      }
+    }
+  }
+  return best;
 }
 
-template <int D, int ROWS, int HELD>
-void launch(const Args& a, hipStream_t s) {
+template <int D, int HELD>
+void launch_held(const Args& a, bool staged, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(a.c.heads) * a.row_tiles * a.splits);
-  if (a.mask)
-    direct_kernel<D, ROWS, HELD, true><<<grid, kThreads, 0, s>>>(a);
-  else
-    direct_kernel<D, ROWS, HELD, false><<<grid, kThreads, 0, s>>>(a);
+  if (staged) {
+    if (a.mask)
+      staged_kernel<D, HELD, true><<<grid, kStagedThreads, 0, s>>>(a);
+    else
+      staged_kernel<D, HELD, false><<<grid, kStagedThreads, 0, s>>>(a);
+  } else {
+    if (a.mask)
+      direct_kernel<D, HELD, true><<<grid, kDirectThreads, 0, s>>>(a);
+    else
+      direct_kernel<D, HELD, false><<<grid, kDirectThreads, 0, s>>>(a);
+  }
 }
 
 template <int D>
-void launch(const Args& a, int tile_rows, hipStream_t s) {
-  const bool int8 = a.c.held == SF_KV_INT8;
-  if (tile_rows == 16) {
-    if (int8)
-      launch<D, 16, SF_KV_INT8>(a, s);
-    else
-      launch<D, 16, SF_KV_E4M3>(a, s);
-  } else {
-    if (int8)
-      launch<D, 32, SF_KV_INT8>(a, s);
-    else
-      launch<D, 32, SF_KV_E4M3>(a, s);
-  }
-  if (a.splits > 1) merge_kernel<D><<<dim3(a.rows, a.c.heads), kThreads, 0, s>>>(a);
+void launch(const Args& a, bool staged, hipStream_t s) {
+  if (a.c.held == SF_KV_INT8)
+    launch_held<D, SF_KV_INT8>(a, staged, s);
+  else
+    launch_held<D, SF_KV_E4M3>(a, staged, s);
+  if (a.splits > 1) merge_kernel<D><<<dim3(a.rows, a.c.heads), kMergeThreads, 0, s>>>(a);
 }
 
 // Keys, and rows over all heads, of a call, so that every index of tiles, rows
@@ -778,9 +1237,9 @@ extern "C" int sf_block_attention(const sf_kv_cache* cache, int batch, int kv_he
       a.part_acc + static_cast<int64_t>(p.splits) * cache->heads * p.rows * cache->head_dim);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (cache->head_dim == 128)
-    launch<128>(a, p.tile_rows, s);
+    launch<128>(a, p.staged, s);
   else
-    launch<64>(a, p.tile_rows, s);
+    launch<64>(a, p.staged, s);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }

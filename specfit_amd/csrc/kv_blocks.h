@@ -33,6 +33,11 @@ __device__ __forceinline__ sf_u32x4 sf_ld16(const void* p) {
   return *(const __attribute__((address_space(1))) sf_u32x4*)(p);
 }
 
+// The same at a uniform address plus a lane's offset in bytes.
+__device__ __forceinline__ sf_u32x4 sf_ld16(const char* p, uint32_t offset) {
+  return *(const __attribute__((address_space(1))) sf_u32x4*)(p + offset);
+}
+
 __device__ __forceinline__ uint32_t sf_pack_bf16(float lo, float hi) {
   const sf_bf16x2 v = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
   return __builtin_bit_cast(uint32_t, v);

@@ -94,7 +94,7 @@ def test_attention_calls_refused_on_the_host():
     assert work(0, 1, 4096, 32, 4, 128) == 0 and work(1, 4096, 4096, 32, 4, 128) == 0
     assert work(1, 1, (1 << 30) + 1, 32, 4, 128) == 0
     for batch, queries, keys, q_heads, kv_heads, dim in (
-            (1, 1, 4097, 32, 4, 128), (1, 61, 1085, 32, 4, 128), (3, 1, 1 << 30, 8, 8, 64),
+            (1, 1, 4097, 32, 4, 128), (1, 128, 32905, 64, 4, 128), (3, 1, 1 << 30, 8, 8, 64),
             (2, 5, 9000, 14, 2, 64)):
         each = batch * queries * q_heads * (dim + 2) * 4
         splits, rest = divmod(work(batch, queries, keys, q_heads, kv_heads, dim), each)

@@ -424,9 +424,9 @@ def test_layouts_of_queries_and_masks(device, kind):
 def test_calls_without_room_for_scratch(device, monkeypatch):
     """With no workspace the keys are not split."""
     g = torch.Generator().manual_seed(8)
-    cache, k, v = _filled(device, g, 1, 2, 64, 900, 1, "int8")
+    cache, k, v = _filled(device, g, 1, 2, 64, 9000, 1, "int8")
     q = _rand(g, 1, 4, 1, 64)
-    assert ops._block_attention_workspace(1, 1, 901, 4, 2, 64) > 0
+    assert ops._block_attention_workspace(1, 1, 9001, 4, 2, 64) > 0
     monkeypatch.setattr(ops, "_block_attention_workspace", lambda *a: 0)
     _check_attention(cache, q, k, v, None, 0.125, "int8")
 
