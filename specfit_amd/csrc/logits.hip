@@ -1,12 +1,12 @@
 // K11: repetition penalties, a bias and an allowed set on rows of logits, and
 // each row's greedy token.
 //
-// A thread keeps the counts (and a shared bias) of its eight vocabulary entries
-// in registers for several rows, so a row costs its logits and one word of its
-// allowed set; the tokens of a row's own path are found by the wavefront that
-// holds their entries.  Bound by the bytes of the logits.  The greedy token is a
-// maximum of (value, lowest index) over partial results of the wavefronts, so
-// no order of arrival changes it.
+// A thread has eight vocabulary entries of a row; the tokens of the row's own path
+// are found by the wavefront that holds their entries.  The greedy token is a
+// maximum of (value, lowest index) over partial results of the wavefronts, so no
+// order of arrival changes it.  Bound by the bytes of the logits, and with
+// penalties by their vector work (a quotient costs three instructions, see
+// `divided`).
 #include <algorithm>
 
 #include "sf_common.h"
@@ -17,7 +17,6 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / SF_WAVE;
 constexpr int kPer = 8;                     // entries of a thread
 constexpr int kChunk = kThreads * kPer;     // of a workgroup
-constexpr int kMaxRows = 8;                 // of a workgroup
 constexpr int kNone = INT32_MIN;            // key of a value that is never chosen
 
 struct RuleArgs {
@@ -27,7 +26,7 @@ struct RuleArgs {
   const int32_t* counts;
   const int32_t* paths;
   int path_length;
-  float repetition, presence, frequency;
+  float repetition, inverse, presence, frequency;  // inverse: of the repetition, or 0
   const float* bias;
   int64_t bias_stride;
   const int32_t* allowed;
@@ -35,7 +34,7 @@ struct RuleArgs {
   void* out;
   int64_t out_stride;
   int2* parts;  // [rows][chunks * kWaves] (key, index), or nullptr
-  int chunks, group;
+  int chunks;
 };
 
 template <int DTYPE>
@@ -71,6 +70,17 @@ __device__ __forceinline__ int order_key(float y) {
   return u >= 0 ? u : u ^ 0x7fffffff;
 }
 
+// x / repetition, correctly rounded.  With the correctly rounded inverse y of b,
+// q = x y is within an ulp or so of x / b, its remainder r = x - q b is exact in a
+// fused multiply-add, and q + r y rounds to the quotient (Markstein, 1990), as long as
+// nothing overflows or loses bits below the normal range: |x| between the two
+// limits, for a repetition that has an inverse here.
+__device__ __forceinline__ float divided(float x, float b, float y) {
+  const float q = x * y;
+  return __builtin_fmaf(__builtin_fmaf(-q, b, x), y, q);
+}
+constexpr float kLeastPlain = 0x1p-90f, kMostPlain = 0x1p100f;
+
 // Entry e of thread tid: VEC neighbours, then the next kThreads * VEC.
 template <int VEC>
 __device__ __forceinline__ int entry(int tid, int e) {
@@ -97,6 +107,10 @@ __device__ __forceinline__ void load_entries(const E* p, int n, E (&x)[kPer]) {
   }
 }
 
+// A workgroup has a chunk of one row.  Two or four rows to a workgroup read the
+// counts once for them, but their registers leave half of the wavefronts: 61 rows of
+// 151936 bf16 logits take 9.4 us with one, 12.5 with two, 15.4 with four (5.9
+// without any rule).
 template <int DTYPE, int VEC, bool PENALTY, bool OUT, bool TOKENS>
 __global__ __launch_bounds__(kThreads) void rules_kernel(const RuleArgs a) {
   using Ty = Type<DTYPE>;
@@ -105,104 +119,119 @@ __global__ __launch_bounds__(kThreads) void rules_kernel(const RuleArgs a) {
   const int wave = threadIdx.x / SF_WAVE;
   const int c0 = blockIdx.x * kChunk;
   const int n = min(kChunk, a.vocab - c0);  // entries of the chunk
-  const int r0 = blockIdx.y * a.group;
-  const int r1 = min(r0 + a.group, a.rows);
+  const int r = blockIdx.y;
 
-  int32_t seen[kPer] = {};
-  if (PENALTY && a.counts) load_entries<VEC>(a.counts + c0, n, seen);
-  float bias[kPer] = {};
-  if (a.bias && a.bias_stride == 0) load_entries<VEC>(a.bias + c0, n, bias);
-
-  for (int r = r0; r < r1; ++r) {
-    Elem raw[kPer];
-    load_entries<VEC>(static_cast<const Elem*>(a.logits) + r * a.stride + c0, n, raw);
-    if (a.bias && a.bias_stride) load_entries<VEC>(a.bias + r * a.bias_stride + c0, n, bias);
-    uint32_t ok = 0;
+  // Everything the row needs is on its way together.
+  Elem raw[kPer];
+  load_entries<VEC>(static_cast<const Elem*>(a.logits) + r * a.stride + c0, n, raw);
+  int32_t count[kPer] = {};
+  if (PENALTY && a.counts) load_entries<VEC>(a.counts + c0, n, count);
+  const int32_t* path = a.paths + static_cast<int64_t>(r) * a.path_length;
+  int own = -1;
+  if (PENALTY && a.paths && lane < a.path_length) own = path[lane];
+  uint32_t good = 0;  // entries that are there and allowed
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) good |= (entry<VEC>(threadIdx.x, e) < n ? 1u : 0u) << e;
+  if (a.allowed) {
+    const int32_t* words = a.allowed + r * a.allowed_stride;
+    uint32_t bits = 0;
 #pragma unroll
     for (int e = 0; e < kPer; e += VEC) {
-      const int at = entry<VEC>(threadIdx.x, e);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) ok |= (at + j < n ? 1u : 0u) << (e + j);
+      // VEC neighbours share a word: chunks and VEC divide or are multiples of 32.
+      const int v = c0 + min(entry<VEC>(threadIdx.x, e), n - 1);
+      bits |= ((static_cast<uint32_t>(words[v / 32]) >> (v % 32)) & ((1u << VEC) - 1u)) << e;
     }
-    if (a.allowed) {
-      const int32_t* words = a.allowed + r * a.allowed_stride;
-      uint32_t bits = 0;
+    good &= bits;
+  }
+
+  float y[kPer];
 #pragma unroll
-      for (int e = 0; e < kPer; e += VEC) {
-        // VEC neighbours share a word: chunks and VEC divide or are multiples of 32.
-        const int v = c0 + min(entry<VEC>(threadIdx.x, e), n - 1);
-        bits |= ((static_cast<uint32_t>(words[v / 32]) >> (v % 32)) & ((1u << VEC) - 1u)) << e;
-      }
-      ok &= bits;
-    }
-    int32_t count[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) count[e] = seen[e];
-    if (PENALTY && a.paths) {
-      const int32_t* path = a.paths + static_cast<int64_t>(r) * a.path_length;
+  for (int e = 0; e < kPer; ++e) y[e] = Ty::load(raw[e]);
+  if (PENALTY) {
+    // The row's own tokens: few chunks have any.
+    if (a.paths)
       for (int p0 = 0; p0 < a.path_length; p0 += SF_WAVE) {
-        const int token = p0 + lane < a.path_length ? path[p0 + lane] : -1;
-        uint64_t here = __ballot(token >= c0 && token < c0 + n);
+        if (p0) own = p0 + lane < a.path_length ? path[p0 + lane] : -1;
+        uint64_t here = __ballot(own >= c0 && own < c0 + n);
         while (here) {  // uniform
           const int at =
-              __builtin_amdgcn_readlane(token, static_cast<int>(__builtin_ctzll(here))) - c0;
+              __builtin_amdgcn_readlane(own, static_cast<int>(__builtin_ctzll(here))) - c0;
           here &= here - 1;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) count[e] += entry<VEC>(threadIdx.x, e) == at;
         }
       }
+    float least = fabsf(y[0]), most = fabsf(y[0]);
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) {
+      least = fminf(least, fabsf(y[e]));
+      most = fmaxf(most, fabsf(y[e]));
     }
-    int best = kNone, index = 0;
-    Elem out[kPer];
+    // (A NaN is in neither: its quotient is NaN both ways.)
+    const bool quick = a.inverse != 0.f && !__any(!(least >= kLeastPlain && most <= kMostPlain));
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      float y = Ty::load(raw[e]);
-      if (PENALTY) {
-        if (__any(count[e] > 0)) {
-          const float x = y < 0.f ? y * a.repetition : y / a.repetition;
-          const float less = a.frequency * static_cast<float>(count[e]);
-          const float z = x - (less + a.presence);
-          if (count[e] > 0) y = z;
-        }
-      }
-      if (a.bias) y += bias[e];
-      if (!((ok >> e) & 1u)) y = -INFINITY;
-      if (OUT) out[e] = Ty::store(y);
-      if (TOKENS) {
-        const int key = order_key(y);
-        if (key > best) {  // entries ascend with e
-          best = key;
-          index = entry<VEC>(threadIdx.x, e);
-        }
+      if (!__any(count[e] > 0)) continue;
+      float x = quick ? divided(y[e], a.repetition, a.inverse) : y[e] / a.repetition;
+      if (y[e] < 0.f) x = y[e] * a.repetition;
+      x -= a.frequency * static_cast<float>(count[e]) + a.presence;
+      if (count[e] > 0) y[e] = x;
+    }
+  }
+  if (a.bias) {
+    float bias[kPer];
+    load_entries<VEC>(a.bias + r * a.bias_stride + c0, n, bias);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) y[e] += bias[e];
+  }
+  Elem out[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(good << (31 - e)) >> 31);
+    y[e] = __uint_as_float((keep & __float_as_uint(y[e])) | (~keep & 0xff800000u));
+    if (OUT) out[e] = Ty::store(y[e]);
+  }
+  if (OUT) {
+    struct __attribute__((aligned(VEC * sizeof(Elem) > 16 ? 16 : VEC * sizeof(Elem)))) Piece {
+      Elem e[VEC];
+    };
+    Elem* to = static_cast<Elem*>(a.out) + r * a.out_stride + c0;
+#pragma unroll
+    for (int e = 0; e < kPer; e += VEC) {
+      const int at = entry<VEC>(threadIdx.x, e);
+      if (at + VEC <= n) {
+        Piece p;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) p.e[j] = out[e + j];
+        *reinterpret_cast<Piece*>(to + at) = p;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at + j < n) to[at + j] = out[e + j];
       }
     }
-    if (OUT) {
-      struct __attribute__((aligned(VEC * sizeof(Elem) > 16 ? 16 : VEC * sizeof(Elem)))) Piece {
-        Elem e[VEC];
-      };
-      Elem* to = static_cast<Elem*>(a.out) + r * a.out_stride + c0;
+  }
+  if (TOKENS) {
+    float most = y[0];  // NaN where one of them is
 #pragma unroll
-      for (int e = 0; e < kPer; e += VEC) {
-        const int at = entry<VEC>(threadIdx.x, e);
-        if (at + VEC <= n) {
-          Piece p;
+    for (int e = 1; e < kPer; ++e) most = __builtin_elementwise_maximum(most, y[e]);
+    const int key = order_key(most);
+    const int top = sf_wave_max_int(key);
+    // The first entry of that value (entries ascend with e).
+    int index = INT32_MAX;
+    if (top == INT32_MAX) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) p.e[j] = out[e + j];
-          *reinterpret_cast<Piece*>(to + at) = p;
-        } else {
+      for (int e = kPer - 1; e >= 0; --e)
+        if (y[e] != y[e]) index = entry<VEC>(threadIdx.x, e);
+    } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (at + j < n) to[at + j] = out[e + j];
-        }
-      }
+      for (int e = kPer - 1; e >= 0; --e)
+        if (y[e] == most) index = entry<VEC>(threadIdx.x, e);
     }
-    if (TOKENS) {
-      const int top = sf_wave_max_int(best);
-      const int low = -sf_wave_max_int(best == top ? -index : INT32_MIN + 1);
-      if (lane == 0)
-        a.parts[(static_cast<int64_t>(r) * a.chunks + blockIdx.x) * kWaves + wave] =
-            make_int2(top, c0 + low);
-    }
+    const int low = -sf_wave_max_int(key == top ? -index : INT32_MIN + 1);
+    if (lane == 0)
+      a.parts[(static_cast<int64_t>(r) * a.chunks + blockIdx.x) * kWaves + wave] =
+          make_int2(top, c0 + low);
   }
 }
 
@@ -233,8 +262,9 @@ __global__ __launch_bounds__(kThreads) void token_kernel(const int2* parts, int 
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 template <int DTYPE, int VEC>
-void launch(const RuleArgs& a, bool penalty, dim3 grid, hipStream_t s) {
+void launch(const RuleArgs& a, bool penalty, hipStream_t s) {
   const bool out = a.out != nullptr, tokens = a.parts != nullptr;
+  const dim3 grid(a.chunks, a.rows);
 #define SF_RULES(P, O, T) rules_kernel<DTYPE, VEC, P, O, T><<<grid, kThreads, 0, s>>>(a)
   if (penalty) {
     if (out && tokens) SF_RULES(true, true, true);
@@ -265,16 +295,20 @@ extern "C" int sf_logit_rules(int dtype, const void* logits, int64_t logits_stri
   if ((dtype != SF_BF16 && dtype != SF_F16 && dtype != SF_F32) || rows < 0 || vocab < 0 ||
       path_length < 0 || !(repetition > 0.f))
     return SF_ERR_INVALID_ARGUMENT;
-  if (vocab > (1 << 30) || rows > (1 << 18)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (vocab > (1 << 30) || rows > 65535) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0 || (!out && !tokens)) return SF_OK;
   if (vocab == 0 || !logits) return SF_ERR_INVALID_ARGUMENT;
   if (tokens && (!workspace || workspace_bytes < sf_logit_rules_workspace(rows, vocab)))
     return SF_ERR_INVALID_ARGUMENT;
   if (tokens && reinterpret_cast<uintptr_t>(workspace) % sizeof(int2)) return SF_ERR_MISALIGNED;
   RuleArgs a = {logits, logits_stride, rows, vocab, counts, path_length ? paths : nullptr,
-                path_length, repetition, presence, frequency, bias, bias_stride, allowed,
+                path_length, repetition,
+                repetition >= 0x1p-20f && repetition <= 0x1p20f
+                    ? static_cast<float>(1.0 / static_cast<double>(repetition))
+                    : 0.f,
+                presence, frequency, bias, bias_stride, allowed,
                 allowed_stride, out, out_stride,
-                tokens ? static_cast<int2*>(workspace) : nullptr, chunks_of(vocab), 1};
+                tokens ? static_cast<int2*>(workspace) : nullptr, chunks_of(vocab)};
   const bool penalty = (counts || a.paths) &&
                        (repetition != 1.f || presence != 0.f || frequency != 0.f);
   const int size = dtype == SF_F32 ? 4 : 2;
@@ -285,18 +319,13 @@ extern "C" int sf_logit_rules(int dtype, const void* logits, int64_t logits_stri
   if (counts) wide = wide && reinterpret_cast<uintptr_t>(counts) % 16 == 0;
   if (bias)
     wide = wide && reinterpret_cast<uintptr_t>(bias) % 16 == 0 && bias_stride % 4 == 0;
-  // Rows of a workgroup: enough workgroups for the 256 CUs first.
-  const int64_t work = static_cast<int64_t>(rows) * a.chunks;
-  a.group = static_cast<int>(std::min<int64_t>(kMaxRows, std::max<int64_t>(1, work / 1024)));
-  const dim3 grid(a.chunks, (rows + a.group - 1) / a.group);
-  if (grid.y > 65535) return SF_ERR_UNSUPPORTED_SHAPE;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == SF_BF16) {
-    wide ? launch<SF_BF16, 8>(a, penalty, grid, s) : launch<SF_BF16, 1>(a, penalty, grid, s);
+    wide ? launch<SF_BF16, 8>(a, penalty, s) : launch<SF_BF16, 1>(a, penalty, s);
   } else if (dtype == SF_F16) {
-    wide ? launch<SF_F16, 8>(a, penalty, grid, s) : launch<SF_F16, 1>(a, penalty, grid, s);
+    wide ? launch<SF_F16, 8>(a, penalty, s) : launch<SF_F16, 1>(a, penalty, s);
   } else {
-    wide ? launch<SF_F32, 4>(a, penalty, grid, s) : launch<SF_F32, 1>(a, penalty, grid, s);
+    wide ? launch<SF_F32, 4>(a, penalty, s) : launch<SF_F32, 1>(a, penalty, s);
   }
   SF_LAUNCH_CHECK();
   if (tokens) {

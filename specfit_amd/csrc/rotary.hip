@@ -78,62 +78,71 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
   __syncthreads();
 
   // A unit of work: two pieces of VEC pairs apart (half layout), one piece of
-  // VEC / 2 pairs (interleaved; VEC 1: a pair), or a piece that is copied.
+  // VEC / 2 pairs (interleaved; VEC 1: a pair), or a piece that is copied.  A
+  // thread keeps its unit (and the unit's sines in registers) over the heads, and
+  // has kAtOnce of them on their way: dividing out token, head and unit for each
+  // piece instead, 8002 tokens of 36 fp32 heads of 128 took 84 us.
   constexpr int kStep = INTERLEAVED ? (VEC > 1 ? VEC : 2) : VEC;
+  constexpr int kPieces = INTERLEAVED ? kStep / VEC : 2;  // of a unit
+  constexpr int kSines = INTERLEAVED ? kStep / 2 : VEC;
+  constexpr int kAtOnce = 4;
   const int turned = (INTERLEAVED ? a.R : half) / kStep;
   const int units = turned + (a.D - a.R) / VEC;
-  const int heads = a.heads[0] + a.heads[1];
-  for (int n = blockIdx.y * kThreads + threadIdx.x; n < count * heads * units;
-       n += gridDim.y * kThreads) {
-    const int u = n % units;
-    int h = (n / units) % heads;
-    const int i = n / units / heads;
-    const int64_t token = first + i;
-    const int64_t b = token / a.T, t = token - b * a.T;
-    const int w = h >= a.heads[0];
-    if (w) h -= a.heads[0];
-    const Elem* x = static_cast<const Elem*>(a.x[w]) + b * a.batch[w] + t * a.tok[w] + h * a.head[w];
-    Elem* y = static_cast<Elem*>(a.out[w]) + ((b * a.heads[w] + h) * a.T + t) * a.D;
-    const float2* cs = turn + i * half;
-    if (u >= turned) {
-      const int d = a.R + (u - turned) * VEC;
-      *reinterpret_cast<Piece*>(y + d) = *reinterpret_cast<const Piece*>(x + d);
-    } else if (!INTERLEAVED) {
-      const int d = u * VEC;
-      const Piece p = *reinterpret_cast<const Piece*>(x + d);
-      const Piece q = *reinterpret_cast<const Piece*>(x + d + half);
-      Piece r, s;
+  const int width = min(units, kThreads);
+  const int rows = kThreads / width;  // heads side by side
+  if (static_cast<int>(threadIdx.x) >= rows * width) return;
+  const int first_head = blockIdx.y * rows + threadIdx.x / width;
+  const int head_step = gridDim.y * rows;
+  for (int u = threadIdx.x % width; u < units; u += width) {
+    const bool copied = u >= turned;
+    // First element of each of the unit's pieces.
+    const int d0 = copied ? a.R + (u - turned) * VEC : u * kStep;
+    const int d1 = INTERLEAVED ? d0 + VEC : d0 + half;
+    const int pieces = copied ? 1 : kPieces;
+    for (int i = 0; i < count; ++i) {
+      const int64_t token = first + i;
+      const int64_t b = token / a.T, t = token - b * a.T;
+      float2 f[kSines] = {};
+      if (!copied) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float2 f = cs[d + e];
-        const float u0 = Ty::load(p.e[e]), u1 = Ty::load(q.e[e]);
-        r.e[e] = Ty::store(__builtin_fmaf(u0, f.x, -(u1 * f.y)));
-        s.e[e] = Ty::store(__builtin_fmaf(u1, f.x, u0 * f.y));
-      }
-      *reinterpret_cast<Piece*>(y + d) = r;
-      *reinterpret_cast<Piece*>(y + d + half) = s;
-    } else {
-      const int d = u * kStep;
-      Elem in[kStep], out[kStep];
-#pragma unroll
-      for (int e = 0; e < kStep; e += VEC) {
-        const Piece p = *reinterpret_cast<const Piece*>(x + d + e);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) in[e + j] = p.e[j];
+        for (int e = 0; e < kSines; ++e)
+          f[e] = turn[i * half + (INTERLEAVED ? d0 / 2 : d0) + e];
       }
 #pragma unroll
-      for (int e = 0; e < kStep; e += 2) {
-        const float2 f = cs[(d + e) / 2];
-        const float u0 = Ty::load(in[e]), u1 = Ty::load(in[e + 1]);
-        out[e] = Ty::store(__builtin_fmaf(u0, f.x, -(u1 * f.y)));
-        out[e + 1] = Ty::store(__builtin_fmaf(u1, f.x, u0 * f.y));
-      }
+      for (int w = 0; w < 2; ++w) {
+        const Elem* x = static_cast<const Elem*>(a.x[w]) + b * a.batch[w] + t * a.tok[w];
+        Elem* y = static_cast<Elem*>(a.out[w]) + (b * a.heads[w] * a.T + t) * a.D;
+        const int64_t out_head = static_cast<int64_t>(a.T) * a.D;
+        for (int h0 = first_head; h0 < a.heads[w]; h0 += kAtOnce * head_step) {
+          Piece p[kAtOnce][2];
 #pragma unroll
-      for (int e = 0; e < kStep; e += VEC) {
-        Piece p;
+          for (int j = 0; j < kAtOnce; ++j) {
+            const int h = h0 + j * head_step;
+            if (h < a.heads[w]) {
+              p[j][0] = *reinterpret_cast<const Piece*>(x + h * a.head[w] + d0);
+              if (pieces > 1) p[j][1] = *reinterpret_cast<const Piece*>(x + h * a.head[w] + d1);
+            }
+          }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) p.e[j] = out[e + j];
-        *reinterpret_cast<Piece*>(y + d + e) = p;
+          for (int j = 0; j < kAtOnce; ++j) {
+            const int h = h0 + j * head_step;
+            if (h >= a.heads[w]) continue;
+            if (!copied) {
+#pragma unroll
+              for (int e = 0; e < kSines; ++e) {
+                // The pair's two elements.
+                Elem& u0 = INTERLEAVED && VEC > 1 ? p[j][0].e[(2 * e) % VEC] : p[j][0].e[e % VEC];
+                Elem& u1 =
+                    INTERLEAVED && VEC > 1 ? p[j][0].e[(2 * e + 1) % VEC] : p[j][1].e[e % VEC];
+                const float v0 = Ty::load(u0), v1 = Ty::load(u1);
+                u0 = Ty::store(__builtin_fmaf(v0, f[e].x, -(v1 * f[e].y)));
+                u1 = Ty::store(__builtin_fmaf(v1, f[e].x, v0 * f[e].y));
+              }
+            }
+            *reinterpret_cast<Piece*>(y + h * out_head + d0) = p[j][0];
+            if (pieces > 1) *reinterpret_cast<Piece*>(y + h * out_head + d1) = p[j][1];
+          }
+        }
       }
     }
   }
@@ -180,11 +189,13 @@ extern "C" int sf_rotary(int dtype, const void* q, int64_t q_stride_batch, int64
       wide = wide && reinterpret_cast<uintptr_t>(a.x[w]) % 16 == 0 &&
              reinterpret_cast<uintptr_t>(a.out[w]) % 16 == 0 && a.batch[w] % vec == 0 &&
              a.tok[w] % vec == 0 && a.head[w] % vec == 0;
-  const int units = wide ? (head_dim - rotary_dim / (interleaved ? 1 : 2)) / vec : head_dim;
-  const int per_token = (q_heads + k_heads) * units;
+  const int step = wide ? vec : 1;
+  const int units = rotary_dim / (interleaved && wide ? vec : 2 * step) +
+                    (head_dim - rotary_dim) / step;
   a.tokens = static_cast<int>(std::min<int64_t>(kMaxTokens, std::max<int64_t>(1, all / 2048)));
-  // A lone token's heads are dealt over workgroups.
-  const int shares = a.tokens > 1 ? 1 : std::min(16, std::max(1, per_token / (4 * kThreads)));
+  // A workgroup of one token takes the heads that stand side by side in it.
+  const int rows = kThreads / std::min(units, kThreads);
+  const int shares = a.tokens > 1 ? 1 : std::min(16, (std::max(q_heads, k_heads) + rows - 1) / rows);
   const dim3 grid(static_cast<uint32_t>((all + a.tokens - 1) / a.tokens), shares);
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool il = interleaved != 0;
