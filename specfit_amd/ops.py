@@ -842,23 +842,20 @@ KV_HELD = {"e4m3": 0, "int8": 1}    # how complete blocks are held
 _KV_MAX_MOVES = 256                 # positions of one sf_kv_compact call
 
 
-class _on_device:
-    """Makes ``device`` current for a launch on it."""
+_get_device = torch._C._cuda_getDevice
 
-    __slots__ = ("_index", "_previous")
 
-    def __init__(self, device: torch.device) -> None:
-        self._index = device.index
-
-    def __enter__(self) -> None:
-        current = torch._C._cuda_getDevice()
-        self._previous = None if self._index in (None, current) else current
-        if self._previous is not None:
-            torch.cuda.set_device(self._index)
-
-    def __exit__(self, *exc) -> None:
-        if self._previous is not None:
-            torch.cuda.set_device(self._previous)
+def _launch(function, device_index: int, *args) -> int:
+    """Calls a library function with its device current (streams given by
+    handle 0 are the current device's)."""
+    previous = _get_device()
+    if previous == device_index:
+        return function(*args)
+    torch.cuda.set_device(device_index)
+    try:
+        return function(*args)
+    finally:
+        torch.cuda.set_device(previous)
 
 
 def _scratch(nbytes: int, device: torch.device, stream: torch.cuda.Stream | None) -> torch.Tensor:
@@ -898,7 +895,7 @@ class KVBlocks:
             device = torch.device("cuda", torch.cuda.current_device())
         self.layers, self.batch, self.kv_heads, self.head_dim = layers, batch, kv_heads, head_dim
         self.capacity_blocks, self.ring_blocks = capacity_blocks, ring_blocks
-        self.held, self.device = held, device
+        self.held, self.device, self.index = held, device, device.index
         heads, width = batch * kv_heads, KV_BLOCK * head_dim
         shape, ring = (layers, heads, capacity_blocks), (layers, heads, ring_blocks)
         self.keys = torch.empty((*shape, width), dtype=torch.uint8, device=device)
@@ -941,12 +938,16 @@ class KVBlocks:
             raise IndexError(f"layer {layer} of a block cache of {self.layers} layers")
         return self._refs[layer]
 
-    def _check_rows(self, name: str, t: torch.Tensor) -> None:
+    def _refuse_rows(self, name: str, t: torch.Tensor) -> None:
+        """Raises what is wrong with rows of keys, values or queries."""
         _require_cuda(name, t, _BF16)
-        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[3] != self.head_dim:
-            raise ValueError(f"{name} must be [{self.batch}, heads, tokens, {self.head_dim}]")
         if t.device != self.device:
             raise ValueError(f"{name} must be on the cache's device")
+        raise ValueError(f"{name} must be [{self.batch}, heads, tokens, {self.head_dim}]")
+
+    def _rows_fit(self, t: torch.Tensor) -> bool:
+        return (isinstance(t, torch.Tensor) and t.dtype is _BF16 and t.get_device() == self.index
+                and t.dim() == 4 and t.shape[0] == self.batch and t.shape[3] == self.head_dim)
 
 
 def kv_append(blocks: KVBlocks, layer: int, key: torch.Tensor, value: torch.Tensor, start: int, *,
@@ -955,21 +956,26 @@ def kv_append(blocks: KVBlocks, layer: int, key: torch.Tensor, value: torch.Tens
     with a unit last one) as tokens start .. start + T - 1 of ``layer``."""
     ref = blocks._check_layer(layer)
     for name, t in (("key", key), ("value", value)):
-        blocks._check_rows(name, t)
-        if t.shape[1] != blocks.kv_heads:
-            raise ValueError(f"{name} must have {blocks.kv_heads} heads")
-    if key.shape != value.shape:
+        if not blocks._rows_fit(t):
+            blocks._refuse_rows(name, t)
+    shape = key.shape
+    if shape != value.shape:
         raise ValueError("key and value differ in shape")
-    if key.stride(3) != 1:
+    if shape[1] != blocks.kv_heads:
+        raise ValueError(f"key and value must have {blocks.kv_heads} heads")
+    kb, kh, kt, kd = key.stride()
+    if kd != 1:
         key = key.contiguous()
-    if value.stride(3) != 1:
+        kb, kh, kt, _ = key.stride()
+    vb, vh, vt, vd = value.stride()
+    if vd != 1:
         value = value.contiguous()
-    (kb, kh, kt, _), (vb, vh, vt, _) = key.stride(), value.stride()
-    with _on_device(blocks.device):
-        rc = _native.lib().sf_kv_append(ref, blocks.kv_heads, key.data_ptr(), kb, kh, kt,
-                                        value.data_ptr(), vb, vh, vt, int(start), key.shape[2],
-                                        _stream_handle(stream, blocks.device))
-    _native.check(rc, "sf_kv_append")
+        vb, vh, vt, _ = value.stride()
+    rc = _launch(_native.lib().sf_kv_append, blocks.index, ref, blocks.kv_heads, key.data_ptr(), kb,
+                 kh, kt, value.data_ptr(), vb, vh, vt, start, shape[2],
+                 _stream_handle(stream, blocks.device))
+    if rc:
+        _native.check(rc, "sf_kv_append")
 
 
 def kv_compact(blocks: KVBlocks, base: int, positions: Sequence[int], end: int, *,
@@ -978,28 +984,27 @@ def kv_compact(blocks: KVBlocks, base: int, positions: Sequence[int], end: int, 
     layer; ``positions`` ascend strictly and ``end`` is the number of tokens
     the layers hold."""
     positions = [int(p) for p in positions]
-    if any(p < 0 or base + p >= end for p in positions) or \
-            any(b <= a for a, b in zip(positions, positions[1:])):
+    last, first = -1, 0
+    for i, p in enumerate(positions):
+        if p <= last:
+            raise ValueError("positions must ascend strictly and name tokens of the cache")
+        first += p == i  # rows that stay where they are: the first ones, as p >= i
+        last = p
+    if base + last >= end:
         raise ValueError("positions must ascend strictly and name tokens of the cache")
-    first = 0
-    while first < len(positions) and positions[first] == first:
-        first += 1  # these rows stay where they are
-    with _on_device(blocks.device):
-        for at in range(first, len(positions), _KV_MAX_MOVES):
-            part = positions[at:at + _KV_MAX_MOVES]
-            rc = _native.lib().sf_kv_compact(
-                blocks._whole_ref, int(base), at,
-                ctypes.cast((ctypes.c_int32 * len(part))(*part), ctypes.c_void_p), len(part),
-                int(end), _stream_handle(stream, blocks.device))
-            _native.check(rc, "sf_kv_compact")
+    for at in range(first, len(positions), _KV_MAX_MOVES):
+        part = positions[at:at + _KV_MAX_MOVES]
+        rc = _launch(_native.lib().sf_kv_compact, blocks.index, blocks._whole_ref, int(base), at,
+                     (ctypes.c_int32 * len(part))(*part), len(part), int(end),
+                     _stream_handle(stream, blocks.device))
+        _native.check(rc, "sf_kv_compact")
 
 
 def kv_fold(blocks: KVBlocks, count: int, *, stream: torch.cuda.Stream | None = None) -> None:
     """Folds the next ``count`` blocks of every layer, complete in the ring,
     into 8 bits; later calls read them from there."""
-    with _on_device(blocks.device):
-        rc = _native.lib().sf_kv_fold(blocks._whole_ref, int(count),
-                                      _stream_handle(stream, blocks.device))
+    rc = _launch(_native.lib().sf_kv_fold, blocks.index, blocks._whole_ref, int(count),
+                 _stream_handle(stream, blocks.device))
     _native.check(rc, "sf_kv_fold")
     blocks.folded += int(count)
 
@@ -1015,9 +1020,8 @@ def kv_read(blocks: KVBlocks, layer: int, start: int, stop: int, *,
     keys = torch.empty(shape, dtype=_BF16, device=blocks.device)
     values = torch.empty(shape, dtype=_BF16, device=blocks.device)
     if stop > start:
-        with _on_device(blocks.device):
-            rc = _native.lib().sf_kv_read(ref, int(start), stop - start, keys.data_ptr(),
-                                          values.data_ptr(), _stream_handle(stream, blocks.device))
+        rc = _launch(_native.lib().sf_kv_read, blocks.index, ref, int(start), stop - start,
+                     keys.data_ptr(), values.data_ptr(), _stream_handle(stream, blocks.device))
         _native.check(rc, "sf_kv_read")
     return keys, values
 
@@ -1044,23 +1048,25 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
     (memory of the current stream) are the caller's to order between the two
     streams."""
     ref = blocks._check_layer(layer)
-    blocks._check_rows("query", query)
+    if not blocks._rows_fit(query):
+        blocks._refuse_rows("query", query)
     B, Hq, Q, D = query.shape
-    if Hq < 1 or Hq % blocks.kv_heads:
+    kv_heads, device = blocks.kv_heads, blocks.device
+    if Hq < 1 or Hq % kv_heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if keys < 0:
         raise ValueError("keys must not be negative")
-    device = blocks.device
     mask_ptr, mask_batch, mask_q, mask_keys = None, 0, 0, 0
     if mask is not None:
-        if mask.dtype != torch.bool:
+        if mask.dtype is not torch.bool:
             raise TypeError("block attention takes a bool mask (True = attend)")
-        if mask.device != device or mask.dim() != 4 or mask.shape[0] not in (1, B) \
+        if mask.get_device() != blocks.index or mask.dim() != 4 or mask.shape[0] not in (1, B) \
                 or mask.shape[1] != 1 or mask.shape[2] != Q or mask.shape[3] > keys:
             raise ValueError(f"mask must be bool [1 or {B}, 1, {Q}, up to {keys} keys]")
-        if mask.stride(3) != 1:
+        mask_batch, _, mask_q, mask_step = mask.stride()
+        if mask_step != 1:
             mask = mask.contiguous()
-        mask_batch, _, mask_q, _ = mask.stride()
+            mask_batch, _, mask_q, _ = mask.stride()
         if mask.shape[0] == 1:
             mask_batch = 0
         mask_keys = mask.shape[3]
@@ -1073,10 +1079,12 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
         # A mask of no keys admits them all: any address but null.
         mask_ptr = mask.data_ptr() if mask_keys else out.data_ptr()
     qb, qh, qt, qd = query.stride()
-    if qd != 1 or (qb | qh | qt) % 8 or query.data_ptr() % 16:
+    q_ptr = query.data_ptr()
+    if qd != 1 or (qb | qh | qt) % 8 or q_ptr % 16:
         query = query.clone(memory_format=torch.contiguous_format)
         qb, qh, qt, _ = query.stride()
-    need = _block_attention_workspace(B, Q, keys, Hq, blocks.kv_heads, D)
+        q_ptr = query.data_ptr()
+    need = _block_attention_workspace(B, Q, keys, Hq, kv_heads, D)
     work_ptr = None
     if need:
         try:
@@ -1084,12 +1092,11 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
             work_ptr = work.data_ptr()
         except torch.OutOfMemoryError:
             need = 0  # the keys are not split then
-    with _on_device(device):
-        rc = _native.lib().sf_block_attention(
-            ref, B, blocks.kv_heads, keys, query.data_ptr(), qb, qh, qt, Q, Hq, mask_ptr,
-            mask_batch, mask_q, mask_keys, float(scale), out.data_ptr(), work_ptr, need,
-            _stream_handle(stream, device))
-    _native.check(rc, "sf_block_attention")
+    rc = _launch(_native.lib().sf_block_attention, blocks.index, ref, B, kv_heads, keys, q_ptr, qb,
+                 qh, qt, Q, Hq, mask_ptr, mask_batch, mask_q, mask_keys, scale, out.data_ptr(),
+                 work_ptr, need, _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_block_attention")
     return out
 
 
@@ -1106,40 +1113,45 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     ``table`` a ``specfit_amd.rotary.RotaryTable`` on the same device.  Returns
     (q, k) as [B, H, T, D] contiguous.  Angles are taken in fp64, so far
     positions keep them; each output is rounded once."""
-    if q.dtype not in _DTYPES:
+    dtype = q.dtype
+    if dtype not in _DTYPES:
         raise ValueError("q must be bf16, fp16 or fp32")
     _require_cuda("q", q)
-    _require_cuda("k", k, q.dtype)
+    _require_cuda("k", k, dtype)
     _require_cuda("positions", positions, torch.int64)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+    if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q and k must be [batch, tokens, heads, head_dim] of the same tokens")
     B, T, Hq, D = q.shape
-    Hk = k.shape[2]
+    Bk, Tk, Hk, Dk = k.shape
+    if Bk != B or Tk != T or Dk != D:
+        raise ValueError("q and k must be [batch, tokens, heads, head_dim] of the same tokens")
     if D != table.head_dim:
         raise ValueError(f"the table is for head dim {table.head_dim}, not {D}")
-    turns = table.turns
-    if k.device != q.device or positions.device != q.device or turns.device != q.device:
+    turns, index, device = table.turns, q.get_device(), q.device
+    if k.get_device() != index or positions.get_device() != index or turns.get_device() != index:
         raise ValueError("q, k, positions and the table must share a device")
-    if positions.dim() == 1:
-        positions = positions[None]
-    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] not in (1, B):
+    shape = positions.shape
+    if len(shape) not in (1, 2) or shape[-1] != T or (len(shape) == 2 and shape[0] not in (1, B)):
         raise ValueError(f"positions must be [{B} or 1, {T}]")
-    if positions.stride(1) != 1:
+    if positions.stride(-1) != 1:
         positions = positions.contiguous()
-    step = positions.stride(0) if positions.shape[0] == B and B > 1 else 0
-    if q.stride(3) != 1:
+    step = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
+    qb, qt, qh, qd = q.stride()
+    if qd != 1:
         q = q.contiguous()
-    if k.stride(3) != 1:
+        qb, qt, qh, _ = q.stride()
+    kb, kt, kh, kd = k.stride()
+    if kd != 1:
         k = k.contiguous()
-    q_out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=q.device)
-    k_out = torch.empty((B, Hk, T, D), dtype=q.dtype, device=q.device)
-    (qb, qt, qh, _), (kb, kt, kh, _) = q.stride(), k.stride()
-    with _on_device(q.device):
-        rc = _native.lib().sf_rotary(
-            _DTYPES[q.dtype], q.data_ptr(), qb, qt, qh, Hq, k.data_ptr(), kb, kt, kh, Hk,
-            positions.data_ptr(), step, turns.data_ptr(), table.factor, B, T, D, table.rotary_dim,
-            table.interleaved, q_out.data_ptr(), k_out.data_ptr(), _stream_handle(stream, q.device))
-    _native.check(rc, "sf_rotary")
+        kb, kt, kh, _ = k.stride()
+    q_out = torch.empty((B, Hq, T, D), dtype=dtype, device=device)
+    k_out = torch.empty((B, Hk, T, D), dtype=dtype, device=device)
+    rc = _launch(_native.lib().sf_rotary, index, _DTYPES[dtype], q.data_ptr(), qb, qt, qh, Hq,
+                 k.data_ptr(), kb, kt, kh, Hk, positions.data_ptr(), step, turns.data_ptr(),
+                 table.factor, B, T, D, table.rotary_dim, table.interleaved, q_out.data_ptr(),
+                 k_out.data_ptr(), _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_rotary")
     return q_out, k_out
 
 
@@ -1151,7 +1163,8 @@ def _logit_rules_workspace(rows: int, vocab: int) -> int:
 
 def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, out,
                  want_tokens, stream):
-    if logits.dtype not in _DTYPES:
+    dtype = logits.dtype
+    if dtype not in _DTYPES:
         raise ValueError("logits must be bf16, fp16 or fp32")
     _require_cuda("logits", logits)
     if logits.dim() != 2:
@@ -1159,45 +1172,47 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
     N, V = logits.shape
     if V == 0:
         raise ValueError("logits must have a vocabulary")
-    if logits.stride(1) != 1:
+    logits_stride, unit = logits.stride()
+    if unit != 1:
         logits = logits.contiguous()
-    device = logits.device
+        logits_stride = logits.stride(0)
+    device, index = logits.device, logits.get_device()
     if not repetition > 0:
         raise ValueError("the repetition penalty must be positive")
     counts_ptr = paths_ptr = bias_ptr = allowed_ptr = None
     length = bias_stride = allowed_stride = 0
     if counts is not None:
         _require_cuda("counts", counts, torch.int32)
-        if counts.shape != (V,) or counts.device != device or not counts.is_contiguous():
+        if counts.dim() != 1 or counts.shape[0] != V or counts.get_device() != index \
+                or not counts.is_contiguous():
             raise ValueError(f"counts must be contiguous int32 [{V}]")
         counts_ptr = counts.data_ptr()
     if paths is not None:
         _require_cuda("paths", paths, torch.int32)
-        if paths.dim() != 2 or paths.shape[0] != N or paths.device != device:
+        if paths.dim() != 2 or paths.shape[0] != N or paths.get_device() != index:
             raise ValueError(f"paths must be int32 [{N}, length]")
-        paths = paths.contiguous()
+        if not paths.is_contiguous():
+            paths = paths.contiguous()
         length, paths_ptr = paths.shape[1], paths.data_ptr()
     if bias is not None:
         _require_cuda("bias", bias, torch.float32)
-        if bias.device != device or bias.shape not in ((V,), (1, V), (N, V)):
+        if bias.get_device() != index or bias.shape not in ((V,), (1, V), (N, V)):
             raise ValueError(f"bias must be fp32 [{V}] or [{N}, {V}]")
         if bias.stride(-1) != 1:
             bias = bias.contiguous()
         bias_stride = bias.stride(0) if bias.dim() == 2 and bias.shape[0] > 1 else 0
-        if bias.dim() == 2 and bias.shape[0] > 1 and bias_stride == 0:
-            bias = bias[0]  # one row expanded
         bias_ptr = bias.data_ptr()
     if allowed is not None:
         words = (V + 31) // 32
         _require_cuda("allowed", allowed, torch.int32)
-        if allowed.device != device or allowed.shape not in ((words,), (1, words), (N, words)):
+        if allowed.get_device() != index or allowed.shape not in ((words,), (1, words), (N, words)):
             raise ValueError(f"allowed must be int32 [{words}] or [{N}, {words}]")
         if allowed.stride(-1) != 1:
             allowed = allowed.contiguous()
         allowed_stride = allowed.stride(0) if allowed.dim() == 2 and allowed.shape[0] > 1 else 0
         allowed_ptr = allowed.data_ptr()
-    tokens = work = None
-    need = 0
+    tokens = tokens_ptr = work_ptr = out_ptr = None
+    need = out_stride = 0
     if want_tokens:
         tokens = torch.empty(N, dtype=torch.int64, device=device)
     if N == 0:
@@ -1205,14 +1220,15 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
     if want_tokens:
         need = _logit_rules_workspace(N, V)
         work = _scratch(need, device, stream)
-    out_ptr, out_stride = (None, 0) if out is None else (out.data_ptr(), out.stride(0))
-    with _on_device(device):
-        rc = _native.lib().sf_logit_rules(
-            _DTYPES[logits.dtype], logits.data_ptr(), logits.stride(0), N, V, counts_ptr, paths_ptr,
-            length, float(repetition), float(presence), float(frequency), bias_ptr, bias_stride,
-            allowed_ptr, allowed_stride, out_ptr, out_stride, _ptr(tokens), _ptr(work), need,
-            _stream_handle(stream, device))
-    _native.check(rc, "sf_logit_rules")
+        tokens_ptr, work_ptr = tokens.data_ptr(), work.data_ptr()
+    if out is not None:
+        out_ptr, out_stride = out.data_ptr(), out.stride(0)
+    rc = _launch(_native.lib().sf_logit_rules, index, _DTYPES[dtype], logits.data_ptr(),
+                 logits_stride, N, V, counts_ptr, paths_ptr, length, repetition, presence,
+                 frequency, bias_ptr, bias_stride, allowed_ptr, allowed_stride, out_ptr, out_stride,
+                 tokens_ptr, work_ptr, need, _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_logit_rules")
     return tokens
 
 
@@ -1233,7 +1249,7 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
     [N, V / 32 up]) is 0 becomes -inf.  Each step is rounded to fp32, the result
     once more to the logits' type.  ``out`` may be ``logits``."""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
             or out.dim() != 2 or out.stride(1) != 1:
         raise ValueError("out must be like logits, with a unit last stride")

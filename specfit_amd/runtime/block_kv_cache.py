@@ -123,7 +123,11 @@ class BlockKVCache:
         """fp32 [2, batch, kv_heads, folded blocks]: the scales of keys (0)
         and values (1)."""
         b = self.blocks
-        return b.scales[:, layer, :, :b.folded].unflatten(1, (b.batch, b.kv_heads))
+        if not 0 <= layer < b.layers:
+            raise IndexError(f"layer {layer} of a block cache of {b.layers} layers")
+        kind, per_layer, head, _ = b.scales.stride()
+        return b.scales.as_strided((2, b.batch, b.kv_heads, b.folded),
+                                   (kind, head * b.kv_heads, head, 1), layer * per_layer)
 
     def _length(self) -> int:
         if len(set(self._lengths)) != 1:
