@@ -1022,13 +1022,72 @@ __global__ __launch_bounds__(kDirectThreads, 1) void direct_kernel(const Args a)
   }
 }
 
-// Merges the splits of a row.  A thread looks at one split's (maximum, sum);
-// groups of D / 4 lanes then add every kGroups-th accumulator, with their loads
-// issued ahead of the weights, and the groups' sums are added in their order.
-// (One after the other, the 128 splits of 8 rows took 16.9 us.)
+// Elements d .. d + 3 of a row, divided by its sum.
+template <int D>
+__device__ __forceinline__ void store_merged(const Args& a, int head, int row, int d, const float4& o,
+                                             float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(a.out + out_row_at(a, head, row) * D + d) =
+      make_uint2(sf_pack_bf16(o.x * inv, o.y * inv), sf_pack_bf16(o.z * inv, o.w * inv));
+}
+
+__device__ __forceinline__ void add_scaled(float4& o, const float4& x, float f) {
+  o.x = __builtin_fmaf(x.x, f, o.x);
+  o.y = __builtin_fmaf(x.y, f, o.y);
+  o.z = __builtin_fmaf(x.z, f, o.z);
+  o.w = __builtin_fmaf(x.w, f, o.w);
+}
+
 constexpr int kMergeWaves = 4;
 constexpr int kMergeThreads = kMergeWaves * SF_WAVE;
+constexpr int kFewSplits = 16;
+constexpr int kManyRows = 512;
 
+// Merges few splits of many rows: D / 4 lanes per row, which go over its splits in
+// their order with the values of four on their way.  Bound by the partial states'
+// bytes: 8192 rows of 8 splits of 128 take 8.5 us (4 TB / s), 13.2 with a workgroup
+// per row; 32 rows of 8 splits take 3.4, and 2.7 with a workgroup per row.
+template <int D>
+__global__ __launch_bounds__(kMergeThreads) void merge_few_kernel(const Args a) {
+  constexpr int kLanes = D / 4, kRows = kMergeThreads / kLanes;
+  const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
+  const int head = blockIdx.y;
+  const int d = 4 * (threadIdx.x % kLanes);
+  if (row >= a.rows) return;
+  const int64_t step = static_cast<int64_t>(a.c.heads) * a.rows;
+  const int64_t at = static_cast<int64_t>(head) * a.rows + row;
+  float2 ml[kFewSplits];
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) ml[s] = a.part_ml[min(s, a.splits - 1) * step + at];
+  float M = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) M = fmaxf(M, ml[s].x);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int s0 = 0; s0 < kFewSplits; s0 += 4) {
+    if (s0 >= a.splits) break;
+    float4 x[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      x[s] = *reinterpret_cast<const float4*>(a.part_acc +
+                                              (min(s0 + s, a.splits - 1) * step + at) * D + d);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (s0 + s >= a.splits || ml[s0 + s].x == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(ml[s0 + s].x - M);
+      l = __builtin_fmaf(ml[s0 + s].y, f, l);
+      add_scaled(o, x[s], f);
+    }
+  }
+  store_merged<D>(a, head, row, d, o, l);
+}
+
+// Merges the splits of a row, if they are many or the rows few.  A thread looks at
+// one split's (maximum, sum); groups of D / 4 lanes then add every kGroups-th
+// accumulator, with their loads issued ahead of the weights, and the groups' sums
+// are added in their order.
+// (One after the other, the 128 splits of 8 rows took 16.9 us.)
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Args a) {
   constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
@@ -1062,28 +1121,19 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Args a) {
   if (threadIdx.x % SF_WAVE == 0) sum_lds[threadIdx.x / SF_WAVE] = wave_sum;
   __syncthreads();
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](const float4& y, float w) {
-    o.x = __builtin_fmaf(y.x, w, o.x);
-    o.y = __builtin_fmaf(y.y, w, o.y);
-    o.z = __builtin_fmaf(y.z, w, o.z);
-    o.w = __builtin_fmaf(y.w, w, o.w);
-  };
 #pragma unroll
   for (int j = 0; j < kLoads; ++j)
-    if (j * kGroups < a.splits && j * kGroups + g < a.splits) add(x[j], weight[j * kGroups + g]);
+    if (j * kGroups < a.splits && j * kGroups + g < a.splits) add_scaled(o, x[j], weight[j * kGroups + g]);
   acc_lds[g][threadIdx.x % kLanes] = o;
   __syncthreads();
   if (g != 0) return;
   o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < kGroups; ++i) add(acc_lds[i][threadIdx.x], 1.f);
+  for (int i = 0; i < kGroups; ++i) add_scaled(o, acc_lds[i][threadIdx.x], 1.f);
   float l = sum_lds[0];
 #pragma unroll
   for (int w = 1; w < kMergeWaves; ++w) l += sum_lds[w];
-  const int64_t to = out_row_at(a, head, row);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(a.out + to * D + d) =
-      make_uint2(sf_pack_bf16(o.x * inv, o.y * inv), sf_pack_bf16(o.z * inv, o.w * inv));
+  store_merged<D>(a, head, row, d, o, l);
 }
 
 // How a call's rows and keys are dealt out.
@@ -1092,38 +1142,43 @@ struct Plan {
   int rows, row_tiles, splits, split_tiles;
 };
 
-// The form and the splits that are expected to take the shortest, in hundredths
-// of a microsecond, of each form unsplit and split over the chip's 256 CUs (one
-// workgroup each).  Measured at 32 / 4 heads of 128: a direct workgroup takes
-// 5 us and 0.25 us per tile of 64 keys, a staged one 6 us and 2.3 us; merging
-// splits is a second kernel of 4.5 us (more with many rows: it moves their fp32
-// states twice).  So the direct form serves decoding and the trees of short
-// contexts (a 61-node tree after 1024 tokens, 488 rows per KV head: 9.4 us direct
-// and unsplit, 17 staged and split, 25 staged), the staged form prompts and
-// large trees (128 nodes and 16 heads after 32777 tokens: 185 us, 1300 direct).
-Plan plan_of(int heads, int group, int queries, int keys) {
+// The form and the splits that are expected to take the shortest, in us, with a
+// workgroup per CU at a time.  Fitted to kernel times on MI355X (head dim 128; 64):
+//   direct  3 + rounds (2 + 0.33 tiles)      (1 + 0.125 tiles)
+//   staged  rounds (8 + 2.45 tiles)          (8 + 1.6 tiles)
+//   splits  the partial states (fp32) at 4.5 MB / us, written and read, and 3 for
+//           the second kernel
+// e.g. at 32 / 4 heads of 128, direct / staged: a 61-node tree after 1024 tokens 9.4 /
+// 20 us (split), 160 nodes after 8000 92 / 52 (split), a prompt of 512 tokens 20 / 26,
+// 1024 46 / 45, 2048 128 / 86; 2000 tokens after 4000 at 16 / 4 heads of 64 85 / 114.
+// tiles: of the longest row tile where there is one round, on average where there
+// are more (as under the causal rule).
+Plan plan_of(int heads, int group, int queries, int keys, int head_dim) {
   const int rows = queries * group;
   const int tiles = (keys + kBlockTokens - 1) / kBlockTokens;
+  const double average = std::max(1., (keys - std::min(queries, keys) / 2) / double(kBlockTokens));
+  const bool wide = head_dim == 128;
   Plan best = {};
   double best_cost = 0;
   for (const bool staged : {false, true}) {
     const int tile_rows = staged ? kStagedRows : kDirectRows;
     const int row_tiles = (rows + tile_rows - 1) / tile_rows;
     const int64_t base = static_cast<int64_t>(heads) * row_tiles;
-    for (const bool split : {false, true}) {
-      int splits = 1, split_tiles = tiles;
-      if (split) {
-        splits = static_cast<int>(std::min<int64_t>(kMaxSplits, 256 / base));
-        if (splits < 2) continue;
-        split_tiles = (tiles + splits - 1) / splits;
-        // The direct form's wavefronts take a tile each at a time.
-        if (!staged) split_tiles = (split_tiles + kDirectWaves - 1) / kDirectWaves * kDirectWaves;
-        splits = (tiles + split_tiles - 1) / split_tiles;
-        if (splits < 2) continue;
-      }
+    int last = 0;
+    for (const int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128}) {
+      if (want > 1 && (base * want > 256 || want > tiles)) break;
+      int split_tiles = (tiles + want - 1) / want;
+      // The direct form's wavefronts take a tile each at a time.
+      if (want > 1 && !staged) split_tiles = (split_tiles + kDirectWaves - 1) / kDirectWaves * kDirectWaves;
+      const int splits = (tiles + split_tiles - 1) / split_tiles;
+      if (splits == last) continue;
+      last = splits;
       const double rounds = static_cast<double>((base * splits + 255) / 256);
-      double cost = rounds * (staged ? 600 + 230. * split_tiles : 500 + 25. * split_tiles);
-      if (splits > 1) cost += 450 + 0.002 * heads * static_cast<double>(rows) * splits;
+      const double each = rounds > 1 ? std::min<double>(average, split_tiles) : split_tiles;
+      double cost = staged ? rounds * (8 + (wide ? 2.45 : 1.6) * each)
+                           : 3 + rounds * (wide ? 2 + 0.33 * each : 1 + 0.125 * each);
+      if (splits > 1)
+        cost += 3 + 2 * 4. * (head_dim + 2) * heads * static_cast<double>(rows) * splits / 4.5e6;
       if (best.rows == 0 || cost < best_cost) {
         best = {staged, rows, row_tiles, splits, split_tiles};
         best_cost = cost;
@@ -1155,7 +1210,12 @@ void launch(const Args& a, bool staged, hipStream_t s) {
     launch_held<D, SF_KV_INT8>(a, staged, s);
   else
     launch_held<D, SF_KV_E4M3>(a, staged, s);
-  if (a.splits > 1) merge_kernel<D><<<dim3(a.rows, a.c.heads), kMergeThreads, 0, s>>>(a);
+  constexpr int kRows = kMergeThreads / (D / 4);
+  if (a.splits > kFewSplits || (a.splits > 1 && a.rows * int64_t{a.c.heads} < kManyRows))
+    merge_kernel<D><<<dim3(a.rows, a.c.heads), kMergeThreads, 0, s>>>(a);
+  else if (a.splits > 1)
+    merge_few_kernel<D>
+        <<<dim3((a.rows + kRows - 1) / kRows, a.c.heads), kMergeThreads, 0, s>>>(a);
 }
 
 // Keys, and rows over all heads, of a call, so that every index of tiles, rows
@@ -1177,7 +1237,7 @@ extern "C" int64_t sf_block_attention_workspace(int batch, int queries, int keys
     return 0;
   const int64_t heads = static_cast<int64_t>(batch) * kv_heads;
   if (!fits(heads, q_heads / kv_heads, queries, keys)) return 0;
-  const Plan p = plan_of(static_cast<int>(heads), q_heads / kv_heads, queries, keys);
+  const Plan p = plan_of(static_cast<int>(heads), q_heads / kv_heads, queries, keys, head_dim);
   if (p.splits == 1) return 0;
   return static_cast<int64_t>(p.splits) * heads * p.rows * (head_dim + 2) * 4;
 }
@@ -1202,7 +1262,7 @@ extern "C" int sf_block_attention(const sf_kv_cache* cache, int batch, int kv_he
   if (reinterpret_cast<uintptr_t>(q) % 16 || q_stride_batch % 8 || q_stride_head % 8 ||
       q_stride_token % 8 || reinterpret_cast<uintptr_t>(out) % 16)
     return SF_ERR_MISALIGNED;
-  Plan p = plan_of(cache->heads, group, queries, keys);
+  Plan p = plan_of(cache->heads, group, queries, keys, cache->head_dim);
   const int64_t need = sf_block_attention_workspace(batch, queries, keys, q_heads, kv_heads,
                                                     cache->head_dim);
   if (p.splits > 1 && (!workspace || workspace_bytes < need)) {
