@@ -13,8 +13,8 @@
 // units, is a reference only: every weight of a row has the same one.
 //
 // Two forms, and a kernel that merges splits of the keys: few rows per KV head go
-// straight from the cache to registers (direct_kernel), many share tiles in LDS
-// (staged_kernel); plan_of chooses.
+// straight from the cache to registers (block_attention_direct_kernel), many share tiles in LDS
+// (block_attention_staged_kernel); plan_of chooses.
 #include <algorithm>
 
 #include "kv_blocks.h"
@@ -529,7 +529,7 @@ __device__ __forceinline__ void add_special(Rows<D, ROWS>& r, const Args& a, int
 // writes before the barrier of iteration i, others last read before that of
 // i - 1).
 template <int D, int HELD, bool MASK>
-__global__ __launch_bounds__(kStagedThreads, 1) void staged_kernel(const Args a) {
+__global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kernel(const Args a) {
   using Sh = Shape<D, 32>;
   using Acc = typename Sh::Acc;
   constexpr int kPieces = kBlockTokens * D / 8;             // of a tile's keys or values, bf16
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(kStagedThreads, 1) void staged_kernel(const Args a)
 // latency (5 us for one tile per wavefront), trees by the conversions of codes
 // and the softmax (0.23 us per tile and CU).
 template <int D, int HELD, bool MASK>
-__global__ __launch_bounds__(kDirectThreads, 1) void direct_kernel(const Args a) {
+__global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kernel(const Args a) {
   constexpr int ROWS = kDirectRows;
   using Sh = Shape<D, ROWS>;
   using Acc = typename Sh::Acc;
@@ -1048,7 +1048,7 @@ constexpr int kManyRows = 512;
 // bytes: 8192 rows of 8 splits of 128 take 8.5 us (4 TB / s), 13.2 with a workgroup
 // per row; 32 rows of 8 splits take 3.4, and 2.7 with a workgroup per row.
 template <int D>
-__global__ __launch_bounds__(kMergeThreads) void merge_few_kernel(const Args a) {
+__global__ __launch_bounds__(kMergeThreads) void block_attention_merge_few_kernel(const Args a) {
   constexpr int kLanes = D / 4, kRows = kMergeThreads / kLanes;
   const int row = blockIdx.x * kRows + threadIdx.x / kLanes;
   const int head = blockIdx.y;
@@ -1089,7 +1089,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_few_kernel(const Args a) 
 // are added in their order.
 // (One after the other, the 128 splits of 8 rows took 16.9 us.)
 template <int D>
-__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const Args a) {
+__global__ __launch_bounds__(kMergeThreads) void block_attention_merge_kernel(const Args a) {
   constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
   constexpr int kLoads = kMaxSplits / kGroups;
   static_assert(kMaxSplits <= kMergeThreads, "a thread per split");
@@ -1193,14 +1193,14 @@ void launch_held(const Args& a, bool staged, hipStream_t s) {
   const dim3 grid(static_cast<uint32_t>(a.c.heads) * a.row_tiles * a.splits);
   if (staged) {
     if (a.mask)
-      staged_kernel<D, HELD, true><<<grid, kStagedThreads, 0, s>>>(a);
+      block_attention_staged_kernel<D, HELD, true><<<grid, kStagedThreads, 0, s>>>(a);
     else
-      staged_kernel<D, HELD, false><<<grid, kStagedThreads, 0, s>>>(a);
+      block_attention_staged_kernel<D, HELD, false><<<grid, kStagedThreads, 0, s>>>(a);
   } else {
     if (a.mask)
-      direct_kernel<D, HELD, true><<<grid, kDirectThreads, 0, s>>>(a);
+      block_attention_direct_kernel<D, HELD, true><<<grid, kDirectThreads, 0, s>>>(a);
     else
-      direct_kernel<D, HELD, false><<<grid, kDirectThreads, 0, s>>>(a);
+      block_attention_direct_kernel<D, HELD, false><<<grid, kDirectThreads, 0, s>>>(a);
   }
 }
 
@@ -1212,9 +1212,9 @@ void launch(const Args& a, bool staged, hipStream_t s) {
     launch_held<D, SF_KV_E4M3>(a, staged, s);
   constexpr int kRows = kMergeThreads / (D / 4);
   if (a.splits > kFewSplits || (a.splits > 1 && a.rows * int64_t{a.c.heads} < kManyRows))
-    merge_kernel<D><<<dim3(a.rows, a.c.heads), kMergeThreads, 0, s>>>(a);
+    block_attention_merge_kernel<D><<<dim3(a.rows, a.c.heads), kMergeThreads, 0, s>>>(a);
   else if (a.splits > 1)
-    merge_few_kernel<D>
+    block_attention_merge_few_kernel<D>
         <<<dim3((a.rows + kRows - 1) / kRows, a.c.heads), kMergeThreads, 0, s>>>(a);
 }
 
@@ -1249,7 +1249,8 @@ extern "C" int sf_block_attention(const sf_kv_cache* cache, int batch, int kv_he
                                   int64_t mask_stride_query, int mask_keys, float scale, void* out,
                                   void* workspace, int64_t workspace_bytes, sf_stream_t stream) {
   if (const int rc = sf_kv_check(cache)) return rc;
-  if (batch < 1 || kv_heads < 1 || batch > cache->heads || batch * kv_heads != cache->heads ||
+  if (batch < 1 || kv_heads < 1 || batch > cache->heads ||
+      static_cast<int64_t>(batch) * kv_heads != cache->heads ||
       queries < 1 || keys < 1 || !q || !out)
     return SF_ERR_INVALID_ARGUMENT;
   if (q_heads < 1 || q_heads % kv_heads) return SF_ERR_UNSUPPORTED_SHAPE;

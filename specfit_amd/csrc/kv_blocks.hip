@@ -380,9 +380,15 @@ int sf_kv_check(const sf_kv_cache* c) {
 
 namespace {
 
+// A start or base above it is refused before it meets a sum.
+int64_t token_capacity(const sf_kv_cache* c) {
+  return static_cast<int64_t>(c->capacity_blocks) * kBlockTokens;
+}
+
 // Tokens [start, end) lie in the capacity, and what is not folded of the
 // sequence up to `end` in the ring.
 bool in_ring(const sf_kv_cache* c, int64_t start, int64_t end) {
+  if (end > token_capacity(c)) return false;
   const int64_t last = (end + kBlockTokens - 1) / kBlockTokens;
   return start >= 0 && start <= end && start >= static_cast<int64_t>(c->folded_blocks) * kBlockTokens &&
          last <= c->capacity_blocks && last - c->folded_blocks <= c->ring_blocks;
@@ -398,7 +404,8 @@ extern "C" int sf_kv_append(const sf_kv_cache* cache, int kv_heads, const void* 
   if (const int rc = sf_kv_check(cache)) return rc;
   if (kv_heads < 1 || cache->heads % kv_heads || tokens < 0) return SF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return SF_OK;
-  if (!k || !v || start < 0 || !in_ring(cache, start, start + tokens))
+  if (!k || !v || start < 0 || start > token_capacity(cache) ||
+      !in_ring(cache, start, start + tokens))
     return SF_ERR_INVALID_ARGUMENT;
   const Rows in = {static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                    k_stride_batch, k_stride_head, k_stride_token,
@@ -423,7 +430,8 @@ extern "C" int sf_kv_compact(const sf_kv_cache* cache, int64_t base, int first,
   if (const int rc = sf_kv_check(cache)) return rc;
   if (count < 0 || count > SF_KV_MAX_MOVES || first < 0 || base < 0) return SF_ERR_INVALID_ARGUMENT;
   if (count == 0) return SF_OK;
-  if (!positions || !in_ring(cache, base + first, end)) return SF_ERR_INVALID_ARGUMENT;
+  if (!positions || base > token_capacity(cache) || !in_ring(cache, base + first, end))
+    return SF_ERR_INVALID_ARGUMENT;
   Moves moves = {};
   for (int i = 0; i < count; ++i) {
     if (positions[i] < first + i || (i && positions[i] <= positions[i - 1]) ||
@@ -467,7 +475,7 @@ extern "C" int sf_kv_fold(const sf_kv_cache* cache, int blocks, sf_stream_t stre
 extern "C" int sf_kv_read(const sf_kv_cache* cache, int64_t start, int tokens, void* k, void* v,
                           sf_stream_t stream) {
   if (const int rc = sf_kv_check(cache)) return rc;
-  if (tokens < 0 || start < 0) return SF_ERR_INVALID_ARGUMENT;
+  if (tokens < 0 || start < 0 || start > token_capacity(cache)) return SF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return SF_OK;
   const int64_t end = start + tokens;
   const int64_t last = (end + kBlockTokens - 1) / kBlockTokens;

@@ -112,7 +112,7 @@ __device__ __forceinline__ void load_entries(const E* p, int n, E (&x)[kPer]) {
 // 151936 bf16 logits take 9.4 us with one, 12.5 with two, 15.4 with four (5.9
 // without any rule).
 template <int DTYPE, int VEC, bool PENALTY, bool OUT, bool TOKENS>
-__global__ __launch_bounds__(kThreads) void rules_kernel(const RuleArgs a) {
+__global__ __launch_bounds__(kThreads) void logit_rules_kernel(const RuleArgs a) {
   using Ty = Type<DTYPE>;
   using Elem = typename Ty::Elem;
   const int lane = threadIdx.x & (SF_WAVE - 1);
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void rules_kernel(const RuleArgs a) {
 }
 
 // The best of a row's partial results: the largest key, then the lowest index.
-__global__ __launch_bounds__(kThreads) void token_kernel(const int2* parts, int count,
+__global__ __launch_bounds__(kThreads) void logit_token_kernel(const int2* parts, int count,
                                                          int64_t* tokens) {
   __shared__ int2 found[kWaves];
   const int2* p = parts + static_cast<int64_t>(blockIdx.x) * count;
@@ -265,7 +265,7 @@ template <int DTYPE, int VEC>
 void launch(const RuleArgs& a, bool penalty, hipStream_t s) {
   const bool out = a.out != nullptr, tokens = a.parts != nullptr;
   const dim3 grid(a.chunks, a.rows);
-#define SF_RULES(P, O, T) rules_kernel<DTYPE, VEC, P, O, T><<<grid, kThreads, 0, s>>>(a)
+#define SF_RULES(P, O, T) logit_rules_kernel<DTYPE, VEC, P, O, T><<<grid, kThreads, 0, s>>>(a)
   if (penalty) {
     if (out && tokens) SF_RULES(true, true, true);
     else if (out) SF_RULES(true, true, false);
@@ -329,7 +329,7 @@ extern "C" int sf_logit_rules(int dtype, const void* logits, int64_t logits_stri
   }
   SF_LAUNCH_CHECK();
   if (tokens) {
-    token_kernel<<<rows, kThreads, 0, s>>>(a.parts, a.chunks * kWaves, tokens);
+    logit_token_kernel<<<rows, kThreads, 0, s>>>(a.parts, a.chunks * kWaves, tokens);
     SF_LAUNCH_CHECK();
   }
   return SF_OK;

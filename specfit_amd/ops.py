@@ -868,6 +868,15 @@ def _scratch(nbytes: int, device: torch.device, stream: torch.cuda.Stream | None
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
+def _dense(t: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """A contiguous copy for a launch on ``stream``, made there: behind what the
+    caller ordered before it, and in memory of that stream's pool."""
+    if stream is None:
+        return t.clone(memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return t.clone(memory_format=torch.contiguous_format)
+
+
 class KVBlocks:
     """Device storage of a block cache (K8): for every layer, sequence and
     key/value head, ``capacity_blocks`` blocks of 64 tokens in 8 bits with a
@@ -965,11 +974,11 @@ def kv_append(blocks: KVBlocks, layer: int, key: torch.Tensor, value: torch.Tens
         raise ValueError(f"key and value must have {blocks.kv_heads} heads")
     kb, kh, kt, kd = key.stride()
     if kd != 1:
-        key = key.contiguous()
+        key = _dense(key, stream)
         kb, kh, kt, _ = key.stride()
     vb, vh, vt, vd = value.stride()
     if vd != 1:
-        value = value.contiguous()
+        value = _dense(value, stream)
         vb, vh, vt, _ = value.stride()
     rc = _launch(_native.lib().sf_kv_append, blocks.index, ref, blocks.kv_heads, key.data_ptr(), kb,
                  kh, kt, value.data_ptr(), vb, vh, vt, start, shape[2],
@@ -1003,10 +1012,13 @@ def kv_compact(blocks: KVBlocks, base: int, positions: Sequence[int], end: int, 
 def kv_fold(blocks: KVBlocks, count: int, *, stream: torch.cuda.Stream | None = None) -> None:
     """Folds the next ``count`` blocks of every layer, complete in the ring,
     into 8 bits; later calls read them from there."""
-    rc = _launch(_native.lib().sf_kv_fold, blocks.index, blocks._whole_ref, int(count),
+    count = int(count)
+    if not 0 <= count <= blocks.capacity_blocks - blocks.folded:
+        raise ValueError("folded blocks out of range")
+    rc = _launch(_native.lib().sf_kv_fold, blocks.index, blocks._whole_ref, count,
                  _stream_handle(stream, blocks.device))
     _native.check(rc, "sf_kv_fold")
-    blocks.folded += int(count)
+    blocks.folded += count
 
 
 def kv_read(blocks: KVBlocks, layer: int, start: int, stop: int, *,
@@ -1054,8 +1066,8 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
     kv_heads, device = blocks.kv_heads, blocks.device
     if Hq < 1 or Hq % kv_heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
-    if keys < 0:
-        raise ValueError("keys must not be negative")
+    if not 0 <= keys < 2 ** 31:
+        raise ValueError("keys must be a number of tokens")
     mask_ptr, mask_batch, mask_q, mask_keys = None, 0, 0, 0
     if mask is not None:
         if mask.dtype is not torch.bool:
@@ -1065,7 +1077,7 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
             raise ValueError(f"mask must be bool [1 or {B}, 1, {Q}, up to {keys} keys]")
         mask_batch, _, mask_q, mask_step = mask.stride()
         if mask_step != 1:
-            mask = mask.contiguous()
+            mask = _dense(mask, stream)
             mask_batch, _, mask_q, _ = mask.stride()
         if mask.shape[0] == 1:
             mask_batch = 0
@@ -1074,14 +1086,17 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
     if Q == 0:
         return out
     if keys == 0:
-        return out.zero_()
+        if stream is None:
+            return out.zero_()
+        with torch.cuda.stream(stream):
+            return out.zero_()
     if mask is not None:
         # A mask of no keys admits them all: any address but null.
         mask_ptr = mask.data_ptr() if mask_keys else out.data_ptr()
     qb, qh, qt, qd = query.stride()
     q_ptr = query.data_ptr()
     if qd != 1 or (qb | qh | qt) % 8 or q_ptr % 16:
-        query = query.clone(memory_format=torch.contiguous_format)
+        query = _dense(query, stream)
         qb, qh, qt, _ = query.stride()
         q_ptr = query.data_ptr()
     need = _block_attention_workspace(B, Q, keys, Hq, kv_heads, D)
@@ -1134,15 +1149,15 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     if len(shape) not in (1, 2) or shape[-1] != T or (len(shape) == 2 and shape[0] not in (1, B)):
         raise ValueError(f"positions must be [{B} or 1, {T}]")
     if positions.stride(-1) != 1:
-        positions = positions.contiguous()
+        positions = _dense(positions, stream)
     step = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
     qb, qt, qh, qd = q.stride()
     if qd != 1:
-        q = q.contiguous()
+        q = _dense(q, stream)
         qb, qt, qh, _ = q.stride()
     kb, kt, kh, kd = k.stride()
     if kd != 1:
-        k = k.contiguous()
+        k = _dense(k, stream)
         kb, kt, kh, _ = k.stride()
     q_out = torch.empty((B, Hq, T, D), dtype=dtype, device=device)
     k_out = torch.empty((B, Hk, T, D), dtype=dtype, device=device)
@@ -1174,7 +1189,7 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
         raise ValueError("logits must have a vocabulary")
     logits_stride, unit = logits.stride()
     if unit != 1:
-        logits = logits.contiguous()
+        logits = _dense(logits, stream)
         logits_stride = logits.stride(0)
     device, index = logits.device, logits.get_device()
     if not repetition > 0:
@@ -1192,14 +1207,14 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
         if paths.dim() != 2 or paths.shape[0] != N or paths.get_device() != index:
             raise ValueError(f"paths must be int32 [{N}, length]")
         if not paths.is_contiguous():
-            paths = paths.contiguous()
+            paths = _dense(paths, stream)
         length, paths_ptr = paths.shape[1], paths.data_ptr()
     if bias is not None:
         _require_cuda("bias", bias, torch.float32)
         if bias.get_device() != index or bias.shape not in ((V,), (1, V), (N, V)):
             raise ValueError(f"bias must be fp32 [{V}] or [{N}, {V}]")
         if bias.stride(-1) != 1:
-            bias = bias.contiguous()
+            bias = _dense(bias, stream)
         bias_stride = bias.stride(0) if bias.dim() == 2 and bias.shape[0] > 1 else 0
         bias_ptr = bias.data_ptr()
     if allowed is not None:
@@ -1208,7 +1223,7 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
         if allowed.get_device() != index or allowed.shape not in ((words,), (1, words), (N, words)):
             raise ValueError(f"allowed must be int32 [{words}] or [{N}, {words}]")
         if allowed.stride(-1) != 1:
-            allowed = allowed.contiguous()
+            allowed = _dense(allowed, stream)
         allowed_stride = allowed.stride(0) if allowed.dim() == 2 and allowed.shape[0] > 1 else 0
         allowed_ptr = allowed.data_ptr()
     tokens = tokens_ptr = work_ptr = out_ptr = None
@@ -1232,6 +1247,18 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
     return tokens
 
 
+def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the bytes between the first and last elements of two tensors
+    meet."""
+    def span(t):
+        first = t.data_ptr()
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return (first, first + (last + 1) * t.element_size()) if t.numel() else (0, 0)
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
                   paths: torch.Tensor | None = None, repetition: float = 1.0,
                   presence: float = 0.0, frequency: float = 0.0,
@@ -1247,7 +1274,8 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
     (frequency * n + presence); then bias (fp32 [V] or [N, V]) is added, and a
     token whose bit v % 32 of word v // 32 of allowed (int32 [V / 32 up] or
     [N, V / 32 up]) is 0 becomes -inf.  Each step is rounded to fp32, the result
-    once more to the logits' type.  ``out`` may be ``logits``."""
+    once more to the logits' type.  ``out`` may be ``logits``, and shares no memory
+    with the arguments otherwise."""
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \
@@ -1255,6 +1283,11 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
         raise ValueError("out must be like logits, with a unit last stride")
     elif out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError("the rows of out must not overlap")
+    else:
+        for t in (logits, counts, paths, bias, allowed):
+            if t is not None and _spans_meet(out, t) and not (
+                    t is logits and t.data_ptr() == out.data_ptr() and t.stride() == out.stride()):
+                raise ValueError("out must be logits or share no memory with the arguments")
     _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, out, False,
                  stream)
     return out

@@ -179,14 +179,18 @@ def summarize(fetch_dir: str, write_dir: str, command: str | None = None) -> str
     return "\n".join(lines) + "\n"
 
 
-# Kernel names of libspecfit_amd (K1-K8), listed in the trace summaries.
+# Kernel names of libspecfit_amd (K1-K11), listed in the trace summaries.
 LIBRARY_KERNELS = ("router_logits_kernel", "router_logits_many_kernel", "router_select_kernel",
                    "dispatch_kernel", "gateup_mfma_kernel", "down_mfma_kernel",
                    "gateup_wide_kernel", "down_wide_kernel", "gateup_generic_kernel",
                    "down_generic_kernel", "combine_kernel", "decode_kernel",
                    "tree_attention_kernel", "tree_attention_tiled_kernel",
                    "tree_attention_merge_kernel", "rms_norm_kernel", "qk_norm_rope_kernel",
-                   "router_topk_scalar_kernel")
+                   "router_topk_scalar_kernel", "kv_append_kernel", "kv_compact_kernel",
+                   "kv_fold_kernel", "kv_read_kernel", "block_attention_direct_kernel",
+                   "block_attention_staged_kernel", "block_attention_merge_kernel",
+                   "block_attention_merge_few_kernel", "rotary_kernel", "logit_rules_kernel",
+                   "logit_token_kernel")
 
 
 FORWARD_START = "router_logits_"  # of few or of many tokens

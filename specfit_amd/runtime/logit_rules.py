@@ -37,11 +37,13 @@ class LogitRules:
         return cls(counts=torch.zeros(vocab_size, dtype=torch.int32, device=device), **kwargs)
 
     def count(self, tokens: torch.Tensor) -> None:
-        """Adds ``tokens`` (int64, any shape) to the histogram."""
+        """Adds ``tokens`` (int64, any shape) to the histogram; those outside
+        the vocabulary, such as a -1 of ``greedy``, count for nothing."""
         if self.counts is None:
             raise ValueError("these rules keep no histogram")
         tokens = tokens.reshape(-1)
-        self.counts.index_add_(0, tokens, torch.ones_like(tokens, dtype=torch.int32))
+        known = (tokens >= 0) & (tokens < self.counts.shape[0])
+        self.counts.index_add_(0, torch.where(known, tokens, 0), known.to(torch.int32))
 
     def adjust(self, logits: torch.Tensor, paths: torch.Tensor | None = None, *,
                allowed: torch.Tensor | None = None,

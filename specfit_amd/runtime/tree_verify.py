@@ -239,7 +239,10 @@ def verify_draft_tree(target, tree: Eagle3DraftTree, pending_seed: torch.Tensor,
     int32 [1 + N, vocab / 32 up] a grammar's set per row (without rules, the
     set alone).  ``commit`` then counts the committed tokens.  A row in which
     nothing is allowed has the verifier token -1, which no draft matches; if
-    the last committed row is one, the pending seed is -1."""
+    the last committed row is one, the pending seed is -1: the sequence ends
+    there, and a call with that seed is refused."""
+    if (rules is not None or allowed is not None) and int(pending_seed.min()) < 0:
+        raise ValueError("the pending seed is no token (nothing was allowed after the last one)")
     verify_ids = tree.verification_token_ids(pending_seed)
     base = cache.get_seq_length()
     device = verify_ids.device

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from specfit_amd import _native, ops
-from specfit_amd.runtime import BlockKVCache, Eagle3DraftTree
+from specfit_amd.runtime import BlockKVCache, Eagle3DraftTree, LogitRules
 from specfit_amd.runtime import block_kv_cache
 
 FAKE = 4096  # never dereferenced: every call below fails, or has no work, before a launch
@@ -218,3 +218,20 @@ def test_path_indices_of_a_tree():
                            tuple(math.log(p) * d for d in (1, 1, 2, 3)))
     assert tree.path_indices().tolist() == [[0, -1, -1, -1], [0, 1, -1, -1], [0, 2, -1, -1],
                                             [0, 1, 3, -1], [0, 1, 3, 4]]
+
+
+def test_starts_past_the_capacity_are_refused():
+    lib, c = _native.lib(), _struct()
+    far = 2 ** 63 - 1
+    for start in (641, far - 5, far):
+        assert _append(c, start, 10) != 0
+        assert lib.sf_kv_read(ctypes.addressof(c), start, 10, FAKE, FAKE, None) != 0
+        assert lib.sf_kv_compact(ctypes.addressof(c), start, 0, (ctypes.c_int32 * 1)(3), 1, far,
+                                 None) != 0
+
+
+def test_tokens_outside_the_vocabulary_are_not_counted():
+    rules = LogitRules.for_vocab(5, "cpu")
+    rules.count(torch.tensor([[0, 4, -1], [5, 4, -7]]))
+    rules.count(torch.empty(0, dtype=torch.int64))
+    assert rules.counts.tolist() == [1, 0, 0, 0, 2]

@@ -484,6 +484,46 @@ def test_another_stream(device):
     assert torch.equal(got, want)
 
 
+def test_another_stream_takes_its_own_copies(device):
+    """Layouts that a call copies first: on the stream it was given, where the
+    caller ordered the inputs, not behind what the current stream still does."""
+    g = torch.Generator().manual_seed(16)
+    key, value, q = (_rand(g, 1, h, n, 64) for h, n in ((2, 90), (2, 90), (4, 3)))
+    swapped = lambda t: t.transpose(2, 3).contiguous().to(device).transpose(2, 3)  # noqa: E731
+    want, got = _cache(device), _cache(device)
+    want.append(0, key.to(device), value.to(device))
+    expected = want.attend(0, q.to(device))
+    mask = torch.rand((1, 1, 90, 3), generator=g).to(device).transpose(2, 3) < 0.5
+    masked = want.attend(0, q.to(device), mask)
+    k2, v2, q2 = swapped(key), swapped(value), swapped(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    ops.kv_append(got.blocks, 0, k2, v2, 0, stream=stream)
+    outs = [ops.block_attention(got.blocks, 0, q2, 90, m, 0.125, stream=stream)
+            for m in (None, mask)]
+    none = ops.block_attention(got.blocks, 0, q2, 0, None, 0.125, stream=stream)
+    with torch.cuda.stream(stream):
+        copies = [t.clone() for t in (*outs, none)]
+    stream.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(copies[0], expected) and torch.equal(copies[1], masked)
+    assert not copies[2].any()
+
+
+def test_token_numbers_past_32_bits_are_refused(device):
+    cache = _cache(device)
+    cache.append(0, *(torch.zeros((1, 2, 70, 64), dtype=torch.bfloat16, device=device),) * 2)
+    q = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16, device=device)
+    for keys in (-1, 2 ** 31, 2 ** 32 + 70):
+        with pytest.raises(ValueError, match="keys"):
+            ops.block_attention(cache.blocks, 0, q, keys, None, 1.0)
+    for count in (-1, 9, 2 ** 32 + 1):
+        with pytest.raises(ValueError, match="folded"):
+            ops.kv_fold(cache.blocks, count)
+    assert cache.folded_tokens == 0
+
+
 def test_repeated_calls_give_the_same_bits(device):
     g = torch.Generator().manual_seed(14)
     for new, mask in ((1, None), (61, "tree"), (300, None)):

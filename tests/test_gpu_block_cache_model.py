@@ -124,6 +124,12 @@ def test_rules_in_the_verification(device):
     nothing = torch.zeros((13, 4), dtype=torch.int32, device=device)
     result = verify_draft_tree(target, tree, seed, cache, allowed=nothing, commit=False)
     assert result.accepted_node_ids == () and int(result.pending_seed) == -1
+    # The sequence ends there.
+    length, counted = cache.get_seq_length(), rules.counts.clone()
+    for again in (dict(rules=rules), dict(allowed=nothing)):
+        with pytest.raises(ValueError, match="seed"):
+            verify_draft_tree(target, tree, result.pending_seed, cache, **again)
+    assert cache.get_seq_length() == length and torch.equal(rules.counts, counted)
     loaded.close()
 
 

@@ -222,3 +222,35 @@ def test_refusals(device):
                 torch.zeros((1, 100), device=device).expand(2, -1)):
         with pytest.raises(ValueError):
             ops.adjust_logits(x, out=out)
+
+
+def test_another_stream_takes_its_own_copies(device):
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn((3, 130), generator=g).to(device)
+    paths = torch.randint(-1, 130, (3, 7), generator=g).int().to(device)
+    bias = torch.randn((3, 130), generator=g).to(device)
+    allowed = _words(g, 3, 130).to(device)
+    args = dict(repetition=1.25, presence=0.5)
+    want = ops.greedy_tokens(x, paths=paths, bias=bias, allowed=allowed, **args)
+    turned = [t.t().contiguous().t() for t in (x, paths, bias, allowed)]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    got = ops.greedy_tokens(turned[0], paths=turned[1], bias=turned[2], allowed=turned[3],
+                            stream=stream, **args)
+    with torch.cuda.stream(stream):
+        got = got.clone()
+    stream.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_out_that_meets_an_argument_is_refused(device):
+    room = torch.zeros((5, 64), device=device)
+    ops.adjust_logits(room[:2], out=room[2:4])
+    with pytest.raises(ValueError, match="share"):
+        ops.adjust_logits(room[:2], out=room[1:3])
+    with pytest.raises(ValueError, match="share"):
+        ops.adjust_logits(room[:2], out=room[2:4], bias=room[3])
+    with pytest.raises(ValueError, match="share"):
+        ops.adjust_logits(room[:2], out=torch.as_strided(room, (2, 64), (128, 1)))

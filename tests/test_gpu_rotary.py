@@ -186,3 +186,21 @@ def test_refusals(device):
         ops.rotary_embed(q, q, positions, table.to("cpu"))
     with pytest.raises(ValueError, match="HIP device"):
         ops.rotary_embed(q.cpu(), q.cpu(), positions.cpu(), table)
+
+
+def test_another_stream_takes_its_own_copies(device):
+    g = torch.Generator().manual_seed(8)
+    table = rotary_frequencies(64, device=device)
+    q, k = (torch.randn((1, 5, h, 64), generator=g).to(device) for h in (4, 2))
+    positions = torch.tensor([[3, 0], [9, 0], [7, 0], [5, 0], [1, 0]], device=device)[:, 0]
+    want = ops.rotary_embed(q, k, positions, table)
+    views = [t.transpose(2, 3).contiguous().transpose(2, 3) for t in (q, k)]
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)
+    got = ops.rotary_embed(*views, positions, table, stream=stream)
+    with torch.cuda.stream(stream):
+        copies = [t.clone() for t in got]
+    stream.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(copies[0], want[0]) and torch.equal(copies[1], want[1])
