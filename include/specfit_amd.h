@@ -43,6 +43,13 @@
  *   sf_qk_norm_rope      tf:162-167  the query/key norms and
  *                        apply_rotary_pos_emb (tf:58-81) of
  *                        Qwen3MoeAttention.forward
+ *   sf_kv_append, sf_kv_compact, sf_kv_fold, sf_kv_read, sf_block_attention
+ *                        the bf16 DynamicCache of the target and its
+ *                        compaction (eagle3_tree.py:833-858), held in 8 bits,
+ *                        and the attention over it
+ *   sf_rotary            apply_rotary_pos_emb with angles from the positions
+ *   sf_logit_rules       the argmax of eagle3_tree.py:1241-1290 with rules on
+ *                        the logits before it
  */
 #ifndef SPECFIT_AMD_H
 #define SPECFIT_AMD_H
@@ -409,7 +416,7 @@ int sf_qk_norm_rope(const void *q, int64_t q_stride_token, const void *k,
                     sf_stream_t stream);
 
 /*
- * K8: the block cache.  Keys and values of a sequence whose complete blocks
+ * K9: the block cache.  Keys and values of a sequence whose complete blocks
  * of SF_KV_BLOCK tokens are held in 8 bits, with one scale per block, head and
  * K or V, and whose last tokens are held in bf16 in a ring of blocks until
  * they are folded.  No counterpart in the reference, whose target keeps a bf16
@@ -490,7 +497,7 @@ int sf_kv_read(const sf_kv_cache *cache, int64_t start, int tokens, void *k,
                void *v, sf_stream_t stream);
 
 /*
- * K9: grouped-query attention over a block cache of `keys` tokens:
+ * K10: grouped-query attention over a block cache of `keys` tokens:
  *   out[b, qi, qh, :] = sum_s p_s * v^[b, h, s, :],
  *   p = softmax over admitted keys s of scale * (q[b, qi, qh, :] . k^[b, h, s, :])
  * h = qh / (q_heads / kv_heads), scores and sums in fp32, p rounded to bf16
@@ -518,7 +525,7 @@ int sf_block_attention(const sf_kv_cache *cache, int batch, int kv_heads,
                        int64_t workspace_bytes, sf_stream_t stream);
 
 /*
- * K10: rotary positions of queries and keys.  For pair i of a head's first
+ * K11: rotary positions of queries and keys.  For pair i of a head's first
  * rotary_dim elements, (a, b) = elements (i, i + rotary_dim / 2), or
  * (2 i, 2 i + 1) if interleaved:
  *   angle = position * turns[i]  (in turns, fp64, reduced before its rounding)
@@ -543,7 +550,7 @@ int sf_rotary(int dtype, const void *q, int64_t q_stride_batch,
               int interleaved, void *q_out, void *k_out, sf_stream_t stream);
 
 /*
- * K11: rules on logits.  With n = counts[v] + occurrences of v in paths[r]
+ * K12: rules on logits.  With n = counts[v] + occurrences of v in paths[r]
  * (entries outside [0, vocab) count for nothing), each step rounded to fp32:
  *   y = x                                        if n == 0
  *   y = (x < 0 ? x * repetition : x / repetition)

@@ -1,4 +1,4 @@
-// K11: repetition penalties, a bias and an allowed set on rows of logits, and
+// K12: repetition penalties, a bias and an allowed set on rows of logits, and
 // each row's greedy token.
 //
 // A thread has eight vocabulary entries of a row; the tokens of the row's own path

@@ -1,4 +1,4 @@
-"""PyTorch-facing wrappers of the C-ABI kernels (K1-K11 and the H2D copy).
+"""PyTorch-facing wrappers of the C-ABI kernels (K1-K12 and the H2D copy).
 
 Tensors are plumbing: each wrapper checks dtype, device, shape and
 contiguity on the host, allocates outputs with the caching allocator and
@@ -836,7 +836,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     return q_out, k_out
 
 
-# ------------------------------------------------------------------ K8 ----
+# ------------------------------------------------------------------ K9 ----
 KV_BLOCK = 64                       # tokens of a cache block (SF_KV_BLOCK)
 KV_HELD = {"e4m3": 0, "int8": 1}    # how complete blocks are held
 _KV_MAX_MOVES = 256                 # positions of one sf_kv_compact call
@@ -878,7 +878,7 @@ def _dense(t: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
 
 
 class KVBlocks:
-    """Device storage of a block cache (K8): for every layer, sequence and
+    """Device storage of a block cache (K9): for every layer, sequence and
     key/value head, ``capacity_blocks`` blocks of 64 tokens in 8 bits with a
     power-of-two scale each for keys and values, and a ring of ``ring_blocks``
     bf16 blocks for the tokens that are not folded yet.  Which tokens are there
@@ -1038,7 +1038,7 @@ def kv_read(blocks: KVBlocks, layer: int, start: int, stop: int, *,
     return keys, values
 
 
-# ------------------------------------------------------------------ K9 ----
+# ----------------------------------------------------------------- K10 ----
 @functools.lru_cache(maxsize=256)
 def _block_attention_workspace(batch: int, queries: int, keys: int, q_heads: int, kv_heads: int,
                                head_dim: int) -> int:
@@ -1050,7 +1050,7 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
                     mask: torch.Tensor | None, scale: float, *,
                     stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """Grouped-query attention over the first ``keys`` tokens of a block
-    cache's layer (K9).
+    cache's layer (K10).
 
     query [batch, Hq, Q, head_dim] bf16, Hq a multiple of the cache's heads;
     mask bool [batch or 1, 1, Q, M] (True = attend) over the last M <= keys
@@ -1115,13 +1115,13 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
     return out
 
 
-# ----------------------------------------------------------------- K10 ----
+# ----------------------------------------------------------------- K11 ----
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table, *,
                  stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Rotary positions of queries and keys (K10).
+    """Rotary positions of queries and keys (K11).
 
     q [B, T, Hq, D] and k [B, T, Hk, D], bf16, fp16 or fp32 (one type, any
     strides with a unit last one); positions int64 [B, T], [1, T] or [T];
@@ -1170,7 +1170,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     return q_out, k_out
 
 
-# ----------------------------------------------------------------- K11 ----
+# ----------------------------------------------------------------- K12 ----
 @functools.lru_cache(maxsize=256)
 def _logit_rules_workspace(rows: int, vocab: int) -> int:
     return _native.lib().sf_logit_rules_workspace(rows, vocab)
@@ -1265,7 +1265,7 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
                   bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
                   out: torch.Tensor | None = None,
                   stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-    """Repetition penalties, a bias and an allowed set on rows of logits (K11).
+    """Repetition penalties, a bias and an allowed set on rows of logits (K12).
 
     logits [N, V] bf16, fp16 or fp32.  n = counts[v] (int32 [V]) + the
     occurrences of v in the row of paths (int32 [N, P]; entries outside the

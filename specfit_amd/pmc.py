@@ -179,7 +179,7 @@ def summarize(fetch_dir: str, write_dir: str, command: str | None = None) -> str
     return "\n".join(lines) + "\n"
 
 
-# Kernel names of libspecfit_amd (K1-K11), listed in the trace summaries.
+# Kernel names of libspecfit_amd (K1-K12), listed in the trace summaries.
 LIBRARY_KERNELS = ("router_logits_kernel", "router_logits_many_kernel", "router_select_kernel",
                    "dispatch_kernel", "gateup_mfma_kernel", "down_mfma_kernel",
                    "gateup_wide_kernel", "down_wide_kernel", "gateup_generic_kernel",

@@ -1,4 +1,4 @@
-"""A key/value cache with its complete blocks in 8 bits (K8, K9).
+"""A key/value cache with its complete blocks in 8 bits (K9, K10).
 
 ``BlockKVCache`` takes the place of the bf16 ``DynamicCache`` that the
 reference's target keeps (src/specfit/runtime/eagle3_tree.py:833-858 and

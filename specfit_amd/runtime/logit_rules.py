@@ -1,4 +1,4 @@
-"""Rules on the logits of a verification step (K11).
+"""Rules on the logits of a verification step (K12).
 
 The reference verifies greedily on the target's bare logits
 (src/specfit/runtime/eagle3_tree.py:1241-1290).  ``LogitRules`` holds what a

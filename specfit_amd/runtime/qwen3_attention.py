@@ -16,11 +16,11 @@ projection whose weight was replaced afterwards (``module.to``, a new
 Parameter) turns the fused GEMM off for that layer.
 
 With a ``BlockKVCache`` as ``past_key_values`` the new keys and values go
-into it and the attention runs over its 8-bit blocks (K9), whatever the
+into it and the attention runs over its 8-bit blocks (K10), whatever the
 config's attention implementation; masks are bool ones (those of sdpa and of
 the tree attention are), or None for causal.  With a rotary table
 (``install_hip_attention(model, rotary=...)``) the rotary embedding takes its
-angles from the position ids (K10), for any batch and head dim, instead of
+angles from the position ids (K11), for any batch and head dim, instead of
 from the model's bf16 cosines.
 """
 from __future__ import annotations

@@ -1,4 +1,4 @@
-"""The block cache and its attention (K8, K9) against plain 64-bit forms.
+"""The block cache and its attention (K9, K10) against plain 64-bit forms.
 
 What the cache gives back and its scales are exact; the attention is held to
 a bound that counts its roundings (see _block_reference.attention)."""

@@ -1,4 +1,4 @@
-"""Rules on logits (K11) against their definition: every step is a
+"""Rules on logits (K12) against their definition: every step is a
 correctly rounded fp32 operation, so values and tokens are exact."""
 import math
 

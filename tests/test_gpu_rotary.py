@@ -1,4 +1,4 @@
-"""Rotary positions (K10) against the formula in 64 bits.
+"""Rotary positions (K11) against the formula in 64 bits.
 
 A turned element is two products and a sum of fp32 values: with sines good to
 2^-22 (their own rounding, that of the reduced angle, 2^-25 of a turn at most, and
