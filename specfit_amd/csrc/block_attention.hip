@@ -9,8 +9,9 @@
 // key scale goes into the factor of a tile's scores, and the value scale, a
 // power of two, into the exponent of its probabilities,
 //   w = 2^(s c_t + (log2 v_scale - M)),  l += v_scale^-1 sum w,  O += w V,
-// so neither costs an instruction per value.  M, a row's maximum in log2
-// units, is a reference only: every weight of a row has the same one.
+// so neither costs an instruction per value.  M, at or a little above a row's
+// maximum in log2 units, is a reference only: every weight of a row has the same
+// one.
 //
 // Two forms, and kernels that merge splits of the keys: few rows per KV head go
 // straight from the cache to registers (the direct kernel), many share tiles in
@@ -66,6 +67,13 @@ struct Args {
   float* part_acc;   // [splits][batch kv_heads][rows][D], splits > 1 only
   float2* part_ml;   // [splits][batch kv_heads][rows]
 };
+
+// M is set this far above the maximum that made it move, so that it rarely has to
+// move again (a move costs a product per accumulator, and with M at the maximum a
+// third of the tiles of a long prompt move one of 32 rows: 128 nodes after 32777
+// tokens 174 -> 170 us).  A row's weights are at most 1, the largest at least
+// 2^-kHeadroom; rounded to bf16 relative to themselves, they lose nothing by it.
+constexpr float kHeadroom = 8.f;
 
 // Above this |M| its rounding could leave p far from 1 at the maximum (2^28 in
 // log2 units: a factor of 2^16), so the scores are scaled before M is taken off.
@@ -248,7 +256,7 @@ struct Rows {
   using Sh = Shape<D, ROWS>;
   using Acc = typename Sh::Acc;
   static constexpr int kN = acc_size<Acc>();
-  float m = -INFINITY, l = 0.f;  // maximum in log2 units; this lane's part of the sum
+  float m = -INFINITY, l = 0.f;  // M, at or above the maximum, in log2 units; this lane's part of the sum
   Acc acc[Sh::kOutTiles];
 
   __device__ __forceinline__ void clear() {
@@ -271,13 +279,14 @@ struct Rows {
     return max_raw(mx[0], mx[1]);
   }
 
-  // Brings the state to the maximum over a tile whose largest score of the lane
-  // is `most`; factor: of the scores, to log2 units.  mul and base: a score's
-  // weight times the value scale is 2^(s mul + base).
+  // Brings M to or above the scores of a tile whose largest of the lane is `most`;
+  // factor: of the scores, to log2 units.  mul and base: a score's weight times the
+  // value scale is 2^(s mul + base).
   __device__ __forceinline__ void raise(Acc (&s)[Sh::kScoreTiles], float most, float factor,
                                         float v_scale, float& mul, float& base) {
-    const float mnew = fmaxf(m, Sh::row_max(most) * factor);
-    if (__any(mnew > m)) {
+    const float top = Sh::row_max(most) * factor;
+    if (__any(top > m)) {
+      const float mnew = top > m ? top + kHeadroom : m;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mnew);
       l *= alpha;
 #pragma unroll

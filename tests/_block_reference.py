@@ -58,12 +58,16 @@ def attention(q, k, v, mask, scale):
     The bound: each weight is off by half a bf16 step of itself, by its score's
     error and by that of the exponential.  A score is a sum of D products whose
     roundings (2^-24 each, D + 2 of them with the factors) are relative to
-    sum |q k|; the maximum taken off in log2 units and the product with the factor
-    add 2 steps of the largest score; an exponential is good to 2^-21.  The sum
-    of the weights has the same but for the bf16 step.  The result is rounded
-    once.  A key whose weight times the value scale 2^e falls below 2^-126 (fp32's
-    least normal number; the row's largest weight is 1) may count for nothing: its
-    part is below 2^-126 |code| <= 2^-126 448 < 2^-117, S of them below S 2^-117."""
+    sum |q k|; the reference taken off in log2 units, at most 8 above the largest
+    score, and the product with the factor add 2 steps of the largest score and of 8
+    (2^-24 8 = 2^-21 each); the value scale's exponent, of at most 128, joins the
+    reference in one more sum (2^-24 128 = 2^-17); an exponential is good to 2^-21;
+    these together stay below 2^-16.
+    The sum of the weights has the same but for the bf16 step.  The result is
+    rounded once.  A key whose weight times the value scale 2^e falls below 2^-126
+    (fp32's least normal number) may count for nothing: its part is below 2^-126
+    |code| <= 2^-126 448 < 2^-117, S of them below S 2^-117, over a sum of weights of
+    at least 2^-8."""
     q = q.cpu().double()
     B, Hq, Q, D = q.shape
     H, S = k.shape[1], k.shape[2]
@@ -83,7 +87,7 @@ def attention(q, k, v, mask, scale):
             p = p / p.sum(1, keepdim=True).clamp_min(1e-300)
             out[b, :, h] = p @ vv
             size = p @ vv.abs()
-            weight = 2.0 ** -24 * ((D + 2) * mag.amax(1) + 4 * mag.amax(1)) * 2 + 2.0 ** -20
+            weight = 2.0 ** -24 * ((D + 2) * mag.amax(1) + 4 * mag.amax(1)) * 2 + 2.0 ** -16
             bound[b, :, h] = (EPS[torch.bfloat16] + weight)[:, None] * size \
-                + EPS[torch.bfloat16] * (1 + EPS[torch.bfloat16]) * out[b, :, h].abs() + S * 2.0 ** -117
+                + EPS[torch.bfloat16] * (1 + EPS[torch.bfloat16]) * out[b, :, h].abs() + S * 2.0 ** -109
     return out, bound
