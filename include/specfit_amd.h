@@ -536,7 +536,8 @@ int sf_block_attention(const sf_kv_cache *cache, int batch, int kv_heads,
  *   positions    int64, (b, t) at b * position_stride + t (0: one row for all)
  *   turns        fp64 [rotary_dim / 2], |position * turns| < 2^51
  *   out          dtype [batch, heads, tokens, head_dim], contiguous
- * dtype: SF_BF16, SF_F16 or SF_F32; rotary_dim even, <= head_dim <= 1024.
+ * dtype: SF_BF16, SF_F16 or SF_F32; rotary_dim even, <= head_dim <= 1024;
+ * batch * tokens < 2^27.
  */
 #define SF_BF16 0
 #define SF_F16 1

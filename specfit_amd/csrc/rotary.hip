@@ -174,7 +174,8 @@ extern "C" int sf_rotary(int dtype, const void* q, int64_t q_stride_batch, int64
     return SF_ERR_UNSUPPORTED_SHAPE;
   const int64_t all = static_cast<int64_t>(batch) * tokens;
   if (all == 0 || q_heads + k_heads == 0) return SF_OK;
-  if (all >= (int64_t{1} << 31)) return SF_ERR_UNSUPPORTED_SHAPE;
+  // Below 2^32 threads of a launch.
+  if (all >= int64_t{kMaxTokens} << 24) return SF_ERR_UNSUPPORTED_SHAPE;
   if (!positions || !turns || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)))
     return SF_ERR_INVALID_ARGUMENT;
   RotaryArgs a = {{q, k}, {q_stride_batch, k_stride_batch}, {q_stride_token, k_stride_token},

@@ -235,3 +235,10 @@ def test_tokens_outside_the_vocabulary_are_not_counted():
     rules.count(torch.tensor([[0, 4, -1], [5, 4, -7]]))
     rules.count(torch.empty(0, dtype=torch.int64))
     assert rules.counts.tolist() == [1, 0, 0, 0, 2]
+
+
+def test_rotary_positions_of_too_many_tokens_are_refused():
+    lib = _native.lib()
+    for batch, tokens in ((1, 2 ** 27), (2 ** 14, 2 ** 14), (2 ** 31 - 1, 2 ** 31 - 1)):
+        assert lib.sf_rotary(0, FAKE, 8, 8, 8, 1, FAKE, 8, 8, 8, 1, FAKE, 0, FAKE, 1.0, batch,
+                             tokens, 2, 2, 0, FAKE, FAKE, None) == 2

@@ -524,6 +524,55 @@ def test_token_numbers_past_32_bits_are_refused(device):
     assert cache.folded_tokens == 0
 
 
+def test_two_streams_at_once(device):
+    """Calls that split their keys, each with scratch memory of its own."""
+    g = torch.Generator().manual_seed(17)
+    cache, _, _ = _filled(device, g, 1, 4, 128, 9000, 3, "int8")
+    assert ops._block_attention_workspace(1, 3, 9003, 16, 4, 128) > 0
+    qs = [_rand(g, 1, 16, 3, 128).to(device) for _ in range(2)]
+    want = [cache.attend(0, q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    outs = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                outs[i].append(cache.attend(0, qs[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+@pytest.mark.parametrize("held,D,rows", [("e4m3", 128, 1), ("int8", 64, 80)])
+def test_offsets_past_32_bits(device, held, D, rows):
+    """The last head of a cache whose codes take more than 4 GiB, with the last
+    blocks of a million tokens: appended, folded, read back and attended to."""
+    heads, blocks = 40 * 128 // D, 16384
+    start, new = (blocks - 3) * BLOCK, 150
+    b = ops.KVBlocks(layers=1, batch=1, kv_heads=heads, head_dim=D, capacity_blocks=blocks,
+                     ring_blocks=3, held=held, device=device)
+    assert (heads - 1) * blocks * BLOCK * D > 2 ** 32
+    b.keys.zero_()
+    b.values.zero_()
+    b.folded = blocks - 3
+    g = torch.Generator().manual_seed(D)
+    k, v, q = (_rand(g, 1, heads, n, D) for n in (new, new, rows))
+    ops.kv_append(b, 0, k.to(device), v.to(device), start)
+    ops.kv_fold(b, 2)
+    got_k, got_v = ops.kv_read(b, 0, start, start + new)
+    kk, vv = held_rows(k, 2, held), held_rows(v, 2, held)
+    assert _same(got_k, kk) and _same(got_v, vv)
+    # The tokens before are there and admit nobody.
+    keys = start + new
+    mask = torch.zeros((1, 1, rows, keys), dtype=torch.bool)
+    mask[..., start:] = torch.rand((rows, new), generator=g) < 0.7
+    mask[..., -1] = True
+    out = ops.block_attention(b, 0, q.to(device), keys, mask.to(device), D ** -0.5)
+    last = heads - 1
+    want, bound = attention(q[:, last:], kk[:, last:], vv[:, last:], mask[..., start:], D ** -0.5)
+    assert ((out[:, :, last:].cpu().double() - want).abs() <= bound).all()
+
+
 def test_repeated_calls_give_the_same_bits(device):
     g = torch.Generator().manual_seed(14)
     for new, mask in ((1, None), (61, "tree"), (300, None)):
