@@ -504,7 +504,10 @@ int sf_kv_read(const sf_kv_cache *cache, int64_t start, int tokens, void *k,
  * for the product with v^, the result rounded to bf16 once.  The mask
  * covers the last mask_keys keys; a key before them is admitted by every row.
  * With mask == NULL key s is admitted when s <= keys - queries + qi.  A row that
- * admits no key gets zeros; what a key that is not admitted holds has no effect.
+ * admits no key gets zeros, and only such a row: one with an admitted score of NaN or
+ * +inf, or with nothing but scores of -inf, is NaN.  An infinite or NaN value of an
+ * admitted key leaves its element infinite or NaN, whatever the key's weight.  What a
+ * key that is not admitted holds has no effect.
  *   q     bf16, element (b, qi, qh, d) at b * q_stride_batch +
  *         qi * q_stride_token + qh * q_stride_head + d, 16-byte aligned rows
  *   mask  uint8/bool, element (b, qi, s) at b * mask_stride_batch +

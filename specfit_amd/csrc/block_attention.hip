@@ -11,7 +11,8 @@
 //   w = 2^(s c_t + (log2 v_scale - M)),  l += v_scale^-1 sum w,  O += w V,
 // so neither costs an instruction per value.  M, at or a little above a row's
 // maximum in log2 units, is a reference only: every weight of a row has the same
-// one.
+// one.  A state whose M is -inf belongs to a row that admits none of its keys; every
+// merge and the last division go by that (see Rows::settle).
 //
 // Two forms, and kernels that merge splits of the keys: few rows per KV head go
 // straight from the cache to registers (the direct kernel), many share tiles in
@@ -74,6 +75,9 @@ struct Args {
 // tokens 174 -> 170 us).  A row's weights are at most 1, the largest at least
 // 2^-kHeadroom; rounded to bf16 relative to themselves, they lose nothing by it.
 constexpr float kHeadroom = 8.f;
+
+// M of a state whose admitted scores were all -inf or NaN.
+constexpr float kLowest = -3.402823466e+38f;
 
 // Above this |M| its rounding could leave p far from 1 at the maximum (2^28 in
 // log2 units: a factor of 2^16), so the scores are scaled before M is taken off.
@@ -340,6 +344,16 @@ struct Rows {
     add_sum(sum, v_scale);
   }
 
+  // After the last tile: the lanes' sums together, and M of a row that admits a key
+  // (`some`, of any lane).  It is still -inf where all scores were -inf or NaN, as the
+  // maximum leaves a NaN out: then the lowest finite value, so that a NaN in l reaches
+  // the result of any merge (its factor may be 0) and a sum of 0 divides 0.
+  __device__ __forceinline__ void settle(bool some) {
+    l = Sh::row_sum(l);
+    const float count = Sh::row_sum(some ? 1.f : 0.f);
+    if (m == -INFINITY && count > 0.f) m = kLowest;
+  }
+
   __device__ __forceinline__ void softmax(Acc (&s)[Sh::kScoreTiles], float factor, float v_scale,
                                           sf_u32x4 (&w)[Sh::kPSteps]) {
     float mul, base;
@@ -377,6 +391,7 @@ struct Admit {
   const uint8_t* row;  // the mask of the lane's row
   int mask_begin, S, lane_end;
   int full;            // keys below it are admitted by all of the wavefront's rows
+  uint32_t some;       // not 0: the row admits a key that the lane knows of
   uint32_t words[Sh::kWords];
 
   __device__ __forceinline__ void load(int lane, int key0) {
@@ -385,6 +400,7 @@ struct Admit {
     for (int g = 0; g < Sh::kWords; ++g) {
       words[g] = admitted(row, key0 + Sh::key(lane, g), mask_begin, S);
       pin(words[g]);
+      some |= words[g];
     }
   }
   // Scores of keys that the row does not admit: -inf.
@@ -576,6 +592,7 @@ __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kern
   admit.mask_begin = a.mask_begin;
   admit.S = a.S;
   admit.lane_end = diag + tok;
+  admit.some = MASK ? a.mask_begin > 0 : diag + tok > 0;
   admit.full = MASK ? min(a.S, a.mask_begin) : max(0, diag + min(wave_row, a.rows - 1) / a.G);
 
   const int64_t cap = static_cast<int64_t>(head) * a.c.capacity_blocks;
@@ -787,7 +804,7 @@ __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kern
   }
   if (special)
     add_special<D, 32, HELD, MASK>(r, a, head, lane, begin, end, 1, admit);
-  r.l = Sh::row_sum(r.l);
+  r.settle(admit.some != 0);
   if (row >= a.rows) return;
   if (a.splits > 1) {
     const int64_t at = (static_cast<int64_t>(split) * a.c.heads + head) * a.rows + row;
@@ -800,7 +817,7 @@ __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kern
             make_float4(r.acc[t][4 * j], r.acc[t][4 * j + 1], r.acc[t][4 * j + 2],
                         r.acc[t][4 * j + 3]);
   } else {
-    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+    const float inv = r.m == -INFINITY ? 0.f : 1.f / r.l;
     uint16_t* out = a.out + out_row_at(a, head, row) * D;
 #pragma unroll
     for (int t = 0; t < Sh::kOutTiles; ++t)
@@ -852,6 +869,7 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
   admit.mask_begin = a.mask_begin;
   admit.S = a.S;
   admit.lane_end = diag + tok;
+  admit.some = MASK ? a.mask_begin > 0 : diag + tok > 0;
   admit.full = MASK ? min(a.S, a.mask_begin) : max(0, diag + first_row / a.G);
 
   const int64_t cap = static_cast<int64_t>(head) * a.c.capacity_blocks;
@@ -986,7 +1004,7 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
   }
   if (special)
     add_special<D, ROWS, HELD, MASK>(r, a, head, lane, begin + wave, end, kDirectWaves, admit);
-  r.l = Sh::row_sum(r.l);
+  r.settle(admit.some != 0);
 
   // Merge the wavefronts' states in their order.
   constexpr int kRow = D + 4;
@@ -1030,18 +1048,18 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
       if (d == 0) a.part_ml[at] = make_float2(M, l);
     } else {
       const int64_t to = out_row_at(a, head, out_row);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = M == -INFINITY ? 0.f : 1.f / l;
       *reinterpret_cast<uint2*>(a.out + to * D + d) =
           make_uint2(sf_pack_bf16(o[0] * inv, o[1] * inv), sf_pack_bf16(o[2] * inv, o[3] * inv));
     }
   }
 }
 
-// Elements d .. d + 3 of a row, divided by its sum.
+// Elements d .. d + 3 of a row with M, divided by its sum.
 template <int D>
 __device__ __forceinline__ void store_merged(const Args& a, int head, int row, int d, const float4& o,
-                                             float l) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+                                             float M, float l) {
+  const float inv = M == -INFINITY ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(a.out + out_row_at(a, head, row) * D + d) =
       make_uint2(sf_pack_bf16(o.x * inv, o.y * inv), sf_pack_bf16(o.z * inv, o.w * inv));
 }
@@ -1095,7 +1113,7 @@ __global__ __launch_bounds__(kMergeThreads) void block_attention_merge_few_kerne
       add_scaled(o, x[s], f);
     }
   }
-  store_merged<D>(a, head, row, d, o, l);
+  store_merged<D>(a, head, row, d, o, M, l);
 }
 
 // Merges the splits of a row, if they are many or the rows few.  A thread looks at
@@ -1148,7 +1166,7 @@ __global__ __launch_bounds__(kMergeThreads) void block_attention_merge_kernel(co
   float l = sum_lds[0];
 #pragma unroll
   for (int w = 1; w < kMergeWaves; ++w) l += sum_lds[w];
-  store_merged<D>(a, head, row, d, o, l);
+  store_merged<D>(a, head, row, d, o, M, l);
 }
 
 // How a call's rows and keys are dealt out.
