@@ -519,6 +519,12 @@ int sf_kv_read(const sf_kv_cache *cache, int64_t start, int tokens, void *k,
  */
 int64_t sf_block_attention_workspace(int batch, int queries, int keys,
                                      int q_heads, int kv_heads, int head_dim);
+/*
+ * Query rows of a KV head that a workgroup takes in such a call: 16 (straight from the
+ * cache) or 256 (tiles shared in LDS), 0 for shapes that the call refuses.
+ */
+int sf_block_attention_rows(int batch, int queries, int keys, int q_heads,
+                            int kv_heads, int head_dim);
 int sf_block_attention(const sf_kv_cache *cache, int batch, int kv_heads,
                        int keys, const void *q, int64_t q_stride_batch,
                        int64_t q_stride_head, int64_t q_stride_token,

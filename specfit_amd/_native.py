@@ -64,6 +64,7 @@ SIGNATURES = {
     "sf_kv_fold": ([_p, _i, _p], _i),
     "sf_kv_read": ([_p, _i64, _i, _p, _p, _p], _i),
     "sf_block_attention_workspace": ([_i, _i, _i, _i, _i, _i], _i64),
+    "sf_block_attention_rows": ([_i, _i, _i, _i, _i, _i], _i),
     "sf_block_attention": ([_p, _i, _i, _i, _p, _i64, _i64, _i64, _i, _i, _p, _i64, _i64, _i, _f,
                             _p, _p, _i64, _p], _i),
     "sf_rotary": ([_i, _p, _i64, _i64, _i64, _i, _p, _i64, _i64, _i64, _i, _p, _i64, _p, _f, _i,

@@ -1261,18 +1261,31 @@ bool fits(int64_t heads, int64_t group, int64_t queries, int64_t keys) {
          queries * group * heads <= kMaxRows;
 }
 
+// False for shapes that no call takes.
+bool plan_for(int batch, int queries, int keys, int q_heads, int kv_heads, int head_dim, Plan* p) {
+  if (batch < 1 || queries < 1 || keys < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
+      (head_dim != 64 && head_dim != 128))
+    return false;
+  const int64_t heads = static_cast<int64_t>(batch) * kv_heads;
+  if (!fits(heads, q_heads / kv_heads, queries, keys)) return false;
+  *p = plan_of(static_cast<int>(heads), q_heads / kv_heads, queries, keys, head_dim);
+  return true;
+}
+
 }  // namespace
 
 extern "C" int64_t sf_block_attention_workspace(int batch, int queries, int keys, int q_heads,
                                                 int kv_heads, int head_dim) {
-  if (batch < 1 || queries < 1 || keys < 1 || kv_heads < 1 || q_heads < 1 || q_heads % kv_heads ||
-      (head_dim != 64 && head_dim != 128))
-    return 0;
-  const int64_t heads = static_cast<int64_t>(batch) * kv_heads;
-  if (!fits(heads, q_heads / kv_heads, queries, keys)) return 0;
-  const Plan p = plan_of(static_cast<int>(heads), q_heads / kv_heads, queries, keys, head_dim);
-  if (p.splits == 1) return 0;
-  return static_cast<int64_t>(p.splits) * heads * p.rows * (head_dim + 2) * 4;
+  Plan p;
+  if (!plan_for(batch, queries, keys, q_heads, kv_heads, head_dim, &p) || p.splits == 1) return 0;
+  return static_cast<int64_t>(p.splits) * batch * kv_heads * p.rows * (head_dim + 2) * 4;
+}
+
+extern "C" int sf_block_attention_rows(int batch, int queries, int keys, int q_heads, int kv_heads,
+                                       int head_dim) {
+  Plan p;
+  if (!plan_for(batch, queries, keys, q_heads, kv_heads, head_dim, &p)) return 0;
+  return p.staged ? kStagedRows : kDirectRows;
 }
 
 extern "C" int sf_block_attention(const sf_kv_cache* cache, int batch, int kv_heads, int keys,
