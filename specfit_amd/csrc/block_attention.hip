@@ -304,15 +304,17 @@ struct Rows {
     mul = factor;
     const bool large = fabsf(m) > kFusedMax && m != -INFINITY;
     if (__any(large)) {
-      const float off = large ? m : 0.f;
+      // Only in the rows that need it: another rounding would change the others' bits.
 #pragma unroll
       for (int t = 0; t < Sh::kScoreTiles; ++t) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) s[t][i] = s[t][i] * factor - off;
+        for (int i = 0; i < kN; ++i) s[t][i] = large ? s[t][i] * factor - m : s[t][i];
         pin(s[t]);
       }
-      if (large) base = shift;
-      mul = 1.f;
+      if (large) {
+        base = shift;
+        mul = 1.f;
+      }
     }
   }
 

@@ -232,3 +232,21 @@ def test_captured_repeated_and_on_two_streams(device, case):
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(o, want[i]) for o in outs[i])
+
+
+@pytest.mark.parametrize("case", FEW, ids=_name)
+def test_a_row_keeps_its_bits_beside_very_large_scores(device, case):
+    """Scores of other rows, up to 2^40 and infinite, change nothing in a row."""
+    B, Hq, H, D, Q, S = case
+    g = torch.Generator().manual_seed(5)
+    q, k, v = _inputs(case, g)
+    q = q * 4  # peaked: a last bit of a score shows
+    cache = _cache(device, case, k, v, "e4m3", (S - 1) // 64)
+    clean = cache.attend(0, q.to(device)).cpu()
+    loud = torch.rand((B, Hq, Q), generator=g) < 0.15
+    loud[:, 0, 0] = True
+    for size in (2.0 ** 40, math.inf):
+        p = torch.where(loud[..., None], (q.float() * size).bfloat16(), q)
+        out = cache.attend(0, p.to(device)).cpu()
+        keep = ~loud.transpose(1, 2)
+        assert torch.equal(out[keep], clean[keep])
