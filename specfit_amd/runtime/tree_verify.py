@@ -240,10 +240,13 @@ def verify_draft_tree(target, tree: Eagle3DraftTree, pending_seed: torch.Tensor,
     set alone).  ``commit`` then counts the committed tokens.  A row in which
     nothing is allowed has the verifier token -1, which no draft matches; if
     the last committed row is one, the pending seed is -1: the sequence ends
-    there, and a call with that seed is refused."""
-    if (rules is not None or allowed is not None) and int(pending_seed.min()) < 0:
-        raise ValueError("the pending seed is no token (nothing was allowed after the last one)")
+    there, and every call with that seed is refused."""
     verify_ids = tree.verification_token_ids(pending_seed)
+    # Also without rules, as a grammar may end before the loop does: the embedding
+    # would be indexed out of range.  (The host waits for the seed's stream anyway, to
+    # copy the tree's inputs.)
+    if int(pending_seed) < 0:
+        raise ValueError("the pending seed is no token (nothing was allowed after the last one)")
     base = cache.get_seq_length()
     device = verify_ids.device
     mask = tree.verification_attention_mask(
