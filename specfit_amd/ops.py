@@ -15,6 +15,7 @@ from typing import Sequence
 import torch
 
 from . import _native
+from .rotary import RotaryTable
 
 _BF16 = torch.bfloat16
 
@@ -1119,15 +1120,18 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table, *,
+def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                 table: RotaryTable, *,
                  stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Rotary positions of queries and keys (K11).
 
     q [B, T, Hq, D] and k [B, T, Hk, D], bf16, fp16 or fp32 (one type, any
     strides with a unit last one); positions int64 [B, T], [1, T] or [T];
-    ``table`` a ``specfit_amd.rotary.RotaryTable`` on the same device.  Returns
+    ``table`` a ``RotaryTable`` on the same device.  Returns
     (q, k) as [B, H, T, D] contiguous.  Angles are taken in fp64, so far
     positions keep them; each output is rounded once."""
+    if not isinstance(table, RotaryTable):
+        raise TypeError("the table must be a RotaryTable")
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError("q must be bf16, fp16 or fp32")

@@ -29,6 +29,15 @@ class RotaryTable:
     factor: float
     turns: torch.Tensor
 
+    def __post_init__(self) -> None:
+        # The kernel reads rotary_dim / 2 doubles one after another.
+        t = self.turns
+        if self.rotary_dim < 2 or self.rotary_dim % 2 or self.rotary_dim > self.head_dim:
+            raise ValueError("rotary_dim must be even and at most head_dim")
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float64 \
+                or t.shape != (self.rotary_dim // 2,) or not t.is_contiguous():
+            raise ValueError(f"turns must be contiguous fp64 [{self.rotary_dim // 2}]")
+
     def to(self, device) -> "RotaryTable":
         return RotaryTable(self.head_dim, self.rotary_dim, self.interleaved, self.factor,
                            self.turns.to(device))
