@@ -154,15 +154,19 @@ class BlockKVCache:
         ops.kv_compact(self.blocks, base_kv_length, positions, end)
         self._lengths = [kept] * len(self._lengths)
 
-    def crop(self, max_length: int) -> None:
+    def crop(self, max_length: int, layer: int | None = None) -> None:
         """Drops the tokens from ``max_length`` on (negative: that many from
-        the end)."""
-        longest = max(self._lengths)
+        the end), in every layer or in one."""
+        if layer is not None and not 0 <= layer < len(self._lengths):
+            raise IndexError(f"layer {layer} of a block cache of {len(self._lengths)} layers")
+        layers = range(len(self._lengths)) if layer is None else (layer,)
+        longest = max(self._lengths[l] for l in layers)
         if max_length < 0:
             max_length = max(0, longest + max_length)
         if max_length < min(longest, self.folded_tokens):
             raise ValueError("tokens of folded blocks cannot be dropped")
-        self._lengths = [min(n, max_length) for n in self._lengths]
+        for l in layers:
+            self._lengths[l] = min(self._lengths[l], max_length)
 
     def reset(self) -> None:
         """Empties the cache."""

@@ -123,9 +123,15 @@ class Qwen3AttentionHip(nn.Module):
                 raise ValueError("a block cache is for inference (no dropout)")
             if self.sliding_window is not None:
                 raise ValueError("a block cache has no sliding window")
+            length = past_key_values.get_seq_length(self.layer_idx)
             past_key_values.append(self.layer_idx, key_states, value_states)
-            attn_output = past_key_values.attend(self.layer_idx, query_states, attention_mask,
-                                                 self.scaling)
+            try:
+                attn_output = past_key_values.attend(self.layer_idx, query_states, attention_mask,
+                                                     self.scaling)
+            except Exception:
+                # Refused (a mask that is not bool, for one): the layers keep one length.
+                past_key_values.crop(length, self.layer_idx)
+                raise
             return self.o_proj(attn_output.reshape(*input_shape, -1)), None
         if past_key_values is not None:
             key_states, value_states = past_key_values.update(key_states, value_states,
