@@ -878,6 +878,14 @@ def _dense(t: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
         return t.clone(memory_format=torch.contiguous_format)
 
 
+def _refuse_gradients(name: str, *tensors: torch.Tensor | None) -> None:
+    """Raises where an output would be cut off from inputs that want gradients."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
 class KVBlocks:
     """Device storage of a block cache (K9): for every layer, sequence and
     key/value head, ``capacity_blocks`` blocks of 64 tokens in 8 bits with a
@@ -963,7 +971,9 @@ class KVBlocks:
 def kv_append(blocks: KVBlocks, layer: int, key: torch.Tensor, value: torch.Tensor, start: int, *,
               stream: torch.cuda.Stream | None = None) -> None:
     """Writes key and value [batch, kv_heads, T, head_dim] (bf16, any strides
-    with a unit last one) as tokens start .. start + T - 1 of ``layer``."""
+    with a unit last one) as tokens start .. start + T - 1 of ``layer``.  No
+    gradients."""
+    _refuse_gradients("kv_append", key, value)
     ref = blocks._check_layer(layer)
     for name, t in (("key", key), ("value", value)):
         if not blocks._rows_fit(t):
@@ -1059,7 +1069,8 @@ def block_attention(blocks: KVBlocks, layer: int, query: torch.Tensor, keys: int
     the end of the keys.  A row that admits no key gives zeros.  Returns
     [batch, Q, Hq, head_dim] bf16.  With ``stream``, the inputs and the output
     (memory of the current stream) are the caller's to order between the two
-    streams."""
+    streams.  No gradients."""
+    _refuse_gradients("block_attention", query)
     ref = blocks._check_layer(layer)
     if not blocks._rows_fit(query):
         blocks._refuse_rows("query", query)
@@ -1129,9 +1140,10 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     strides with a unit last one); positions int64 [B, T], [1, T] or [T];
     ``table`` a ``RotaryTable`` on the same device.  Returns
     (q, k) as [B, H, T, D] contiguous.  Angles are taken in fp64, so far
-    positions keep them; each output is rounded once."""
+    positions keep them; each output is rounded once.  No gradients."""
     if not isinstance(table, RotaryTable):
         raise TypeError("the table must be a RotaryTable")
+    _refuse_gradients("rotary_embed", q, k)
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError("q must be bf16, fp16 or fp32")
@@ -1279,7 +1291,8 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
     token whose bit v % 32 of word v // 32 of allowed (int32 [V / 32 up] or
     [N, V / 32 up]) is 0 becomes -inf.  Each step is rounded to fp32, the result
     once more to the logits' type.  ``out`` may be ``logits``, and shares no memory
-    with the arguments otherwise."""
+    with the arguments otherwise.  No gradients."""
+    _refuse_gradients("adjust_logits", logits, bias)
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device \

@@ -21,7 +21,8 @@ config's attention implementation; masks are bool ones (those of sdpa and of
 the tree attention are), or None for causal.  With a rotary table
 (``install_hip_attention(model, rotary=...)``) the rotary embedding takes its
 angles from the position ids (K11), for any batch and head dim, instead of
-from the model's bf16 cosines.
+from the model's bf16 cosines.  Neither has gradients: inputs that want them are
+refused.
 """
 from __future__ import annotations
 
