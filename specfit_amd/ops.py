@@ -1263,16 +1263,26 @@ def _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, a
     return tokens
 
 
-def _spans_meet(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the bytes between the first and last elements of two tensors
-    meet."""
+def _may_share(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether two tensors may have bytes in common: the spans between their first
+    and last elements meet, and they are not columns side by side in rows of one
+    length."""
     def span(t):
         first = t.data_ptr()
         last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         return (first, first + (last + 1) * t.element_size()) if t.numel() else (0, 0)
 
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    (a0, a1), (b0, b1) = span(out), span(t)
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if out.dim() != 2 or t.dim() != 2 or out.stride(1) != 1 or t.stride(1) != 1:
+        return True
+    step = out.stride(0) * out.element_size()
+    if step <= 0 or t.stride(0) * t.element_size() != step:
+        return True
+    behind = (b0 - a0) % step
+    return behind < out.shape[1] * out.element_size() or \
+        behind + t.shape[1] * t.element_size() > step
 
 
 def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
@@ -1291,7 +1301,7 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
     token whose bit v % 32 of word v // 32 of allowed (int32 [V / 32 up] or
     [N, V / 32 up]) is 0 becomes -inf.  Each step is rounded to fp32, the result
     once more to the logits' type.  ``out`` may be ``logits``, and shares no memory
-    with the arguments otherwise.  No gradients."""
+    with the arguments otherwise (they may be columns of one buffer).  No gradients."""
     _refuse_gradients("adjust_logits", logits, bias)
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
@@ -1302,7 +1312,7 @@ def adjust_logits(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
         raise ValueError("the rows of out must not overlap")
     else:
         for t in (logits, counts, paths, bias, allowed):
-            if t is not None and _spans_meet(out, t) and not (
+            if t is not None and _may_share(out, t) and not (
                     t is logits and t.data_ptr() == out.data_ptr() and t.stride() == out.stride()):
                 raise ValueError("out must be logits or share no memory with the arguments")
     _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, out, False,
