@@ -500,8 +500,9 @@ int sf_kv_read(const sf_kv_cache *cache, int64_t start, int tokens, void *k,
  * K10: grouped-query attention over a block cache of `keys` tokens:
  *   out[b, qi, qh, :] = sum_s p_s * v^[b, h, s, :],
  *   p = softmax over admitted keys s of scale * (q[b, qi, qh, :] . k^[b, h, s, :])
- * h = qh / (q_heads / kv_heads), scores and sums in fp32, p rounded to bf16
- * for the product with v^, the result rounded to bf16 once.  The mask
+ * h = qh / (q_heads / kv_heads), scores and sums in fp32, the result rounded to bf16
+ * once; for the product with v^, p is kept to 2^-16 of itself where a workgroup takes 16
+ * rows (sf_block_attention_rows), and rounded to bf16 where it takes 256.  The mask
  * covers the last mask_keys keys; a key before them is admitted by every row.
  * With mask == NULL key s is admitted when s <= keys - queries + qi.  A row that
  * admits no key gets zeros, and only such a row: one with an admitted score of NaN or

@@ -320,11 +320,11 @@ struct Rows {
 
   // The n-th pair of scores to weights times the value scale, as bf16 into w (the
   // B operands of the values' product, in the order of the lane's scores), and
-  // added to sum.
+  // added to sum; returns the weights themselves.
   static constexpr int kPairs = Sh::kScoreTiles * kN / 2;
-  static __device__ __forceinline__ void weigh_pair(const Acc (&s)[Sh::kScoreTiles], int n,
-                                                    float mul, float base, float (&sum)[2],
-                                                    sf_u32x4 (&w)[Sh::kPSteps]) {
+  static __device__ __forceinline__ float2 weigh_pair(const Acc (&s)[Sh::kScoreTiles], int n,
+                                                      float mul, float base, float (&sum)[2],
+                                                      sf_u32x4 (&w)[Sh::kPSteps]) {
     const float p0 =
         __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * n / kN][2 * n % kN], mul, base));
     const float p1 =
@@ -332,6 +332,7 @@ struct Rows {
     sum[0] += p0;
     sum[1] += p1;
     w[n / 4][n % 4] = sf_pack_bf16(p0, p1);
+    return make_float2(p0, p1);
   }
   __device__ __forceinline__ void add_sum(const float (&sum)[2], float v_scale) {
     // 1 / v_scale, a power of two.
@@ -356,11 +357,22 @@ struct Rows {
     if (m == -INFINITY && count > 0.f) m = kLowest;
   }
 
+  // All of a tile's weights, in two terms: w, and what its rounding to bf16 left, also
+  // as bf16 (2^-16 of a weight is lost, where w alone loses up to 2^-8).
   __device__ __forceinline__ void softmax(Acc (&s)[Sh::kScoreTiles], float factor, float v_scale,
-                                          sf_u32x4 (&w)[Sh::kPSteps]) {
+                                          sf_u32x4 (&w)[Sh::kPSteps],
+                                          sf_u32x4 (&rest)[Sh::kPSteps]) {
     float mul, base;
     raise(s, top(s), factor, v_scale, mul, base);
-    weigh(s, mul, base, v_scale, w);
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < kPairs; ++n) {
+      const float2 p = weigh_pair(s, n, mul, base, sum, w);
+      const uint32_t pair = w[n / 4][n % 4];
+      rest[n / 4][n % 4] = sf_pack_bf16(p.x - __uint_as_float(pair << 16),
+                                        p.y - __uint_as_float(pair & 0xffff0000u));
+    }
+    add_sum(sum, v_scale);
   }
 };
 
@@ -561,6 +573,12 @@ __device__ __forceinline__ void add_special(Rows<D, ROWS>& r, const Args& a, int
 // product of a library reaches 1150).  Without the exponentials it is 5% less,
 // without the staging 14%.  Two groups of 32 rows per wavefront, for half of the
 // reads of LDS, spill: 2150 us.
+//
+// Probabilities meet the values as bf16, so that a row's error is 0.0023 of its norm
+// against 64 bits where 0.0017 are the result's own rounding (e4m3 codes of the values
+// are off by up to 2^-4).  What their rounding left, as a second product (the direct
+// kernel has it), would cost about a quarter more: 594 -> 729 us here, 165 -> 195 for
+// 128 nodes after 32777 tokens, with the products alone.
 template <int D, int HELD, bool MASK>
 __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kernel(const Args a) {
   using Sh = Shape<D, 32>;
@@ -837,7 +855,11 @@ __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kern
 // LDS, no barrier).  Decoding long contexts is bound by the cache's bytes
 // (131072 int8 keys of 4 heads of 128: 24 us, 5.6 TB/s), short calls by
 // latency (5 us for one tile per wavefront), trees by the conversions of codes
-// and the softmax (0.23 us per tile and CU).
+// and the softmax (0.23 us per tile and CU).  The matrix unit has room for
+// probabilities in two terms, so that a row's error is the rounding of the result
+// (0.0016 - 0.0017 of its norm; 0.0019 - 0.0024 with one term): append and attention
+// of 131072 keys 34.6 -> 35.1 us, of 16 padded sequences 20.5 -> 21.2, of a tree of 61
+// nodes 16.4 both ways.
 template <int D, int HELD, bool MASK>
 __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kernel(const Args a) {
   constexpr int ROWS = kDirectRows;
@@ -944,8 +966,8 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
     }
     __builtin_amdgcn_sched_barrier(0);  // keep conversions next to their products
     admit.restrict_scores(s, lane, tile * kBlockTokens);
-    sf_u32x4 w[Sh::kPSteps];
-    r.softmax(s, factor, scale_v, w);
+    sf_u32x4 w[Sh::kPSteps], rest[Sh::kPSteps];
+    r.softmax(s, factor, scale_v, w, rest);
     __builtin_amdgcn_sched_barrier(0);
     auto add_values = [&](auto finite) {
 #pragma unroll
@@ -954,8 +976,12 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
         for (int p = 0; p < kValuePairs; ++p) {
           sf_u32x4 x, y;
           sf_codes_frags<HELD>(vr[t * kValuePairs + p], x, y);
-          r.acc[t] = Sh::mma(finite(x), w[2 * p], r.acc[t]);
-          r.acc[t] = Sh::mma(finite(y), w[2 * p + 1], r.acc[t]);
+          x = finite(x);
+          y = finite(y);
+          r.acc[t] = Sh::mma(x, w[2 * p], r.acc[t]);
+          r.acc[t] = Sh::mma(y, w[2 * p + 1], r.acc[t]);
+          r.acc[t] = Sh::mma(x, rest[2 * p], r.acc[t]);
+          r.acc[t] = Sh::mma(y, rest[2 * p + 1], r.acc[t]);
         }
     };
     if (flag & kFlagValue)
@@ -989,14 +1015,17 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
 #pragma unroll
       for (int k = 0; k < Sh::kPSteps; ++k) v16[t][k] = sf_ld16(vp + 16 * Sh::value_piece16(t, k));
     admit.restrict_scores(s, lane, tile * kBlockTokens);
-    sf_u32x4 w[Sh::kPSteps];
-    r.softmax(s, a.scale_log2, 1.f, w);
+    sf_u32x4 w[Sh::kPSteps], rest[Sh::kPSteps];
+    r.softmax(s, a.scale_log2, 1.f, w, rest);
     auto add_values = [&](auto finite) {
 #pragma unroll
       for (int t = 0; t < Sh::kOutTiles; ++t)
 #pragma unroll
-        for (int k = 0; k < Sh::kPSteps; ++k)
-          r.acc[t] = Sh::mma(finite(v16[t][k]), w[k], r.acc[t]);
+        for (int k = 0; k < Sh::kPSteps; ++k) {
+          const sf_u32x4 x = finite(v16[t][k]);
+          r.acc[t] = Sh::mma(x, w[k], r.acc[t]);
+          r.acc[t] = Sh::mma(x, rest[k], r.acc[t]);
+        }
     };
     if (flag)
       add_values([](const sf_u32x4& x) { return entries<false>(x, 3); });

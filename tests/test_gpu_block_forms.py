@@ -250,3 +250,24 @@ def test_a_row_keeps_its_bits_beside_very_large_scores(device, case):
         out = cache.attend(0, p.to(device)).cpu()
         keep = ~loud.transpose(1, 2)
         assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("held", ("e4m3", "int8"))
+@pytest.mark.parametrize("case", ((1, 8, 2, 64, 1, 3), (4, 8, 2, 128, 1, 9), (2, 16, 4, 128, 5, 20),
+                                  (2, 8, 4, 64, 30, 70), (2, 64, 4, 128, 9, 300)), ids=_name)
+def test_weights_of_the_direct_form(device, case, held):
+    """Kept to 2^-16 of themselves (two bf16 terms of half steps 2^-8 each), where one
+    term would lose 2^-8; beside it S sums of up to a step, 2^-23, of the values' sizes."""
+    assert form_of(case)[0] == 16
+    B, Hq, H, D, Q, S = case
+    g = torch.Generator().manual_seed(S)
+    q, k, v = _inputs(case, g)
+    folded = (S - 1) // 64
+    scale = D ** -0.5
+    out = _cache(device, case, k, v, held, folded).attend(0, q.to(device), None, scale)
+    kk, vv = (held_rows(t, folded, held) for t in (k, v))
+    want, bound = attention(q, kk, vv, None, scale)
+    size, _ = attention(q, kk, vv.abs(), None, scale)
+    bound = bound - (2.0 ** -8 - 2.0 ** -16 - S * 2.0 ** -23) * size
+    worst = ((out.cpu().double() - want).abs() / bound).max().item()
+    assert worst <= 1.0, worst
