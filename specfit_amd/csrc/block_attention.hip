@@ -398,6 +398,23 @@ __device__ __forceinline__ sf_u32x4 entries(const sf_u32x4& v, int kind) {
   return r;
 }
 
+// A piece of codes with zeros for those that stand for NaN.
+template <int HELD>
+__device__ __forceinline__ sf_u32x4 finite_codes(const sf_u32x4& v) {
+  sf_u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t y = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = (v[j] >> (8 * i)) & 0xffu;
+      if (HELD == SF_KV_INT8 ? x != 0x80u : (x & 0x7fu) != 0x7fu) y |= x << (8 * i);
+    }
+    r[j] = y;
+  }
+  return r;
+}
+
 // What a lane needs to restrict the scores of a tile: its mask's bytes, loaded
 // with the tile's keys, or the keys that its row sees without a mask.
 template <typename Sh, bool MASK>
@@ -969,25 +986,24 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
     sf_u32x4 w[Sh::kPSteps], rest[Sh::kPSteps];
     r.softmax(s, factor, scale_v, w, rest);
     __builtin_amdgcn_sched_barrier(0);
-    auto add_values = [&](auto finite) {
+    if (flag & kFlagValue) {  // in place: a second copy of the products takes registers
 #pragma unroll
-      for (int t = 0; t < Sh::kOutTiles; ++t)
+      for (int n = 0; n < kPieces; ++n) {
+        vr[n] = finite_codes<HELD>(vr[n]);
+        pin(vr[n]);
+      }
+    }
 #pragma unroll
-        for (int p = 0; p < kValuePairs; ++p) {
-          sf_u32x4 x, y;
-          sf_codes_frags<HELD>(vr[t * kValuePairs + p], x, y);
-          x = finite(x);
-          y = finite(y);
-          r.acc[t] = Sh::mma(x, w[2 * p], r.acc[t]);
-          r.acc[t] = Sh::mma(y, w[2 * p + 1], r.acc[t]);
-          r.acc[t] = Sh::mma(x, rest[2 * p], r.acc[t]);
-          r.acc[t] = Sh::mma(y, rest[2 * p + 1], r.acc[t]);
-        }
-    };
-    if (flag & kFlagValue)
-      add_values([](const sf_u32x4& x) { return entries<HELD == SF_KV_INT8>(x, 3); });
-    else
-      add_values([](const sf_u32x4& x) { return x; });
+    for (int t = 0; t < Sh::kOutTiles; ++t)
+#pragma unroll
+      for (int p = 0; p < kValuePairs; ++p) {
+        sf_u32x4 x, y;
+        sf_codes_frags<HELD>(vr[t * kValuePairs + p], x, y);
+        r.acc[t] = Sh::mma(x, w[2 * p], r.acc[t]);
+        r.acc[t] = Sh::mma(y, w[2 * p + 1], r.acc[t]);
+        r.acc[t] = Sh::mma(x, rest[2 * p], r.acc[t]);
+        r.acc[t] = Sh::mma(y, rest[2 * p + 1], r.acc[t]);
+      }
     special |= flag;
     if (tile + kDirectWaves < end8) load_values(tile + kDirectWaves);
   }
@@ -1017,20 +1033,22 @@ __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kern
     admit.restrict_scores(s, lane, tile * kBlockTokens);
     sf_u32x4 w[Sh::kPSteps], rest[Sh::kPSteps];
     r.softmax(s, a.scale_log2, 1.f, w, rest);
-    auto add_values = [&](auto finite) {
+    if (flag) {
 #pragma unroll
       for (int t = 0; t < Sh::kOutTiles; ++t)
 #pragma unroll
         for (int k = 0; k < Sh::kPSteps; ++k) {
-          const sf_u32x4 x = finite(v16[t][k]);
-          r.acc[t] = Sh::mma(x, w[k], r.acc[t]);
-          r.acc[t] = Sh::mma(x, rest[k], r.acc[t]);
+          v16[t][k] = entries<false>(v16[t][k], 3);
+          pin(v16[t][k]);
         }
-    };
-    if (flag)
-      add_values([](const sf_u32x4& x) { return entries<false>(x, 3); });
-    else
-      add_values([](const sf_u32x4& x) { return x; });
+    }
+#pragma unroll
+    for (int t = 0; t < Sh::kOutTiles; ++t)
+#pragma unroll
+      for (int k = 0; k < Sh::kPSteps; ++k) {
+        r.acc[t] = Sh::mma(v16[t][k], w[k], r.acc[t]);
+        r.acc[t] = Sh::mma(v16[t][k], rest[k], r.acc[t]);
+      }
     special |= flag;
   }
   if (special)
