@@ -142,13 +142,14 @@ __device__ __forceinline__ uint32_t admitted(const uint8_t* row, int key, int ma
   return w;
 }
 
-// The shapes of the two direct forms.  Both read the same pieces: the key of a
-// row of the A operand and the contraction's order of d are free, as long as
-// queries, scores and values agree on them.
+// The shapes of the matrix instructions: 32 rows in the staged kernel, 16 in the
+// direct one.  Both read the same pieces: the key of a row of the A operand and the
+// contraction's order of d are free, as long as queries, scores and values agree on
+// them.
 template <int D, int ROWS>
 struct Shape;
 
-// v_mfma_f32_32x32x16_bf16: kScores registers hold, for query row lane % 32,
+// v_mfma_f32_32x32x16_bf16: the 32 scores of a lane are, for query row lane % 32,
 // keys 8 g + 4 (lane / 32) + i of the tile in register 4 g + i.
 template <int D>
 struct Shape<D, 32> {
@@ -586,7 +587,7 @@ __device__ __forceinline__ void add_special(Rows<D, ROWS>& r, const Args& a, int
 // i - 1).
 //
 // Bound by the matrix unit at the clock that its power allows: 2048 e4m3 queries
-// after 16000 keys, 32 heads of 128, take 605 us, 940 TFLOP/s (a large matrix
+// after 16000 keys, 32 heads of 128, take 595 - 605 us, 940 TFLOP/s (a large matrix
 // product of a library reaches 1150).  Without the exponentials it is 5% less,
 // without the staging 14%.  Two groups of 32 rows per wavefront, for half of the
 // reads of LDS, spill: 2150 us.
@@ -594,8 +595,8 @@ __device__ __forceinline__ void add_special(Rows<D, ROWS>& r, const Args& a, int
 // Probabilities meet the values as bf16, so that a row's error is 0.0023 of its norm
 // against 64 bits where 0.0017 are the result's own rounding (e4m3 codes of the values
 // are off by up to 2^-4).  What their rounding left, as a second product (the direct
-// kernel has it), would cost about a quarter more: 594 -> 729 us here, 165 -> 195 for
-// 128 nodes after 32777 tokens, with the products alone.
+// kernel has it), costs a third more: 602 -> 833 us here, 165 -> 212 for 128 nodes after
+// 32777 tokens (729 and 195 by its matrix instructions alone).
 template <int D, int HELD, bool MASK>
 __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kernel(const Args a) {
   using Sh = Shape<D, 32>;
@@ -867,16 +868,16 @@ __global__ __launch_bounds__(kStagedThreads, 1) void block_attention_staged_kern
 }
 
 // The form of few rows: 16 rows per workgroup, whose eight wavefronts take every
-// eighth tile and merge their states in LDS.  Operands go straight from the
-// cache into registers, whose order is that of the matrix instructions (no
-// LDS, no barrier).  Decoding long contexts is bound by the cache's bytes
-// (131072 int8 keys of 4 heads of 128: 24 us, 5.6 TB/s), short calls by
-// latency (5 us for one tile per wavefront), trees by the conversions of codes
-// and the softmax (0.23 us per tile and CU).  The matrix unit has room for
+// eighth tile and merge their states in LDS.  Until then operands go straight from
+// the cache into registers, whose order is that of the matrix instructions: the
+// loop over tiles needs no LDS and no barrier.  Decoding long contexts is bound by
+// the cache's bytes (131072 int8 keys of 4 heads of 128: 25 us, 5.4 TB/s), short calls
+// by latency (5.3 us for one tile per wavefront), trees by the conversions of codes
+// and the softmax (10.2 us for 61 nodes after 1024).  The matrix unit has room for
 // probabilities in two terms, so that a row's error is the rounding of the result
-// (0.0016 - 0.0017 of its norm; 0.0019 - 0.0024 with one term): append and attention
-// of 131072 keys 34.6 -> 35.1 us, of 16 padded sequences 20.5 -> 21.2, of a tree of 61
-// nodes 16.4 both ways.
+// (0.0016 - 0.0017 of its norm; 0.0019 - 0.0022 with one term).  Kernel times with one
+// and with two: 131072 keys 26.3 and 26.6 us, the tree 8.7 and 9.5, 512 tokens of 32 / 4
+// heads of 128 18.7 and 19.1, 2000 after 4000 of 16 / 4 heads of 64 80 and 94.
 template <int D, int HELD, bool MASK>
 __global__ __launch_bounds__(kDirectThreads, 1) void block_attention_direct_kernel(const Args a) {
   constexpr int ROWS = kDirectRows;
@@ -1230,9 +1231,11 @@ struct Plan {
 //   staged  rounds (8 + 2.45 tiles)          (8 + 1.6 tiles)
 //   splits  the partial states (fp32) at 4.5 MB / us, written and read, and 3 for
 //           the second kernel
-// e.g. at 32 / 4 heads of 128, direct / staged: a 61-node tree after 1024 tokens 9.4 /
-// 20 us (split), 160 nodes after 8000 92 / 52 (split), a prompt of 512 tokens 20 / 26,
-// 1024 46 / 45, 2048 128 / 86; 2000 tokens after 4000 at 16 / 4 heads of 64 85 / 114.
+// The direct figures are from probabilities in one term (the second adds 2 - 9%, for
+// heads of 64 up to 17%).  As the kernels are, in e4m3 at 32 / 4 heads of 128, direct / staged:
+// a 61-node tree after 1024 tokens 9.5 / 19 us (split), 160 nodes after 8000 70 / 48
+// (split), a prompt of 512 tokens 19 / 23, 1024 45 / 43, 2048 120 / 79; of 64: a prompt of
+// 1000 21 / 30, 4000 168 / 112; 2000 tokens after 4000 at 16 / 4 heads of 64 93 / 91.
 // tiles: of the longest row tile where there is one round, on average where there
 // are more (as under the causal rule).
 Plan plan_of(int heads, int group, int queries, int keys, int head_dim) {

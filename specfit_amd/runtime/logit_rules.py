@@ -23,7 +23,10 @@ class LogitRules:
                 that occurred
     presence    taken off every token that occurred
     frequency   taken off for each occurrence
-    bias        fp32 [vocab] or [rows, vocab], added to every token"""
+    bias        fp32 [vocab] or [rows, vocab], added to every token
+
+    All penalties go by the same occurrences; for others, ``adjust`` with two
+    rules in turn (on fp32 logits, so that nothing is rounded in between)."""
 
     counts: torch.Tensor | None = None
     repetition: float = 1.0
