@@ -7,26 +7,21 @@ import math
 import pytest
 import torch
 
-from specfit_amd import ops
+from _block_forms import ONE_OF_EACH
 from specfit_amd.runtime import BlockKVCache
 
 pytestmark = pytest.mark.gpu
 
-# batch, query heads, KV heads, D, queries, keys, splits
-CASES = [
-    (1, 8, 2, 128, 1, 27, 1), (1, 8, 2, 128, 1, 65, 1), (1, 8, 2, 64, 1, 129, 1),
-    (1, 4, 2, 64, 30, 30, 1), (2, 8, 2, 128, 61, 500, 1),   # 16 rows to a workgroup
-    (1, 8, 2, 64, 1, 9001, 18), (1, 32, 1, 128, 64, 2000, 2),
-    (8, 64, 4, 128, 32, 32, 1), (3, 256, 1, 64, 32, 32, 1), (4, 32, 4, 128, 256, 256, 1),
-    (1, 32, 4, 128, 300, 2300, 6),                          # 256 rows to a workgroup
-]
-IDS = ["x".join(map(str, c[:6])) for c in CASES]
+# batch, query heads, KV heads, D, queries, keys
+CASES = [(1, 8, 2, 128, 1, 27), (1, 8, 2, 128, 1, 65), (1, 8, 2, 64, 1, 129), (1, 4, 2, 64, 30, 30),
+         (2, 8, 2, 128, 61, 500), (1, 32, 1, 128, 64, 2000), (8, 64, 4, 128, 32, 32),
+         (3, 256, 1, 64, 32, 32), (4, 32, 4, 128, 256, 256), (1, 32, 4, 128, 300, 2300)]
+CASES += [c for c in ONE_OF_EACH.values() if c not in CASES]
+IDS = ["x".join(map(str, c)) for c in CASES]
 
 
 def _inputs(case, seed=0):
-    B, Hq, H, D, Q, S, splits = case
-    work = ops._block_attention_workspace(B, Q, S, Hq, H, D)
-    assert work == (0 if splits == 1 else splits * B * Hq * Q * (D + 2) * 4)
+    B, Hq, H, D, Q, S = case
     g = torch.Generator().manual_seed(seed)
     return [torch.randn((B, h, n, D), generator=g).to(torch.bfloat16)
             for h, n in ((Hq, Q), (H, S), (H, S))]
@@ -34,7 +29,7 @@ def _inputs(case, seed=0):
 
 def _attend(device, case, q, k, v, mask=None, held="e4m3"):
     """The last token is in bf16, and so are those of its block."""
-    B, _, H, D, _, S, _ = case
+    B, _, H, D, _, S = case
     cache = BlockKVCache(1, H, D, S, batch=B, held=held, tail_tokens=S, device=device)
     folded = (S - 1) // 64 * 64
     if folded:
@@ -53,7 +48,7 @@ def _check(out, clean, bad):
 @pytest.mark.parametrize("masked", (False, True))
 @pytest.mark.parametrize("case", CASES, ids=IDS)
 def test_nan_queries(device, case, masked):
-    B, Hq, _, _, Q, S, _ = case
+    B, Hq, _, _, Q, S = case
     q, k, v = _inputs(case)
     g = torch.Generator().manual_seed(1)
     mask = None
@@ -75,7 +70,7 @@ def test_nan_queries(device, case, masked):
 @pytest.mark.parametrize("case", CASES, ids=IDS)
 def test_a_nan_key(device, case, where, held):
     """In every mask's reach (causal), and as the only key of some rows."""
-    B, Hq, H, _, Q, S, _ = case
+    B, Hq, H, _, Q, S = case
     q, k, v = _inputs(case)
     place = 0 if where == "first" else S - 1
     k[-1, -1, place, 5] = 0.0  # the block's scale is that of its finite values
@@ -104,7 +99,7 @@ def test_a_nan_key(device, case, where, held):
 def test_scores_of_minus_infinity(device, case):
     """A key whose score is -inf counts for nothing beside others; a row that
     admits no others has no softmax."""
-    B, Hq, H, _, Q, S, _ = case
+    B, Hq, H, _, Q, S = case
     q, k, v = _inputs(case)
     q[..., 0] = q[..., 0].abs() + 1
     damaged = k.clone()

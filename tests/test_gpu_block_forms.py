@@ -6,20 +6,16 @@ import math
 import pytest
 import torch
 
-from _block_forms import CASES, form_of
+from _block_forms import CASES, ONE_OF_EACH, form_of, splits_of
 from _block_reference import attention, held_rows
 from specfit_amd import ops
 from specfit_amd.runtime import BlockKVCache
 
 pytestmark = pytest.mark.gpu
 
-NAMES = ["x".join(map(str, c)) for c in CASES]
-STAGED = [c for c, f in CASES.items() if f[0] == 256]
-STAGED_SPLIT = [c for c in STAGED if CASES[c][1] > 1]
-# One of each kernel and way of merging.
-FEW = [(8, 128, 2, 128, 17, 77), (3, 64, 1, 64, 200, 200), (5, 16, 4, 128, 333, 833),
-       (3, 32, 1, 64, 300, 4300), (1, 128, 2, 128, 17, 6017), (2, 64, 4, 128, 9, 300),
-       (1, 8, 2, 64, 1, 9001), (1, 32, 1, 128, 64, 2000)]
+EACH = list(ONE_OF_EACH.values())
+ALL = CASES + [c for c in EACH if c not in CASES]
+SPLIT = [c for c in ALL if splits_of(c) > 1]
 
 
 def _name(case):
@@ -79,10 +75,9 @@ def _check(out, q, k, v, mask, scale):
 @pytest.mark.parametrize("kind,held,part", [
     ("causal", "e4m3", "all"), ("causal", "int8", "none"), ("tree", "int8", "all"),
     ("tree", "e4m3", "half"), ("padded", "e4m3", "all"), ("rows", "int8", "half")])
-@pytest.mark.parametrize("case", CASES, ids=NAMES)
+@pytest.mark.parametrize("case", ALL, ids=_name)
 def test_forms(device, case, kind, held, part):
     """``part``: of the complete blocks before the last tokens, in 8 bits."""
-    assert form_of(case) == CASES[case]
     B, Hq, H, D, Q, S = case
     g = torch.Generator().manual_seed(Q + S)
     q, k, v = _inputs(case, g)
@@ -109,7 +104,7 @@ def test_forms(device, case, kind, held, part):
 
 
 @pytest.mark.parametrize("held", ("e4m3", "int8"))
-@pytest.mark.parametrize("case", FEW, ids=_name)
+@pytest.mark.parametrize("case", EACH, ids=_name)
 def test_values_that_are_not_finite(device, case, held):
     """In a folded block, in the last block and in the first: NaN where the codes hold
     them, as they are in bf16; only in the element and the rows that admit the key."""
@@ -135,7 +130,7 @@ def test_values_that_are_not_finite(device, case, held):
 
 
 @pytest.mark.parametrize("scale", (0.0, -0.3, 40.0))
-@pytest.mark.parametrize("case", FEW, ids=_name)
+@pytest.mark.parametrize("case", EACH, ids=_name)
 def test_scales_of_the_scores(device, case, scale):
     B, Hq, H, D, Q, S = case
     g = torch.Generator().manual_seed(S)
@@ -146,7 +141,7 @@ def test_scales_of_the_scores(device, case, scale):
     _check(out[-1:, :, -1:], q[-1:, -1:], kk, vv, None, scale)
 
 
-@pytest.mark.parametrize("case", [c for c in FEW if CASES[c][0] == 256], ids=_name)
+@pytest.mark.parametrize("case", EACH, ids=_name)
 def test_blocks_of_very_different_scales(device, case):
     """Value scales change from block to block by up to 2^40, key scales by 2^10."""
     B, Hq, H, D, Q, S = case
@@ -184,7 +179,7 @@ def test_layouts(device, case, kind):
         assert torch.equal(got, cache.attend(0, q.to(device), whole.to(device)))
 
 
-@pytest.mark.parametrize("case", STAGED_SPLIT, ids=_name)
+@pytest.mark.parametrize("case", SPLIT, ids=_name)
 def test_without_room_for_scratch(device, case, monkeypatch):
     """The same keys in one piece: the result moves by roundings only."""
     B, Hq, H, D, Q, S = case
@@ -198,8 +193,7 @@ def test_without_room_for_scratch(device, case, monkeypatch):
     _check(out[-1:, :, -1:], q[-1:, -1:], kk, vv, None, D ** -0.5)
 
 
-@pytest.mark.parametrize("case", ((5, 32, 4, 128, 130, 260), (5, 16, 4, 128, 333, 833),
-                                  (1, 128, 2, 64, 17, 20017)), ids=_name)
+@pytest.mark.parametrize("case", EACH, ids=_name)
 def test_captured_repeated_and_on_two_streams(device, case):
     B, Hq, H, D, Q, S = case
     g = torch.Generator().manual_seed(12)
@@ -234,7 +228,7 @@ def test_captured_repeated_and_on_two_streams(device, case):
         assert all(torch.equal(o, want[i]) for o in outs[i])
 
 
-@pytest.mark.parametrize("case", FEW, ids=_name)
+@pytest.mark.parametrize("case", EACH, ids=_name)
 def test_a_row_keeps_its_bits_beside_very_large_scores(device, case):
     """Scores of other rows, up to 2^40 and infinite, change nothing in a row."""
     B, Hq, H, D, Q, S = case
@@ -253,12 +247,13 @@ def test_a_row_keeps_its_bits_beside_very_large_scores(device, case):
 
 
 @pytest.mark.parametrize("held", ("e4m3", "int8"))
-@pytest.mark.parametrize("case", ((1, 8, 2, 64, 1, 3), (4, 8, 2, 128, 1, 9), (2, 16, 4, 128, 5, 20),
-                                  (2, 8, 4, 64, 30, 70), (2, 64, 4, 128, 9, 300)), ids=_name)
+@pytest.mark.parametrize("case", [c for c in ((1, 8, 2, 64, 1, 3), (4, 8, 2, 128, 1, 9),
+                                              (2, 16, 4, 128, 5, 20), (2, 8, 4, 64, 30, 70),
+                                              (2, 64, 4, 128, 9, 300)) if form_of(c)[0] == 16],
+                         ids=_name)
 def test_weights_of_the_direct_form(device, case, held):
     """Kept to 2^-16 of themselves (two bf16 terms of half steps 2^-8 each), where one
     term would lose 2^-8; beside it S sums of up to a step, 2^-23, of the values' sizes."""
-    assert form_of(case)[0] == 16
     B, Hq, H, D, Q, S = case
     g = torch.Generator().manual_seed(S)
     q, k, v = _inputs(case, g)
