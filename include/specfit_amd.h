@@ -48,6 +48,12 @@
  *                        compaction (eagle3_tree.py:833-858), held in 8 bits,
  *                        and the attention over it
  *   sf_rotary            apply_rotary_pos_emb with angles from the positions
+ *   sf_mx_quantize, sf_mx_values, sf_mx_linear, sf_mx_grouped_swiglu
+ *                        the model's linear layers and experts
+ *                        (qwen3_offloaded_experts.py:38-62) with weights held
+ *                        in microscaled 4 bits
+ *   sf_add_rms_norm      the residual's addition and the norm behind it, of a
+ *                        decoder layer
  *   sf_logit_rules       the argmax of eagle3_tree.py:1241-1290 with rules on
  *                        the logits before it
  */
@@ -588,6 +594,93 @@ int sf_logit_rules(int dtype, const void *logits, int64_t logits_stride,
                    int64_t allowed_stride, void *out, int64_t out_stride,
                    int64_t *tokens, void *workspace, int64_t workspace_bytes,
                    sf_stream_t stream);
+
+/*
+ * K13: microscaled values.  32 neighbours of a row share the scale 2^e, held
+ * as the byte e + 127, e the least integer from -127 up at which no value
+ * rounds past the type's largest; values are rounded to nearest, ties to even.
+ * A block with an infinity or a NaN has the byte 255 and reads as NaN.
+ * With tiles = ceil(dim / 128), quads = ceil(dim / 512):
+ *   held 0  rows in e4m3: codes [rows, tiles * 128] (zeros behind the row's
+ *           end), scales [rows, quads * 16], the byte of block b (0..3) of tile
+ *           t at t / 4 * 16 + b * 4 + t % 4
+ *   held 1  a weight in e2m1: codes [R][tiles][4][16][16] with R = 2 * ceil(rows /
+ *           32): 16 bytes of block b and row r of row tile and tile, the first of
+ *           two values in the low half; scales [R][quads][4][16][4], the
+ *           byte of tile t in t % 4; rows behind the last are zeros
+ * Bytes of the last quad's missing tiles are neither written nor read.
+ *   dtype       0 bf16, 1 fp16, 2 fp32
+ *   x           [rows, dim], row stride row_stride; batch of them (held 1 only)
+ *               at batch_stride elements, the outputs at codes_batch_stride and
+ *               scales_batch_stride bytes
+ * codes 16-byte and scales 4-byte aligned.  dim <= 2^30.
+ */
+int sf_mx_quantize(int dtype, const void *x, int64_t row_stride,
+                   int64_t batch_stride, int rows, int dim, int batch,
+                   int held, void *codes, int64_t codes_batch_stride,
+                   void *scales, int64_t scales_batch_stride,
+                   sf_stream_t stream);
+
+/* The values held, to out [rows, dim] (contiguous, dtype as above). */
+int sf_mx_values(int held, const void *codes, const void *scales, int rows,
+                 int dim, int dtype, void *out, sf_stream_t stream);
+
+/*
+ * K14: the residual's addition and RMSNorm, with an 8-bit output.
+ *   s = x + residual                   rounded to dtype (x without a residual)
+ *   y = s * r * weight                 fp32; r = fp32(1 / sqrt(mean(s^2) + eps)),
+ *                                      the mean in 64 bits
+ *   sum = s, normed = y rounded to dtype, codes and scales = y in e4m3 (K13)
+ * x and residual [rows, dim] with row strides; the outputs contiguous, each of
+ * them NULL if not wanted (sum needs a residual; codes and scales go together).
+ */
+int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
+                    const void *residual, int64_t residual_stride, int rows,
+                    int dim, const void *weight, double eps, void *sum,
+                    void *normed, void *codes, void *scales,
+                    sf_stream_t stream);
+
+/*
+ * K15: out[m, n] = T(sum_k x[m, k] w[n, k] + bias[n]), fp32 sums.
+ *   x_dtype   3: rows in e4m3 (K13), x_scales theirs; 0 bf16 or 1 fp16: at most
+ *             16 rows of row stride x_stride, rounded to e4m3 here (dim and
+ *             x_stride multiples of 8)
+ *   codes, scales   a weight in e2m1 [out_features, dim]
+ *   bias      [out_features] of out_dtype, or NULL
+ *   out_dtype 0 bf16, 1 fp16; out has row stride out_stride
+ * x 16-byte, codes 16-byte, scales and x_scales 4-byte aligned.
+ */
+int sf_mx_linear(int x_dtype, const void *x, const void *x_scales,
+                 int64_t x_stride, int rows, int dim, const void *codes,
+                 const void *scales, int out_features, const void *bias,
+                 int out_dtype, void *out, int64_t out_stride,
+                 sf_stream_t stream);
+
+/*
+ * K16: K3 with the experts' weights in microscaled 4 bits, over every expert
+ * e < num_experts that has rows and, with a table, slot_of_expert[e] >= 0.
+ *   a       = e4m3(silu(x[t] . gate^T) * (x[t] . up^T))        fp32 up to a
+ *   rows[r] = bf16((a . down^T) * route_weights[perm_pos[r]])
+ *   x_dtype         as sf_mx_linear (0: at most 16 tokens)
+ *   slots           records of sf_mx_expert_bytes at slot_stride bytes: the codes
+ *                   of gate [I, H], up [I, H], down [H, I] and then their
+ *                   scales (held 1), at the byte offsets that
+ *                   sf_mx_expert_parts writes (6)
+ *   slot_of_expert  device int32 [num_experts], or NULL: expert e in slot e
+ *   act, act_scales scratch: rows in e4m3 [tokens * top_k, intermediate_size]
+ *   out_rows        bf16 [tokens * top_k, hidden_size]
+ * slots and slot_stride 16-byte, out_rows 8-byte aligned.
+ */
+int64_t sf_mx_expert_bytes(int hidden_size, int intermediate_size);
+int sf_mx_expert_parts(int hidden_size, int intermediate_size, int64_t *offsets);
+int sf_mx_grouped_swiglu(int x_dtype, const void *x, const void *x_scales,
+                         int64_t x_stride, const int32_t *perm_pos,
+                         const int32_t *offsets, const void *route_weights,
+                         int tokens, int top_k, int hidden_size,
+                         int intermediate_size, int num_experts,
+                         const int32_t *slot_of_expert, const void *slots,
+                         int64_t slot_stride, void *act, void *act_scales,
+                         void *out_rows, sf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -22,7 +22,7 @@ OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ("abi.hip", "router.hip", "dispatch.hip", "swiglu.hip", "combine.hip",
            "attention.hip", "norm.hip", "codec.hip", "kv_blocks.hip", "block_attention.hip",
-           "rotary.hip", "logits.hip")
+           "rotary.hip", "logits.hip", "mx_quantize.hip", "mx_linear.hip", "mx_experts.hip")
 
 HIPCC_FLAGS = (
     f"--offload-arch={OFFLOAD_ARCH}",

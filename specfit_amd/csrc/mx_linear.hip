@@ -1,0 +1,145 @@
+// K15: rows times a weight in microscaled 4 bits,
+//   out[m, n] = T(sum_k x[m, k] w[n, k] + bias[n]),
+// x in e4m3 (rounded here where rows come in 16 bits), w in e2m1.  Products are
+// exact, the matrix unit adds a block's in its own fixed order and width and
+// accumulates in fp32.
+#include "mx_product.h"
+
+namespace {
+
+using namespace sf_mx;
+
+constexpr int kThreads = 256, kWaves = kThreads / SF_WAVE;
+
+struct Linear {
+  const void* x;
+  const uint8_t* x_scales;
+  int64_t x_stride;
+  int rows, dim, out_features;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const void* bias;
+  int out_dtype;
+  char* out;
+  int64_t out_stride;
+  bool wide;  // 4 outputs at a time fit the output's alignment
+};
+
+__device__ __forceinline__ void store4(const Linear& p, int row, int n, f32x4 v) {
+  if (row >= p.rows || n >= p.out_features) return;
+  const int left = min(4, p.out_features - n);
+  if (p.bias) {
+    for (int i = 0; i < left; ++i)
+      v[i] += p.out_dtype == kFp16 ? element<kFp16>(static_cast<const char*>(p.bias) + 2 * (n + i))
+                                   : element<kBf16>(static_cast<const char*>(p.bias) + 2 * (n + i));
+  }
+  char* o = p.out + (row * p.out_stride + n) * 2;
+  const u32x2 w = p.out_dtype == kFp16 ? u32x2{narrow2<kFp16>(v[0], v[1]), narrow2<kFp16>(v[2], v[3])}
+                                       : u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
+  if (p.wide && left == 4) {
+    *reinterpret_cast<u32x2*>(o) = w;
+    return;
+  }
+  for (int i = 0; i < left; ++i)
+    reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+}
+
+// Few rows: a wavefront takes NT row tiles of the weight and one of KS parts of
+// the sum straight from memory; the parts meet in LDS.
+template <int MT, int NT, int KS, int XDT>
+__global__ __launch_bounds__(kThreads) void linear_direct_kernel(Linear p) {
+  constexpr int kAhead = MT * NT <= 4 ? 4 : MT * NT <= 8 ? 2 : 1;
+  __shared__ f32x4 part[KS > 1 ? kWaves * NT * MT * SF_WAVE : 1];
+  const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
+  const int g = lane >> 4, c = lane & 15;
+  const int group = blockIdx.x * (kWaves / KS) + wave / KS;  // of NT row tiles
+  const int row_tile_count = row_tiles(p.out_features);
+  const int row0 = blockIdx.y * (16 * MT);
+  WeightSource w[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    w[n].set(p.codes, p.scales, min(group * NT + n, row_tile_count - 1), p.dim, lane);
+  RowSource<XDT> x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    x[m].set(p.x, p.x_scales, min(row0 + 16 * m + c, p.rows - 1), p.x_stride, p.dim, g);
+  int begin, end;
+  part_of(tiles(p.dim), wave % KS, KS, begin, end);
+  f32x4 acc[NT][MT] = {};
+  accumulate<MT, NT, XDT, kAhead>(acc, w, x, begin, end, p.dim, g);
+  if (KS == 1) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) store4(p, row0 + 16 * m + c, (group * NT + n) * 16 + 4 * g, acc[n][m]);
+    return;
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) part[(wave * NT * MT + n * MT + m) * SF_WAVE + lane] = acc[n][m];
+  __syncthreads();
+  // Each group's NT * MT results over its KS wavefronts.
+#pragma unroll
+  for (int i = 0; i < (NT * MT + KS - 1) / KS; ++i) {
+    const int item = i * KS + wave % KS;
+    if (item >= NT * MT) break;  // wave-uniform
+    f32x4 v = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) v += part[((wave / KS * KS + k) * NT * MT + item) * SF_WAVE + lane];
+    store4(p, row0 + item % MT * 16 + c, (group * NT + item / MT) * 16 + 4 * g, v);
+  }
+}
+
+template <int MT, int NT, int KS, int XDT>
+void launch_direct(const Linear& p, hipStream_t s) {
+  const int groups = (row_tiles(p.out_features) - 1) / NT + 1, per = kWaves / KS;
+  linear_direct_kernel<MT, NT, KS, XDT><<<dim3((groups - 1) / per + 1, (p.rows - 1) / (16 * MT) + 1),
+                                          dim3(kThreads), 0, s>>>(p);
+}
+
+// Rows of 16-bit values are rounded by every wavefront that reads them, which
+// is cheaper than a launch of its own for one tile of rows only.
+constexpr int kMostRawRows = 16;
+
+}  // namespace
+
+extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, int rows,
+                            int dim, const void* codes, const void* scales, int out_features,
+                            const void* bias, int out_dtype, void* out, int64_t out_stride,
+                            sf_stream_t stream) {
+  if (rows < 0 || dim < 1 || out_features < 1 || x_stride < 0 || out_stride < out_features ||
+      (out_dtype != kBf16 && out_dtype != kFp16) ||
+      (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows))
+    return SF_ERR_INVALID_ARGUMENT;
+  // 32-bit element and tile numbers within a row, grids within their limits.
+  if (dim > 1 << 24 || out_features > 1 << 28 || rows > 1 << 20 || (x_dtype != kRows && rows > kMostRawRows))
+    return SF_ERR_UNSUPPORTED_SHAPE;
+  if (rows == 0) return SF_OK;
+  if (!x || !codes || !scales || !out || (x_dtype == kRows && !x_scales)) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4) || !aligned(out, 2) ||
+      (bias && !aligned(bias, 2)))
+    return SF_ERR_MISALIGNED;
+  if (x_dtype == kRows) {
+    if (!aligned(x_scales, 4)) return SF_ERR_MISALIGNED;
+  } else if (x_stride % 8 || dim % 8) {
+    return SF_ERR_MISALIGNED;
+  }
+  const Linear p = {x, static_cast<const uint8_t*>(x_scales), x_stride, rows, dim, out_features,
+                    static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), bias,
+                    out_dtype, static_cast<char*>(out), out_stride,
+                    aligned(out, 8) && out_stride % 4 == 0};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (x_dtype == kBf16)
+    launch_direct<1, 1, 4, kBf16>(p, s);
+  else if (x_dtype == kFp16)
+    launch_direct<1, 1, 4, kFp16>(p, s);
+  else if (rows <= 16)
+    launch_direct<1, 1, 4, kRows>(p, s);
+  else if (rows <= 32)
+    launch_direct<2, 2, 4, kRows>(p, s);
+  else
+    launch_direct<4, 2, 2, kRows>(p, s);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}

@@ -1,4 +1,4 @@
-"""PyTorch-facing wrappers of the C-ABI kernels (K1-K12 and the H2D copy).
+"""PyTorch-facing wrappers of the C-ABI kernels (K1-K16 and the H2D copy).
 
 Tensors are plumbing: each wrapper checks dtype, device, shape and
 contiguity on the host, allocates outputs with the caching allocator and
@@ -14,7 +14,8 @@ from typing import Sequence
 
 import torch
 
-from . import _native
+from . import _native, mx
+from .mx import MXRows, MXWeight
 from .rotary import RotaryTable
 
 _BF16 = torch.bfloat16
@@ -1331,3 +1332,339 @@ def greedy_tokens(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
     as adjust_logits."""
     return _logit_rules(logits, counts, paths, repetition, presence, frequency, bias, allowed, None,
                         True, stream)
+
+
+# ------------------------------------------------------- K13: microscaled --
+_MX_E4M3, _MX_E2M1, _MX_ROWS = 0, 1, 3
+_MX_RAW_ROWS = 16   # rows of 16-bit values that a product takes as they are
+
+
+def _new(shape, dtype: torch.dtype, device: torch.device,
+         stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """Memory that a launch on ``stream`` writes and a later one there reads."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _as_rows(name: str, x: torch.Tensor, stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """x [..., dim] as [rows, dim] with a unit last stride: a view where the
+    rows share one stride, else a copy."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} must have at least one column")
+    if x.stride(-1) != 1:
+        x = _dense(x, stream)
+    if x.dim() == 2:
+        return x
+    rows = x.numel() // x.shape[-1]
+    try:
+        return x.view(rows, x.shape[-1])
+    except RuntimeError:
+        return _dense(x, stream).view(rows, x.shape[-1])
+
+
+def _mx_rows(shape, dtype: torch.dtype, device: torch.device,
+             stream: torch.cuda.Stream | None) -> MXRows:
+    rows = 1
+    for s in shape[:-1]:
+        rows *= s
+    code, scale = mx.row_bytes(shape[-1])
+    buf = _new(rows * (code + scale), torch.uint8, device, stream)
+    return MXRows(buf[:rows * code], buf[rows * code:], tuple(shape), dtype)
+
+
+def _mx_quantize_into(x: torch.Tensor, out: MXRows, stream: torch.cuda.Stream | None) -> None:
+    flat = _as_rows("x", x, stream)
+    rc = _launch(_native.lib().sf_mx_quantize, x.get_device(), _DTYPES[x.dtype], flat.data_ptr(),
+                 flat.stride(0), 0, flat.shape[0], flat.shape[1], 1, _MX_E4M3, out.codes.data_ptr(),
+                 0, out.scales.data_ptr(), 0, _stream_handle(stream, x.device))
+    if rc:
+        _native.check(rc, "sf_mx_quantize")
+
+
+def mx_quantize(x: torch.Tensor, *, stream: torch.cuda.Stream | None = None) -> MXRows:
+    """x [..., dim] (bf16, fp16 or fp32, any strides) in e4m3 with a
+    power-of-two scale for each 32 values of a row (K13).  No gradients."""
+    _refuse_gradients("mx_quantize", x)
+    _require_cuda("x", x)
+    if x.dtype not in _DTYPES:
+        raise ValueError("x must be bf16, fp16 or fp32")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have at least one column")
+    out = _mx_rows(x.shape, x.dtype, x.device, None)
+    if out.rows:
+        _mx_quantize_into(x, out, stream)
+    return out
+
+
+def mx_quantize_weight(weight: torch.Tensor, *,
+                       stream: torch.cuda.Stream | None = None) -> MXWeight:
+    """weight [rows, dim] (bf16, fp16 or fp32) in e2m1 with a power-of-two
+    scale for each 32 values of a row (K13).  No gradients."""
+    _refuse_gradients("mx_quantize_weight", weight)
+    _require_cuda("weight", weight)
+    if weight.dtype not in _DTYPES:
+        raise ValueError("weight must be bf16, fp16 or fp32")
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError("weight must be [rows, dim]")
+    if weight.stride(1) != 1:
+        weight = _dense(weight, stream)
+    rows, dim = weight.shape
+    code, scale = mx.weight_bytes(rows, dim)
+    out = MXWeight(torch.empty(code, dtype=torch.uint8, device=weight.device),
+                   torch.empty(scale, dtype=torch.uint8, device=weight.device), rows, dim)
+    rc = _launch(_native.lib().sf_mx_quantize, weight.get_device(), _DTYPES[weight.dtype],
+                 weight.data_ptr(), weight.stride(0), 0, rows, dim, 1, _MX_E2M1,
+                 out.codes.data_ptr(), 0, out.scales.data_ptr(), 0,
+                 _stream_handle(stream, weight.device))
+    if rc:
+        _native.check(rc, "sf_mx_quantize")
+    return out
+
+
+def mx_values(t: MXRows | MXWeight, dtype: torch.dtype = _BF16, *,
+              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The values that microscaled rows or a weight hold, in bf16, fp16 or
+    fp32 (K13)."""
+    if not isinstance(t, (MXRows, MXWeight)):
+        raise TypeError("mx_values takes MXRows or an MXWeight")
+    _require_cuda("codes", t.codes)
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be bf16, fp16 or fp32")
+    out = torch.empty(t.shape, dtype=dtype, device=t.device)
+    if out.numel():
+        held = _MX_E4M3 if isinstance(t, MXRows) else _MX_E2M1
+        rc = _launch(_native.lib().sf_mx_values, t.codes.get_device(), held, t.codes.data_ptr(),
+                     t.scales.data_ptr(), t.rows, t.dim, _DTYPES[dtype], out.data_ptr(),
+                     _stream_handle(stream, t.device))
+        if rc:
+            _native.check(rc, "sf_mx_values")
+    return out
+
+
+# ----------------------------------------------------------------- K14 ----
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,
+                 *, normed: bool = True, quantized: bool = False,
+                 stream: torch.cuda.Stream | None = None
+                 ) -> tuple[torch.Tensor, torch.Tensor | None, MXRows | None]:
+    """The residual's addition and RMSNorm in one kernel, with an output in
+    microscaled e4m3 for ``mx_linear`` and ``mx_grouped_swiglu`` (K14).
+
+    s = x + residual rounded to their type (x itself without one), y = s /
+    sqrt(mean(s^2) + eps) * weight over the last dimension, the mean in 64
+    bits.  Returns (s, y rounded to the type, y in e4m3); the second is None
+    without ``normed``, the third without ``quantized``.  Both are rounded once,
+    from fp32: ``rms_norm`` instead rounds the normed value to bf16 before the
+    weight, as Qwen3MoeRMSNorm does.  x and residual [..., dim], bf16, fp16 or
+    fp32, any strides; weight [dim] of their type.  No gradients."""
+    _refuse_gradients("add_rms_norm", x, residual, weight)
+    _require_cuda("x", x)
+    dtype, device = x.dtype, x.device
+    if dtype not in _DTYPES:
+        raise ValueError("x must be bf16, fp16 or fp32")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have at least one column")
+    dim = x.shape[-1]
+    _require_cuda("weight", weight, dtype)
+    if weight.shape != (dim,) or weight.stride(0) != 1 or weight.device != device:
+        raise ValueError(f"weight must be a contiguous [{dim}] tensor on x's device")
+    if residual is not None:
+        _require_cuda("residual", residual, dtype)
+        if residual.shape != x.shape or residual.device != device:
+            raise ValueError("residual must be like x")
+    if not normed and not quantized:
+        raise ValueError("add_rms_norm needs an output: normed or quantized")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    total = x if residual is None else torch.empty(x.shape, dtype=dtype, device=device)
+    y = torch.empty(x.shape, dtype=dtype, device=device) if normed else None
+    q = _mx_rows(x.shape, dtype, device, None) if quantized else None
+    if x.numel() == 0:
+        return total, y, q
+    flat = _as_rows("x", x, stream)
+    rows, res_ptr, res_stride = flat.shape[0], None, 0
+    if residual is not None:
+        residual = _as_rows("residual", residual, stream)
+        res_ptr, res_stride = residual.data_ptr(), residual.stride(0)
+    rc = _launch(_native.lib().sf_add_rms_norm, x.get_device(), _DTYPES[dtype], flat.data_ptr(),
+                 flat.stride(0), res_ptr, res_stride, rows, dim, weight.data_ptr(), eps,
+                 None if residual is None else total.data_ptr(), _ptr(y),
+                 None if q is None else q.codes.data_ptr(),
+                 None if q is None else q.scales.data_ptr(), _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_add_rms_norm")
+    return total, y, q
+
+
+# ----------------------------------------------------------------- K15 ----
+def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | None = None, *,
+              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """x weight^T + bias with the weight in microscaled 4 bits (K15).
+
+    x [..., dim], bf16 or fp16 (rounded to e4m3 as ``mx_quantize`` does) or the
+    MXRows of such; bias [rows of the weight] of that type.  fp32 sums,
+    rounded once to x's type.  With ``stream``, the inputs and the output
+    (memory of the current stream) are the caller's to order between the two
+    streams.  No gradients."""
+    if not isinstance(weight, MXWeight):
+        raise TypeError("the weight must be an MXWeight")
+    held = isinstance(x, MXRows)
+    if held:
+        _refuse_gradients("mx_linear", bias)
+        _require_cuda("x", x.codes)
+    else:
+        _refuse_gradients("mx_linear", x, bias)
+        _require_cuda("x", x)
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if dtype not in (_BF16, torch.float16):
+        raise ValueError("a product's rows must come from bf16 or fp16")
+    if len(shape) < 1 or shape[-1] != weight.dim:
+        raise ValueError(f"x must be [..., {weight.dim}]")
+    index = weight.codes.get_device()
+    if weight.device != device:
+        raise ValueError("x and the weight must share a device")
+    if bias is not None:
+        _require_cuda("bias", bias, dtype)
+        if bias.shape != (weight.rows,) or bias.stride(0) != 1 or bias.device != device:
+            raise ValueError(f"bias must be a contiguous [{weight.rows}] tensor on x's device")
+    out = torch.empty((*shape[:-1], weight.rows), dtype=dtype, device=device)
+    if out.numel() == 0:
+        return out
+    kind, x_ptr, scale_ptr, stride = _MX_ROWS, 0, None, 0
+    if not held:
+        flat = _as_rows("x", x, stream)
+        if flat.shape[0] <= _MX_RAW_ROWS and weight.dim % 8 == 0 and flat.stride(0) % 8 == 0 \
+                and flat.data_ptr() % 16 == 0:
+            kind, x_ptr, stride = _DTYPES[dtype], flat.data_ptr(), flat.stride(0)
+        else:
+            x = _mx_rows(shape, dtype, device, stream)
+            _mx_quantize_into(flat, x, stream)
+    if kind == _MX_ROWS:
+        x_ptr, scale_ptr = x.codes.data_ptr(), x.scales.data_ptr()
+    rc = _launch(_native.lib().sf_mx_linear, index, kind, x_ptr, scale_ptr, stride,
+                 out.numel() // weight.rows, weight.dim, weight.codes.data_ptr(),
+                 weight.scales.data_ptr(), weight.rows, _ptr(bias), _DTYPES[dtype], out.data_ptr(),
+                 weight.rows, _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_mx_linear")
+    return out
+
+
+# ----------------------------------------------------------------- K16 ----
+@functools.lru_cache(maxsize=64)
+def mx_expert_bytes(hidden_size: int, intermediate_size: int) -> int:
+    """Bytes of one expert's record: the codes of gate, up and down as
+    MXWeights hold them, then their scales."""
+    n = _native.lib().sf_mx_expert_bytes(hidden_size, intermediate_size)
+    if n < 0:
+        raise ValueError("unsupported expert shape")
+    return n
+
+
+def mx_quantize_experts(packed: torch.Tensor, hidden_size: int, intermediate_size: int, *,
+                        out: torch.Tensor | None = None,
+                        stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Experts packed as [gate | up | down] (bf16, fp16 or fp32 [n, 3*H*I]) as
+    records in e2m1 (uint8 [n, mx_expert_bytes(H, I)]), for
+    ``mx_grouped_swiglu``.  No gradients."""
+    H, I = hidden_size, intermediate_size
+    _refuse_gradients("mx_quantize_experts", packed)
+    _require_cuda("packed experts", packed)
+    if packed.dtype not in _DTYPES:
+        raise ValueError("packed experts must be bf16, fp16 or fp32")
+    nbytes = mx_expert_bytes(H, I)
+    if packed.dim() != 2 or packed.shape[1] != 3 * H * I or packed.stride(1) != 1:
+        raise ValueError(f"packed experts must be [n, {3 * H * I}] with a unit last stride")
+    n = packed.shape[0]
+    if out is None:
+        out = torch.empty((n, nbytes), dtype=torch.uint8, device=packed.device)
+    elif out.shape != (n, nbytes) or out.dtype != torch.uint8 or out.device != packed.device \
+            or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous uint8 [{n}, {nbytes}]")
+    at = (ctypes.c_int64 * 6)()
+    lib = _native.lib()
+    _native.check(lib.sf_mx_expert_parts(H, I, at), "sf_mx_expert_parts")
+    size, base, src = packed.element_size(), out.data_ptr(), packed.data_ptr()
+    parts = ((0, I, H, at[0], at[3]), (H * I, I, H, at[1], at[4]), (2 * H * I, H, I, at[2], at[5]))
+    for first in range(0, n, 32768):
+        count = min(32768, n - first)
+        for start, rows, dim, codes, scales in parts:
+            rc = _launch(lib.sf_mx_quantize, packed.get_device(), _DTYPES[packed.dtype],
+                         src + (first * packed.stride(0) + start) * size, dim, packed.stride(0),
+                         rows, dim, count, _MX_E2M1, base + first * nbytes + codes, nbytes,
+                         base + first * nbytes + scales, nbytes,
+                         _stream_handle(stream, packed.device))
+            _native.check(rc, "sf_mx_quantize")
+    return out
+
+
+def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
+                      route_weights: torch.Tensor | None, slot_storage: torch.Tensor,
+                      hidden_size: int, intermediate_size: int, out_rows: torch.Tensor, *,
+                      slot_of_expert: torch.Tensor | None = None,
+                      stream: torch.cuda.Stream | None = None) -> None:
+    """Grouped SwiGLU over the dispatched rows with the experts' weights in
+    microscaled 4 bits (K16), the counterpart of ``grouped_swiglu_table``.
+
+    hidden [tokens, H] bf16, or its MXRows; ``slot_storage`` uint8 [slots,
+    mx_expert_bytes(H, I)] records; expert e's is that of slot
+    ``slot_of_expert[e]`` (int32 [num_experts]; -1: its rows are left as they
+    are), or of slot e without a table.  ``out_rows`` bf16 [tokens * top_k, H]
+    takes each route's row times its weight, for ``combine``.  The
+    activation silu(gate) * up is rounded once, from fp32 to e4m3.  No
+    gradients."""
+    H, I, T, K, E = hidden_size, intermediate_size, plan.tokens, plan.top_k, plan.num_experts
+    held = isinstance(hidden, MXRows)
+    if held:
+        _require_cuda("hidden_states", hidden.codes)
+    else:
+        _refuse_gradients("mx_grouped_swiglu", hidden)
+        _require_cuda("hidden_states", hidden, _BF16)
+    _refuse_gradients("mx_grouped_swiglu", route_weights)
+    if tuple(hidden.shape) != (T, H):
+        raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
+    device = hidden.device
+    nbytes = mx_expert_bytes(H, I)
+    _require_cuda("slot storage", slot_storage, torch.uint8)
+    if slot_storage.dim() != 2 or slot_storage.shape[1] != nbytes or slot_storage.stride(1) != 1 \
+            or slot_storage.stride(0) < nbytes or slot_storage.device != device \
+            or slot_storage.data_ptr() % 16 or slot_storage.stride(0) % 16:
+        raise ValueError(f"slot storage must be 16-byte aligned uint8 [slots, {nbytes}]")
+    if slot_of_expert is None:
+        if slot_storage.shape[0] < E:
+            raise ValueError("without a table, every expert needs a slot")
+    else:
+        _require_cuda("slot_of_expert", slot_of_expert, torch.int32)
+        if slot_of_expert.numel() != E or not slot_of_expert.is_contiguous() \
+                or slot_of_expert.device != device:
+            raise ValueError("slot_of_expert must be contiguous int32 [num_experts]")
+    _require_cuda("out_rows", out_rows, _BF16)
+    if out_rows.shape != (T * K, H) or not out_rows.is_contiguous() or out_rows.device != device:
+        raise ValueError("out_rows must be contiguous bf16 [tokens * top_k, hidden]")
+    if route_weights is not None:
+        _require_cuda("route weights", route_weights, _BF16)
+        if route_weights.numel() != T * K or not route_weights.is_contiguous() \
+                or route_weights.device != device:
+            raise ValueError("route weights must be contiguous bf16 [tokens*top_k]")
+    if T * K == 0:
+        return
+    kind, stride, scale_ptr = _MX_ROWS, 0, None
+    if not held:
+        hidden = _as_rows("hidden_states", hidden, stream)
+        if T <= _MX_RAW_ROWS and H % 8 == 0 and hidden.stride(0) % 8 == 0 \
+                and hidden.data_ptr() % 16 == 0:
+            kind, stride, x_ptr = 0, hidden.stride(0), hidden.data_ptr()
+        else:
+            flat, hidden = hidden, _mx_rows((T, H), _BF16, device, stream)
+            _mx_quantize_into(flat, hidden, stream)
+    if kind == _MX_ROWS:
+        x_ptr, scale_ptr = hidden.codes.data_ptr(), hidden.scales.data_ptr()
+    act = _mx_rows((T * K, I), _BF16, device, stream)
+    rc = _launch(_native.lib().sf_mx_grouped_swiglu, out_rows.get_device(), kind, x_ptr, scale_ptr,
+                 stride, plan.perm_pos.data_ptr(), plan.offsets.data_ptr(), _ptr(route_weights), T,
+                 K, H, I, E, _ptr(slot_of_expert), slot_storage.data_ptr(), slot_storage.stride(0),
+                 act.codes.data_ptr(), act.scales.data_ptr(), out_rows.data_ptr(),
+                 _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_mx_grouped_swiglu")

@@ -1,0 +1,79 @@
+"""Routed experts of one decoder layer held in HBM in microscaled 4 bits (K16).
+
+Drop-in for transformers' ``Qwen3MoeExperts`` (tf:215-246): the same forward
+arguments, every expert resident.  An expert of the Qwen3-30B-A3B shape takes
+2.5 MB instead of 9.4, so the 48 layers of that model take 15 GB and the 94 of
+Qwen3-235B-A22B 117 of a GPU's 288 GB; ``Qwen3OffloadedExperts`` is for experts
+that have to stay exact and stream.  A forward reads nothing back to the host
+and can be captured into a graph.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from .. import ops
+
+
+class Qwen3MXExperts(nn.Module):
+    def __init__(self, records: torch.Tensor, *, hidden_size: int, intermediate_size: int) -> None:
+        """``records``: uint8 [experts, ops.mx_expert_bytes(H, I)] on a GPU, as
+        ``ops.mx_quantize_experts`` makes them."""
+        super().__init__()
+        nbytes = ops.mx_expert_bytes(hidden_size, intermediate_size)
+        if records.dtype != torch.uint8 or records.dim() != 2 or records.shape[1] != nbytes \
+                or not records.is_contiguous():
+            raise ValueError(f"records must be contiguous uint8 [experts, {nbytes}]")
+        if not 1 <= records.shape[0] <= 256:
+            raise ValueError("a layer has 1 to 256 experts")
+        self.hidden_size = hidden_size
+        self.intermediate_size = intermediate_size
+        self.register_buffer("records", records)
+
+    @property
+    def num_experts(self) -> int:
+        return self.records.shape[0]
+
+    @classmethod
+    def from_packed(cls, packed: torch.Tensor, *, hidden_size: int,
+                    intermediate_size: int) -> "Qwen3MXExperts":
+        """From [gate | up | down] packed experts [experts, 3*H*I] on a GPU."""
+        return cls(ops.mx_quantize_experts(packed, hidden_size, intermediate_size),
+                   hidden_size=hidden_size, intermediate_size=intermediate_size)
+
+    @classmethod
+    def from_module(cls, experts: nn.Module) -> "Qwen3MXExperts":
+        """From an HF ``Qwen3MoeExperts`` on a GPU (shares no storage)."""
+        gate_up, down = experts.gate_up_proj.detach(), experts.down_proj.detach()
+        E, H, I = down.shape
+        records = torch.empty((E, ops.mx_expert_bytes(H, I)), dtype=torch.uint8, device=down.device)
+        for e in range(E):  # one expert's copy at a time, not the layer's
+            packed = torch.cat([gate_up[e].reshape(-1), down[e].reshape(-1)])[None]
+            ops.mx_quantize_experts(packed, H, I, out=records[e:e + 1])
+        return cls(records, hidden_size=H, intermediate_size=I)
+
+    def forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
+                top_k_weights: torch.Tensor) -> torch.Tensor:
+        """Sum over a token's experts of weight * expert(token), bf16 [tokens,
+        H].  Routes to experts that the layer does not have count for nothing."""
+        if hidden_states.dim() != 2 or hidden_states.shape[1] != self.hidden_size:
+            raise ValueError(f"hidden_states must have shape [tokens, {self.hidden_size}]")
+        if top_k_index.dim() != 2 or top_k_index.shape[0] != hidden_states.shape[0]:
+            raise ValueError("top_k_index must have shape [tokens, top_k]")
+        if top_k_weights.shape != top_k_index.shape:
+            raise ValueError("top_k_weights must match top_k_index shape")
+        if hidden_states.dtype != torch.bfloat16:
+            raise ValueError("hidden_states must be bfloat16")
+        for t in (hidden_states, top_k_index, top_k_weights):
+            if t.device != self.records.device:
+                raise ValueError("hidden_states and routes must be on the experts' device")
+        T, K = top_k_index.shape
+        if T * K == 0:
+            return torch.zeros_like(hidden_states)
+        plan = ops.dispatch(top_k_index, self.num_experts)
+        rows = torch.empty((T * K, self.hidden_size), dtype=torch.bfloat16,
+                           device=hidden_states.device)
+        weights = top_k_weights.to(torch.bfloat16).contiguous().view(-1)
+        ops.mx_grouped_swiglu(hidden_states, plan, weights, self.records, self.hidden_size,
+                              self.intermediate_size, rows)
+        return ops.combine(rows, top_k_index, plan, self.hidden_size, accumulate_fp32=True)

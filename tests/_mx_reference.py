@@ -1,0 +1,108 @@
+"""Microscaled values and products in 64 bits, from their definition."""
+import torch
+
+BLOCK = 32
+LARGEST = {"e4m3": (464.0, True), "e2m1": (7.0, False)}   # what still rounds to the largest
+FOUR = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
+
+
+def grid(held):
+    """The type's magnitudes, ascending."""
+    if held == "e2m1":
+        return FOUR
+    codes = torch.arange(127, dtype=torch.uint8)
+    return codes.view(torch.float8_e4m3fn).double()
+
+
+def round_to(y, held):
+    """y to the nearest of the type's values, ties to the even code."""
+    g = grid(held).to(y.device)
+    a = y.abs()
+    hi = torch.searchsorted(g, a).clamp_max(g.numel() - 1)
+    lo = (hi - 1).clamp_min(0)
+    down, up = a - g[lo], g[hi] - a
+    code = torch.where((down < up) | ((down == up) & (lo % 2 == 0)), lo, hi)
+    code = torch.where(g[hi] == a, hi, code)
+    return torch.where(y < 0, -g[code], g[code])
+
+
+def quantize(x, held):
+    """(values held, scale bytes) of x [rows, dim] (any float type)."""
+    x = x.double()
+    rows, dim = x.shape
+    n = -(-dim // BLOCK)
+    pad = torch.zeros((rows, n * BLOCK), dtype=torch.float64, device=x.device)
+    pad[:, :dim] = x
+    pad = pad.view(rows, n, BLOCK)
+    limit, included = LARGEST[held]
+    top = pad.abs().amax(2)
+    bad = ~torch.isfinite(pad).all(2)
+    top = torch.where(bad, 0.0, top)
+    byte = torch.zeros((rows, n), dtype=torch.long, device=x.device)
+    for b in range(254, -1, -1):     # the least that holds it, by trying all
+        holds = top <= limit * 2.0 ** (b - 127) if included else top < limit * 2.0 ** (b - 127)
+        byte = torch.where(holds, b, byte)
+    scale = torch.exp2(byte.double() - 127)[..., None]
+    values = round_to(torch.where(bad[..., None], 0.0, pad) / scale, held) * scale
+    values = torch.where(bad[..., None], torch.nan, values)
+    return values.view(rows, -1)[:, :dim], torch.where(bad, 255, byte)
+
+
+def product_slack(x, w):
+    """What the matrix unit may lose of each output x w^T: it lines eight
+    neighbouring products up with the largest of them and cuts each at 2^-13
+    of its power of two (the product of two significands is below 4, so the
+    largest is at least that power), and adds in fp32.  [rows, outs]."""
+    rows, dim = x.shape
+    pad = -dim % 8
+    x = torch.nn.functional.pad(x.abs(), (0, pad)).view(rows, -1, 8)
+    w = torch.nn.functional.pad(w.abs(), (0, pad)).view(w.shape[0], -1, 8)
+    slack = torch.zeros((rows, w.shape[0]), dtype=torch.float64, device=x.device)
+    total = torch.zeros_like(slack)
+    for at in range(x.shape[1]):
+        p = x[:, None, at] * w[None, :, at]
+        slack += 8 * 2.0 ** -13 * p.amax(2)
+        total += p.sum(2)
+    return slack + total * x.shape[1] * 2.0 ** -24
+
+
+def half_step(y, dtype):
+    """Half a step of dtype around y."""
+    tiny = torch.finfo(dtype).tiny
+    return y.abs().clamp_min(tiny) * torch.finfo(dtype).eps / 2
+
+
+def experts(hidden, index, weights, packed, hidden_size, intermediate_size, table=None):
+    """Outputs of K16's chain with its roundings, and what they may be off by
+    beyond it: the product's slack, and where the activation lies so near a
+    border that it may fall on the other side, a step of it."""
+    H, I = hidden_size, intermediate_size
+    x = quantize(hidden, "e4m3")[0]
+    out = torch.zeros((hidden.shape[0], H), dtype=torch.float64, device=hidden.device)
+    slack = torch.zeros_like(out)
+    for e in range(packed.shape[0]):
+        token, slot = torch.nonzero(index == e, as_tuple=True)
+        if not token.numel():
+            continue
+        gate, up, down = (quantize(p.view(r, d), "e2m1")[0] for p, r, d in zip(
+            packed[e].split(H * I), (I, I, H), (H, H, I)))
+        g, u = x[token] @ gate.t(), x[token] @ up.t()
+        dg, du = product_slack(x[token], gate), product_slack(x[token], up)
+        silu = g * torch.sigmoid(g)
+        a = silu * u
+        # |silu'| <= 1.1; eight steps of fp32 in exp, quotient and products.
+        da = 1.1 * dg * (u.abs() + du) + silu.abs() * du + 8 * 2.0 ** -24 * a.abs()
+        q, byte = quantize(a, "e4m3")
+        scale = torch.exp2(byte.double() - 127).repeat_interleave(BLOCK, dim=1)[:, :I]
+        # Off by da before the rounding: the rounded value moves by at most
+        # da and the two half steps around it, where it moves at all.
+        step = torch.maximum(q.abs() * 2.0 ** -3, scale * 2.0 ** -9)
+        moves = (quantize(a + da, "e4m3")[0] != q) | (quantize(a - da, "e4m3")[0] != q)
+        dq = torch.where(moves, da + step, 0.0)
+        y = q @ down.t()
+        dy = product_slack(q, down) + dq @ down.abs().t()
+        r = weights[token, slot].double()[:, None]
+        row = y * r
+        out.index_add_(0, token, row)
+        slack.index_add_(0, token, dy * r.abs() + half_step(row, torch.bfloat16) * 1.01)
+    return out, slack + half_step(out, torch.bfloat16) + slack * 2.0 ** -8

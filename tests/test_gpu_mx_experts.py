@@ -1,0 +1,160 @@
+"""Experts with 4-bit weights (K16) against a 64-bit reference."""
+import pytest
+import torch
+
+import _mx_reference as ref
+from specfit_amd import ops
+from specfit_amd.runtime import Qwen3MXExperts
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _case(tokens, hidden, inner, experts, top_k, seed=0, favourite=None, distinct=True):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    h = torch.randn((tokens, hidden), generator=g, device=DEV).to(torch.bfloat16)
+    packed = (torch.randn((experts, 3 * hidden * inner), generator=g, device=DEV)
+              * 1.5 * hidden ** -0.5).to(torch.bfloat16)
+    scores = torch.rand((tokens, experts), generator=g, device=DEV)
+    if favourite is not None:
+        scores[:, favourite] += 1
+    index = torch.topk(scores, top_k, dim=1).indices
+    if not distinct:
+        index = torch.randint(0, experts, (tokens, top_k), generator=g, device=DEV)
+    weights = torch.softmax(torch.randn((tokens, top_k), generator=g, device=DEV), 1)
+    return h, packed, index, weights.to(torch.bfloat16)
+
+
+def _check(got, h, index, weights, packed, hidden, inner):
+    want, slack = ref.experts(h, index, weights, packed, hidden, inner)
+    assert (got.double() - want).abs().le(slack).all()
+    if want.norm() > 0:
+        # Roundings to 8 bits fall on the other side for a few values only.
+        assert (got.double() - want).norm() <= 2.0 ** -7 * want.norm()
+
+
+SHAPES = [(1, 64, 32, 8, 3), (5, 64, 32, 8, 3), (40, 64, 32, 8, 3), (7, 1000, 424, 20, 2),
+          (3, 33, 17, 4, 1), (16, 2048, 768, 16, 8), (17, 2048, 768, 16, 8), (61, 256, 160, 128, 8),
+          (150, 256, 96, 4, 2), (300, 512, 256, 6, 2), (1, 4096, 1536, 8, 8), (600, 128, 64, 3, 1)]
+
+
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", SHAPES)
+def test_experts(tokens, hidden, inner, experts, top_k):
+    h, packed, index, weights = _case(tokens, hidden, inner, experts, top_k)
+    module = Qwen3MXExperts.from_packed(packed, hidden_size=hidden, intermediate_size=inner)
+    _check(module(h, index, weights), h, index, weights, packed, hidden, inner)
+
+
+@pytest.mark.parametrize("tokens", [20, 200, 700])
+def test_a_favourite_takes_every_token(tokens):
+    h, packed, index, weights = _case(tokens, 256, 128, 40, 2, favourite=11)
+    module = Qwen3MXExperts.from_packed(packed, hidden_size=256, intermediate_size=128)
+    _check(module(h, index, weights), h, index, weights, packed, 256, 128)
+
+
+def test_the_same_expert_twice_and_experts_that_are_not_there():
+    h, packed, index, weights = _case(30, 96, 64, 5, 4, distinct=False)
+    index[3, 1], index[7] = 99, -1
+    module = Qwen3MXExperts.from_packed(packed, hidden_size=96, intermediate_size=64)
+    got = module(h, index, weights)
+    _check(got, h, index, weights, packed, 96, 64)
+    assert not got[7].any()
+
+
+def test_a_slot_table_and_rows_that_are_left_alone():
+    H, I, E, K = 128, 96, 6, 2
+    h, packed, index, weights = _case(50, H, I, E, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    slots = torch.zeros((4, records.shape[1]), dtype=torch.uint8, device=DEV)
+    table = torch.tensor([2, -1, 0, -1, 3, 1], dtype=torch.int32, device=DEV)
+    for e, s in enumerate(table.tolist()):
+        if s >= 0:
+            slots[s] = records[e]
+    plan = ops.dispatch(index, E)
+    full = torch.empty((50 * K, H), dtype=torch.bfloat16, device=DEV)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), records, H, I, full)
+    some = torch.full_like(full, 7.0)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), slots, H, I, some, slot_of_expert=table)
+    expert = index.flatten()[plan.perm_pos.long()]
+    there = table[expert] >= 0
+    assert torch.equal(some[there], full[there]) and (some[~there] == 7).all()
+
+
+def test_rows_and_tensor_give_the_same_and_no_weights_means_one():
+    H, I, E, K = 256, 64, 8, 2
+    h, packed, index, _ = _case(12, H, I, E, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    plan = ops.dispatch(index, E)
+    a, b = (torch.empty((12 * K, H), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ops.mx_grouped_swiglu(h, plan, None, records, H, I, a)
+    ops.mx_grouped_swiglu(ops.mx_quantize(h), plan, None, records, H, I, b)
+    ones = torch.ones((12, K), dtype=torch.bfloat16, device=DEV)
+    c = torch.empty_like(a)
+    ops.mx_grouped_swiglu(h, plan, ones.view(-1), records, H, I, c)
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_non_finite_tokens_stay_alone():
+    h, packed, index, weights = _case(40, 128, 64, 4, 2)
+    h[5, 9], h[17, 100] = float("inf"), float("nan")
+    module = Qwen3MXExperts.from_packed(packed, hidden_size=128, intermediate_size=64)
+    bad = torch.isnan(module(h, index, weights)).all(1)
+    assert bad.nonzero().flatten().tolist() == [5, 17]
+    assert not torch.isnan(module(h, index, weights)[~bad]).any()
+
+
+def test_from_an_hf_module():
+    from transformers import Qwen3MoeConfig
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeExperts
+
+    config = Qwen3MoeConfig(hidden_size=64, moe_intermediate_size=48, num_experts=6)
+    hf = Qwen3MoeExperts(config).to(torch.bfloat16).to(DEV)
+    with torch.no_grad():
+        for p in hf.parameters():
+            p.normal_(0, 0.2)
+    packed = torch.cat([hf.gate_up_proj.detach().flatten(1), hf.down_proj.detach().flatten(1)], 1)
+    ours = Qwen3MXExperts.from_module(hf)
+    again = Qwen3MXExperts.from_packed(packed, hidden_size=64, intermediate_size=48)
+    assert torch.equal(ours.records, again.records)
+    h, _, index, weights = _case(9, 64, 48, 6, 2)
+    _check(ours(h, index, weights), h, index, weights, packed, 64, 48)
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 300])
+def test_captured_and_replayed(tokens):
+    H, I, E, K = 256, 128, 16, 4
+    h, packed, index, weights = _case(tokens, H, I, E, K)
+    module = Qwen3MXExperts.from_packed(packed, hidden_size=H, intermediate_size=I)
+    h_in, index_in, w_in = h.clone(), index.clone(), weights.clone()
+    module(h_in, index_in, w_in)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = module(h_in, index_in, w_in)
+    for seed in range(3):
+        h, _, index, weights = _case(tokens, H, I, E, K, seed=seed + 5)
+        h_in.copy_(h)
+        index_in.copy_(index)
+        w_in.copy_(weights)
+        graph.replay()
+        eager = module(h, index, weights)
+        assert torch.equal(out, eager)
+
+
+def test_on_another_stream():
+    h, packed, index, weights = _case(33, 128, 64, 6, 2)
+    records = ops.mx_quantize_experts(packed, 128, 64)
+    plan = ops.dispatch(index, 6)
+    want = torch.empty((66, 128), dtype=torch.bfloat16, device=DEV)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), records, 128, 64, want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = torch.zeros_like(want)
+    side.wait_stream(torch.cuda.current_stream())
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), records, 128, 64, got, stream=side)
+    x = h[:, :100]
+    w = ops.mx_quantize_weight(torch.randn((40, 100), device=DEV))
+    side.wait_stream(torch.cuda.current_stream())
+    y = ops.mx_linear(x, w, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(y, ops.mx_linear(x, w))
