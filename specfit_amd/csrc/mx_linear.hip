@@ -98,6 +98,41 @@ void launch_direct(const Linear& p, hipStream_t s) {
                                           dim3(kThreads), 0, s>>>(p);
 }
 
+// Many rows: a workgroup takes kRows of them by kOut of the weight's.
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void linear_tiled_kernel(Linear p, int row_groups) {
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
+  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
+  const int row0 = blockIdx.x % row_groups * T::kRows, tile0 = blockIdx.x / row_groups * (T::kOut / 16);
+  const int last_tile = row_tiles(p.out_features) - 1;
+  f32x16 acc[T::FN][T::FM];
+  multiply<T>(acc, static_cast<const uint8_t*>(p.x), p.x_scales, p.codes, p.scales, p.dim,
+              [&](int r) { return min(row0 + r, p.rows - 1); },
+              [&](int i) { return min(tile0 + i, last_tile); }, stage0, stage1, scales);
+  const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
+  const int wn = wave / T::WM, wm = wave % T::WM;
+#pragma unroll
+  for (int m = 0; m < T::FM; ++m) {
+    const int row = row0 + (wm * T::FM + m) * 32 + (lane & 31);
+#pragma unroll
+    for (int n = 0; n < T::FN; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store4(p, row, tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 4 * (lane >> 5),
+               f32x4{acc[n][m][4 * i], acc[n][m][4 * i + 1], acc[n][m][4 * i + 2], acc[n][m][4 * i + 3]});
+  }
+}
+
+template <class T>
+int launch_tiled(const Linear& p, hipStream_t s) {
+  const int row_groups = (p.rows - 1) / T::kRows + 1, out_groups = (p.out_features - 1) / T::kOut + 1;
+  if (static_cast<int64_t>(row_groups) * out_groups > 0x7fffffff) return SF_ERR_UNSUPPORTED_SHAPE;
+  linear_tiled_kernel<T><<<dim3(row_groups * out_groups), dim3(T::kThreads), 0, s>>>(p, row_groups);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
 // Rows of 16-bit values are rounded by every wavefront that reads them, which
 // is cheaper than a launch of its own for one tile of rows only.
 constexpr int kMostRawRows = 16;
@@ -138,6 +173,8 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
     launch_direct<1, 1, 4, kRows>(p, s);
   else if (rows <= 32)
     launch_direct<2, 2, 4, kRows>(p, s);
+  else if (rows > 128)
+    return launch_tiled<Tiling<2, 2, 4, 2>>(p, s);
   else
     launch_direct<4, 2, 2, kRows>(p, s);
   SF_LAUNCH_CHECK();

@@ -158,4 +158,188 @@ __device__ __forceinline__ void part_of(int count, int i, int n, int& begin, int
   end = count * (i + 1) / n;
 }
 
+// ------------------------------------------------------- tiles of many rows --
+// WN x WM wavefronts, each FN x FM products of 32 weight rows by 32 rows on
+// v_mfma_scale_f32_32x32x64_f8f6f4.  A stage is one tile (128 values) of the
+// workgroup's rows and weight rows; two stages alternate, the next one on its
+// way into LDS (loads that write it themselves) while the present one is
+// multiplied.  The scales of four tiles come together, ahead of them.
+//
+// LDS: rows keep their 128 bytes together, piece p (16 bytes) of row r in slot
+// p ^ (r & 7): the loads then take whole lines from memory, and eight lanes
+// reading a piece of eight rows meet eight different slots.  Weight pieces
+// stay in the operand's order.
+template <int WN_, int WM_, int FN_, int FM_>
+struct Tiling {
+  static constexpr int WN = WN_, WM = WM_, FN = FN_, FM = FM_;
+  static constexpr int kWaves = WN * WM, kThreads = kWaves * SF_WAVE;
+  static constexpr int kRows = 32 * FM * WM, kOut = 32 * FN * WN;  // of a workgroup
+  static constexpr int kRowLoads = kRows / 8 / kWaves, kOutLoads = kOut / 16 / kWaves;
+  static_assert(kRows / 8 % kWaves == 0 && kOut / 16 % kWaves == 0, "whole loads for a wavefront");
+  static constexpr int kRowScaleLoads = kRows / 64, kOutScaleLoads = kOut / 64;
+  struct Stage {
+    uint8_t rows[kRows * kTile];
+    uint8_t out[kOut * kTile / 2];
+  };
+  struct Scales {
+    uint8_t rows[kRows * 16];
+    uint8_t out[kOut * 16];
+  };
+};
+
+__device__ __forceinline__ void to_lds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// All of this wavefront's loads have landed and its LDS reads are done; then
+// all wavefronts'.  The builtins rather than assembly: the compiler then knows
+// that nothing is under way and adds no waits of its own.
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_sched_barrier(0);   // the products before the wait, not behind it
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ i32x8 operand4(const uint8_t* at) {
+  const u32x4 v = *reinterpret_cast<const u32x4*>(at);
+  return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]),
+               0, 0, 0, 0};
+}
+
+__device__ __forceinline__ i32x8 operand8(const uint8_t* lo, const uint8_t* hi) {
+  const u32x4 a = *reinterpret_cast<const u32x4*>(lo), b = *reinterpret_cast<const u32x4*>(hi);
+  return i32x8{static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]),
+               static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3])};
+}
+
+// acc[n][m] = the workgroup's rows times its weight rows.  row_at(r) is row r's
+// number (r < kRows; any valid row for those past the end), out_tile(i) the row
+// tile of the weight's i-th 16 rows as an offset of tiles from w and ws.
+template <class T, class RowAt, class OutTile>
+__device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint8_t* x, const uint8_t* x_scales,
+                                         const uint8_t* w, const uint8_t* w_scales, int dim, RowAt row_at,
+                                         OutTile out_tile, typename T::Stage& stage0, typename T::Stage& stage1,
+                                         typename T::Scales (&scales)[2]) {
+  const int lane = threadIdx.x & (SF_WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / SF_WAVE);
+  const int wn = wave / T::WM, wm = wave % T::WM;
+  const int kt = tiles(dim), kq = quads(dim);
+  const int r = lane & 31, g = lane >> 5;
+  // This wavefront's loads: 8 rows each, and 16 weight rows each.
+  const uint8_t* row_from[T::kRowLoads];
+#pragma unroll
+  for (int i = 0; i < T::kRowLoads; ++i) {
+    const int row = (wave * T::kRowLoads + i) * 8 + lane / 8;
+    row_from[i] = x + static_cast<int64_t>(row_at(row)) * (static_cast<int64_t>(kt) * kTile) +
+                  (lane % 8 ^ (row & 7)) * 16;
+  }
+  const uint8_t* out_from[T::kOutLoads];
+#pragma unroll
+  for (int i = 0; i < T::kOutLoads; ++i)
+    out_from[i] = w + (static_cast<int64_t>(out_tile(wave * T::kOutLoads + i)) * kt) * 1024;
+
+  const auto load_stage = [&](typename T::Stage& s, int t) {
+#pragma unroll
+    for (int i = 0; i < T::kRowLoads; ++i)
+      to_lds(row_from[i] + static_cast<int64_t>(t) * kTile, s.rows + (wave * T::kRowLoads + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < T::kOutLoads; ++i)
+      to_lds(out_from[i] + static_cast<int64_t>(t) * 1024 + lane * 16, s.out + (wave * T::kOutLoads + i) * 1024);
+  };
+  const auto load_scales = [&](int q) {
+    typename T::Scales& s = scales[q % 2];
+#pragma unroll
+    for (int i = 0; i < (T::kRowScaleLoads + T::kWaves - 1) / T::kWaves; ++i) {
+      const int at = wave + i * T::kWaves;  // 64 rows
+      if (at < T::kRowScaleLoads)
+        to_lds(x_scales + static_cast<int64_t>(row_at(at * 64 + lane)) * (static_cast<int64_t>(kq) * 16) + q * 16,
+               s.rows + at * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < (T::kOutScaleLoads + T::kWaves - 1) / T::kWaves; ++i) {
+      const int at = T::kWaves - 1 - wave + i * T::kWaves;  // four row tiles, 256 bytes each
+      if (at < T::kOutScaleLoads)
+        to_lds(w_scales + (static_cast<int64_t>(out_tile(at * 4 + lane / 16)) * kq + q) * 256 + lane % 16 * 16,
+               s.out + at * 1024);
+    }
+  };
+
+#pragma unroll
+  for (int n = 0; n < T::FN; ++n)
+#pragma unroll
+    for (int m = 0; m < T::FM; ++m) acc[n][m] = f32x16{};
+  // Scale words of blocks g and 2 + g (the tile's halves), the present tile's
+  // byte lowest.
+  uint32_t ws[T::FN][2], xs[T::FM][2];
+  const auto read_scales = [&](int q) {
+    const typename T::Scales& s = scales[q % 2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < T::FN; ++n)
+        ws[n][h] = *reinterpret_cast<const uint32_t*>(s.out + ((wn * T::FN + n) * 2 + r / 16) * 256 +
+                                                      (2 * h + g) * 64 + r % 16 * 4);
+#pragma unroll
+      for (int m = 0; m < T::FM; ++m)
+        xs[m][h] = *reinterpret_cast<const uint32_t*>(s.rows + ((wm * T::FM + m) * 32 + r) * 16 + (2 * h + g) * 4);
+    }
+  };
+  const auto step = [&](typename T::Stage& here) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x8 a[T::FN], b[T::FM];
+#pragma unroll
+      for (int n = 0; n < T::FN; ++n)
+        a[n] = operand4(here.out + ((wn * T::FN + n) * 2 + r / 16) * 1024 + (2 * h + g) * 256 + r % 16 * 16);
+#pragma unroll
+      for (int m = 0; m < T::FM; ++m) {
+        const int row = (wm * T::FM + m) * 32 + r;
+        const uint8_t* at = here.rows + row * kTile;
+        b[m] = operand8(at + ((4 * h + g) ^ (row & 7)) * 16, at + ((4 * h + 2 + g) ^ (row & 7)) * 16);
+      }
+#pragma unroll
+      for (int n = 0; n < T::FN; ++n)
+#pragma unroll
+        for (int m = 0; m < T::FM; ++m)
+          acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              a[n], b[m], acc[n][m], 4, 0, 0, static_cast<int>(ws[n][h]), 0, static_cast<int>(xs[m][h]));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < T::FN; ++n) ws[n][h] >>= 8;
+#pragma unroll
+      for (int m = 0; m < T::FM; ++m) xs[m][h] >>= 8;
+    }
+  };
+
+  load_stage(stage0, 0);
+  load_scales(0);
+  meet();
+  int t = 0;
+  for (; t + 2 <= kt; t += 2) {
+    if (t % 4 == 0) {
+      read_scales(t / 4);
+      if (t + 4 < kt) load_scales(t / 4 + 1);
+    }
+    load_stage(stage1, t + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    step(stage0);
+    meet();
+    // No branch here, or the products above would be moved behind it: past the
+    // end the last tile comes once more, unread.
+    load_stage(stage0, min(t + 2, kt - 1));
+    __builtin_amdgcn_sched_barrier(0);
+    step(stage1);
+    meet();
+  }
+  if (t < kt) {
+    if (t % 4 == 0) read_scales(t / 4);
+    step(stage0);
+  }
+}
+
 }  // namespace sf_mx
