@@ -9,8 +9,6 @@ namespace {
 
 using namespace sf_mx;
 
-constexpr int kThreads = 256, kWaves = kThreads / SF_WAVE;
-
 struct Linear {
   const void* x;
   const uint8_t* x_scales;
@@ -46,13 +44,13 @@ __device__ __forceinline__ void store4(const Linear& p, int row, int n, f32x4 v)
 
 // Few rows: a wavefront takes NT row tiles of the weight and one of KS parts of
 // the sum straight from memory; the parts meet in LDS.
-template <int MT, int NT, int KS, int XDT>
-__global__ __launch_bounds__(kThreads) void linear_direct_kernel(Linear p) {
+template <int MT, int NT, int KS, int WAVES, int XDT>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void linear_direct_kernel(Linear p) {
   constexpr int kAhead = MT * NT <= 4 ? 4 : MT * NT <= 8 ? 2 : 1;
-  __shared__ f32x4 part[KS > 1 ? kWaves * NT * MT * SF_WAVE : 1];
+  __shared__ f32x4 part[KS > 1 ? WAVES * NT * MT * SF_WAVE : 1];
   const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
   const int g = lane >> 4, c = lane & 15;
-  const int group = blockIdx.x * (kWaves / KS) + wave / KS;  // of NT row tiles
+  const int group = blockIdx.x * (WAVES / KS) + wave / KS;  // of NT row tiles
   const int row_tile_count = row_tiles(p.out_features);
   const int row0 = blockIdx.y * (16 * MT);
   WeightSource w[NT];
@@ -91,20 +89,22 @@ __global__ __launch_bounds__(kThreads) void linear_direct_kernel(Linear p) {
   }
 }
 
-template <int MT, int NT, int KS, int XDT>
+template <int MT, int NT, int KS, int WAVES, int XDT>
 void launch_direct(const Linear& p, hipStream_t s) {
-  const int groups = (row_tiles(p.out_features) - 1) / NT + 1, per = kWaves / KS;
-  linear_direct_kernel<MT, NT, KS, XDT><<<dim3((groups - 1) / per + 1, (p.rows - 1) / (16 * MT) + 1),
-                                          dim3(kThreads), 0, s>>>(p);
+  const int groups = (row_tiles(p.out_features) - 1) / NT + 1, per = WAVES / KS;
+  linear_direct_kernel<MT, NT, KS, WAVES, XDT><<<dim3((groups - 1) / per + 1, (p.rows - 1) / (16 * MT) + 1),
+                                                 dim3(WAVES * SF_WAVE), 0, s>>>(p);
 }
 
 // Many rows: a workgroup takes kRows of them by kOut of the weight's.
 template <class T>
-__global__ __launch_bounds__(T::kThreads, 2) void linear_tiled_kernel(Linear p, int row_groups) {
+__global__ __launch_bounds__(T::kThreads, 2) void linear_tiled_kernel(Linear p, int row_groups, int out_groups) {
   __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
   __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
   __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
-  const int row0 = blockIdx.x % row_groups * T::kRows, tile0 = blockIdx.x / row_groups * (T::kOut / 16);
+  int row_group, out_group;
+  tile_of(blockIdx.x, row_groups, out_groups, row_group, out_group);
+  const int row0 = row_group * T::kRows, tile0 = out_group * (T::kOut / 16);
   const int last_tile = row_tiles(p.out_features) - 1;
   f32x16 acc[T::FN][T::FM];
   multiply<T>(acc, static_cast<const uint8_t*>(p.x), p.x_scales, p.codes, p.scales, p.dim,
@@ -128,7 +128,7 @@ template <class T>
 int launch_tiled(const Linear& p, hipStream_t s) {
   const int row_groups = (p.rows - 1) / T::kRows + 1, out_groups = (p.out_features - 1) / T::kOut + 1;
   if (static_cast<int64_t>(row_groups) * out_groups > 0x7fffffff) return SF_ERR_UNSUPPORTED_SHAPE;
-  linear_tiled_kernel<T><<<dim3(row_groups * out_groups), dim3(T::kThreads), 0, s>>>(p, row_groups);
+  linear_tiled_kernel<T><<<dim3(row_groups * out_groups), dim3(T::kThreads), 0, s>>>(p, row_groups, out_groups);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
@@ -136,6 +136,36 @@ int launch_tiled(const Linear& p, hipStream_t s) {
 // Rows of 16-bit values are rounded by every wavefront that reads them, which
 // is cheaper than a launch of its own for one tile of rows only.
 constexpr int kMostRawRows = 16;
+
+int64_t groups(int n, int per) { return (n - 1) / per + 1; }
+
+// Few rows, or too small a product for tiles: 16 rows by NT row tiles of the
+// weight in a workgroup of KS wavefronts that cut the sum.
+template <int XDT>
+int launch_few(const Linear& p, hipStream_t s) {
+  const int64_t units = groups(p.rows, 16) * row_tiles(p.out_features);
+  if (XDT == kRows && units >= 2048)
+    launch_direct<2, 4, 4, 4, kRows>(p, s);
+  else if (XDT == kRows && units >= 1024)
+    launch_direct<1, 4, 4, 4, kRows>(p, s);
+  else if (units >= 320)
+    launch_direct<1, 2, 8, 8, XDT>(p, s);
+  else
+    launch_direct<1, 1, 8, 8, XDT>(p, s);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
+// The largest tiles that give the 256 CUs a workgroup each.
+int launch_rows(const Linear& p, hipStream_t s) {
+  constexpr int kCus = 256;
+  const int m = p.rows, n = p.out_features;
+  if (m <= 32 && groups(n, 128) >= kCus) return launch_tiled<Tiling<2, 1, 2, 1>>(p, s);
+  if (m > 64 && groups(m, 128) * groups(n, 256) >= kCus) return launch_tiled<Tiling<2, 2, 4, 2>>(p, s);
+  if (m > 32 && groups(m, 64) * groups(n, 128) >= kCus) return launch_tiled<Tiling<2, 2, 2, 1>>(p, s);
+  if (m > 32 && groups(m, 64) * groups(n, 64) >= kCus) return launch_tiled<Tiling<2, 2, 1, 1>>(p, s);
+  return launch_few<kRows>(p, s);
+}
 
 }  // namespace
 
@@ -165,18 +195,7 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
                     out_dtype, static_cast<char*>(out), out_stride,
                     aligned(out, 8) && out_stride % 4 == 0};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (x_dtype == kBf16)
-    launch_direct<1, 1, 4, kBf16>(p, s);
-  else if (x_dtype == kFp16)
-    launch_direct<1, 1, 4, kFp16>(p, s);
-  else if (rows <= 16)
-    launch_direct<1, 1, 4, kRows>(p, s);
-  else if (rows <= 32)
-    launch_direct<2, 2, 4, kRows>(p, s);
-  else if (rows > 128)
-    return launch_tiled<Tiling<2, 2, 4, 2>>(p, s);
-  else
-    launch_direct<4, 2, 2, kRows>(p, s);
-  SF_LAUNCH_CHECK();
-  return SF_OK;
+  if (x_dtype == kBf16) return launch_few<kBf16>(p, s);
+  if (x_dtype == kFp16) return launch_few<kFp16>(p, s);
+  return launch_rows(p, s);
 }

@@ -166,8 +166,9 @@ __device__ __forceinline__ void part_of(int count, int i, int n, int& begin, int
 // multiplied.  The scales of four tiles come together, ahead of them.
 //
 // LDS: rows keep their 128 bytes together, piece p (16 bytes) of row r in slot
-// p ^ (r & 7): the loads then take whole lines from memory, and eight lanes
-// reading a piece of eight rows meet eight different slots.  Weight pieces
+// p ^ (r / 2 & 7): the loads then take whole lines from memory, and the sixteen
+// lanes that read a piece of sixteen rows together meet sixteen different
+// places of the 64 banks, a pair of rows apart in each slot.  Weight pieces
 // stay in the operand's order.
 template <int WN_, int WM_, int FN_, int FM_>
 struct Tiling {
@@ -176,16 +177,32 @@ struct Tiling {
   static constexpr int kRows = 32 * FM * WM, kOut = 32 * FN * WN;  // of a workgroup
   static constexpr int kRowLoads = kRows / 8 / kWaves, kOutLoads = kOut / 16 / kWaves;
   static_assert(kRows / 8 % kWaves == 0 && kOut / 16 % kWaves == 0, "whole loads for a wavefront");
-  static constexpr int kRowScaleLoads = kRows / 64, kOutScaleLoads = kOut / 64;
+  static constexpr int kRowScaleLoads = (kRows + 63) / 64, kOutScaleLoads = (kOut + 63) / 64;
   struct Stage {
     uint8_t rows[kRows * kTile];
     uint8_t out[kOut * kTile / 2];
   };
   struct Scales {
-    uint8_t rows[kRows * 16];
-    uint8_t out[kOut * 16];
+    uint8_t rows[kRowScaleLoads * 1024];
+    uint8_t out[kOutScaleLoads * 1024];
   };
 };
+
+// Which tile a workgroup takes.  Neighbouring workgroups run on different XCDs,
+// each with its own L2: an XCD gets a run of the tiles, the run goes by bands of
+// kBand row groups, so that what runs together shares rows and weights there.
+constexpr int kXcds = 8, kBand = 8;
+
+__device__ __forceinline__ void tile_of(int id, int row_groups, int out_groups, int& row_group, int& out_group) {
+  const int total = row_groups * out_groups, each = total / kXcds, more = total % kXcds;
+  const int xcd = id % kXcds;
+  const int at = xcd * each + min(xcd, more) + id / kXcds;
+  const int band = at / (kBand * out_groups);
+  const int first = band * kBand, rows_here = min(kBand, row_groups - first);
+  const int in_band = at - band * kBand * out_groups;
+  row_group = first + in_band % rows_here;
+  out_group = in_band / rows_here;
+}
 
 __device__ __forceinline__ void to_lds(const uint8_t* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
@@ -234,7 +251,7 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
   for (int i = 0; i < T::kRowLoads; ++i) {
     const int row = (wave * T::kRowLoads + i) * 8 + lane / 8;
     row_from[i] = x + static_cast<int64_t>(row_at(row)) * (static_cast<int64_t>(kt) * kTile) +
-                  (lane % 8 ^ (row & 7)) * 16;
+                  (lane % 8 ^ (row / 2 & 7)) * 16;
   }
   const uint8_t* out_from[T::kOutLoads];
 #pragma unroll
@@ -288,24 +305,28 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
     }
   };
   const auto step = [&](typename T::Stage& here) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x8 a[T::FN], b[T::FM];
-#pragma unroll
-      for (int n = 0; n < T::FN; ++n)
-        a[n] = operand4(here.out + ((wn * T::FN + n) * 2 + r / 16) * 1024 + (2 * h + g) * 256 + r % 16 * 16);
+    i32x8 a[2][T::FN], b[2][T::FM];
+    const auto read = [&](int h) {
 #pragma unroll
       for (int m = 0; m < T::FM; ++m) {
         const int row = (wm * T::FM + m) * 32 + r;
         const uint8_t* at = here.rows + row * kTile;
-        b[m] = operand8(at + ((4 * h + g) ^ (row & 7)) * 16, at + ((4 * h + 2 + g) ^ (row & 7)) * 16);
+        b[h][m] = operand8(at + ((4 * h + g) ^ (row / 2 & 7)) * 16, at + ((4 * h + 2 + g) ^ (row / 2 & 7)) * 16);
       }
+#pragma unroll
+      for (int n = 0; n < T::FN; ++n)
+        a[h][n] = operand4(here.out + ((wn * T::FN + n) * 2 + r / 16) * 1024 + (2 * h + g) * 256 + r % 16 * 16);
+    };
+    read(0);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h) read(1);
 #pragma unroll
       for (int n = 0; n < T::FN; ++n)
 #pragma unroll
         for (int m = 0; m < T::FM; ++m)
           acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-              a[n], b[m], acc[n][m], 4, 0, 0, static_cast<int>(ws[n][h]), 0, static_cast<int>(xs[m][h]));
+              a[h][n], b[h][m], acc[n][m], 4, 0, 0, static_cast<int>(ws[n][h]), 0, static_cast<int>(xs[m][h]));
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
