@@ -12,8 +12,6 @@ namespace {
 
 using namespace sf_mx;
 
-constexpr int kThreads = 256, kWaves = kThreads / SF_WAVE;
-
 // The parts of an expert's record: codes of gate, up and down, then their
 // scales in that order.
 struct Record {
@@ -38,7 +36,7 @@ struct Experts {
   const int32_t* perm_pos;
   const int32_t* offsets;
   const uint16_t* route_weights;
-  int top_k, hidden, inner;
+  int top_k, hidden, inner, num_experts;
   const int32_t* slot_of_expert;
   const uint8_t* slots;
   int64_t slot_stride;
@@ -48,148 +46,297 @@ struct Experts {
   uint16_t* rows;       // bf16 [tokens * top_k, hidden]
 };
 
-// The weights of the expert of this workgroup; null where it has none to do.
-__device__ __forceinline__ const uint8_t* expert_of(const Experts& p, int e, int& begin, int& end) {
-  begin = p.offsets[e];
-  end = p.offsets[e + 1];
-  const int slot = p.slot_of_expert ? p.slot_of_expert[e] : e;
-  return begin < end && slot >= 0 ? p.slots + slot * p.slot_stride : nullptr;
+// The rows of one workgroup: up to PER of one expert's.  Chunk `id` of all
+// experts' in turn, found by every wavefront from the dispatch's offsets: a lane
+// counts the chunks of four experts, a scan over the lanes places them.
+struct Chunk {
+  const uint8_t* weights;  // null: there is no such chunk
+  int begin, end;          // its rows
+};
+
+template <int PER>
+__device__ __forceinline__ Chunk chunk_of(const Experts& p, int id) {
+  constexpr int kEach = SF_MAX_EXPERTS / SF_WAVE;
+  const int lane = threadIdx.x & (SF_WAVE - 1);
+  int first[kEach + 1], slot[kEach], before[kEach], mine = 0;
+#pragma unroll
+  for (int i = 0; i <= kEach; ++i) first[i] = p.offsets[min(lane * kEach + i, p.num_experts)];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = min(lane * kEach + i, p.num_experts - 1);
+    slot[i] = p.slot_of_expert ? p.slot_of_expert[e] : e;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    before[i] = mine;
+    if (slot[i] >= 0) mine += (first[i + 1] - first[i] + PER - 1) / PER;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < SF_WAVE; d *= 2) {
+    const int v = __shfl_up(upto, d);
+    if (lane >= d) upto += v;
+  }
+  const uint64_t past = __ballot(upto > id);
+  if (past == 0) return {nullptr, 0, 0};
+  const int owner = __builtin_ctzll(past);
+  int own_slot = 0, begin = 0, end = 0;
+  const int at = id - (upto - mine);  // of the owner's chunks
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    // The last of its experts that starts at or before `at` and has rows.
+    if (before[i] <= at && slot[i] >= 0 && first[i + 1] > first[i]) {
+      own_slot = slot[i];
+      begin = first[i] + (at - before[i]) * PER;
+      end = first[i + 1];
+    }
+  }
+  own_slot = __builtin_amdgcn_readlane(own_slot, owner);
+  begin = __builtin_amdgcn_readlane(begin, owner);
+  end = min(__builtin_amdgcn_readlane(end, owner), begin + PER);
+  return {p.slots + own_slot * p.slot_stride, begin, end};
 }
 
-// A workgroup: 32 columns of gate and up of one expert, the hidden size cut
-// over its wavefronts, so that the 32 activations are one block of the next
-// product's rows.
-template <int MT, int XDT>
-__global__ __launch_bounds__(kThreads) void gate_up_direct_kernel(Experts p) {
-  constexpr int kAhead = MT == 1 ? 2 : 1;
-  __shared__ f32x4 part[kWaves * 4 * MT * SF_WAVE];
-  int row_begin, row_end;
-  const uint8_t* weights = expert_of(p, blockIdx.y, row_begin, row_end);
-  if (!weights) return;
+// At most this many chunks.
+int64_t most_chunks(int64_t routes, int experts, int per) {
+  return min(routes, static_cast<int64_t>(experts)) + routes / per;
+}
+
+__device__ __forceinline__ float swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+
+// Where row `row` of the activations and the scale byte of its block lie.
+__device__ __forceinline__ uint8_t* act_row(const Experts& p, int row) {
+  return p.act + row * (static_cast<int64_t>(tiles(p.inner)) * kTile);
+}
+__device__ __forceinline__ uint8_t* act_scale(const Experts& p, int row, int block) {
+  return p.act_scales + row * (static_cast<int64_t>(quads(p.inner)) * 16) + block / 16 * 16 + block % 4 * 4 +
+         block / 4 % 4;
+}
+
+// Few rows.  A workgroup: 32 columns of gate and up for 16 rows of one expert,
+// the hidden size cut over its wavefronts, so that the 32 activations are one
+// block of the next product's rows.
+template <int WAVES, int XDT>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p, int blocks) {
+  constexpr int kAhead = 2;
+  __shared__ f32x4 part[WAVES * 4 * SF_WAVE];
+  const Chunk chunk = chunk_of<16>(p, blockIdx.x / blocks);
+  if (!chunk.weights) return;
   const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
   const int g = lane >> 4, c = lane & 15;
-  const int block = blockIdx.x;
-  const int64_t act_width = static_cast<int64_t>(tiles(p.inner)) * kTile;
-  const int64_t act_scale_width = static_cast<int64_t>(quads(p.inner)) * 16;
-  const int scale_at = block / 16 * 16 + block % 4 * 4 + block / 4 % 4;
+  const int block = blockIdx.x % blocks;
+  const int row = min(chunk.begin + c, chunk.end - 1);
   if (block * kBlock >= p.inner) {  // behind the activations' end, within their last tile: zeros
-    for (int i = threadIdx.x; i < (row_end - row_begin) * 8; i += kThreads) {
-      const int64_t row = row_begin + i / 8;
-      *reinterpret_cast<uint32_t*>(p.act + row * act_width + block * kBlock + i % 8 * 4) = 0;
-      if (i % 8 == 0) p.act_scales[row * act_scale_width + scale_at] = 0;
+    if (wave == 0) {
+      *reinterpret_cast<u32x2*>(act_row(p, row) + block * kBlock + 8 * g) = u32x2{0u, 0u};
+      if (g == 0) *act_scale(p, row, block) = 0;
     }
     return;
   }
   WeightSource w[4];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    w[n].set(weights, weights + p.record.gate_scales, 2 * block + n, p.hidden, lane);
-    w[2 + n].set(weights + p.record.up_codes, weights + p.record.up_scales, 2 * block + n, p.hidden, lane);
+    w[n].set(chunk.weights, chunk.weights + p.record.gate_scales, 2 * block + n, p.hidden, lane);
+    w[2 + n].set(chunk.weights + p.record.up_codes, chunk.weights + p.record.up_scales, 2 * block + n, p.hidden,
+                 lane);
   }
+  RowSource<XDT> x[1];
+  x[0].set(p.x, p.x_scales, p.perm_pos[row] / p.top_k, p.x_stride, p.hidden, g);
   int begin, end;
-  part_of(tiles(p.hidden), wave, kWaves, begin, end);
-  for (int row0 = row_begin; row0 < row_end; row0 += 16 * MT) {
-    RowSource<XDT> x[MT];
+  part_of(tiles(p.hidden), wave, WAVES, begin, end);
+  f32x4 acc[4][1] = {};
+  accumulate<1, 4, XDT, kAhead>(acc, w, x, begin, end, p.hidden, g);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int token = p.perm_pos[min(row0 + 16 * m + c, row_end - 1)] / p.top_k;
-      x[m].set(p.x, p.x_scales, token, p.x_stride, p.hidden, g);
-    }
-    f32x4 acc[4][MT] = {};
-    accumulate<MT, 4, XDT, kAhead>(acc, w, x, begin, end, p.hidden, g);
+  for (int n = 0; n < 4; ++n) part[(wave * 4 + n) * SF_WAVE + lane] = acc[n][0];
+  __syncthreads();
+  if (wave > 0) return;
+  f32x4 v[4] = {};
 #pragma unroll
-    for (int n = 0; n < 4; ++n)
+  for (int k = 0; k < WAVES; ++k)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) part[((wave * MT + m) * 4 + n) * SF_WAVE + lane] = acc[n][m];
-    __syncthreads();
-    if (wave < MT) {  // a wavefront to 16 rows: a lane 4 + 4 of its row's 32
-      const int row = row0 + 16 * wave + c;
-      f32x4 v[4] = {};
+    for (int n = 0; n < 4; ++n) v[n] += part[(k * 4 + n) * SF_WAVE + lane];
+  float a[8];  // of row c: columns 4 g .. + 3 and 16 + 4 g .. + 3 of the block
+  uint32_t top = 0;
 #pragma unroll
-      for (int k = 0; k < kWaves; ++k)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) v[n] += part[((k * MT + wave) * 4 + n) * SF_WAVE + lane];
-      float a[8];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float gate = v[i / 4][i % 4], up = v[2 + i / 4][i % 4];
-        a[i] = gate / (1.0f + __expf(-gate)) * up;
-        top = max(top, magnitude(a[i]));
-      }
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-      const uint32_t byte = scale_byte<kE4m3>(top);
-      uint32_t lo = 0, hi = 0;
-      if (byte != 255) {
-        const float s = inverse_scale(byte);
-        lo = e4m3x4(a[0] * s, a[1] * s, a[2] * s, a[3] * s);
-        hi = e4m3x4(a[4] * s, a[5] * s, a[6] * s, a[7] * s);
-      }
-      if (row < row_end) {
-        uint8_t* o = p.act + row * act_width + block * kBlock + 4 * g;
-        *reinterpret_cast<uint32_t*>(o) = lo;
-        *reinterpret_cast<uint32_t*>(o + 16) = hi;
-        if (g == 0) p.act_scales[row * act_scale_width + scale_at] = static_cast<uint8_t>(byte);
-      }
-    }
-    __syncthreads();
+  for (int i = 0; i < 8; ++i) {
+    a[i] = swiglu(v[i / 4][i % 4], v[2 + i / 4][i % 4]);
+    top = max(top, magnitude(a[i]));
+  }
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+  const uint32_t byte = scale_byte<kE4m3>(top);
+  const float s = byte == 255 ? 0.f : inverse_scale(byte);
+  if (chunk.begin + c < chunk.end) {
+    uint8_t* o = act_row(p, row) + block * kBlock + 4 * g;
+    *reinterpret_cast<uint32_t*>(o) = byte == 255 ? 0u : e4m3x4(a[0] * s, a[1] * s, a[2] * s, a[3] * s);
+    *reinterpret_cast<uint32_t*>(o + 16) = byte == 255 ? 0u : e4m3x4(a[4] * s, a[5] * s, a[6] * s, a[7] * s);
+    if (g == 0) *act_scale(p, row, block) = static_cast<uint8_t>(byte);
   }
 }
 
-// A wavefront: NT row tiles of down over the whole inner size.
-template <int MT, int NT>
-__global__ __launch_bounds__(kThreads) void down_direct_kernel(Experts p) {
-  constexpr int kAhead = MT * NT <= 2 ? 4 : 2;
-  int row_begin, row_end;
-  const uint8_t* weights = expert_of(p, blockIdx.y, row_begin, row_end);
-  if (!weights) return;
+__device__ __forceinline__ void store_row4(const Experts& p, int row, int h, f32x4 v) {
+  uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
+  if (p.hidden % 4 == 0) {
+    if (h < p.hidden)
+      *reinterpret_cast<u32x2*>(o) = u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
+  } else {
+    for (int i = 0; i < 4; ++i)
+      if (h + i < p.hidden) o[i] = sf_f32_to_bf16(v[i]);
+  }
+}
+
+__device__ __forceinline__ float route_weight(const Experts& p, int row) {
+  return p.route_weights ? sf_bf16_to_f32(p.route_weights[p.perm_pos[row]]) : 1.0f;
+}
+
+// A wavefront: NT row tiles of down for 16 rows, over the whole inner size.
+template <int WAVES, int NT>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void down_few_kernel(Experts p, int blocks) {
+  constexpr int kAhead = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+  const Chunk chunk = chunk_of<16>(p, blockIdx.x / blocks);
+  if (!chunk.weights) return;
   const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
   const int g = lane >> 4, c = lane & 15;
-  const int group = blockIdx.x * kWaves + wave, last = row_tiles(p.hidden) - 1;
+  const int group = blockIdx.x % blocks * WAVES + wave, last = row_tiles(p.hidden) - 1;
   if (group * NT > last) return;
   WeightSource w[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-    w[n].set(weights + p.record.down_codes, weights + p.record.down_scales, min(group * NT + n, last), p.inner,
-             lane);
-  for (int row0 = row_begin; row0 < row_end; row0 += 16 * MT) {
-    RowSource<kRows> x[MT];
-    float route[MT];
+    w[n].set(chunk.weights + p.record.down_codes, chunk.weights + p.record.down_scales, min(group * NT + n, last),
+             p.inner, lane);
+  const int row = min(chunk.begin + c, chunk.end - 1);
+  RowSource<kRows> x[1];
+  x[0].set(p.act, p.act_scales, row, 0, p.inner, g);
+  const float route = route_weight(p, row);
+  f32x4 acc[NT][1] = {};
+  accumulate<1, NT, kRows, kAhead>(acc, w, x, 0, tiles(p.inner), p.inner, g);
+  if (chunk.begin + c >= chunk.end) return;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = min(row0 + 16 * m + c, row_end - 1);
-      x[m].set(p.act, p.act_scales, row, 0, p.inner, g);
-      route[m] = p.route_weights ? sf_bf16_to_f32(p.route_weights[p.perm_pos[row]]) : 1.0f;
-    }
-    f32x4 acc[NT][MT] = {};
-    accumulate<MT, NT, kRows, kAhead>(acc, w, x, 0, tiles(p.inner), p.inner, g);
+  for (int n = 0; n < NT; ++n) store_row4(p, row, (group * NT + n) * 16 + 4 * g, acc[n][0] * route);
+}
+
+// Many rows by tiles.  Half of a wavefront's weight rows are gate's, the other
+// half the same of up's.
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void gate_up_tiled_kernel(Experts p, int blocks) {
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
+  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
+  const Chunk chunk = chunk_of<T::kRows>(p, blockIdx.x / blocks);
+  if (!chunk.weights) return;
+  const int col0 = blockIdx.x % blocks * (T::kOut / 2);
+  const int up_tiles = row_tiles(p.inner);
+  f32x16 acc[T::FN][T::FM];
+  multiply<T>(acc, static_cast<const uint8_t*>(p.x), p.x_scales, chunk.weights,
+              chunk.weights + p.record.gate_scales, p.hidden,
+              [&](int r) { return p.perm_pos[min(chunk.begin + r, chunk.end - 1)] / p.top_k; },
+              [&](int i) {
+                const int wn = i / (2 * T::FN), j = i % (2 * T::FN);
+                const int tile = min(col0 / 16 + wn * T::FN + j % T::FN, up_tiles - 1);
+                return j < T::FN ? tile : up_tiles + tile;
+              },
+              stage0, stage1, scales);
+  const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
+  const int wn = wave / T::WM, wm = wave % T::WM, g = lane >> 5;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = row0 + 16 * m + c;
-      if (row >= row_end) continue;
+  for (int m = 0; m < T::FM; ++m) {
+    const int row = chunk.begin + (wm * T::FM + m) * 32 + (lane & 31);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int h = (group * NT + n) * 16 + 4 * g;
-        const f32x4 v = acc[n][m] * route[m];
-        uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
-        if (h + 4 <= p.hidden && p.hidden % 4 == 0) {
-          *reinterpret_cast<u32x2*>(o) = u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
-        } else {
-          for (int i = 0; i < 4; ++i)
-            if (h + i < p.hidden) o[i] = sf_f32_to_bf16(v[i]);
-        }
+    for (int n = 0; n < T::FN / 2; ++n) {
+      const int block = col0 / kBlock + wn * (T::FN / 2) + n;
+      const bool held = block * kBlock < p.inner;
+      float a[16];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        a[i] = held ? swiglu(acc[n][m][i], acc[T::FN / 2 + n][m][i]) : 0.f;
+        top = max(top, magnitude(a[i]));
+      }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+      const uint32_t byte = scale_byte<kE4m3>(top);
+      const float s = byte == 255 ? 0.f : inverse_scale(byte);
+      if (row < chunk.end && block < tiles(p.inner) * 4) {
+        uint8_t* o = act_row(p, row) + block * kBlock + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint32_t*>(o + 8 * i) =
+              byte == 255 ? 0u : e4m3x4(a[4 * i] * s, a[4 * i + 1] * s, a[4 * i + 2] * s, a[4 * i + 3] * s);
+        if (g == 0) *act_scale(p, row, block) = static_cast<uint8_t>(byte);
       }
     }
   }
 }
 
-template <int MT, int XDT>
-void launch_direct(const Experts& p, int num_experts, hipStream_t s) {
-  gate_up_direct_kernel<MT, XDT><<<dim3(tiles(p.inner) * 4, num_experts), dim3(kThreads), 0, s>>>(p);
-  constexpr int NT = 2;
-  const int groups = (row_tiles(p.hidden) - 1) / NT + 1;
-  down_direct_kernel<MT, NT><<<dim3((groups - 1) / kWaves + 1, num_experts), dim3(kThreads), 0, s>>>(p);
+template <class T>
+__global__ __launch_bounds__(T::kThreads, 2) void down_tiled_kernel(Experts p, int blocks) {
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
+  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
+  const Chunk chunk = chunk_of<T::kRows>(p, blockIdx.x / blocks);
+  if (!chunk.weights) return;
+  const int tile0 = blockIdx.x % blocks * (T::kOut / 16), last = row_tiles(p.hidden) - 1;
+  f32x16 acc[T::FN][T::FM];
+  multiply<T>(acc, p.act, p.act_scales, chunk.weights + p.record.down_codes, chunk.weights + p.record.down_scales,
+              p.inner, [&](int r) { return min(chunk.begin + r, chunk.end - 1); },
+              [&](int i) { return min(tile0 + i, last); }, stage0, stage1, scales);
+  const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
+  const int wn = wave / T::WM, wm = wave % T::WM;
+#pragma unroll
+  for (int m = 0; m < T::FM; ++m) {
+    const int row = chunk.begin + (wm * T::FM + m) * 32 + (lane & 31);
+    if (row >= chunk.end) continue;
+    const float route = route_weight(p, row);
+#pragma unroll
+    for (int n = 0; n < T::FN; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        store_row4(p, row, tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 4 * (lane >> 5),
+                   f32x4{acc[n][m][4 * i], acc[n][m][4 * i + 1], acc[n][m][4 * i + 2], acc[n][m][4 * i + 3]} * route);
+  }
+}
+
+int groups(int n, int per) { return (n - 1) / per + 1; }
+
+constexpr int64_t kMostGroups = 0x7fffffff;
+
+template <int WAVES, int XDT>
+int gate_up_few(const Experts& p, int64_t routes, hipStream_t s) {
+  const int blocks = tiles(p.inner) * 4;
+  const int64_t grid = most_chunks(routes, p.num_experts, 16) * blocks;
+  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  gate_up_few_kernel<WAVES, XDT><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
+template <int WAVES, int NT>
+int down_few(const Experts& p, int64_t routes, hipStream_t s) {
+  const int blocks = groups(groups(row_tiles(p.hidden), NT), WAVES);
+  const int64_t grid = most_chunks(routes, p.num_experts, 16) * blocks;
+  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  down_few_kernel<WAVES, NT><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
+template <class T>
+int gate_up_tiled(const Experts& p, int64_t routes, hipStream_t s) {
+  const int blocks = groups(tiles(p.inner) * 4, T::kOut / 64);
+  const int64_t grid = most_chunks(routes, p.num_experts, T::kRows) * blocks;
+  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  gate_up_tiled_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s>>>(p, blocks);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
+template <class T>
+int down_tiled(const Experts& p, int64_t routes, hipStream_t s) {
+  const int blocks = groups(p.hidden, T::kOut);
+  const int64_t grid = most_chunks(routes, p.num_experts, T::kRows) * blocks;
+  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  down_tiled_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s>>>(p, blocks);
+  SF_LAUNCH_CHECK();
+  return SF_OK;
 }
 
 }  // namespace
@@ -231,17 +378,26 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
     if (tokens > 16) return SF_ERR_UNSUPPORTED_SHAPE;
   }
   const Experts p = {x, static_cast<const uint8_t*>(x_scales), x_stride, perm_pos, offsets,
-                     static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size,
+                     static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size, num_experts,
                      slot_of_expert, static_cast<const uint8_t*>(slots), slot_stride,
                      record_of(hidden_size, intermediate_size), static_cast<uint8_t*>(act),
                      static_cast<uint8_t*>(act_scales), static_cast<uint16_t*>(out_rows)};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
+  // By the routes to an expert on average: how many rows share its weights.
+  int rc;
   if (x_dtype == kBf16)
-    launch_direct<1, kBf16>(p, num_experts, s);
-  else if (static_cast<int64_t>(tokens) * top_k <= 8 * num_experts)
-    launch_direct<1, kRows>(p, num_experts, s);
+    rc = gate_up_few<4, kBf16>(p, routes, s);
+  else if (routes <= num_experts)
+    rc = gate_up_few<4, kRows>(p, routes, s);
+  else if (routes <= 16 * num_experts)
+    rc = gate_up_tiled<Tiling<4, 1, 2, 1>>(p, routes, s);
+  else if (routes <= 96 * num_experts)
+    rc = gate_up_tiled<Tiling<4, 1, 2, 2>>(p, routes, s);
   else
-    launch_direct<4, kRows>(p, num_experts, s);
-  SF_LAUNCH_CHECK();
-  return SF_OK;
+    rc = gate_up_tiled<Tiling<2, 2, 4, 2>>(p, routes, s);
+  if (rc) return rc;
+  if (routes <= 8 * num_experts) return down_few<1, 2>(p, routes, s);
+  if (routes <= 96 * num_experts) return down_tiled<Tiling<4, 1, 2, 2>>(p, routes, s);
+  return down_tiled<Tiling<2, 2, 4, 2>>(p, routes, s);
 }

@@ -258,6 +258,12 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
   for (int i = 0; i < T::kOutLoads; ++i)
     out_from[i] = w + (static_cast<int64_t>(out_tile(wave * T::kOutLoads + i)) * kt) * 1024;
 
+  const uint8_t* scales_from[(T::kRowScaleLoads + T::kWaves - 1) / T::kWaves];
+#pragma unroll
+  for (int i = 0; i < (T::kRowScaleLoads + T::kWaves - 1) / T::kWaves; ++i)  // 64 rows each
+    scales_from[i] = x_scales + static_cast<int64_t>(row_at(min((wave + i * T::kWaves) * 64 + lane, T::kRows - 1))) *
+                                    (static_cast<int64_t>(kq) * 16);
+
   const auto load_stage = [&](typename T::Stage& s, int t) {
 #pragma unroll
     for (int i = 0; i < T::kRowLoads; ++i)
@@ -270,10 +276,8 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
     typename T::Scales& s = scales[q % 2];
 #pragma unroll
     for (int i = 0; i < (T::kRowScaleLoads + T::kWaves - 1) / T::kWaves; ++i) {
-      const int at = wave + i * T::kWaves;  // 64 rows
-      if (at < T::kRowScaleLoads)
-        to_lds(x_scales + static_cast<int64_t>(row_at(at * 64 + lane)) * (static_cast<int64_t>(kq) * 16) + q * 16,
-               s.rows + at * 1024);
+      const int at = wave + i * T::kWaves;
+      if (at < T::kRowScaleLoads) to_lds(scales_from[i] + q * 16, s.rows + at * 1024);
     }
 #pragma unroll
     for (int i = 0; i < (T::kOutScaleLoads + T::kWaves - 1) / T::kWaves; ++i) {
