@@ -682,6 +682,23 @@ int sf_mx_grouped_swiglu(int x_dtype, const void *x, const void *x_scales,
                          int64_t slot_stride, void *act, void *act_scales,
                          void *out_rows, sf_stream_t stream);
 
+/*
+ * K16 for few tokens, without a dispatch: out[t] = bf16(sum over k of
+ * route_weights[t, k] * expert(index[t, k])(x[t])), summed in fp32.
+ *   index           int64 [tokens, top_k]; an expert outside 0 .. num_experts - 1
+ *                   or in no slot counts for nothing
+ *   route_weights   bf16 [tokens, top_k]
+ *   out             bf16 [tokens, hidden_size]
+ * The rest as above; out 2-byte aligned.
+ */
+int sf_mx_routed_swiglu(int x_dtype, const void *x, const void *x_scales,
+                        int64_t x_stride, const int64_t *index,
+                        const void *route_weights, int tokens, int top_k,
+                        int hidden_size, int intermediate_size, int num_experts,
+                        const int32_t *slot_of_expert, const void *slots,
+                        int64_t slot_stride, void *act, void *act_scales,
+                        void *out, sf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -113,21 +113,17 @@ __device__ __forceinline__ uint8_t* act_scale(const Experts& p, int row, int blo
          block / 4 % 4;
 }
 
-// Few rows.  A workgroup: 32 columns of gate and up for 16 rows of one expert,
-// the hidden size cut over its wavefronts, so that the 32 activations are one
-// block of the next product's rows.
-template <int WAVES, int XDT>
-__global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p, int blocks) {
-  constexpr int kAhead = 2;
-  __shared__ f32x4 part[WAVES * 4 * SF_WAVE];
-  const Chunk chunk = chunk_of<16>(p, blockIdx.x / blocks);
-  if (!chunk.weights) return;
+// 32 columns of gate and up for 16 rows of one expert, the hidden size cut over
+// the workgroup's wavefronts, so that the 32 activations are one block of the
+// next product's rows.  Lane c of sixteen: x's row x_row, to row `row` of the
+// activations where `live`.
+template <int WAVES, int XDT, int AHEAD>
+__device__ __forceinline__ void gate_up_block(const Experts& p, const uint8_t* weights, int block, int64_t x_row,
+                                              int row, bool live, f32x4* part) {
   const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
-  const int g = lane >> 4, c = lane & 15;
-  const int block = blockIdx.x % blocks;
-  const int row = min(chunk.begin + c, chunk.end - 1);
+  const int g = lane >> 4;
   if (block * kBlock >= p.inner) {  // behind the activations' end, within their last tile: zeros
-    if (wave == 0) {
+    if (wave == 0 && live) {
       *reinterpret_cast<u32x2*>(act_row(p, row) + block * kBlock + 8 * g) = u32x2{0u, 0u};
       if (g == 0) *act_scale(p, row, block) = 0;
     }
@@ -136,16 +132,15 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p,
   WeightSource w[4];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    w[n].set(chunk.weights, chunk.weights + p.record.gate_scales, 2 * block + n, p.hidden, lane);
-    w[2 + n].set(chunk.weights + p.record.up_codes, chunk.weights + p.record.up_scales, 2 * block + n, p.hidden,
-                 lane);
+    w[n].set(weights, weights + p.record.gate_scales, 2 * block + n, p.hidden, lane);
+    w[2 + n].set(weights + p.record.up_codes, weights + p.record.up_scales, 2 * block + n, p.hidden, lane);
   }
   RowSource<XDT> x[1];
-  x[0].set(p.x, p.x_scales, p.perm_pos[row] / p.top_k, p.x_stride, p.hidden, g);
+  x[0].set(p.x, p.x_scales, x_row, p.x_stride, p.hidden, g);
   int begin, end;
   part_of(tiles(p.hidden), wave, WAVES, begin, end);
   f32x4 acc[4][1] = {};
-  accumulate<1, 4, XDT, kAhead>(acc, w, x, begin, end, p.hidden, g);
+  accumulate<1, 4, XDT, AHEAD>(acc, w, x, begin, end, p.hidden, g);
 #pragma unroll
   for (int n = 0; n < 4; ++n) part[(wave * 4 + n) * SF_WAVE + lane] = acc[n][0];
   __syncthreads();
@@ -166,12 +161,24 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p,
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
   const uint32_t byte = scale_byte<kE4m3>(top);
   const float s = byte == 255 ? 0.f : inverse_scale(byte);
-  if (chunk.begin + c < chunk.end) {
+  if (live) {
     uint8_t* o = act_row(p, row) + block * kBlock + 4 * g;
     *reinterpret_cast<uint32_t*>(o) = byte == 255 ? 0u : e4m3x4(a[0] * s, a[1] * s, a[2] * s, a[3] * s);
     *reinterpret_cast<uint32_t*>(o + 16) = byte == 255 ? 0u : e4m3x4(a[4] * s, a[5] * s, a[6] * s, a[7] * s);
     if (g == 0) *act_scale(p, row, block) = static_cast<uint8_t>(byte);
   }
+}
+
+// Few rows: a workgroup takes 16 of one expert's.
+template <int WAVES, int XDT>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p, int blocks) {
+  __shared__ f32x4 part[WAVES * 4 * SF_WAVE];
+  const Chunk chunk = chunk_of<16>(p, blockIdx.x / blocks);
+  if (!chunk.weights) return;
+  const int c = threadIdx.x & 15;
+  const int row = min(chunk.begin + c, chunk.end - 1);
+  gate_up_block<WAVES, XDT, 2>(p, chunk.weights, blockIdx.x % blocks, p.perm_pos[row] / p.top_k, row,
+                               chunk.begin + c < chunk.end, part);
 }
 
 __device__ __forceinline__ void store_row4(const Experts& p, int row, int h, f32x4 v) {
@@ -218,13 +225,8 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void down_few_kernel(Experts p, in
 // Many rows by tiles.  Half of a wavefront's weight rows are gate's, the other
 // half the same of up's.
 template <class T>
-__global__ __launch_bounds__(T::kThreads, 2) void gate_up_tiled_kernel(Experts p, int blocks) {
-  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
-  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
-  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
-  const Chunk chunk = chunk_of<T::kRows>(p, blockIdx.x / blocks);
-  if (!chunk.weights) return;
-  const int col0 = blockIdx.x % blocks * (T::kOut / 2);
+__device__ __forceinline__ void gate_up_tile(const Experts& p, const Chunk& chunk, int col0, typename T::Stage& stage0,
+                                             typename T::Stage& stage1, typename T::Scales (&scales)[2]) {
   const int up_tiles = row_tiles(p.inner);
   f32x16 acc[T::FN][T::FM];
   multiply<T>(acc, static_cast<const uint8_t*>(p.x), p.x_scales, chunk.weights,
@@ -268,13 +270,9 @@ __global__ __launch_bounds__(T::kThreads, 2) void gate_up_tiled_kernel(Experts p
 }
 
 template <class T>
-__global__ __launch_bounds__(T::kThreads, 2) void down_tiled_kernel(Experts p, int blocks) {
-  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
-  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
-  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
-  const Chunk chunk = chunk_of<T::kRows>(p, blockIdx.x / blocks);
-  if (!chunk.weights) return;
-  const int tile0 = blockIdx.x % blocks * (T::kOut / 16), last = row_tiles(p.hidden) - 1;
+__device__ __forceinline__ void down_tile(const Experts& p, const Chunk& chunk, int tile0, typename T::Stage& stage0,
+                                          typename T::Stage& stage1, typename T::Scales (&scales)[2]) {
+  const int last = row_tiles(p.hidden) - 1;
   f32x16 acc[T::FN][T::FM];
   multiply<T>(acc, p.act, p.act_scales, chunk.weights + p.record.down_codes, chunk.weights + p.record.down_scales,
               p.inner, [&](int r) { return min(chunk.begin + r, chunk.end - 1); },
@@ -292,6 +290,106 @@ __global__ __launch_bounds__(T::kThreads, 2) void down_tiled_kernel(Experts p, i
       for (int i = 0; i < 4; ++i)
         store_row4(p, row, tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 4 * (lane >> 5),
                    f32x4{acc[n][m][4 * i], acc[n][m][4 * i + 1], acc[n][m][4 * i + 2], acc[n][m][4 * i + 3]} * route);
+  }
+}
+
+// A chunk's workgroup takes the lowest of its tilings that holds its rows: an
+// expert's last chunk is rarely full.  All have the same wavefronts and weight
+// rows, the tallest first.
+template <class T, class...>
+struct First {
+  using type = T;
+};
+
+template <bool GATE_UP, class T, class... Lower>
+__device__ __forceinline__ void fitting_tile(const Experts& p, const Chunk& chunk, int out0, void* stage0, void* stage1,
+                                             void* scales) {
+  if constexpr (sizeof...(Lower) > 0) {
+    if (chunk.end - chunk.begin <= First<Lower...>::type::kRows) {
+      fitting_tile<GATE_UP, Lower...>(p, chunk, out0, stage0, stage1, scales);
+      return;
+    }
+  }
+  auto& s0 = *static_cast<typename T::Stage*>(stage0);
+  auto& s1 = *static_cast<typename T::Stage*>(stage1);
+  auto& sc = *static_cast<typename T::Scales(*)[2]>(scales);
+  if constexpr (GATE_UP)
+    gate_up_tile<T>(p, chunk, out0, s0, s1, sc);
+  else
+    down_tile<T>(p, chunk, out0, s0, s1, sc);
+}
+
+template <bool GATE_UP, class T, class... Lower>
+__global__ __launch_bounds__(T::kThreads, 2) void experts_tiled_kernel(Experts p, int blocks) {
+  static_assert(((Lower::kThreads == T::kThreads && Lower::kOut == T::kOut && Lower::kRows < T::kRows) && ...), "");
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
+  __shared__ __attribute__((aligned(16))) typename T::Stage stage1;
+  __shared__ __attribute__((aligned(16))) typename T::Scales scales[2];
+  // Eight chunks in turn: neighbouring workgroups run on different XCDs, so a
+  // chunk's stay on one and read its rows from one L2.
+  const int id = blockIdx.x / kXcds;
+  const Chunk chunk = chunk_of<T::kRows>(p, id / blocks * kXcds + blockIdx.x % kXcds);
+  if (!chunk.weights) return;
+  const int out0 = id % blocks * (GATE_UP ? T::kOut / 2 : T::kOut / 16);
+  fitting_tile<GATE_UP, T, Lower...>(p, chunk, out0, &stage0, &stage1, &scales);
+}
+
+// ------------------------------------------------ a token's own few routes --
+// Routes that hardly share experts, without a dispatch: each multiplies its
+// token's row by its expert's weights, the second kernel adds a token's up.
+struct Routes {
+  const int64_t* index;
+  const uint16_t* weights;
+  uint16_t* out;  // bf16 [tokens, hidden]
+};
+
+__device__ __forceinline__ const uint8_t* weights_of(const Experts& p, int64_t e) {
+  if (e < 0 || e >= p.num_experts) return nullptr;
+  const int slot = p.slot_of_expert ? p.slot_of_expert[e] : static_cast<int>(e);
+  return slot < 0 ? nullptr : p.slots + slot * p.slot_stride;
+}
+
+template <int WAVES, int XDT>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void routed_gate_up_kernel(Experts p, Routes r, int blocks) {
+  __shared__ f32x4 part[WAVES * 4 * SF_WAVE];
+  const int route = blockIdx.x / blocks;
+  const uint8_t* weights = weights_of(p, r.index[route]);
+  if (!weights) return;
+  gate_up_block<WAVES, XDT, 2>(p, weights, blockIdx.x % blocks, route / p.top_k, route, (threadIdx.x & 15) == 0, part);
+}
+
+// A workgroup: 16 columns of one token's output.  Its wavefronts take the
+// routes in turn, and parts of the inner size where there are fewer routes.
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * SF_WAVE) void routed_down_kernel(Experts p, Routes r, int cuts) {
+  __shared__ float part[WAVES][16];
+  const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
+  const int g = lane >> 4;
+  const int all = row_tiles(p.hidden), token = blockIdx.x / all, tile = blockIdx.x % all;
+  f32x4 sum = {};
+  for (int item = wave; item < p.top_k * cuts; item += WAVES) {  // wave-uniform
+    const int route = token * p.top_k + item / cuts;
+    const uint8_t* weights = weights_of(p, r.index[route]);
+    if (!weights) continue;
+    WeightSource w[1];
+    w[0].set(weights + p.record.down_codes, weights + p.record.down_scales, tile, p.inner, lane);
+    RowSource<kRows> x[1];
+    x[0].set(p.act, p.act_scales, route, 0, p.inner, g);
+    int begin, end;
+    part_of(tiles(p.inner), item % cuts, cuts, begin, end);
+    f32x4 acc[1][1] = {};
+    accumulate<1, 1, kRows, 6>(acc, w, x, begin, end, p.inner, g);
+    sum += acc[0][0] * sf_bf16_to_f32(r.weights[route]);
+  }
+  if ((lane & 15) == 0)
+    for (int i = 0; i < 4; ++i) part[wave][4 * g + i] = sum[i];
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) v += part[k][threadIdx.x];
+    const int h = tile * 16 + threadIdx.x;
+    if (h < p.hidden) r.out[static_cast<int64_t>(token) * p.hidden + h] = sf_f32_to_bf16(v);
   }
 }
 
@@ -319,23 +417,55 @@ int down_few(const Experts& p, int64_t routes, hipStream_t s) {
   return SF_OK;
 }
 
-template <class T>
-int gate_up_tiled(const Experts& p, int64_t routes, hipStream_t s) {
-  const int blocks = groups(tiles(p.inner) * 4, T::kOut / 64);
-  const int64_t grid = most_chunks(routes, p.num_experts, T::kRows) * blocks;
-  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
-  gate_up_tiled_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s>>>(p, blocks);
+template <bool GATE_UP, class T, class... Lower>
+int tiled(const Experts& p, int64_t routes, hipStream_t s) {
+  const int blocks = GATE_UP ? groups(tiles(p.inner) * 4, T::kOut / 64) : groups(p.hidden, T::kOut);
+  const int64_t chunks = (most_chunks(routes, p.num_experts, T::kRows) + kXcds - 1) / kXcds * kXcds;
+  if (chunks * blocks > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  experts_tiled_kernel<GATE_UP, T, Lower...>
+      <<<dim3(static_cast<unsigned>(chunks * blocks)), dim3(T::kThreads), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
 
-template <class T>
-int down_tiled(const Experts& p, int64_t routes, hipStream_t s) {
-  const int blocks = groups(p.hidden, T::kOut);
-  const int64_t grid = most_chunks(routes, p.num_experts, T::kRows) * blocks;
-  if (grid > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
-  down_tiled_kernel<T><<<dim3(static_cast<unsigned>(grid)), dim3(T::kThreads), 0, s>>>(p, blocks);
+using Tiles32 = Tiling<4, 1, 2, 1>;
+using Tiles64 = Tiling<4, 1, 2, 2>;
+using Tiles128 = Tiling<2, 2, 4, 2>;
+
+template <int WAVES, int XDT>
+int routed(const Experts& p, const Routes& r, int64_t routes, hipStream_t s) {
+  const int blocks = tiles(p.inner) * 4;
+  const int64_t down = routes / p.top_k * row_tiles(p.hidden);
+  if (routes * blocks > kMostGroups || down > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
+  routed_gate_up_kernel<WAVES, XDT>
+      <<<dim3(static_cast<unsigned>(routes * blocks)), dim3(WAVES * SF_WAVE), 0, s>>>(p, r, blocks);
   SF_LAUNCH_CHECK();
+  routed_down_kernel<WAVES>
+      <<<dim3(static_cast<unsigned>(down)), dim3(WAVES * SF_WAVE), 0, s>>>(p, r, max(1, WAVES / p.top_k));
+  SF_LAUNCH_CHECK();
+  return SF_OK;
+}
+
+// What both entry points ask of their arguments.
+int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, int tokens, int top_k, int hidden_size,
+          int intermediate_size, int num_experts, const void* slots, int64_t slot_stride, const void* act,
+          const void* act_scales) {
+  if (tokens < 0 || top_k < 1 || num_experts < 1 || x_stride < 0 || (x_dtype != kBf16 && x_dtype != kRows))
+    return SF_ERR_INVALID_ARGUMENT;
+  const int64_t bytes = sf_mx_expert_bytes(hidden_size, intermediate_size);
+  if (bytes < 0) return SF_ERR_INVALID_ARGUMENT;
+  if (num_experts > SF_MAX_EXPERTS || top_k > SF_MAX_TOPK) return SF_ERR_TOO_MANY_EXPERTS;
+  if (static_cast<int64_t>(tokens) * top_k > 1 << 28) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (tokens == 0) return SF_OK;
+  if (!x || (x_dtype == kRows && !x_scales) || !slots || !act || !act_scales || slot_stride < bytes)
+    return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !aligned(slots, 16) || slot_stride % 16 || !aligned(act, 16) || !aligned(act_scales, 4) ||
+      (x_dtype == kRows && !aligned(x_scales, 4)))
+    return SF_ERR_MISALIGNED;
+  if (x_dtype != kRows) {
+    if (x_stride % 8 || hidden_size % 8) return SF_ERR_MISALIGNED;
+    if (tokens > 16) return SF_ERR_UNSUPPORTED_SHAPE;
+  }
   return SF_OK;
 }
 
@@ -360,23 +490,12 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
                                     int intermediate_size, int num_experts, const int32_t* slot_of_expert,
                                     const void* slots, int64_t slot_stride, void* act, void* act_scales,
                                     void* out_rows, sf_stream_t stream) {
-  if (tokens < 0 || top_k < 1 || num_experts < 1 || x_stride < 0 || (x_dtype != kBf16 && x_dtype != kRows))
-    return SF_ERR_INVALID_ARGUMENT;
-  const int64_t bytes = sf_mx_expert_bytes(hidden_size, intermediate_size);
-  if (bytes < 0) return SF_ERR_INVALID_ARGUMENT;
-  if (num_experts > SF_MAX_EXPERTS || top_k > SF_MAX_TOPK) return SF_ERR_TOO_MANY_EXPERTS;
-  if (static_cast<int64_t>(tokens) * top_k > 1 << 28) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
+                           slots, slot_stride, act, act_scales))
+    return rc;
   if (tokens == 0) return SF_OK;
-  if (!x || (x_dtype == kRows && !x_scales) || !perm_pos || !offsets || !slots || !act || !act_scales ||
-      !out_rows || slot_stride < bytes)
-    return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(x, 16) || !aligned(slots, 16) || slot_stride % 16 || !aligned(act, 16) || !aligned(act_scales, 4) ||
-      !aligned(out_rows, 8) || (x_dtype == kRows && !aligned(x_scales, 4)))
-    return SF_ERR_MISALIGNED;
-  if (x_dtype != kRows) {
-    if (x_stride % 8 || hidden_size % 8) return SF_ERR_MISALIGNED;
-    if (tokens > 16) return SF_ERR_UNSUPPORTED_SHAPE;
-  }
+  if (!perm_pos || !offsets || !out_rows) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(out_rows, 8)) return SF_ERR_MISALIGNED;
   const Experts p = {x, static_cast<const uint8_t*>(x_scales), x_stride, perm_pos, offsets,
                      static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size, num_experts,
                      slot_of_expert, static_cast<const uint8_t*>(slots), slot_stride,
@@ -391,13 +510,44 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
   else if (routes <= num_experts)
     rc = gate_up_few<4, kRows>(p, routes, s);
   else if (routes <= 16 * num_experts)
-    rc = gate_up_tiled<Tiling<4, 1, 2, 1>>(p, routes, s);
+    rc = tiled<true, Tiles32>(p, routes, s);
   else if (routes <= 96 * num_experts)
-    rc = gate_up_tiled<Tiling<4, 1, 2, 2>>(p, routes, s);
+    rc = tiled<true, Tiles64, Tiles32>(p, routes, s);
   else
-    rc = gate_up_tiled<Tiling<2, 2, 4, 2>>(p, routes, s);
+    rc = tiled<true, Tiles128, Tiles64, Tiles32>(p, routes, s);
   if (rc) return rc;
   if (routes <= 8 * num_experts) return down_few<1, 2>(p, routes, s);
-  if (routes <= 96 * num_experts) return down_tiled<Tiling<4, 1, 2, 2>>(p, routes, s);
-  return down_tiled<Tiling<2, 2, 4, 2>>(p, routes, s);
+  if (routes <= 96 * num_experts) return tiled<false, Tiles64, Tiles32>(p, routes, s);
+  return tiled<false, Tiles128, Tiles64, Tiles32>(p, routes, s);
+}
+
+extern "C" int sf_mx_routed_swiglu(int x_dtype, const void* x, const void* x_scales, int64_t x_stride,
+                                   const int64_t* index, const void* route_weights, int tokens, int top_k,
+                                   int hidden_size, int intermediate_size, int num_experts,
+                                   const int32_t* slot_of_expert, const void* slots, int64_t slot_stride, void* act,
+                                   void* act_scales, void* out, sf_stream_t stream) {
+  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
+                           slots, slot_stride, act, act_scales))
+    return rc;
+  if (tokens == 0) return SF_OK;
+  if (!index || !route_weights || !out) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(index, 8) || !aligned(route_weights, 2) || !aligned(out, 2)) return SF_ERR_MISALIGNED;
+  Experts p = {};
+  p.x = x;
+  p.x_scales = static_cast<const uint8_t*>(x_scales);
+  p.x_stride = x_stride;
+  p.top_k = top_k;
+  p.hidden = hidden_size;
+  p.inner = intermediate_size;
+  p.num_experts = num_experts;
+  p.slot_of_expert = slot_of_expert;
+  p.slots = static_cast<const uint8_t*>(slots);
+  p.slot_stride = slot_stride;
+  p.record = record_of(hidden_size, intermediate_size);
+  p.act = static_cast<uint8_t*>(act);
+  p.act_scales = static_cast<uint8_t*>(act_scales);
+  const Routes r = {index, static_cast<const uint16_t*>(route_weights), static_cast<uint16_t*>(out)};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
+  return x_dtype == kBf16 ? routed<8, kBf16>(p, r, routes, s) : routed<8, kRows>(p, r, routes, s);
 }

@@ -11,6 +11,7 @@ plain order in which checkpoints hold microscaled weights.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -23,6 +24,14 @@ def _up(n: int, to: int) -> int:
     return -(-n // to)
 
 
+def _rows(shape: tuple) -> int:
+    n = 1
+    for s in shape[:-1]:
+        n *= s
+    return n
+
+
+@functools.lru_cache(maxsize=256)
 def row_bytes(dim: int) -> tuple[int, int]:
     """Bytes of codes and of scales that one of MXRows' rows takes."""
     return _up(dim, TILE) * TILE, _up(dim, 4 * TILE) * 16
@@ -40,39 +49,58 @@ def _check(name: str, t: torch.Tensor, nbytes: int) -> None:
         raise ValueError(f"{name} must be {nbytes} contiguous uint8")
 
 
-@dataclass(frozen=True, eq=False)
 class MXRows:
     """Activations in e4m3: ``shape`` [..., dim], ``dtype`` the type they came
     in and a product with them gives."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    shape: tuple
-    dtype: torch.dtype
+    __slots__ = ("shape", "dtype", "rows", "dim", "_codes", "_scales", "_both")
 
-    def __post_init__(self) -> None:
-        if len(self.shape) < 1 or self.shape[-1] < 1:
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple,
+                 dtype: torch.dtype) -> None:
+        shape = tuple(shape)
+        if len(shape) < 1 or shape[-1] < 1:
             raise ValueError("rows must have at least one column")
+        self.shape, self.dtype, self.dim = shape, dtype, shape[-1]
+        self.rows = _rows(shape)
         code, scale = row_bytes(self.dim)
-        _check("codes", self.codes, self.rows * code)
-        _check("scales", self.scales, self.rows * scale)
-        if self.codes.device != self.scales.device:
+        _check("codes", codes, self.rows * code)
+        _check("scales", scales, self.rows * scale)
+        if codes.device != scales.device:
             raise ValueError("codes and scales must share a device")
+        self._codes, self._scales, self._both = codes, scales, None
+
+    @classmethod
+    def _of(cls, both: torch.Tensor, shape: tuple, rows: int, dtype: torch.dtype) -> "MXRows":
+        """Over one buffer, the codes in front (what the operators make: a
+        call that only passes them on makes no views)."""
+        new = cls.__new__(cls)
+        new.shape, new.dtype, new.rows, new.dim = shape, dtype, rows, shape[-1]
+        new._codes = new._scales = None
+        new._both = both
+        return new
 
     @property
-    def dim(self) -> int:
-        return self.shape[-1]
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            self._codes = self._both[:self.rows * row_bytes(self.dim)[0]]
+        return self._codes
 
     @property
-    def rows(self) -> int:
-        n = 1
-        for s in self.shape[:-1]:
-            n *= s
-        return n
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._both[self.rows * row_bytes(self.dim)[0]:]
+        return self._scales
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._both is None else self._both).device
+
+    def _pointers(self) -> tuple[int, int]:
+        """Addresses of the codes and of the scales."""
+        if self._both is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self._both.data_ptr()
+        return at, at + self.rows * row_bytes(self.dim)[0]
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values held, [..., dim] (exact in any of the three types but for
@@ -115,6 +143,9 @@ class MXWeight:
     @property
     def device(self) -> torch.device:
         return self.codes.device
+
+    def _pointers(self) -> tuple[int, int]:
+        return self.codes.data_ptr(), self.scales.data_ptr()
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values held, [rows, dim]."""

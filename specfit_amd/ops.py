@@ -1364,21 +1364,17 @@ def _as_rows(name: str, x: torch.Tensor, stream: torch.cuda.Stream | None) -> to
         return _dense(x, stream).view(rows, x.shape[-1])
 
 
-def _mx_rows(shape, dtype: torch.dtype, device: torch.device,
+def _mx_rows(shape, rows: int, dtype: torch.dtype, device: torch.device,
              stream: torch.cuda.Stream | None) -> MXRows:
-    rows = 1
-    for s in shape[:-1]:
-        rows *= s
     code, scale = mx.row_bytes(shape[-1])
-    buf = _new(rows * (code + scale), torch.uint8, device, stream)
-    return MXRows(buf[:rows * code], buf[rows * code:], tuple(shape), dtype)
+    return MXRows._of(_new(rows * (code + scale), torch.uint8, device, stream), shape, rows, dtype)
 
 
-def _mx_quantize_into(x: torch.Tensor, out: MXRows, stream: torch.cuda.Stream | None) -> None:
-    flat = _as_rows("x", x, stream)
-    rc = _launch(_native.lib().sf_mx_quantize, x.get_device(), _DTYPES[x.dtype], flat.data_ptr(),
-                 flat.stride(0), 0, flat.shape[0], flat.shape[1], 1, _MX_E4M3, out.codes.data_ptr(),
-                 0, out.scales.data_ptr(), 0, _stream_handle(stream, x.device))
+def _mx_quantize_into(flat: torch.Tensor, out: MXRows, stream: torch.cuda.Stream | None) -> None:
+    codes, scales = out._pointers()
+    rc = _launch(_native.lib().sf_mx_quantize, flat.get_device(), _DTYPES[flat.dtype],
+                 flat.data_ptr(), flat.stride(0), 0, out.rows, out.dim, 1, _MX_E4M3, codes, 0, scales,
+                 0, _stream_handle(stream, flat.device))
     if rc:
         _native.check(rc, "sf_mx_quantize")
 
@@ -1392,9 +1388,10 @@ def mx_quantize(x: torch.Tensor, *, stream: torch.cuda.Stream | None = None) -> 
         raise ValueError("x must be bf16, fp16 or fp32")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must have at least one column")
-    out = _mx_rows(x.shape, x.dtype, x.device, None)
+    flat = _as_rows("x", x, stream)
+    out = _mx_rows(x.shape, flat.shape[0], x.dtype, x.device, None)
     if out.rows:
-        _mx_quantize_into(x, out, stream)
+        _mx_quantize_into(flat, out, stream)
     return out
 
 
@@ -1429,15 +1426,17 @@ def mx_values(t: MXRows | MXWeight, dtype: torch.dtype = _BF16, *,
     fp32 (K13)."""
     if not isinstance(t, (MXRows, MXWeight)):
         raise TypeError("mx_values takes MXRows or an MXWeight")
-    _require_cuda("codes", t.codes)
     if dtype not in _DTYPES:
         raise ValueError("dtype must be bf16, fp16 or fp32")
-    out = torch.empty(t.shape, dtype=dtype, device=t.device)
-    if out.numel():
-        held = _MX_E4M3 if isinstance(t, MXRows) else _MX_E2M1
-        rc = _launch(_native.lib().sf_mx_values, t.codes.get_device(), held, t.codes.data_ptr(),
-                     t.scales.data_ptr(), t.rows, t.dim, _DTYPES[dtype], out.data_ptr(),
-                     _stream_handle(stream, t.device))
+    device = t.device
+    if device.type != "cuda":
+        raise ValueError("codes must be on a HIP device")
+    out = torch.empty(t.shape, dtype=dtype, device=device)
+    if t.rows:
+        codes, scales = t._pointers()
+        rc = _launch(_native.lib().sf_mx_values, device.index,
+                     _MX_E4M3 if isinstance(t, MXRows) else _MX_E2M1, codes, scales, t.rows, t.dim,
+                     _DTYPES[dtype], out.data_ptr(), _stream_handle(stream, device))
         if rc:
             _native.check(rc, "sf_mx_values")
     return out
@@ -1477,21 +1476,23 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
         raise ValueError("add_rms_norm needs an output: normed or quantized")
     if not eps >= 0:
         raise ValueError("eps must not be negative")
-    total = x if residual is None else torch.empty(x.shape, dtype=dtype, device=device)
-    y = torch.empty(x.shape, dtype=dtype, device=device) if normed else None
-    q = _mx_rows(x.shape, dtype, device, None) if quantized else None
-    if x.numel() == 0:
-        return total, y, q
     flat = _as_rows("x", x, stream)
-    rows, res_ptr, res_stride = flat.shape[0], None, 0
+    rows, res_ptr, res_stride, y, q = flat.shape[0], None, 0, None, None
+    total, total_ptr, codes, scales = x, None, None, None
     if residual is not None:
+        total = torch.empty_like(x, memory_format=torch.contiguous_format)
         residual = _as_rows("residual", residual, stream)
-        res_ptr, res_stride = residual.data_ptr(), residual.stride(0)
+        total_ptr, res_ptr, res_stride = total.data_ptr(), residual.data_ptr(), residual.stride(0)
+    if normed:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if quantized:
+        q = _mx_rows(x.shape, rows, dtype, device, None)
+        codes, scales = q._pointers()
+    if rows == 0:
+        return total, y, q
     rc = _launch(_native.lib().sf_add_rms_norm, x.get_device(), _DTYPES[dtype], flat.data_ptr(),
-                 flat.stride(0), res_ptr, res_stride, rows, dim, weight.data_ptr(), eps,
-                 None if residual is None else total.data_ptr(), _ptr(y),
-                 None if q is None else q.codes.data_ptr(),
-                 None if q is None else q.scales.data_ptr(), _stream_handle(stream, device))
+                 flat.stride(0), res_ptr, res_stride, rows, dim, weight.data_ptr(), eps, total_ptr,
+                 _ptr(y), codes, scales, _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_add_rms_norm")
     return total, y, q
@@ -1512,7 +1513,8 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
     held = isinstance(x, MXRows)
     if held:
         _refuse_gradients("mx_linear", bias)
-        _require_cuda("x", x.codes)
+        if x.device.type != "cuda":
+            raise ValueError("x must be on a HIP device")
     else:
         _refuse_gradients("mx_linear", x, bias)
         _require_cuda("x", x)
@@ -1521,7 +1523,7 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
         raise ValueError("a product's rows must come from bf16 or fp16")
     if len(shape) < 1 or shape[-1] != weight.dim:
         raise ValueError(f"x must be [..., {weight.dim}]")
-    index = weight.codes.get_device()
+    index = device.index
     if weight.device != device:
         raise ValueError("x and the weight must share a device")
     if bias is not None:
@@ -1538,10 +1540,10 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
                 and flat.data_ptr() % 16 == 0:
             kind, x_ptr, stride = _DTYPES[dtype], flat.data_ptr(), flat.stride(0)
         else:
-            x = _mx_rows(shape, dtype, device, stream)
+            x = _mx_rows(shape, flat.shape[0], dtype, device, stream)
             _mx_quantize_into(flat, x, stream)
     if kind == _MX_ROWS:
-        x_ptr, scale_ptr = x.codes.data_ptr(), x.scales.data_ptr()
+        x_ptr, scale_ptr = x._pointers()
     rc = _launch(_native.lib().sf_mx_linear, index, kind, x_ptr, scale_ptr, stride,
                  out.numel() // weight.rows, weight.dim, weight.codes.data_ptr(),
                  weight.scales.data_ptr(), weight.rows, _ptr(bias), _DTYPES[dtype], out.data_ptr(),
@@ -1599,6 +1601,38 @@ def mx_quantize_experts(packed: torch.Tensor, hidden_size: int, intermediate_siz
     return out
 
 
+def _mx_slots(slot_storage: torch.Tensor, slot_of_expert: torch.Tensor | None, num_experts: int,
+              hidden_size: int, intermediate_size: int, device: torch.device) -> None:
+    nbytes = mx_expert_bytes(hidden_size, intermediate_size)
+    _require_cuda("slot storage", slot_storage, torch.uint8)
+    if slot_storage.dim() != 2 or slot_storage.shape[1] != nbytes or slot_storage.stride(1) != 1 \
+            or slot_storage.stride(0) < nbytes or slot_storage.device != device \
+            or slot_storage.data_ptr() % 16 or slot_storage.stride(0) % 16:
+        raise ValueError(f"slot storage must be 16-byte aligned uint8 [slots, {nbytes}]")
+    if slot_of_expert is None:
+        if slot_storage.shape[0] < num_experts:
+            raise ValueError("without a table, every expert needs a slot")
+    else:
+        _require_cuda("slot_of_expert", slot_of_expert, torch.int32)
+        if slot_of_expert.numel() != num_experts or not slot_of_expert.is_contiguous() \
+                or slot_of_expert.device != device:
+            raise ValueError("slot_of_expert must be contiguous int32 [num_experts]")
+
+
+def _mx_hidden(hidden: torch.Tensor | MXRows, tokens: int, hidden_size: int,
+               stream: torch.cuda.Stream | None):
+    """(what owns the memory, type, rows, scales, row stride) of the tokens as
+    the kernels take them: few bf16 rows as they are, others in e4m3."""
+    if not isinstance(hidden, MXRows):
+        hidden = _as_rows("hidden_states", hidden, stream)
+        at, stride = hidden.data_ptr(), hidden.stride(0)
+        if tokens <= _MX_RAW_ROWS and hidden_size % 8 == 0 and stride % 8 == 0 and at % 16 == 0:
+            return hidden, 0, at, None, stride
+        flat, hidden = hidden, _mx_rows((tokens, hidden_size), tokens, _BF16, hidden.device, stream)
+        _mx_quantize_into(flat, hidden, stream)
+    return hidden, _MX_ROWS, *hidden._pointers(), 0
+
+
 def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
                       route_weights: torch.Tensor | None, slot_storage: torch.Tensor,
                       hidden_size: int, intermediate_size: int, out_rows: torch.Tensor, *,
@@ -1617,7 +1651,8 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
     H, I, T, K, E = hidden_size, intermediate_size, plan.tokens, plan.top_k, plan.num_experts
     held = isinstance(hidden, MXRows)
     if held:
-        _require_cuda("hidden_states", hidden.codes)
+        if hidden.device.type != "cuda":
+            raise ValueError("hidden_states must be on a HIP device")
     else:
         _refuse_gradients("mx_grouped_swiglu", hidden)
         _require_cuda("hidden_states", hidden, _BF16)
@@ -1625,20 +1660,7 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
     if tuple(hidden.shape) != (T, H):
         raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
     device = hidden.device
-    nbytes = mx_expert_bytes(H, I)
-    _require_cuda("slot storage", slot_storage, torch.uint8)
-    if slot_storage.dim() != 2 or slot_storage.shape[1] != nbytes or slot_storage.stride(1) != 1 \
-            or slot_storage.stride(0) < nbytes or slot_storage.device != device \
-            or slot_storage.data_ptr() % 16 or slot_storage.stride(0) % 16:
-        raise ValueError(f"slot storage must be 16-byte aligned uint8 [slots, {nbytes}]")
-    if slot_of_expert is None:
-        if slot_storage.shape[0] < E:
-            raise ValueError("without a table, every expert needs a slot")
-    else:
-        _require_cuda("slot_of_expert", slot_of_expert, torch.int32)
-        if slot_of_expert.numel() != E or not slot_of_expert.is_contiguous() \
-                or slot_of_expert.device != device:
-            raise ValueError("slot_of_expert must be contiguous int32 [num_experts]")
+    _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
     _require_cuda("out_rows", out_rows, _BF16)
     if out_rows.shape != (T * K, H) or not out_rows.is_contiguous() or out_rows.device != device:
         raise ValueError("out_rows must be contiguous bf16 [tokens * top_k, hidden]")
@@ -1649,22 +1671,57 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
             raise ValueError("route weights must be contiguous bf16 [tokens*top_k]")
     if T * K == 0:
         return
-    kind, stride, scale_ptr = _MX_ROWS, 0, None
-    if not held:
-        hidden = _as_rows("hidden_states", hidden, stream)
-        if T <= _MX_RAW_ROWS and H % 8 == 0 and hidden.stride(0) % 8 == 0 \
-                and hidden.data_ptr() % 16 == 0:
-            kind, stride, x_ptr = 0, hidden.stride(0), hidden.data_ptr()
-        else:
-            flat, hidden = hidden, _mx_rows((T, H), _BF16, device, stream)
-            _mx_quantize_into(flat, hidden, stream)
-    if kind == _MX_ROWS:
-        x_ptr, scale_ptr = hidden.codes.data_ptr(), hidden.scales.data_ptr()
-    act = _mx_rows((T * K, I), _BF16, device, stream)
+    hidden, kind, x_ptr, scale_ptr, stride = _mx_hidden(hidden, T, H, stream)
+    scratch = _mx_rows((T * K, I), T * K, _BF16, device, stream)
+    act, act_scales = scratch._pointers()
     rc = _launch(_native.lib().sf_mx_grouped_swiglu, out_rows.get_device(), kind, x_ptr, scale_ptr,
                  stride, plan.perm_pos.data_ptr(), plan.offsets.data_ptr(), _ptr(route_weights), T,
                  K, H, I, E, _ptr(slot_of_expert), slot_storage.data_ptr(), slot_storage.stride(0),
-                 act.codes.data_ptr(), act.scales.data_ptr(), out_rows.data_ptr(),
-                 _stream_handle(stream, device))
+                 act, act_scales, out_rows.data_ptr(), _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_mx_grouped_swiglu")
+
+
+def mx_routed_swiglu(hidden: torch.Tensor | MXRows, index: torch.Tensor,
+                     route_weights: torch.Tensor, slot_storage: torch.Tensor, hidden_size: int,
+                     intermediate_size: int, *, slot_of_expert: torch.Tensor | None = None,
+                     stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """The routed experts' sum for few tokens (K16's form without a dispatch):
+    bf16 [tokens, H], for each token the sum over its routes of weight *
+    expert, in fp32 and rounded once.
+
+    ``index`` int64 [tokens, top_k], ``route_weights`` bf16 like it; hidden and
+    the experts as ``mx_grouped_swiglu`` takes them, as many experts as the
+    table has entries, or slots without one.  Every route reads its expert's
+    weights for itself, so this is for routes that hardly share any.  Routes to
+    experts that are not there or in no slot count for nothing.  No gradients."""
+    H, I = hidden_size, intermediate_size
+    _refuse_gradients("mx_routed_swiglu", None if isinstance(hidden, MXRows) else hidden,
+                      route_weights)
+    _require_cuda("top_k_index", index, torch.int64)
+    if index.dim() != 2 or not index.is_contiguous():
+        raise ValueError("top_k_index must be contiguous [tokens, top_k]")
+    T, K = index.shape
+    device = index.device
+    if not isinstance(hidden, MXRows):
+        _require_cuda("hidden_states", hidden, _BF16)
+    if tuple(hidden.shape) != (T, H) or hidden.device != device:
+        raise ValueError(f"hidden_states must be [{T}, {H}] on the routes' device")
+    _require_cuda("route weights", route_weights, _BF16)
+    if route_weights.shape != index.shape or not route_weights.is_contiguous() \
+            or route_weights.device != device:
+        raise ValueError("route weights must be contiguous bf16 [tokens, top_k]")
+    E = slot_storage.shape[0] if slot_of_expert is None else slot_of_expert.numel()
+    _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
+    if T * K == 0:
+        return torch.zeros((T, H), dtype=_BF16, device=device)
+    out = torch.empty((T, H), dtype=_BF16, device=device)
+    hidden, kind, x_ptr, scale_ptr, stride = _mx_hidden(hidden, T, H, stream)
+    scratch = _mx_rows((T * K, I), T * K, _BF16, device, stream)
+    rc = _launch(_native.lib().sf_mx_routed_swiglu, device.index, kind, x_ptr, scale_ptr, stride,
+                 index.data_ptr(), route_weights.data_ptr(), T, K, H, I, E, _ptr(slot_of_expert),
+                 slot_storage.data_ptr(), slot_storage.stride(0), *scratch._pointers(),
+                 out.data_ptr(), _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_mx_routed_swiglu")
+    return out

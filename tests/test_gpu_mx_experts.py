@@ -158,3 +158,54 @@ def test_on_another_stream():
     y = ops.mx_linear(x, w, stream=side)
     side.synchronize()
     assert torch.equal(got, want) and torch.equal(y, ops.mx_linear(x, w))
+
+
+def _routed(h, index, weights, packed, hidden, inner, **more):
+    records = ops.mx_quantize_experts(packed, hidden, inner)
+    return ops.mx_routed_swiglu(h, index, weights, records, hidden, inner, **more)
+
+
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", SHAPES[:10] + [(3, 2048, 768, 128, 1), (2, 520, 200, 9, 5),
+                                                                          (1, 64, 32, 40, 16)])
+def test_routed(tokens, hidden, inner, experts, top_k):
+    h, packed, index, weights = _case(tokens, hidden, inner, experts, top_k, seed=3)
+    got = _routed(h, index, weights, packed, hidden, inner)
+    _check(got, h, index, weights, packed, hidden, inner)
+    assert torch.equal(got, _routed(ops.mx_quantize(h), index, weights, packed, hidden, inner))
+
+
+def test_routed_with_a_table_repeats_and_experts_that_are_not_there():
+    h, packed, index, weights = _case(9, 96, 64, 5, 4, distinct=False)
+    index[3, 1], index[7], index[2, 0], index[1, 3] = 99, -1, 2 ** 40, -2 ** 40
+    table = torch.tensor([2, -1, 0, 3, 1], dtype=torch.int32, device=DEV)
+    records = ops.mx_quantize_experts(packed, 96, 64)
+    slots = torch.zeros((4, records.shape[1]), dtype=torch.uint8, device=DEV)
+    slots[table[table >= 0].long()] = records[table >= 0]
+    got = ops.mx_routed_swiglu(h, index, weights, slots, 96, 64, slot_of_expert=table)
+    there = torch.where(index == 1, -1, index)
+    _check(got, h, there, weights, packed, 96, 64)
+    assert not got[7].any()
+    h[5, 9] = float("nan")
+    assert torch.isnan(ops.mx_routed_swiglu(h, index, weights, records, 96, 64)).all(1).tolist() \
+        == [i == 5 for i in range(9)]
+
+
+def test_routed_captured_and_on_another_stream():
+    h, packed, index, weights = _case(2, 256, 128, 16, 4)
+    records = ops.mx_quantize_experts(packed, 256, 128)
+    want = ops.mx_routed_swiglu(h, index, weights, records, 256, 128)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    columns = h.t().contiguous().t()
+    side.wait_stream(torch.cuda.current_stream())
+    got = ops.mx_routed_swiglu(columns, index, weights, records, 256, 128, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.mx_routed_swiglu(h, index, weights, records, 256, 128)
+    for seed in range(3):
+        new, _, i2, w2 = _case(2, 256, 128, 16, 4, seed=seed + 5)
+        h.copy_(new), index.copy_(i2), weights.copy_(w2)
+        graph.replay()
+        assert torch.equal(out, ops.mx_routed_swiglu(h, index, weights, records, 256, 128))
