@@ -165,6 +165,12 @@ __device__ __forceinline__ void part_of(int count, int i, int n, int& begin, int
 // way into LDS (loads that write it themselves) while the present one is
 // multiplied.  The scales of four tiles come together, ahead of them.
 //
+// Where the operands of a whole tile fit beside the accumulators they are read
+// first, and the stage that they leave takes the tile after the next: twice the
+// time for a load, for a second meeting (us, one ahead and two: 61 x 2,048 x
+// 151,936 44.8 / 41.4; experts of 1,024 tokens 112.7 / 109.7; with 4 x 2 products
+// the registers do not suffice, 8,192^3 423 / 433).
+//
 // LDS: rows keep their 128 bytes together, piece p (16 bytes) of row r in slot
 // p ^ (r / 2 & 7): the loads then take whole lines from memory, and the sixteen
 // lanes that read a piece of sixteen rows together meet sixteen different
@@ -175,6 +181,7 @@ struct Tiling {
   static constexpr int WN = WN_, WM = WM_, FN = FN_, FM = FM_;
   static constexpr int kWaves = WN * WM, kThreads = kWaves * SF_WAVE;
   static constexpr int kRows = 32 * FM * WM, kOut = 32 * FN * WN;  // of a workgroup
+  static constexpr bool kTwoAhead = FN * FM <= 4;
   static constexpr int kRowLoads = kRows / 8 / kWaves, kOutLoads = kOut / 16 / kWaves;
   static_assert(kRows / 8 % kWaves == 0 && kOut / 16 % kWaves == 0, "whole loads for a wavefront");
   static constexpr int kRowScaleLoads = (kRows + 63) / 64, kOutScaleLoads = (kOut + 63) / 64;
@@ -209,12 +216,16 @@ __device__ __forceinline__ void to_lds(const uint8_t* from, uint8_t* to) {
                                    (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
-// All of this wavefront's loads have landed and its LDS reads are done; then
-// all wavefronts'.  The builtins rather than assembly: the compiler then knows
-// that nothing is under way and adds no waits of its own.
+// Operands of s_waitcnt: at most n vector memory loads under way; no LDS reads.
+constexpr int loads_left(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
+constexpr int kLdsRead = 0xc07f;
+
+// This wavefront's wait, then all wavefronts' meeting.  The builtins rather than
+// assembly: the compiler then knows what has landed and adds no waits of its own.
+template <int WAIT>
 __device__ __forceinline__ void meet() {
-  __builtin_amdgcn_sched_barrier(0);   // the products before the wait, not behind it
-  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_sched_barrier(0);  // the products before the wait, not behind it
+  __builtin_amdgcn_s_waitcnt(WAIT);
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -308,7 +319,15 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
         xs[m][h] = *reinterpret_cast<const uint32_t*>(s.rows + ((wm * T::FM + m) * 32 + r) * 16 + (2 * h + g) * 4);
     }
   };
-  const auto step = [&](typename T::Stage& here) {
+  const auto step = [&](typename T::Stage& here, typename T::Stage& other, int t) {
+    if (t % 4 == 0) read_scales(t / 4);
+    const auto request = [&](typename T::Stage& s, int ahead) {
+      if (t % 4 == 0 && t + 4 < kt) load_scales(t / 4 + 1);
+      // No branch here, or the products would be moved behind it: past the end
+      // the last tile comes once more, unread.
+      load_stage(s, min(t + ahead, kt - 1));
+      __builtin_amdgcn_sched_barrier(0);
+    };
     i32x8 a[2][T::FN], b[2][T::FM];
     const auto read = [&](int h) {
 #pragma unroll
@@ -321,10 +340,18 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
       for (int n = 0; n < T::FN; ++n)
         a[h][n] = operand4(here.out + ((wn * T::FN + n) * 2 + r / 16) * 1024 + (2 * h + g) * 256 + r % 16 * 16);
     };
-    read(0);
+    if constexpr (T::kTwoAhead) {
+      read(0);
+      read(1);
+      meet<kLdsRead>();
+      request(here, 2);
+    } else {
+      request(other, 1);
+      read(0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if (h) read(1);
+      if (!T::kTwoAhead && h) read(1);
 #pragma unroll
       for (int n = 0; n < T::FN; ++n)
 #pragma unroll
@@ -339,32 +366,21 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
 #pragma unroll
       for (int m = 0; m < T::FM; ++m) xs[m][h] >>= 8;
     }
+    // Two ahead: the loads of this step stay under way.
+    meet<T::kTwoAhead ? loads_left(T::kRowLoads + T::kOutLoads) : loads_left(0) & kLdsRead>();
   };
 
-  load_stage(stage0, 0);
   load_scales(0);
-  meet();
+  load_stage(stage0, 0);
+  if constexpr (T::kTwoAhead) load_stage(stage1, min(1, kt - 1));
+  meet<loads_left(0)>();
   int t = 0;
   for (; t + 2 <= kt; t += 2) {
-    if (t % 4 == 0) {
-      read_scales(t / 4);
-      if (t + 4 < kt) load_scales(t / 4 + 1);
-    }
-    load_stage(stage1, t + 1);
-    __builtin_amdgcn_sched_barrier(0);
-    step(stage0);
-    meet();
-    // No branch here, or the products above would be moved behind it: past the
-    // end the last tile comes once more, unread.
-    load_stage(stage0, min(t + 2, kt - 1));
-    __builtin_amdgcn_sched_barrier(0);
-    step(stage1);
-    meet();
+    step(stage0, stage1, t);
+    step(stage1, stage0, t + 1);
   }
-  if (t < kt) {
-    if (t % 4 == 0) read_scales(t / 4);
-    step(stage0);
-  }
+  if (t < kt) step(stage0, stage1, t);
+  __builtin_amdgcn_s_waitcnt(loads_left(0));  // nothing on its way into LDS that is given back
 }
 
 }  // namespace sf_mx
