@@ -77,15 +77,19 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
   }
 }
 
-// 8 neighbours at p (16-byte aligned) as fp32.
+// Pieces of 16 bytes that start at any element: one load or store all the same.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+
+// 8 neighbours at p as fp32.
 template <int DT>
 __device__ __forceinline__ void load8(const char* p, float (&f)[8]) {
   if (DT == kFp32) {
-    const f32x4 a = ld<f32x4>(p), b = ld<f32x4>(p + 16);
+    const f32x4 a = ld<f32x4_any>(p), b = ld<f32x4_any>(p + 16);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
   } else {
-    const u32x4 v = ld<u32x4>(p);
+    const u32x4 v = ld<u32x4_any>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) unpack2<DT>(v[i], f[2 * i], f[2 * i + 1]);
   }

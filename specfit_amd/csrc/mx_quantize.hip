@@ -15,7 +15,7 @@ constexpr int kThreads = 256;
 // ------------------------------------------------------------------ K13 ----
 // Rows to e4m3.  A lane takes 8 neighbours, so a block is four lanes of one
 // DPP quad, and loads and stores of a wavefront lie in a piece.
-template <int DT, bool VEC>
+template <int DT>
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const char* __restrict__ x,
                                                                  int64_t row_stride, int dim,
                                                                  int chunks, int64_t total,
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const char* __r
   const int c = static_cast<int>(at - row * chunks);
   const char* p = x + (row * row_stride + 8 * c) * size_of<DT>();
   float f[8] = {};
-  if (VEC && 8 * c + 8 <= dim) {
+  if (8 * c + 8 <= dim) {
     load8<DT>(p, f);
   } else {
 #pragma unroll
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const char* __r
 // A weight to e2m1 tiles: a wavefront takes 16 rows by 512 columns, a lane one
 // block of each of four tiles -- no exchange between lanes, and codes (1 KiB)
 // and scales (256 bytes) leave in a piece.
-template <int DT, bool VEC>
+template <int DT>
 __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(
     const char* __restrict__ x, int64_t row_stride, int64_t batch_stride, int rows, int dim,
     uint8_t* __restrict__ codes, int64_t codes_batch, uint8_t* __restrict__ scales,
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(
     const int k0 = (4 * q + j) * kTile + b * kBlock;
     float f[4][8] = {};
     if (row < rows) {
-      if (VEC && k0 + kBlock <= dim) {
+      if (k0 + kBlock <= dim) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) load8<DT>(x + static_cast<int64_t>(k0 + 8 * i) * size_of<DT>(), f[i]);
       } else {
@@ -97,14 +97,14 @@ __global__ __launch_bounds__(kThreads) void quantize_weight_kernel(
 
 // 8 values to out; past the row's end nothing.
 template <int DT>
-__device__ __forceinline__ void store8(const float (&f)[8], char* p, int left, bool vec) {
-  if (vec && left >= 8) {
+__device__ __forceinline__ void store8(const float (&f)[8], char* p, int left) {
+  if (left >= 8) {
     if (DT == kFp32) {
-      *reinterpret_cast<f32x4*>(p) = f32x4{f[0], f[1], f[2], f[3]};
-      *reinterpret_cast<f32x4*>(p + 16) = f32x4{f[4], f[5], f[6], f[7]};
+      *reinterpret_cast<f32x4_any*>(p) = f32x4{f[0], f[1], f[2], f[3]};
+      *reinterpret_cast<f32x4_any*>(p + 16) = f32x4{f[4], f[5], f[6], f[7]};
     } else {
-      *reinterpret_cast<u32x4*>(p) = u32x4{narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]),
-                                          narrow2<DT>(f[4], f[5]), narrow2<DT>(f[6], f[7])};
+      *reinterpret_cast<u32x4_any*>(p) = u32x4{narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]),
+                                              narrow2<DT>(f[4], f[5]), narrow2<DT>(f[6], f[7])};
     }
     return;
   }
@@ -122,7 +122,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void rows_values_kernel(const uint8_t* __restrict__ codes,
                                                                const uint8_t* __restrict__ scales,
                                                                int dim, int chunks, int64_t total,
-                                                               bool vec, char* __restrict__ out) {
+                                                               char* __restrict__ out) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (at >= total) return;
   const int64_t row = total <= 0x7fffffff
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(kThreads) void rows_values_kernel(const uint8_t* __
     const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w[i]), true);
     f[4 * i] = a[0] * s, f[4 * i + 1] = a[1] * s, f[4 * i + 2] = b[0] * s, f[4 * i + 3] = b[1] * s;
   }
-  store8<DT>(f, out + (row * dim + 8 * c) * size_of<DT>(), dim - 8 * c, vec);
+  store8<DT>(f, out + (row * dim + 8 * c) * size_of<DT>(), dim - 8 * c);
 }
 
 // A wavefront to 16 rows of a tile, four rows at a time: sixteen lanes write
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void rows_values_kernel(const uint8_t* __
 template <int DT>
 __global__ __launch_bounds__(kThreads) void weight_values_kernel(const uint8_t* __restrict__ codes,
                                                                  const uint8_t* __restrict__ scales,
-                                                                 int rows, int dim, bool vec,
+                                                                 int rows, int dim,
                                                                  char* __restrict__ out) {
   const int lane = threadIdx.x & (SF_WAVE - 1);
   const int kt = tiles(dim), kq = quads(dim);
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void weight_values_kernel(const uint8_t* 
     const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.0f, 3);
     f[0] = a[0] * s, f[1] = a[1] * s, f[2] = b[0] * s, f[3] = b[1] * s;
     f[4] = d[0] * s, f[5] = d[1] * s, f[6] = e[0] * s, f[7] = e[1] * s;
-    store8<DT>(f, out + (row * dim + k) * size_of<DT>(), dim - k, vec);
+    store8<DT>(f, out + (row * dim + k) * size_of<DT>(), dim - k);
   }
 }
 
@@ -209,10 +209,10 @@ __device__ __forceinline__ double row_sum(double v, double* part) {
   return v;
 }
 
-template <int DT, bool VEC>
+template <int DT>
 __device__ __forceinline__ void load_sum(const char* x, const char* res, int c, int dim, float (&f)[8]) {
   const int64_t off = static_cast<int64_t>(c) * 8 * size_of<DT>();
-  if (VEC && 8 * c + 8 <= dim) {
+  if (8 * c + 8 <= dim) {
     load8<DT>(x + off, f);
     if (res) {
       float g[8];
@@ -232,7 +232,7 @@ __device__ __forceinline__ void load_sum(const char* x, const char* res, int c, 
   }
 }
 
-template <int DT, int LANES, int CHUNKS, bool VEC>
+template <int DT, int LANES, int CHUNKS>
 __global__ __launch_bounds__(kThreads) void add_rms_norm_kernel(
     const char* __restrict__ x, int64_t x_stride, const char* __restrict__ residual,
     int64_t residual_stride, int rows, int dim, const char* __restrict__ weight, double eps,
@@ -253,16 +253,16 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_kernel(
   const int steps = CHUNKS ? CHUNKS : (chunks + LANES - 1) / LANES;
   if (CHUNKS) {
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) load_sum<DT, VEC>(xr, rr, lane + j * LANES, dim, f[j]);
+    for (int j = 0; j < kHeld; ++j) load_sum<DT>(xr, rr, lane + j * LANES, dim, f[j]);
   }
 #pragma unroll kHeld
   for (int j = 0; j < steps; ++j) {
     float(&v)[8] = f[CHUNKS ? j : 0];
     const int c = lane + j * LANES;
-    if (!CHUNKS) load_sum<DT, VEC>(xr, rr, c, dim, v);
+    if (!CHUNKS) load_sum<DT>(xr, rr, c, dim, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) total = __builtin_fma(static_cast<double>(v[i]), static_cast<double>(v[i]), total);
-    if (sr && 8 * c < dim) store8<DT>(v, sr + static_cast<int64_t>(c) * 8 * size_of<DT>(), dim - 8 * c, VEC);
+    if (sr && 8 * c < dim) store8<DT>(v, sr + static_cast<int64_t>(c) * 8 * size_of<DT>(), dim - 8 * c);
   }
   total = row_sum<LANES>(total, part);
   const float r = static_cast<float>(1.0 / sqrt(total / dim + eps));
@@ -270,11 +270,11 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_kernel(
   for (int j = 0; j < steps; ++j) {
     float(&v)[8] = f[CHUNKS ? j : 0];
     const int c = lane + j * LANES;
-    if (!CHUNKS) load_sum<DT, VEC>(xr, rr, c, dim, v);
+    if (!CHUNKS) load_sum<DT>(xr, rr, c, dim, v);
     if (c >= chunks) continue;  // whole quads
     const char* wp = weight + static_cast<int64_t>(c) * 8 * size_of<DT>();
     float w[8] = {};
-    if (VEC && 8 * c + 8 <= dim) {
+    if (8 * c + 8 <= dim) {
       load8<DT>(wp, w);
     } else {
 #pragma unroll
@@ -284,21 +284,21 @@ __global__ __launch_bounds__(kThreads) void add_rms_norm_kernel(
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = 8 * c + i < dim ? v[i] * r * w[i] : 0.f;
-    if (nr && 8 * c < dim) store8<DT>(y, nr + static_cast<int64_t>(c) * 8 * size_of<DT>(), dim - 8 * c, VEC);
+    if (nr && 8 * c < dim) store8<DT>(y, nr + static_cast<int64_t>(c) * 8 * size_of<DT>(), dim - 8 * c);
     if (codes)
       store_rows_chunk(y, c, codes + row * chunks * 8,
                        scales + row * (static_cast<int64_t>((chunks + 63) / 64) * 16));
   }
 }
 
-template <int DT, bool VEC>
+template <int DT>
 void launch_norm(const char* x, int64_t xs, const char* res, int64_t rs, int rows, int dim,
                  const char* weight, double eps, char* sum, char* normed, uint8_t* codes,
                  uint8_t* scales, hipStream_t s) {
   const int chunks = tiles(dim) * 16;
   const unsigned all = static_cast<unsigned>(rows), quarter = static_cast<unsigned>((rows - 1) / 4 + 1);
 #define SF_NORM(LANES, CHUNKS, GRID)                                                             \
-  add_rms_norm_kernel<DT, LANES, CHUNKS, VEC><<<dim3(GRID), dim3(kThreads), 0, s>>>(             \
+  add_rms_norm_kernel<DT, LANES, CHUNKS><<<dim3(GRID), dim3(kThreads), 0, s>>>(             \
       x, xs, res, rs, rows, dim, weight, eps, sum, normed, codes, scales)
   if (chunks <= 64)
     SF_NORM(64, 1, quarter);
@@ -313,37 +313,24 @@ void launch_norm(const char* x, int64_t xs, const char* res, int64_t rs, int row
 #undef SF_NORM
 }
 
-template <int DT>
-bool fits16(const void* p, int64_t stride) {
-  return aligned(p, 16) && stride * size_of<DT>() % 16 == 0;
-}
-
 constexpr int64_t kMostGroups = 0x7fffffff;
 
 template <int DT>
 int quantize(const char* x, int64_t row_stride, int64_t batch_stride, int rows, int dim, int batch,
              int held, uint8_t* codes, int64_t codes_batch, uint8_t* scales, int64_t scales_batch,
              hipStream_t s) {
-  const bool vec = fits16<DT>(x, row_stride) && (batch == 1 || batch_stride * size_of<DT>() % 16 == 0);
   if (held == kE4m3) {
     const int chunks = tiles(dim) * 16;
     const int64_t total = static_cast<int64_t>(rows) * chunks, groups = (total - 1) / kThreads + 1;
     if (groups > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
     const dim3 grid(static_cast<unsigned>(groups));
-    if (vec)
-      quantize_rows_kernel<DT, true><<<grid, dim3(kThreads), 0, s>>>(x, row_stride, dim, chunks, total, codes, scales);
-    else
-      quantize_rows_kernel<DT, false><<<grid, dim3(kThreads), 0, s>>>(x, row_stride, dim, chunks, total, codes, scales);
+    quantize_rows_kernel<DT><<<grid, dim3(kThreads), 0, s>>>(x, row_stride, dim, chunks, total, codes, scales);
   } else {
     const int64_t groups = (static_cast<int64_t>(row_tiles(rows)) * quads(dim) - 1) / (kThreads / SF_WAVE) + 1;
     if (groups > kMostGroups || batch > 65535) return SF_ERR_UNSUPPORTED_SHAPE;
     const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(batch));
-    if (vec)
-      quantize_weight_kernel<DT, true><<<grid, dim3(kThreads), 0, s>>>(
-          x, row_stride, batch_stride, rows, dim, codes, codes_batch, scales, scales_batch);
-    else
-      quantize_weight_kernel<DT, false><<<grid, dim3(kThreads), 0, s>>>(
-          x, row_stride, batch_stride, rows, dim, codes, codes_batch, scales, scales_batch);
+    quantize_weight_kernel<DT><<<grid, dim3(kThreads), 0, s>>>(x, row_stride, batch_stride, rows, dim, codes,
+                                                               codes_batch, scales, scales_batch);
   }
   SF_LAUNCH_CHECK();
   return SF_OK;
@@ -352,19 +339,18 @@ int quantize(const char* x, int64_t row_stride, int64_t batch_stride, int rows, 
 template <int DT>
 int values(int held, const uint8_t* codes, const uint8_t* scales, int rows, int dim, char* out,
            hipStream_t s) {
-  const bool vec = fits16<DT>(out, dim);
   if (held == kE4m3) {
     const int chunks = tiles(dim) * 16;
     const int64_t total = static_cast<int64_t>(rows) * chunks, groups = (total - 1) / kThreads + 1;
     if (groups > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
     rows_values_kernel<DT><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(
-        codes, scales, dim, chunks, total, vec, out);
+        codes, scales, dim, chunks, total, out);
   } else {
     const int64_t units = static_cast<int64_t>((rows - 1) / 16 + 1) * tiles(dim);
     const int64_t groups = (units - 1) / (kThreads / SF_WAVE) + 1;
     if (groups > kMostGroups) return SF_ERR_UNSUPPORTED_SHAPE;
     weight_values_kernel<DT><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, s>>>(
-        codes, scales, rows, dim, vec, out);
+        codes, scales, rows, dim, out);
   }
   SF_LAUNCH_CHECK();
   return SF_OK;
@@ -385,7 +371,7 @@ extern "C" int sf_mx_quantize(int dtype, const void* x, int64_t row_stride, int6
   if (dim > kMostColumns) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0 || batch == 0) return SF_OK;
   if (!x || !codes || !scales) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(codes, 16) || !aligned(scales, 4) || codes_batch_stride % 16 || scales_batch_stride % 4)
+  if (!aligned(x, dtype == kFp32 ? 4 : 2) || !aligned(codes, 16) || !aligned(scales, 4) || codes_batch_stride % 16 || scales_batch_stride % 4)
     return SF_ERR_MISALIGNED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const char* xp = static_cast<const char*>(x);
@@ -408,7 +394,7 @@ extern "C" int sf_mx_values(int held, const void* codes, const void* scales, int
   if (dim > kMostColumns) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0) return SF_OK;
   if (!codes || !scales || !out) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(codes, 16)) return SF_ERR_MISALIGNED;
+  if (!aligned(codes, 16) || !aligned(out, dtype == kFp32 ? 4 : 2)) return SF_ERR_MISALIGNED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const auto* cp = static_cast<const uint8_t*>(codes);
   const auto* sp = static_cast<const uint8_t*>(scales);
@@ -429,28 +415,21 @@ extern "C" int sf_add_rms_norm(int dtype, const void* x, int64_t x_stride, const
   if (rows == 0) return SF_OK;
   if (!x || !weight || !codes != !scales || (sum && !residual) || (!sum && !normed && !codes))
     return SF_ERR_INVALID_ARGUMENT;
-  if (codes && !aligned(codes, 8)) return SF_ERR_MISALIGNED;
+  const uintptr_t size = dtype == kFp32 ? 4 : 2;
+  if (!aligned(x, size) || !aligned(residual, size) || !aligned(weight, size) || !aligned(sum, size) ||
+      !aligned(normed, size) || !aligned(codes, 8))
+    return SF_ERR_MISALIGNED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const char *xp = static_cast<const char*>(x), *rp = static_cast<const char*>(residual),
              *wp = static_cast<const char*>(weight);
   char *sp = static_cast<char*>(sum), *np = static_cast<char*>(normed);
   auto *cp = static_cast<uint8_t*>(codes), *kp = static_cast<uint8_t*>(scales);
-#define SF_NORM_TYPE(DT)                                                                          \
-  {                                                                                               \
-    const bool vec = fits16<DT>(x, x_stride) && (!rp || fits16<DT>(rp, residual_stride)) &&       \
-                     aligned(wp, 16) && (!sp || fits16<DT>(sp, dim)) && (!np || fits16<DT>(np, dim)); \
-    if (vec)                                                                                      \
-      launch_norm<DT, true>(xp, x_stride, rp, residual_stride, rows, dim, wp, eps, sp, np, cp, kp, s); \
-    else                                                                                          \
-      launch_norm<DT, false>(xp, x_stride, rp, residual_stride, rows, dim, wp, eps, sp, np, cp, kp, s); \
-  }
   if (dtype == kBf16)
-    SF_NORM_TYPE(kBf16)
+    launch_norm<kBf16>(xp, x_stride, rp, residual_stride, rows, dim, wp, eps, sp, np, cp, kp, s);
   else if (dtype == kFp16)
-    SF_NORM_TYPE(kFp16)
+    launch_norm<kFp16>(xp, x_stride, rp, residual_stride, rows, dim, wp, eps, sp, np, cp, kp, s);
   else
-    SF_NORM_TYPE(kFp32)
-#undef SF_NORM_TYPE
+    launch_norm<kFp32>(xp, x_stride, rp, residual_stride, rows, dim, wp, eps, sp, np, cp, kp, s);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
