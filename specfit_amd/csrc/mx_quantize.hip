@@ -302,6 +302,8 @@ void launch_norm(const char* x, int64_t xs, const char* res, int64_t rs, int row
       x, xs, res, rs, rows, dim, weight, eps, sum, normed, codes, scales)
   if (chunks <= 64)
     SF_NORM(64, 1, quarter);
+  else if (chunks <= 128 && rows >= 2048)
+    SF_NORM(64, 2, quarter);
   else if (chunks <= 256)
     SF_NORM(256, 1, all);
   else if (chunks <= 512)

@@ -1650,13 +1650,11 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
     gradients."""
     H, I, T, K, E = hidden_size, intermediate_size, plan.tokens, plan.top_k, plan.num_experts
     held = isinstance(hidden, MXRows)
-    if held:
-        if hidden.device.type != "cuda":
-            raise ValueError("hidden_states must be on a HIP device")
-    else:
-        _refuse_gradients("mx_grouped_swiglu", hidden)
+    _refuse_gradients("mx_grouped_swiglu", None if held else hidden, route_weights)
+    if not held:
         _require_cuda("hidden_states", hidden, _BF16)
-    _refuse_gradients("mx_grouped_swiglu", route_weights)
+    elif hidden.device.type != "cuda":
+        raise ValueError("hidden_states must be on a HIP device")
     if tuple(hidden.shape) != (T, H):
         raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
     device = hidden.device

@@ -14,7 +14,7 @@ from .qwen3_expert_prefetch import Qwen3ExpertPrefetch
 from .qwen3_offloaded_model import (LoadedOffloadedQwen3, PackedExpertBackingMode,
                                     Qwen3LoadTimings, build_offloaded_qwen3, load_offloaded_qwen3)
 from .qwen3_attention import Qwen3AttentionHip, install_hip_attention
-from .qwen3_mx_experts import Qwen3MXExperts
+from .qwen3_mx_experts import Qwen3MXExperts, install_mx_experts
 from .qwen3_norm import Qwen3RMSNormHip, install_hip_norms
 from .qwen3_router import Qwen3MoeTopKRouterHip
 from .replay import (ExpertAccessReplayResult, LogicalReplayError, LogicalReplayEvent,
@@ -27,7 +27,7 @@ from .tree_verify import (Eagle3DraftTree, TreeVerification, compact_tree_cache,
                           verify_draft_tree)
 
 __all__ = [
-    "BlockKVCache", "LogitRules", "Qwen3MXExperts",
+    "BlockKVCache", "LogitRules", "Qwen3MXExperts", "install_mx_experts",
     "CacheSlotSnapshot", "CacheTransition", "CacheTransitionCounters",
     "CacheTransitionObserver", "ExpertCacheStats", "ExpertExecutionPolicy", "ExpertKey",
     "ExpertLease", "GpuExpertCache", "GpuExpertCacheSnapshot", "NoEvictableSlotError",

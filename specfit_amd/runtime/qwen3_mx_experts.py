@@ -63,6 +63,8 @@ class Qwen3MXExperts(nn.Module):
     @classmethod
     def from_module(cls, experts: nn.Module) -> "Qwen3MXExperts":
         """From an HF ``Qwen3MoeExperts`` on a GPU (shares no storage)."""
+        if type(experts.act_fn).__name__ not in ("SiLUActivation", "SiLU"):
+            raise ValueError("the experts' activation must be silu")
         gate_up, down = experts.gate_up_proj.detach(), experts.down_proj.detach()
         E, H, I = down.shape
         records = torch.empty((E, ops.mx_expert_bytes(H, I)), dtype=torch.uint8, device=down.device)
@@ -107,3 +109,18 @@ class Qwen3MXExperts(nn.Module):
         ops.mx_grouped_swiglu(hidden_states, plan, weights.view(-1), self.records, self.hidden_size,
                               self.intermediate_size, rows)
         return ops.combine(rows, top_k_index, plan, self.hidden_size, accumulate_fp32=True)
+
+
+def install_mx_experts(model: nn.Module) -> int:
+    """Replace the experts of every Qwen3-MoE layer of ``model`` that are
+    transformers' own, on a GPU, with a ``Qwen3MXExperts`` of their weights in
+    4 bits; returns how many.  Layers whose experts are offloaded stay."""
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeExperts
+
+    targets = [(name, mod) for name, mod in model.named_modules()
+               if isinstance(mod, Qwen3MoeExperts)]
+    for name, mod in targets:
+        parent_name, _, attr = name.rpartition(".")
+        parent = model.get_submodule(parent_name) if parent_name else model
+        setattr(parent, attr, Qwen3MXExperts.from_module(mod))
+    return len(targets)

@@ -209,3 +209,38 @@ def test_routed_captured_and_on_another_stream():
         h.copy_(new), index.copy_(i2), weights.copy_(w2)
         graph.replay()
         assert torch.equal(out, ops.mx_routed_swiglu(h, index, weights, records, 256, 128))
+
+
+@torch.inference_mode()
+def test_a_model_with_mx_experts_prompt_and_decoding():
+    """Every layer's experts in a model's own forwards, a prompt and single
+    tokens after it, against the reference on what the layer was given."""
+    from transformers import Qwen3MoeConfig, Qwen3MoeForCausalLM
+
+    from specfit_amd.runtime import install_hip_attention, install_hip_norms, install_mx_experts
+
+    torch.manual_seed(3)
+    config = Qwen3MoeConfig(vocab_size=96, hidden_size=64, intermediate_size=48, moe_intermediate_size=32,
+                            num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                            num_experts=6, num_experts_per_tok=2, norm_topk_prob=True)
+    model = Qwen3MoeForCausalLM(config).to(torch.bfloat16).eval().to(DEV)
+    packed = {}
+    for i, layer in enumerate(model.model.layers):
+        experts = layer.mlp.experts
+        for p in experts.parameters():
+            p.normal_(0, 0.2)
+        packed[i] = torch.cat([experts.gate_up_proj.flatten(1), experts.down_proj.flatten(1)], 1)
+    assert install_mx_experts(model) == 2 and install_mx_experts(model) == 0
+    install_hip_norms(model), install_hip_attention(model)
+    seen = []
+    for i, layer in enumerate(model.model.layers):
+        assert isinstance(layer.mlp.experts, Qwen3MXExperts)
+        layer.mlp.experts.register_forward_hook(lambda m, a, o, i=i: seen.append((i, *a, o)))
+    ids = torch.randint(0, 96, (1, 300), device=DEV)
+    out = model(input_ids=ids, use_cache=True)
+    for _ in range(3):
+        assert torch.isfinite(out.logits).all()
+        out = model(input_ids=out.logits[:, -1:].argmax(-1), past_key_values=out.past_key_values, use_cache=True)
+    assert len(seen) == 8 and {s[1].shape[0] for s in seen} == {300, 1}
+    for i, hidden, index, weights, got in seen:
+        _check(got, hidden, index, weights.to(torch.bfloat16), packed[i], 64, 32)
