@@ -633,6 +633,7 @@ int sf_mx_values(int held, const void *codes, const void *scales, int rows,
  *   sum = s, normed = y rounded to dtype, codes and scales = y in e4m3 (K13)
  * x and residual [rows, dim] with row strides; the outputs contiguous, each of
  * them NULL if not wanted (sum needs a residual; codes and scales go together).
+ * Fewer than 2^24 rows, 2^26 of up to 512 columns.
  */
 int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
                     const void *residual, int64_t residual_stride, int rows,
@@ -648,7 +649,7 @@ int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
  *   codes, scales   a weight in e2m1 [out_features, dim]
  *   bias      [out_features] of out_dtype, or NULL
  *   out_dtype 0 bf16, 1 fp16; out has row stride out_stride
- * x 16-byte, codes 16-byte, scales and x_scales 4-byte aligned.
+ * x, x_scales, codes and scales 16-byte aligned; rows <= 2^20.
  */
 int sf_mx_linear(int x_dtype, const void *x, const void *x_scales,
                  int64_t x_stride, int rows, int dim, const void *codes,
@@ -669,7 +670,8 @@ int sf_mx_linear(int x_dtype, const void *x, const void *x_scales,
  *   slot_of_expert  device int32 [num_experts], or NULL: expert e in slot e
  *   act, act_scales scratch: rows in e4m3 [tokens * top_k, intermediate_size]
  *   out_rows        bf16 [tokens * top_k, hidden_size]
- * slots and slot_stride 16-byte, out_rows 8-byte aligned.
+ * x, x_scales, slots, slot_stride, act and act_scales 16-byte, out_rows 8-byte
+ * aligned.
  */
 int64_t sf_mx_expert_bytes(int hidden_size, int intermediate_size);
 int sf_mx_expert_parts(int hidden_size, int intermediate_size, int64_t *offsets);

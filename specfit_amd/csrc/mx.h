@@ -181,6 +181,9 @@ __device__ __forceinline__ void store_rows_chunk(const float (&f)[8], int c, uin
   }
 }
 
+// A grid's work-items are counted in 32 bits.
+inline bool grid_fits(int64_t groups, int threads) { return groups <= 0xffffffffll / threads; }
+
 inline bool aligned(const void* p, uintptr_t to) {
   return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0;
 }

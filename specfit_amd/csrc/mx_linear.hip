@@ -127,7 +127,7 @@ __global__ __launch_bounds__(T::kThreads, 2) void linear_tiled_kernel(Linear p, 
 template <class T>
 int launch_tiled(const Linear& p, hipStream_t s) {
   const int row_groups = (p.rows - 1) / T::kRows + 1, out_groups = (p.out_features - 1) / T::kOut + 1;
-  if (static_cast<int64_t>(row_groups) * out_groups > 0x7fffffff) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (!grid_fits(static_cast<int64_t>(row_groups) * out_groups, T::kThreads)) return SF_ERR_UNSUPPORTED_SHAPE;
   linear_tiled_kernel<T><<<dim3(row_groups * out_groups), dim3(T::kThreads), 0, s>>>(p, row_groups, out_groups);
   SF_LAUNCH_CHECK();
   return SF_OK;
@@ -182,11 +182,11 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
     return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0) return SF_OK;
   if (!x || !codes || !scales || !out || (x_dtype == kRows && !x_scales)) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 4) || !aligned(out, 2) ||
+  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, 2) ||
       (bias && !aligned(bias, 2)))
     return SF_ERR_MISALIGNED;
   if (x_dtype == kRows) {
-    if (!aligned(x_scales, 4)) return SF_ERR_MISALIGNED;
+    if (!aligned(x_scales, 16)) return SF_ERR_MISALIGNED;
   } else if (x_stride % 8 || dim % 8) {
     return SF_ERR_MISALIGNED;
   }

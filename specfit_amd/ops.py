@@ -1355,9 +1355,11 @@ def _as_rows(name: str, x: torch.Tensor, stream: torch.cuda.Stream | None) -> to
         raise ValueError(f"{name} must have at least one column")
     if x.stride(-1) != 1:
         x = _dense(x, stream)
-    if x.dim() == 2:
+    if x.dim() == 2 and x.shape[0] <= 0x7FFFFFFF:
         return x
     rows = x.numel() // x.shape[-1]
+    if rows > 0x7FFFFFFF:
+        raise ValueError(f"{name} has too many rows")
     try:
         return x.view(rows, x.shape[-1])
     except RuntimeError:
@@ -1655,9 +1657,9 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
         _require_cuda("hidden_states", hidden, _BF16)
     elif hidden.device.type != "cuda":
         raise ValueError("hidden_states must be on a HIP device")
-    if tuple(hidden.shape) != (T, H):
-        raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
     device = hidden.device
+    if tuple(hidden.shape) != (T, H) or plan.perm_pos.device != device:
+        raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
     _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
     _require_cuda("out_rows", out_rows, _BF16)
     if out_rows.shape != (T * K, H) or not out_rows.is_contiguous() or out_rows.device != device:

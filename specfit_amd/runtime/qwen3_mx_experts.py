@@ -77,36 +77,32 @@ class Qwen3MXExperts(nn.Module):
                 top_k_weights: torch.Tensor) -> torch.Tensor:
         """Sum over a token's experts of weight * expert(token), bf16 [tokens,
         H].  Routes to experts that the layer does not have count for nothing."""
-        if hidden_states.dim() != 2 or hidden_states.shape[1] != self.hidden_size:
-            raise ValueError(f"hidden_states must have shape [tokens, {self.hidden_size}]")
-        if top_k_index.dim() != 2 or top_k_index.shape[0] != hidden_states.shape[0]:
+        records = self.records
+        if top_k_index.dim() != 2:
             raise ValueError("top_k_index must have shape [tokens, top_k]")
+        if _without_dispatch(top_k_index.numel(), *records.shape):
+            return ops.mx_routed_swiglu(hidden_states, top_k_index.contiguous(),
+                                        top_k_weights.to(torch.bfloat16).contiguous(), records,
+                                        self.hidden_size, self.intermediate_size)
+        if hidden_states.shape != (top_k_index.shape[0], self.hidden_size):
+            raise ValueError(f"hidden_states must have shape [tokens, {self.hidden_size}]")
         if top_k_weights.shape != top_k_index.shape:
             raise ValueError("top_k_weights must match top_k_index shape")
-        if hidden_states.dtype != torch.bfloat16:
-            raise ValueError("hidden_states must be bfloat16")
         for t in (hidden_states, top_k_index, top_k_weights):
-            if t.device != self.records.device:
+            if t.device != records.device:
                 raise ValueError("hidden_states and routes must be on the experts' device")
-        T, K = top_k_index.shape
-        if T * K == 0:
-            return torch.zeros_like(hidden_states)
-        if torch.cuda.current_device() != self.records.get_device():
-            with torch.cuda.device(self.records.device):
-                return self._experts(hidden_states, top_k_index, top_k_weights)
-        return self._experts(hidden_states, top_k_index, top_k_weights)
+        if records.is_cuda and torch.cuda.current_device() != records.get_device():
+            with torch.cuda.device(records.device):
+                return self._dispatched(hidden_states, top_k_index, top_k_weights)
+        return self._dispatched(hidden_states, top_k_index, top_k_weights)
 
-    def _experts(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
-                 top_k_weights: torch.Tensor) -> torch.Tensor:
-        T, K = top_k_index.shape
-        weights = top_k_weights.to(torch.bfloat16).contiguous()
-        if _without_dispatch(T * K, self.num_experts, self.records.shape[1]):
-            return ops.mx_routed_swiglu(hidden_states, top_k_index.contiguous(), weights,
-                                        self.records, self.hidden_size, self.intermediate_size)
+    def _dispatched(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
+                    top_k_weights: torch.Tensor) -> torch.Tensor:
         plan = ops.dispatch(top_k_index, self.num_experts)
-        rows = torch.empty((T * K, self.hidden_size), dtype=torch.bfloat16,
+        rows = torch.empty((top_k_index.numel(), self.hidden_size), dtype=torch.bfloat16,
                            device=hidden_states.device)
-        ops.mx_grouped_swiglu(hidden_states, plan, weights.view(-1), self.records, self.hidden_size,
+        weights = top_k_weights.to(torch.bfloat16).contiguous().view(-1)
+        ops.mx_grouped_swiglu(hidden_states, plan, weights, self.records, self.hidden_size,
                               self.intermediate_size, rows)
         return ops.combine(rows, top_k_index, plan, self.hidden_size, accumulate_fp32=True)
 

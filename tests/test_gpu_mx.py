@@ -135,7 +135,7 @@ def _norm_reference(x, residual, weight, eps):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("residual", [True, False])
 @pytest.mark.parametrize("rows,dim", [(1, 1), (1, 2048), (5, 64), (7, 100), (61, 520), (3, 1001),
-                                      (4, 4096), (2, 5000), (3, 9000), (2, 20001), (300, 256)])
+                                      (4, 4096), (2, 5000), (3, 9000), (2, 20001), (300, 256), (2050, 800), (2100, 1001)])
 def test_add_rms_norm(rows, dim, residual, dtype):
     x = _normal(rows, rows, dim).to(dtype)
     res = _normal(dim, rows, dim).to(dtype) * 3 if residual else None
@@ -301,3 +301,93 @@ def test_norm_then_products_as_a_layer_runs_them():
     s = (b.double() + total.double()).to(torch.bfloat16)
     assert torch.equal(total2, s)
     assert torch.equal(q2.values(), ops.mx_quantize(_norm_reference(s, None, wn, 1e-6)[1]).values())
+
+
+def test_weights_from_a_checkpoints_order():
+    rows, dim = 50, 300
+    g = _gen(0)
+    codes = torch.randint(0, 256, (rows, 160), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.randint(120, 132, (rows, 10), generator=g, device=DEV, dtype=torch.uint8)
+    w = MXWeight.from_blocks(codes, scales, dim)
+    four = torch.cat([ref.FOUR, -ref.FOUR]).to(DEV)
+    want = (four[torch.stack([codes & 15, codes >> 4], -1).flatten(1).long()]
+            * torch.exp2(scales.double() - 127).repeat_interleave(32, 1))[:, :dim]
+    assert torch.equal(w.values(torch.float32).double(), want)
+    # One value of a row at a time picks one column of the weight.
+    x = torch.eye(dim, dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(ops.mx_linear(x, w).double(), want.t())
+
+
+def test_far_rows_and_outputs():
+    """Offsets past 32 bits: what lies there equals what it is by itself."""
+    rows, dim = 290_000, 8192
+    x = torch.empty((rows, dim), dtype=torch.bfloat16, device=DEV).normal_(generator=_gen(1))
+    w = (1 + 0.1 * _normal(2, dim)).to(torch.bfloat16)
+    q = ops.mx_quantize(x)
+    tail = x[-700:].clone()
+    assert torch.equal(q.codes.view(rows, dim)[-700:], ops.mx_quantize(tail).codes.view(700, dim))
+    values = q.values()
+    assert torch.equal(values[-700:], ops.mx_quantize(tail).values())
+    del values
+    total, y, nq = ops.add_rms_norm(x, x, w, 1e-6, quantized=True)
+    t2, y2, nq2 = ops.add_rms_norm(tail, tail, w, 1e-6, quantized=True)
+    assert torch.equal(total[-700:], t2) and torch.equal(y[-700:], y2)
+    assert torch.equal(nq.codes.view(rows, dim)[-700:], nq2.codes.view(700, dim))
+    del total, y, nq
+    weight = ops.mx_quantize_weight(x)              # 290,000 outputs
+    assert torch.equal(weight.values()[-672:], ops.mx_quantize_weight(x[-672:]).values())
+    out = ops.mx_linear(tail[:31], weight)
+    assert torch.equal(out[:, -672:], ops.mx_linear(tail[:31], ops.mx_quantize_weight(x[-672:])))
+    weight = ops.mx_quantize_weight(x[:8000])
+    out = ops.mx_linear(q, weight)                  # 2.3e9 outputs
+    # Whatever the tile, the same products are added in the same order.
+    assert torch.equal(out[-600:], ops.mx_linear(x[-600:], weight))
+
+
+def test_captured_chains_replay_each_their_own():
+    """Two graphs of a layer's calls, replayed in turn, with eager work between."""
+    rows, dim = 40, 512
+    weights = [ops.mx_quantize_weight(0.05 * _normal(s, n, dim)) for s, n in ((1, 300), (2, dim))]
+    wn = torch.ones(dim, dtype=torch.bfloat16, device=DEV)
+
+    def chain(h, o):
+        total, _, q = ops.add_rms_norm(o, h, wn, 1e-6, normed=False, quantized=True)
+        return ops.mx_linear(q, weights[0]), ops.add_rms_norm(ops.mx_linear(total, weights[1]), total, wn, 1e-6)[1]
+
+    inputs = [[_normal(s + i, rows, dim).to(torch.bfloat16) for i in range(2)] for s in (3, 5)]
+    graphs, outs = [], []
+    for h, o in inputs:
+        chain(h, o)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(chain(h, o))
+        graphs.append(graph)
+    for step in range(4):
+        for h, o in inputs:
+            h.copy_(_normal(10 + step, rows, dim)), o.copy_(_normal(20 + step, rows, dim))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (h, o), out in zip(inputs, outs):
+            want = chain(h, o)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_each_operator_on_another_stream():
+    rows, dim = 70, 384
+    x = _normal(0, rows, dim).to(torch.bfloat16)
+    wide = _normal(1, dim, rows).to(torch.bfloat16).t()     # copied to dense rows, on the stream
+    w = torch.ones(dim, dtype=torch.bfloat16, device=DEV)
+    want = (ops.mx_quantize(wide).values(), ops.mx_quantize_weight(wide).values(),
+            *ops.add_rms_norm(x, wide, w, 1e-6)[:2], ops.mx_linear(wide, ops.mx_quantize_weight(x)))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    q, wq = ops.mx_quantize(wide, stream=side), ops.mx_quantize_weight(wide, stream=side)
+    xw = ops.mx_quantize_weight(x, stream=side)
+    got = (ops.mx_values(q, stream=side), ops.mx_values(wq, stream=side),
+           *ops.add_rms_norm(x, wide, w, 1e-6, stream=side)[:2], ops.mx_linear(wide, xw, stream=side))
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
