@@ -183,7 +183,7 @@ __device__ __forceinline__ void gate_up_block(const Experts& p, const uint8_t* w
   }
 }
 
-// Few rows: a workgroup takes 16 of one expert's.
+// Few rows, as they come: a workgroup takes 16 of one expert's.
 template <int WAVES, int XDT>
 __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p, int blocks) {
   __shared__ f32x4 part[WAVES * 4 * SF_WAVE];
@@ -333,12 +333,11 @@ __device__ __forceinline__ void fitting_tile(const Experts& p, const Chunk& chun
     down_tile<T>(p, chunk, out0, s0, s1, sc);
 }
 
-// What counts as a short chunk: only beside tall tiles does the order pay for the
-// second scan (us, in turn and sorted: 2,048 tokens 165 / 153, of 64 experts 126 /
-// 118; by 64 rows, 1,024 tokens 110 / 112, 400 with favourites 84.5 / 87).
+// What counts as a short chunk: rows that a lower tiling holds (us, chunks in turn
+// and sorted: 2,048 tokens of 128 experts 165 / 153, of 64 experts 126 / 118).
 template <class... Lower>
 constexpr int light_rows() {
-  if constexpr (sizeof...(Lower) > 1)
+  if constexpr (sizeof...(Lower) > 0)
     return First<Lower...>::type::kRows;
   else
     return 0;
@@ -527,21 +526,24 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
                      static_cast<uint8_t*>(act_scales), static_cast<uint16_t*>(out_rows)};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t routes = static_cast<int64_t>(tokens) * top_k;
-  // By the routes to an expert on average: how many rows share its weights.
+  // By the routes to an expert on average: how many rows share its weights.  us
+  // of both products; experts of 2,048 x 768, 4,096 x 1,536 and 1,000 x 424:
+  //   gate and up by tiles of at most 32 and of 128 rows
+  //     16 routes an expert    70.9 / 76.5    67.7 / 68.3    21.7 / 22.8
+  //     32                     90.5 / 87.5    91.0 / 78.5    32.1 / 30.4
+  //   down by wavefronts and by tiles of at most 128 rows
+  //     4                      63.9 / 66.1    67.3 / 64.8    21.1 / 21.5
+  //     8                      67.5 / 67.3    68.5 / 65.6    22.0 / 21.7
+  //     16                     77.2 / 70.7    78.0 / 68.1    23.9 / 22.0
   int rc;
   if (x_dtype == kBf16)
     rc = gate_up_few<4, kBf16>(p, routes, s);
-  else if (routes <= num_experts)
-    rc = gate_up_few<4, kRows>(p, routes, s);
   else if (routes <= 16 * num_experts)
     rc = tiled<true, Tiles32>(p, routes, s);
-  else if (routes <= 96 * num_experts)
-    rc = tiled<true, Tiles64, Tiles32>(p, routes, s);
   else
     rc = tiled<true, Tiles128, Tiles64, Tiles32>(p, routes, s);
   if (rc) return rc;
   if (routes <= 8 * num_experts) return down_few<1, 2>(p, routes, s);
-  if (routes <= 96 * num_experts) return tiled<false, Tiles64, Tiles32>(p, routes, s);
   return tiled<false, Tiles128, Tiles64, Tiles32>(p, routes, s);
 }
 

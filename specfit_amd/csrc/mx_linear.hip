@@ -139,16 +139,22 @@ constexpr int kMostRawRows = 16;
 
 int64_t groups(int n, int per) { return (n - 1) / per + 1; }
 
-// Few rows, or too small a product for tiles: 16 rows by NT row tiles of the
-// weight in a workgroup of KS wavefronts that cut the sum.
+// Few rows, or too small a product for tiles: 16 or 32 rows by NT row tiles of
+// the weight in a workgroup of KS wavefronts that cut the sum, so that some
+// thousand wavefronts have loads under way.  More row tiles to a wavefront where
+// rows are read for each of them again (us, rows x dim x outputs; 1, 2 and 4 row
+// tiles of 16 rows, then 4 of 32):
+//   1 x 2,048 x 2,048     4.2   3.6   5.3          64 x 2,048 x 2,048     5.5   4.5   6.3   6.9
+//   1 x 2,048 x 20,000    6.4   6.4   8.9          64 x 2,048 x 5,120    10.3   7.9   7.3   7.1
+//   16 x 2,048 x 16,384   8.8   6.4   7.5          32 x 4,096 x 9,216    17.7  13.2  11.3  11.0
 template <int XDT>
 int launch_few(const Linear& p, hipStream_t s) {
   const int64_t units = groups(p.rows, 16) * row_tiles(p.out_features);
-  if (XDT == kRows && units >= 2048)
+  if (XDT == kRows && p.rows > 16 && units >= 2048)
     launch_direct<2, 4, 4, 4, kRows>(p, s);
-  else if (XDT == kRows && units >= 1024)
+  else if (XDT == kRows && p.rows > 16 && units >= 1024)
     launch_direct<1, 4, 4, 4, kRows>(p, s);
-  else if (units >= 320)
+  else if (units >= 128)
     launch_direct<1, 2, 8, 8, XDT>(p, s);
   else
     launch_direct<1, 1, 8, 8, XDT>(p, s);
@@ -156,14 +162,30 @@ int launch_few(const Linear& p, hipStream_t s) {
   return SF_OK;
 }
 
-// The largest tiles that give the 256 CUs a workgroup each.
+// Tiles where they make work for the 256 CUs, the larger the better they fill
+// them; at most 2 workgroups of the largest run on a CU together, 4 of the others.
+// us; direct form, then tiles of 32 x 128, 64 x 64, 64 x 128 and 128 x 256 rows and
+// outputs:
+//   16 x 2,048 x 40,000    12.9  13.5  13.5  14.2         16 x 2,048 x 80,000    22.7  19.5  19.8  19.5
+//   32 x 2,048 x 16,384     8.1   9.1   8.4   9.7         32 x 2,048 x 32,768    12.6  12.5  12.7  13.1
+//   256 x 2,048 x 2,048     7.0   8.4   7.8   9.1         128 x 2,048 x 5,120     9.2   8.9   8.3   9.6
+//   1,024 x 2,048 x 2,048         10.4   9.3  10.0        1,024 x 2,048 x 5,120         18.2  18.3  16.8  19.9
+//   2,048 x 4,096 x 9,216               101.9  81.3  86.4     (576 of the largest)
+//   1,536 x 4,096 x 9,216                78.2  61.4  56.1     (432)
+//   8,192 x 2,048 x 2,048                48.6  40.4  35.0     (512)
 int launch_rows(const Linear& p, hipStream_t s) {
   constexpr int kCus = 256;
   const int m = p.rows, n = p.out_features;
-  if (m <= 32 && groups(n, 128) >= kCus) return launch_tiled<Tiling<2, 1, 2, 1>>(p, s);
-  if (m > 64 && groups(m, 128) * groups(n, 256) >= kCus) return launch_tiled<Tiling<2, 2, 4, 2>>(p, s);
-  if (m > 32 && groups(m, 64) * groups(n, 128) >= kCus) return launch_tiled<Tiling<2, 2, 2, 1>>(p, s);
-  if (m > 32 && groups(m, 64) * groups(n, 64) >= kCus) return launch_tiled<Tiling<2, 2, 1, 1>>(p, s);
+  if (m <= 32) {
+    if (groups(n, 128) >= (m <= 16 ? 2 * kCus : kCus)) return launch_tiled<Tiling<2, 1, 2, 1>>(p, s);
+    return launch_few<kRows>(p, s);
+  }
+  const int64_t large = groups(m, 128) * groups(n, 256);
+  // The largest in one nearly full round, or in several.
+  if (m > 64 && (large >= 4 * kCus || (large <= 2 * kCus && large * 5 >= 2 * kCus * 4)))
+    return launch_tiled<Tiling<2, 2, 4, 2>>(p, s);
+  if (groups(m, 64) * groups(n, 128) >= 2 * kCus) return launch_tiled<Tiling<2, 2, 2, 1>>(p, s);
+  if (groups(m, 64) * groups(n, 64) >= kCus * 5 / 8) return launch_tiled<Tiling<2, 2, 1, 1>>(p, s);
   return launch_few<kRows>(p, s);
 }
 

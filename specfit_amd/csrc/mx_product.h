@@ -359,6 +359,18 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
           acc[n][m] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
               a[h][n], b[h][m], acc[n][m], 4, 0, 0, static_cast<int>(ws[n][h]), 0, static_cast<int>(xs[m][h]));
     }
+    if constexpr (!T::kTwoAhead) {
+      // All of the first half's reads, then the second half's among the first's
+      // products.
+      constexpr int kReads = T::FN + 2 * T::FM, kProducts = T::FN * T::FM, kMfma = 0x8, kDsRead = 0x100;
+      __builtin_amdgcn_sched_group_barrier(kDsRead, kReads, 0);
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, (kReads + kProducts - 1) / kProducts, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kMfma, kProducts, 0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll

@@ -1337,6 +1337,11 @@ def greedy_tokens(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
 # ------------------------------------------------------- K13: microscaled --
 _MX_E4M3, _MX_E2M1, _MX_ROWS = 0, 1, 3
 _MX_RAW_ROWS = 16   # rows of 16-bit values that a product takes as they are
+# ... of a weight up to this size: every wavefront rounds the rows it reads, which costs more
+# than a launch of its own where there are many of them.  us on the device, as they are and
+# with the launch (4 more on the host): 1 row of 2,048 x 5,120 outputs 5.4 / 6.0, x 16,384
+# 9.4 / 7.5, x 40,000 22 / 13.5, x 151,936 77 / 36; 16 rows 7.2 / 7.2, 12 / 8.7, 30 / 15, 103 / 37.
+_MX_RAW_WEIGHT = 1 << 25
 
 
 def _new(shape, dtype: torch.dtype, device: torch.device,
@@ -1538,8 +1543,8 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
     kind, x_ptr, scale_ptr, stride = _MX_ROWS, 0, None, 0
     if not held:
         flat = _as_rows("x", x, stream)
-        if flat.shape[0] <= _MX_RAW_ROWS and weight.dim % 8 == 0 and flat.stride(0) % 8 == 0 \
-                and flat.data_ptr() % 16 == 0:
+        if flat.shape[0] <= _MX_RAW_ROWS and weight.rows * weight.dim <= _MX_RAW_WEIGHT \
+                and weight.dim % 8 == 0 and flat.stride(0) % 8 == 0 and flat.data_ptr() % 16 == 0:
             kind, x_ptr, stride = _DTYPES[dtype], flat.data_ptr(), flat.stride(0)
         else:
             x = _mx_rows(shape, flat.shape[0], dtype, device, stream)

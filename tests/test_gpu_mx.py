@@ -209,9 +209,11 @@ def _exact_case(seed, rows, dim, out, dtype):
 
 LINEAR = [(1, 128, 16), (1, 2048, 5120), (2, 64, 24), (3, 40, 33), (16, 1000, 100), (17, 768, 2048),
           (32, 2048, 64), (33, 100, 47), (61, 2048, 1000), (64, 4096, 256), (100, 520, 330),
-          (129, 128, 512), (255, 1024, 257), (256, 896, 512), (300, 136, 1030), (512, 2048, 768), (20, 64, 33000), (60, 200, 33000),
+          (129, 128, 512), (255, 1024, 257), (256, 896, 512), (300, 136, 1030), (512, 2048, 768), (20, 64, 33000),
+          (60, 200, 33000),
           (128, 64, 66000), (600, 640, 2500), (400, 96, 1100),
-          (1000, 320, 96), (1, 8000, 48), (5, 2080, 4096), (2000, 1152, 4200)]
+          (1000, 320, 96), (1, 8000, 48), (5, 2080, 4096), (2000, 1152, 4200), (16, 64, 70000),
+          (7, 2048, 17000), (1600, 128, 9000), (4100, 72, 8000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
