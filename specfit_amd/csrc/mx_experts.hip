@@ -5,7 +5,15 @@
 //   rows[r] = bf16((a . down^T) * route_weight)
 // with fp32 sums and one rounding between them: the activation is what the
 // second product reads, so it is rounded once, from fp32, to that product's
-// type.
+// type.  A route's row is rounded to bf16 for the combine, which halves what the
+// two exchange (8 routes of a token: 0.0024 of the outputs' norm against 64 bits,
+// 0.0016 without); the form without a dispatch adds in fp32 and rounds once.
+//
+// 128 experts of 2,048 x 768, 8 to a token, one MI355X; gate and up, then down:
+//   1 token (no dispatch)        7.6 + 5.6 us   latency of two dependent launches
+//   61 tokens, favourites         36 + 20 us    4.2 and 3.7 TB/s of weights
+//   2,048 tokens                  74 + 59 us    1.4 and 0.9 PFLOP/s, the weights' 214
+//                                               and 107 MB arriving meanwhile
 #include "mx_product.h"
 
 namespace {

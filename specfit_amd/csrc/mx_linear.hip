@@ -2,7 +2,13 @@
 //   out[m, n] = T(sum_k x[m, k] w[n, k] + bias[n]),
 // x in e4m3 (rounded here where rows come in 16 bits), w in e2m1.  Products are
 // exact, the matrix unit adds a block's in its own fixed order and width and
-// accumulates in fp32.
+// accumulates in fp32; the output is rounded once, to the type that x came in.
+//
+// One MI355X (a large copy moves 5.0 TB/s, an 8,192^3 library product in e4m3 runs
+// at 2,650 TFLOP/s):
+//   1 x 2,048 x 5,120            5.5 us   latency: eight wavefronts cut the sum
+//   61 x 2,048 x 151,936        41 us   the weight's 165 MB at 4.5 TB/s with the output
+//   4,096 x 4,096 x 9,216      133 us   2,330 TFLOP/s, the chip's power: zeros take 115
 #include "mx_product.h"
 
 namespace {
@@ -134,7 +140,7 @@ int launch_tiled(const Linear& p, hipStream_t s) {
 }
 
 // Rows of 16-bit values are rounded by every wavefront that reads them, which
-// is cheaper than a launch of its own for one tile of rows only.
+// is cheaper than a launch of its own for one tile of rows and few wavefronts only.
 constexpr int kMostRawRows = 16;
 
 int64_t groups(int n, int per) { return (n - 1) / per + 1; }

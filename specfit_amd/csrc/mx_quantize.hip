@@ -3,7 +3,15 @@
 //
 // Formats and layouts are in mx.h.  All of it is memory traffic: a block's
 // scale is an integer maximum over the magnitudes' bits, a code the conversion
-// instruction's result on the value times an exact power of two.
+// instruction's result on the value times an exact power of two.  A lane holds 8
+// neighbours, which is a whole 16-byte load of 16-bit values and a quarter of a
+// block, whatever the row's alignment.
+//
+// bf16, one MI355X (a large copy moves 5.0 TB/s):
+//   8,192 x 4,096 to e4m3     20.8 us   4.9 TB/s     and back   17.4 us   5.8 TB/s
+//   151,936 x 2,048 to e2m1    150 us   5.3 TB/s     and back    125 us   6.3 TB/s
+//   8,192 x 4,096 residual, norm, e4m3 output   59 us   5.1 TB/s
+//   1 x 2,048: 1.6 (values) to 3 us, a launch's latency
 #include "mx.h"
 
 namespace {
@@ -193,6 +201,7 @@ __global__ __launch_bounds__(kThreads) void weight_values_kernel(const uint8_t* 
 // for each output.  The mean is kept in 64 bits: r is then the same whatever
 // the order of the sum, so are the 8-bit codes, whose borders a last bit of r
 // would move values across, and the 64-bit work hides under the row's traffic.
+// Addition and products are single fp32 operations (no contraction).
 //
 // LANES (a wavefront or a workgroup of four) take a row, a lane chunks of 8
 // at LANES * 8 from each other, CHUNKS of them in registers between the two

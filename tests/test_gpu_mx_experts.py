@@ -35,7 +35,9 @@ def _check(got, h, index, weights, packed, hidden, inner):
 
 SHAPES = [(1, 64, 32, 8, 3), (5, 64, 32, 8, 3), (40, 64, 32, 8, 3), (7, 1000, 424, 20, 2),
           (3, 33, 17, 4, 1), (16, 2048, 768, 16, 8), (17, 2048, 768, 16, 8), (61, 256, 160, 128, 8),
-          (150, 256, 96, 4, 2), (300, 512, 256, 6, 2), (1, 4096, 1536, 8, 8), (600, 128, 64, 3, 1)]
+          (150, 256, 96, 4, 2), (300, 512, 256, 6, 2), (1, 4096, 1536, 8, 8), (600, 128, 64, 3, 1),
+          (33, 64, 32, 1, 1), (50, 64, 32, 256, 3), (400, 1000, 424, 3, 1), (300, 33, 17, 2, 1),
+          (700, 136, 200, 5, 5)]
 
 
 @pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", SHAPES)
