@@ -701,6 +701,28 @@ int sf_mx_routed_swiglu(int x_dtype, const void *x, const void *x_scales,
                         int64_t slot_stride, void *act, void *act_scales,
                         void *out, sf_stream_t stream);
 
+/*
+ * A layer's routed experts in one call: sf_mx_routed_swiglu, or sf_dispatch,
+ * sf_mx_grouped_swiglu and sf_combine (fp32 sums of the routes' bf16 rows),
+ * expert e in slot e.
+ *   x_dtype     0 bf16 rows of row stride x_stride, any number and alignment of
+ *               them; 3 rows in e4m3 as above
+ *   workspace   sf_mx_experts_workspace bytes (-1: an unsupported shape),
+ *               16-byte aligned; calls that may overlap need one each
+ * sf_mx_experts_form says which it is: 1 without a dispatch, 0 with one (-1: an
+ * unsupported shape).
+ */
+int sf_mx_experts_form(int tokens, int top_k, int hidden_size,
+                       int intermediate_size, int num_experts);
+int64_t sf_mx_experts_workspace(int tokens, int top_k, int hidden_size,
+                                int intermediate_size, int num_experts);
+int sf_mx_experts(int x_dtype, const void *x, const void *x_scales,
+                  int64_t x_stride, const int64_t *index,
+                  const void *route_weights, int tokens, int top_k,
+                  int hidden_size, int intermediate_size, int num_experts,
+                  const void *slots, int64_t slot_stride, void *workspace,
+                  void *out, sf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

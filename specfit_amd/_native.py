@@ -80,6 +80,9 @@ SIGNATURES = {
     "sf_mx_expert_parts": ([_i, _i, _p], _i),
     "sf_mx_routed_swiglu": ([_i, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i64, _p, _p, _p,
                              _p], _i),
+    "sf_mx_experts_form": ([_i, _i, _i, _i, _i], _i),
+    "sf_mx_experts_workspace": ([_i, _i, _i, _i, _i], _i64),
+    "sf_mx_experts": ([_i, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _p, _i64, _p, _p, _p], _i),
     "sf_mx_grouped_swiglu": ([_i, _p, _p, _i64, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i64, _p, _p,
                               _p, _p], _i),
 }

@@ -14,6 +14,8 @@
 //   61 tokens, favourites         36 + 20 us    4.2 and 3.7 TB/s of weights
 //   2,048 tokens                  74 + 59 us    1.4 and 0.9 PFLOP/s, the weights' 214
 //                                               and 107 MB arriving meanwhile
+#include <cmath>
+
 #include "mx_product.h"
 
 namespace {
@@ -500,6 +502,49 @@ int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, in
   return SF_OK;
 }
 
+// Routes that read their experts for themselves save a dispatch, a combine and the
+// launches of both: about 10 us on the device and 10 on the host.  They read an
+// expert again for each further route to it, with even routing routes - E (1 -
+// (1 - 1 / E)^routes) times; 10 us are 40 MB of such reads.  us a call on the
+// device, without dispatch and with it:
+//   128 experts of 2048 x 768, 8 a token    1 token 12 / 21   4: 24 / 30   8: 42 / 42   12: 60 / 53
+//   32 experts of 4096 x 1536, 8 a token    1 token 27 / 34   2: 40 / 45   3: 57 / 55   4: 71 / 67
+//   100 experts of 1000 x 424, 2 a token    1 token 8 / 15    16: 14 / 19  32: 19 / 23
+// Beyond 128 routes the products' idle rows would count.
+bool without_dispatch(int64_t routes, int experts, int64_t expert_bytes) {
+  if (routes > 128) return false;
+  const double again = routes - experts * (1.0 - std::pow(1.0 - 1.0 / experts, static_cast<double>(routes)));
+  return again * static_cast<double>(expert_bytes) <= 40e6;
+}
+
+// sf_mx_experts' workspace: what each part starts at, in bytes.
+struct Workspace {
+  int64_t act, act_scales, x, x_scales, meta, perm, inv, rows, bytes;
+};
+
+Workspace workspace_of(int tokens, int top_k, int hidden, int inner, int experts, bool dispatched) {
+  Workspace w = {};
+  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += (bytes + 255) / 256 * 256;
+    return from;
+  };
+  w.act = take(routes * tiles(inner) * kTile);
+  w.act_scales = take(routes * quads(inner) * 16);
+  w.x = take(static_cast<int64_t>(tokens) * tiles(hidden) * kTile);
+  w.x_scales = take(static_cast<int64_t>(tokens) * quads(hidden) * 16);
+  if (dispatched) {
+    w.meta = take(8ll * (experts + 1));
+    w.perm = take(4 * routes);
+    w.inv = take(4 * routes);
+    w.rows = take(2 * routes * hidden);
+  }
+  w.bytes = at;
+  return w;
+}
+
 }  // namespace
 
 extern "C" int64_t sf_mx_expert_bytes(int hidden_size, int intermediate_size) {
@@ -584,4 +629,55 @@ extern "C" int sf_mx_routed_swiglu(int x_dtype, const void* x, const void* x_sca
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int64_t routes = static_cast<int64_t>(tokens) * top_k;
   return x_dtype == kBf16 ? routed<8, kBf16>(p, r, routes, s) : routed<8, kRows>(p, r, routes, s);
+}
+
+extern "C" int sf_mx_experts_form(int tokens, int top_k, int hidden_size, int intermediate_size, int num_experts) {
+  const int64_t bytes = sf_mx_expert_bytes(hidden_size, intermediate_size);
+  if (tokens < 0 || top_k < 1 || num_experts < 1 || bytes < 0) return -1;
+  return without_dispatch(static_cast<int64_t>(tokens) * top_k, num_experts, bytes);
+}
+
+extern "C" int64_t sf_mx_experts_workspace(int tokens, int top_k, int hidden_size, int intermediate_size,
+                                           int num_experts) {
+  const int form = sf_mx_experts_form(tokens, top_k, hidden_size, intermediate_size, num_experts);
+  if (form < 0 || top_k > SF_MAX_TOPK || num_experts > SF_MAX_EXPERTS) return -1;
+  return workspace_of(tokens, top_k, hidden_size, intermediate_size, num_experts, form == 0).bytes;
+}
+
+extern "C" int sf_mx_experts(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, const int64_t* index,
+                             const void* route_weights, int tokens, int top_k, int hidden_size, int intermediate_size,
+                             int num_experts, const void* slots, int64_t slot_stride, void* workspace, void* out,
+                             sf_stream_t stream) {
+  const int64_t bytes = sf_mx_experts_workspace(tokens, top_k, hidden_size, intermediate_size, num_experts);
+  if (bytes < 0) return SF_ERR_INVALID_ARGUMENT;
+  if (tokens == 0) return SF_OK;
+  if (!x || !index || !route_weights || !slots || !workspace || !out) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(workspace, 16) || !aligned(out, 2)) return SF_ERR_MISALIGNED;
+  const bool dispatched = !sf_mx_experts_form(tokens, top_k, hidden_size, intermediate_size, num_experts);
+  const Workspace w = workspace_of(tokens, top_k, hidden_size, intermediate_size, num_experts, dispatched);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  // Few rows are rounded by the wavefronts that read them.
+  if (x_dtype == kBf16 && (tokens > 16 || hidden_size % 8 || x_stride % 8 || !aligned(x, 16))) {
+    if (const int rc = sf_mx_quantize(kBf16, x, x_stride, 0, tokens, hidden_size, 1, kE4m3, base + w.x, 0,
+                                      base + w.x_scales, 0, stream))
+      return rc;
+    x_dtype = kRows;
+    x = base + w.x;
+    x_scales = base + w.x_scales;
+  }
+  if (!dispatched)
+    return sf_mx_routed_swiglu(x_dtype, x, x_scales, x_stride, index, route_weights, tokens, top_k, hidden_size,
+                               intermediate_size, num_experts, nullptr, slots, slot_stride, base + w.act,
+                               base + w.act_scales, out, stream);
+  int32_t* counts = reinterpret_cast<int32_t*>(base + w.meta);
+  int32_t* offsets = counts + num_experts + 1;
+  int32_t* perm = reinterpret_cast<int32_t*>(base + w.perm);
+  int32_t* inv = reinterpret_cast<int32_t*>(base + w.inv);
+  if (const int rc = sf_dispatch(index, tokens, top_k, num_experts, counts, offsets, perm, inv, nullptr, stream))
+    return rc;
+  if (const int rc = sf_mx_grouped_swiglu(x_dtype, x, x_scales, x_stride, perm, offsets, route_weights, tokens, top_k,
+                                          hidden_size, intermediate_size, num_experts, nullptr, slots, slot_stride,
+                                          base + w.act, base + w.act_scales, base + w.rows, stream))
+    return rc;
+  return sf_combine(base + w.rows, index, inv, nullptr, tokens, top_k, num_experts, hidden_size, 1, out, stream);
 }

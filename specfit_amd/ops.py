@@ -1730,3 +1730,63 @@ def mx_routed_swiglu(hidden: torch.Tensor | MXRows, index: torch.Tensor,
     if rc:
         _native.check(rc, "sf_mx_routed_swiglu")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _mx_experts_workspace(tokens: int, top_k: int, hidden_size: int, intermediate_size: int,
+                          num_experts: int) -> int:
+    n = _native.lib().sf_mx_experts_workspace(tokens, top_k, hidden_size, intermediate_size,
+                                              num_experts)
+    if n < 0:
+        raise ValueError("unsupported number of experts, or of experts to a token")
+    return n
+
+
+def mx_experts(hidden: torch.Tensor | MXRows, index: torch.Tensor, route_weights: torch.Tensor,
+               records: torch.Tensor, hidden_size: int, intermediate_size: int, *,
+               stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """A layer's routed experts with weights in microscaled 4 bits, every
+    expert resident (K16): bf16 [tokens, H], for each token the sum over its
+    routes of weight * expert.
+
+    hidden [tokens, H] bf16 or its MXRows, ``index`` int64 and ``route_weights``
+    bf16 [tokens, top_k], ``records`` uint8 [experts, mx_expert_bytes(H, I)].
+    Few routes run as ``mx_routed_swiglu``, others as ``dispatch``,
+    ``mx_grouped_swiglu`` and ``combine`` with fp32 sums.  Routes to experts that
+    are not there count for nothing.  Nothing is read back to the host.  With
+    ``stream``, the inputs and the output (memory of the current stream) are the
+    caller's to order between the two streams.  No gradients."""
+    H, I = hidden_size, intermediate_size
+    held = isinstance(hidden, MXRows)
+    _refuse_gradients("mx_experts", None if held else hidden, route_weights)
+    _require_cuda("top_k_index", index, torch.int64)
+    if index.dim() != 2 or not index.is_contiguous():
+        raise ValueError("top_k_index must be contiguous [tokens, top_k]")
+    T, K = index.shape
+    device = index.device
+    if not held:
+        _require_cuda("hidden_states", hidden, _BF16)
+    if tuple(hidden.shape) != (T, H) or hidden.device != device:
+        raise ValueError(f"hidden_states must be [{T}, {H}] on the routes' device")
+    _require_cuda("route weights", route_weights, _BF16)
+    if route_weights.shape != index.shape or not route_weights.is_contiguous() \
+            or route_weights.device != device:
+        raise ValueError("route weights must be contiguous bf16 [tokens, top_k]")
+    E = records.shape[0]
+    _mx_slots(records, None, E, H, I, device)
+    if T * K == 0:
+        return torch.zeros((T, H), dtype=_BF16, device=device)
+    out = torch.empty((T, H), dtype=_BF16, device=device)
+    workspace = _new(_mx_experts_workspace(T, K, H, I, E), torch.uint8, device, stream)
+    if held:
+        kind, stride, (x, scales) = _MX_ROWS, 0, hidden._pointers()
+    else:
+        hidden = _as_rows("hidden_states", hidden, stream)
+        kind, stride, x, scales = 0, hidden.stride(0), hidden.data_ptr(), None
+    rc = _launch(_native.lib().sf_mx_experts, device.index, kind, x, scales, stride,
+                 index.data_ptr(), route_weights.data_ptr(), T, K, H, I, E, records.data_ptr(),
+                 records.stride(0), workspace.data_ptr(), out.data_ptr(),
+                 _stream_handle(stream, device))
+    if rc:
+        _native.check(rc, "sf_mx_experts")
+    return out

@@ -9,29 +9,10 @@ and can be captured into a graph.
 """
 from __future__ import annotations
 
-import functools
-
 import torch
 from torch import nn
 
 from .. import ops
-
-# Routes that read their experts for themselves save a dispatch, a combine and
-# the launches of both: about 10 us on the device, and 20 on the host.  They
-# read an expert again for each further route to it, with even routing
-# routes - E (1 - (1 - 1/E)^routes) times; 10 us are 40 MB of such reads.
-# us a call on the device, without dispatch and with it:
-#   128 experts of 2048 x 768, 8 a token    1 token 12 / 21   4: 24 / 30   8: 42 / 42   12: 60 / 53
-#   32 experts of 4096 x 1536, 8 a token    1 token 27 / 34   2: 40 / 45   3: 57 / 55   4: 71 / 67
-#   100 experts of 1000 x 424, 2 a token    1 token 8 / 15    16: 14 / 19  32: 19 / 23
-_READ_AGAIN = 40_000_000
-_MOST_ROUTES = 128   # beyond, the products' idle rows would count
-
-
-@functools.lru_cache(maxsize=1024)
-def _without_dispatch(routes: int, experts: int, expert_bytes: int) -> bool:
-    again = routes - experts * (1 - (1 - 1 / experts) ** routes)
-    return routes <= _MOST_ROUTES and again * expert_bytes <= _READ_AGAIN
 
 
 class Qwen3MXExperts(nn.Module):
@@ -77,34 +58,10 @@ class Qwen3MXExperts(nn.Module):
                 top_k_weights: torch.Tensor) -> torch.Tensor:
         """Sum over a token's experts of weight * expert(token), bf16 [tokens,
         H].  Routes to experts that the layer does not have count for nothing."""
-        records = self.records
-        if top_k_index.dim() != 2:
-            raise ValueError("top_k_index must have shape [tokens, top_k]")
-        if _without_dispatch(top_k_index.numel(), *records.shape):
-            return ops.mx_routed_swiglu(hidden_states, top_k_index.contiguous(),
-                                        top_k_weights.to(torch.bfloat16).contiguous(), records,
-                                        self.hidden_size, self.intermediate_size)
-        if hidden_states.shape != (top_k_index.shape[0], self.hidden_size):
-            raise ValueError(f"hidden_states must have shape [tokens, {self.hidden_size}]")
-        if top_k_weights.shape != top_k_index.shape:
-            raise ValueError("top_k_weights must match top_k_index shape")
-        for t in (hidden_states, top_k_index, top_k_weights):
-            if t.device != records.device:
-                raise ValueError("hidden_states and routes must be on the experts' device")
-        if records.is_cuda and torch.cuda.current_device() != records.get_device():
-            with torch.cuda.device(records.device):
-                return self._dispatched(hidden_states, top_k_index, top_k_weights)
-        return self._dispatched(hidden_states, top_k_index, top_k_weights)
-
-    def _dispatched(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
-                    top_k_weights: torch.Tensor) -> torch.Tensor:
-        plan = ops.dispatch(top_k_index, self.num_experts)
-        rows = torch.empty((top_k_index.numel(), self.hidden_size), dtype=torch.bfloat16,
-                           device=hidden_states.device)
-        weights = top_k_weights.to(torch.bfloat16).contiguous().view(-1)
-        ops.mx_grouped_swiglu(hidden_states, plan, weights, self.records, self.hidden_size,
-                              self.intermediate_size, rows)
-        return ops.combine(rows, top_k_index, plan, self.hidden_size, accumulate_fp32=True)
+        if top_k_weights.dtype != torch.bfloat16:
+            top_k_weights = top_k_weights.to(torch.bfloat16)
+        return ops.mx_experts(hidden_states, top_k_index.contiguous(), top_k_weights.contiguous(),
+                              self.records, self.hidden_size, self.intermediate_size)
 
 
 def install_mx_experts(model: nn.Module) -> int:

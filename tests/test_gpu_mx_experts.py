@@ -213,6 +213,44 @@ def test_routed_captured_and_on_another_stream():
         assert torch.equal(out, ops.mx_routed_swiglu(h, index, weights, records, 256, 128))
 
 
+@pytest.mark.parametrize("tokens", [2, 12, 90])
+def test_one_call_takes_any_rows(tokens):
+    H, I, E, K = 128, 64, 6, 3
+    h, packed, index, weights = _case(tokens, H, I, E, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    want = ops.mx_experts(h, index, weights, records, H, I)
+    _check(want, h, index, weights, packed, H, I)
+    wide = torch.zeros((tokens, 2 * H + 1), dtype=torch.bfloat16, device=DEV)
+    for at in (3, 8, H + 1):
+        wide[:, at:at + H] = h
+        # Rows rounded here or beforehand: the same codes, so the same bits in one form.
+        assert torch.equal(ops.mx_experts(wide[:, at:at + H], index, weights, records, H, I),
+                           ops.mx_experts(ops.mx_quantize(h), index, weights, records, H, I))
+    columns = h.t().contiguous().t()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got = ops.mx_experts(columns, index, weights, records, H, I, stream=side)
+    side.synchronize()
+    assert torch.equal(got, ops.mx_experts(ops.mx_quantize(h), index, weights, records, H, I))
+
+
+def test_two_calls_at_once():
+    """Each call has scratch memory of its own."""
+    H, I, E, K = 512, 256, 16, 4
+    cases = [_case(t, H, I, E, K, seed=t) for t in (1, 300)]
+    records = [ops.mx_quantize_experts(c[1], H, I) for c in cases]
+    want = [ops.mx_experts(c[0], c[2], c[3], r, H, I) for c, r in zip(cases, records)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, r) in enumerate(zip(cases, records)):
+            got[i].append(ops.mx_experts(c[0], c[2], c[3], r, H, I, stream=streams[i]))
+    torch.cuda.synchronize()
+    for outs, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in outs)
+
+
 @torch.inference_mode()
 def test_a_model_with_mx_experts_prompt_and_decoding():
     """Every layer's experts in a model's own forwards, a prompt and single

@@ -7,7 +7,6 @@ import torch
 from specfit_amd import _native, mx, ops
 from specfit_amd.mx import MXRows, MXWeight
 from specfit_amd.runtime import Qwen3MXExperts
-from specfit_amd.runtime.qwen3_mx_experts import _without_dispatch
 
 INVALID, UNSUPPORTED, MISALIGNED, TOO_MANY = 1, 2, 3, 4
 
@@ -102,7 +101,8 @@ def test_operators_refuse_what_they_cannot_do():
                  lambda: ops.mx_quantize_experts(torch.zeros((1, 3 * 64 * 32), dtype=torch.bfloat16), 64, 32),
                  lambda: ops.mx_grouped_swiglu(x, plan, None, slots, 64, 32, rows),
                  lambda: ops.mx_grouped_swiglu(_held(), plan, None, slots, 64, 32, rows),
-                 lambda: ops.mx_routed_swiglu(x, index, routes, slots, 64, 32)]:
+                 lambda: ops.mx_routed_swiglu(x, index, routes, slots, 64, 32),
+                 lambda: ops.mx_experts(x, index, routes, slots, 64, 32)]:
         with pytest.raises(ValueError, match="device"):     # there is no host form
             call()
     with pytest.raises(TypeError):
@@ -124,7 +124,9 @@ def test_operators_refuse_inputs_that_want_gradients():
                  lambda: ops.mx_grouped_swiglu(x, plan, None, x, 64, 32, x),
                  lambda: ops.mx_grouped_swiglu(_held(), plan, x, x, 64, 32, x),
                  lambda: ops.mx_routed_swiglu(x, plain, plain, plain, 64, 32),
-                 lambda: ops.mx_routed_swiglu(_held(), plain, x, plain, 64, 32)]:
+                 lambda: ops.mx_routed_swiglu(_held(), plain, x, plain, 64, 32),
+                 lambda: ops.mx_experts(x, plain, plain, plain, 64, 32),
+                 lambda: ops.mx_experts(_held(), plain, x, plain, 64, 32)]:
         with pytest.raises(ValueError, match="no gradient"):
             call()
 
@@ -204,6 +206,14 @@ def test_the_library_refuses_before_any_launch():
     assert g(3, p, p, 0, p, p, None, 2, 2, 64, 32, 4, None, p, big + 8, p, p, p, None) == misaligned
     assert g(3, p, p, 0, p, p, None, 2, 2, 64, 32, 257, None, p, big, p, p, p, None) not in (0, INVALID, misaligned)
     assert g(0, p, None, 64, p, p, None, 17, 2, 64, 32, 4, None, p, big, p, p, p, None) == unsupported
+    e = lib.sf_mx_experts
+    assert e(0, p, None, 64, p, p, 0, 2, 64, 32, 4, p, big, p, p, None) == 0
+    assert e(0, p, None, 64, p, p, 2, 2, 64, 32, 257, p, big, p, p, None) == INVALID
+    assert e(0, p, None, 64, p, p, 2, 2, 64, 32, 4, p, big, None, p, None) == INVALID
+    assert e(3, p, None, 0, p, p, 2, 2, 64, 32, 4, p, big, p, p, None) == INVALID
+    assert e(1, p, None, 64, p, p, 2, 2, 64, 32, 4, p, big, p, p, None) == INVALID
+    assert e(0, p, None, 64, p, p, 2, 2, 64, 32, 4, p, big, p + 4, p, None) == misaligned
+    assert e(0, p, None, 64, p, p, 2, 2, 64, 32, 4, p, big - 16, p, p, None) == INVALID
     r = lib.sf_mx_routed_swiglu
     assert r(3, p, p, 0, p, p, 0, 2, 64, 32, 4, None, p, big, p, p, p, None) == 0
     assert r(3, p, p, 0, p, None, 2, 2, 64, 32, 4, None, p, big, p, p, p, None) == INVALID
@@ -212,7 +222,19 @@ def test_the_library_refuses_before_any_launch():
 
 
 def test_few_routes_go_without_a_dispatch():
-    nbytes = ops.mx_expert_bytes(2048, 768)
-    assert _without_dispatch(8, 128, nbytes) and _without_dispatch(1, 1, nbytes)
-    assert not _without_dispatch(61 * 8, 128, nbytes) and not _without_dispatch(129, 256, 100)
-    assert not _without_dispatch(32, 8, ops.mx_expert_bytes(4096, 1536))
+    form = _native.lib().sf_mx_experts_form
+    assert form(1, 8, 2048, 768, 128) == form(8, 8, 2048, 768, 128) == form(1, 1, 64, 32, 1) == 1
+    assert form(61, 8, 2048, 768, 128) == form(43, 3, 64, 32, 256) == form(4, 8, 4096, 1536, 8) == 0
+    assert form(-1, 8, 2048, 768, 128) == form(1, 0, 64, 32, 4) == form(1, 1, 0, 32, 4) == -1
+
+
+def test_the_workspace_holds_every_part():
+    size = _native.lib().sf_mx_experts_workspace
+    for tokens, top_k, hidden, inner, experts in [(1, 8, 2048, 768, 128), (500, 2, 33, 17, 6), (64, 8, 96, 300, 256)]:
+        routes = tokens * top_k
+        parts = [routes * sum(mx.row_bytes(inner)), tokens * sum(mx.row_bytes(hidden))]
+        if not _native.lib().sf_mx_experts_form(tokens, top_k, hidden, inner, experts):
+            parts += [8 * (experts + 1), 8 * routes, 2 * routes * hidden]
+        assert sum(parts) <= size(tokens, top_k, hidden, inner, experts) <= sum(parts) + 8 * 256
+    assert size(1, 8, 64, 32, 257) == size(1, 8, 0, 32, 4) == size(1, 0, 64, 32, 4) == -1
+    assert size(0, 2, 64, 32, 4) >= 0
