@@ -643,19 +643,24 @@ int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
 
 /*
  * K15: out[m, n] = T(sum_k x[m, k] w[n, k] + bias[n]), fp32 sums.
- *   x_dtype   3: rows in e4m3 (K13), x_scales theirs; 0 bf16 or 1 fp16: at most
- *             16 rows of row stride x_stride, rounded to e4m3 here (dim and
- *             x_stride multiples of 8)
+ *   x_dtype   3: rows in e4m3 (K13), x_scales theirs; 0 bf16 or 1 fp16: rows of
+ *             row stride x_stride, rounded to e4m3 here
+ *   workspace 16-byte aligned, rows * (tiles * 128 + quads * 16) bytes as K13 has
+ *             them, for rows that are rounded beforehand.  NULL where
+ *             sf_mx_linear_workspace is 0 (-1: an unsupported shape) and, for
+ *             x_dtype 0 and 1, x is 16-byte aligned and x_stride a multiple of 8
  *   codes, scales   a weight in e2m1 [out_features, dim]
  *   bias      [out_features] of out_dtype, or NULL
  *   out_dtype 0 bf16, 1 fp16; out has row stride out_stride
- * x, x_scales, codes and scales 16-byte aligned; rows <= 2^20.
+ * codes, scales and, for x_dtype 3, x and x_scales 16-byte aligned; rows <= 2^20.
  */
 int sf_mx_linear(int x_dtype, const void *x, const void *x_scales,
                  int64_t x_stride, int rows, int dim, const void *codes,
                  const void *scales, int out_features, const void *bias,
                  int out_dtype, void *out, int64_t out_stride,
-                 sf_stream_t stream);
+                 void *workspace, sf_stream_t stream);
+int64_t sf_mx_linear_workspace(int x_dtype, int rows, int dim,
+                               int out_features);
 
 /*
  * K16: K3 with the experts' weights in microscaled 4 bits, over every expert

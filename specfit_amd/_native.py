@@ -75,7 +75,8 @@ SIGNATURES = {
     "sf_mx_quantize": ([_i, _p, _i64, _i64, _i, _i, _i, _i, _p, _i64, _p, _i64, _p], _i),
     "sf_mx_values": ([_i, _p, _p, _i, _i, _i, _p, _p], _i),
     "sf_add_rms_norm": ([_i, _p, _i64, _p, _i64, _i, _i, _p, ctypes.c_double, _p, _p, _p, _p, _p], _i),
-    "sf_mx_linear": ([_i, _p, _p, _i64, _i, _i, _p, _p, _i, _p, _i, _p, _i64, _p], _i),
+    "sf_mx_linear": ([_i, _p, _p, _i64, _i, _i, _p, _p, _i, _p, _i, _p, _i64, _p, _p], _i),
+    "sf_mx_linear_workspace": ([_i, _i, _i, _i], _i64),
     "sf_mx_expert_bytes": ([_i, _i], _i64),
     "sf_mx_expert_parts": ([_i, _i, _p], _i),
     "sf_mx_routed_swiglu": ([_i, _p, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _p, _p, _i64, _p, _p, _p,

@@ -139,9 +139,17 @@ int launch_tiled(const Linear& p, hipStream_t s) {
   return SF_OK;
 }
 
-// Rows of 16-bit values are rounded by every wavefront that reads them, which
-// is cheaper than a launch of its own for one tile of rows and few wavefronts only.
+// Rows of 16-bit values are rounded by every wavefront that reads them where that
+// is cheaper than a launch of its own: one tile of rows and few wavefronts.  us on
+// the device, as they are and with the launch (4 more on the host):
+//   1 row of 2,048 by 5,120   5.4 / 6.0   16,384   9.4 / 7.5   40,000   22 / 13.5   151,936   77 / 36
+//   16 rows                   7.2 / 7.2           12.2 / 8.7            30 / 15.4            103 / 37
 constexpr int kMostRawRows = 16;
+constexpr int64_t kMostRawWeight = 1 << 25;  // values
+
+bool as_they_are(int rows, int dim, int out_features) {
+  return rows <= kMostRawRows && dim % 8 == 0 && static_cast<int64_t>(dim) * out_features <= kMostRawWeight;
+}
 
 int64_t groups(int n, int per) { return (n - 1) / per + 1; }
 
@@ -197,25 +205,43 @@ int launch_rows(const Linear& p, hipStream_t s) {
 
 }  // namespace
 
+extern "C" int64_t sf_mx_linear_workspace(int x_dtype, int rows, int dim, int out_features) {
+  if (rows < 0 || dim < 1 || out_features < 1 || dim > 1 << 24 || rows > 1 << 20 ||
+      (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows))
+    return -1;
+  if (x_dtype == kRows || as_they_are(rows, dim, out_features)) return 0;
+  return rows * (static_cast<int64_t>(tiles(dim)) * kTile + static_cast<int64_t>(quads(dim)) * 16);
+}
+
 extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, int rows,
                             int dim, const void* codes, const void* scales, int out_features,
-                            const void* bias, int out_dtype, void* out, int64_t out_stride,
+                            const void* bias, int out_dtype, void* out, int64_t out_stride, void* workspace,
                             sf_stream_t stream) {
   if (rows < 0 || dim < 1 || out_features < 1 || x_stride < 0 || out_stride < out_features ||
       (out_dtype != kBf16 && out_dtype != kFp16) ||
       (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows))
     return SF_ERR_INVALID_ARGUMENT;
   // 32-bit element and tile numbers within a row, grids within their limits.
-  if (dim > 1 << 24 || out_features > 1 << 28 || rows > 1 << 20 || (x_dtype != kRows && rows > kMostRawRows))
-    return SF_ERR_UNSUPPORTED_SHAPE;
+  if (dim > 1 << 24 || out_features > 1 << 28 || rows > 1 << 20) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0) return SF_OK;
   if (!x || !codes || !scales || !out || (x_dtype == kRows && !x_scales)) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, 2) ||
-      (bias && !aligned(bias, 2)))
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, 2) || !aligned(bias, 2) || !aligned(workspace, 16) ||
+      !aligned(x_scales, 16))
     return SF_ERR_MISALIGNED;
+  const bool fits = aligned(x, 16) && x_stride % 8 == 0;
   if (x_dtype == kRows) {
-    if (!aligned(x_scales, 16)) return SF_ERR_MISALIGNED;
-  } else if (x_stride % 8 || dim % 8) {
+    if (!aligned(x, 16)) return SF_ERR_MISALIGNED;
+  } else if (workspace && (!fits || !as_they_are(rows, dim, out_features))) {
+    uint8_t* held = static_cast<uint8_t*>(workspace);
+    uint8_t* held_scales = held + rows * (static_cast<int64_t>(tiles(dim)) * kTile);
+    if (const int rc = sf_mx_quantize(x_dtype, x, x_stride, 0, rows, dim, 1, kE4m3, held, 0, held_scales, 0, stream))
+      return rc;
+    x_dtype = kRows;
+    x = held;
+    x_scales = held_scales;
+  } else if (rows > kMostRawRows) {
+    return SF_ERR_UNSUPPORTED_SHAPE;
+  } else if (!fits || dim % 8) {
     return SF_ERR_MISALIGNED;
   }
   const Linear p = {x, static_cast<const uint8_t*>(x_scales), x_stride, rows, dim, out_features,

@@ -387,7 +387,8 @@ extern "C" int sf_mx_quantize(int dtype, const void* x, int64_t row_stride, int6
   if (dim > kMostColumns) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0 || batch == 0) return SF_OK;
   if (!x || !codes || !scales) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(x, dtype == kFp32 ? 4 : 2) || !aligned(codes, 16) || !aligned(scales, 4) || codes_batch_stride % 16 || scales_batch_stride % 4)
+  if (!aligned(x, dtype == kFp32 ? 4 : 2) || !aligned(codes, 16) || !aligned(scales, 4) ||
+      codes_batch_stride % 16 || scales_batch_stride % 4)
     return SF_ERR_MISALIGNED;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const char* xp = static_cast<const char*>(x);
@@ -395,11 +396,14 @@ extern "C" int sf_mx_quantize(int dtype, const void* x, int64_t row_stride, int6
   auto* sp = static_cast<uint8_t*>(scales);
   switch (dtype) {
     case kBf16:
-      return quantize<kBf16>(xp, row_stride, batch_stride, rows, dim, batch, held, cp, codes_batch_stride, sp, scales_batch_stride, s);
+      return quantize<kBf16>(xp, row_stride, batch_stride, rows, dim, batch, held, cp,
+                             codes_batch_stride, sp, scales_batch_stride, s);
     case kFp16:
-      return quantize<kFp16>(xp, row_stride, batch_stride, rows, dim, batch, held, cp, codes_batch_stride, sp, scales_batch_stride, s);
+      return quantize<kFp16>(xp, row_stride, batch_stride, rows, dim, batch, held, cp,
+                             codes_batch_stride, sp, scales_batch_stride, s);
     default:
-      return quantize<kFp32>(xp, row_stride, batch_stride, rows, dim, batch, held, cp, codes_batch_stride, sp, scales_batch_stride, s);
+      return quantize<kFp32>(xp, row_stride, batch_stride, rows, dim, batch, held, cp,
+                             codes_batch_stride, sp, scales_batch_stride, s);
   }
 }
 

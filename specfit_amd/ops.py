@@ -1336,12 +1336,7 @@ def greedy_tokens(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
 
 # ------------------------------------------------------- K13: microscaled --
 _MX_E4M3, _MX_E2M1, _MX_ROWS = 0, 1, 3
-_MX_RAW_ROWS = 16   # rows of 16-bit values that a product takes as they are
-# ... of a weight up to this size: every wavefront rounds the rows it reads, which costs more
-# than a launch of its own where there are many of them.  us on the device, as they are and
-# with the launch (4 more on the host): 1 row of 2,048 x 5,120 outputs 5.4 / 6.0, x 16,384
-# 9.4 / 7.5, x 40,000 22 / 13.5, x 151,936 77 / 36; 16 rows 7.2 / 7.2, 12 / 8.7, 30 / 15, 103 / 37.
-_MX_RAW_WEIGHT = 1 << 25
+_MX_RAW_ROWS = 16   # rows of 16-bit values that the experts take as they are
 
 
 def _new(shape, dtype: torch.dtype, device: torch.device,
@@ -1506,6 +1501,14 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
 
 
 # ----------------------------------------------------------------- K15 ----
+@functools.lru_cache(maxsize=1024)
+def _mx_linear_workspace(kind: int, rows: int, dim: int, out_features: int) -> int:
+    n = _native.lib().sf_mx_linear_workspace(kind, rows, dim, out_features)
+    if n < 0:
+        raise ValueError("a product takes at most 2^20 rows of 2^24 columns")
+    return n
+
+
 def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | None = None, *,
               stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """x weight^T + bias with the weight in microscaled 4 bits (K15).
@@ -1540,21 +1543,23 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
     out = torch.empty((*shape[:-1], weight.rows), dtype=dtype, device=device)
     if out.numel() == 0:
         return out
-    kind, x_ptr, scale_ptr, stride = _MX_ROWS, 0, None, 0
-    if not held:
-        flat = _as_rows("x", x, stream)
-        if flat.shape[0] <= _MX_RAW_ROWS and weight.rows * weight.dim <= _MX_RAW_WEIGHT \
-                and weight.dim % 8 == 0 and flat.stride(0) % 8 == 0 and flat.data_ptr() % 16 == 0:
-            kind, x_ptr, stride = _DTYPES[dtype], flat.data_ptr(), flat.stride(0)
+    workspace = None
+    if held:
+        kind, rows, stride, (x_ptr, scale_ptr) = _MX_ROWS, x.rows, 0, x._pointers()
+    else:
+        x = _as_rows("x", x, stream)
+        kind, rows, stride = _DTYPES[dtype], x.shape[0], x.stride(0)
+        x_ptr, scale_ptr = x.data_ptr(), None
+        if stride % 8 or x_ptr % 16:
+            nbytes = rows * sum(mx.row_bytes(weight.dim))
         else:
-            x = _mx_rows(shape, flat.shape[0], dtype, device, stream)
-            _mx_quantize_into(flat, x, stream)
-    if kind == _MX_ROWS:
-        x_ptr, scale_ptr = x._pointers()
-    rc = _launch(_native.lib().sf_mx_linear, index, kind, x_ptr, scale_ptr, stride,
-                 out.numel() // weight.rows, weight.dim, weight.codes.data_ptr(),
-                 weight.scales.data_ptr(), weight.rows, _ptr(bias), _DTYPES[dtype], out.data_ptr(),
-                 weight.rows, _stream_handle(stream, device))
+            nbytes = _mx_linear_workspace(kind, rows, weight.dim, weight.rows)
+        if nbytes:
+            workspace = _new(nbytes, torch.uint8, device, stream)
+    rc = _launch(_native.lib().sf_mx_linear, index, kind, x_ptr, scale_ptr, stride, rows, weight.dim,
+                 weight.codes.data_ptr(), weight.scales.data_ptr(), weight.rows, _ptr(bias),
+                 _DTYPES[dtype], out.data_ptr(), weight.rows, _ptr(workspace),
+                 _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_mx_linear")
     return out

@@ -187,7 +187,8 @@ def test_the_library_refuses_before_any_launch():
     assert n(0, p, 8, p, 8, 2, 8, p, 1e-6, None, None, None, None, None) == INVALID  # no output
     assert n(0, p, 8, p, 8, 2, 8, p, 1e-6, None, None, p, None, None) == INVALID     # codes without scales
     assert n(2, p + 2, 8, p, 8, 2, 8, p, 1e-6, p, p, p, p, None) == misaligned
-    lin = lib.sf_mx_linear
+    def lin(*args):                     # without a workspace
+        return lib.sf_mx_linear(*args[:-1], None, args[-1])
     assert lin(3, p, p, 0, 0, 64, p, p, 32, None, 0, p, 32, None) == 0
     assert lin(2, p, p, 64, 2, 64, p, p, 32, None, 0, p, 32, None) == INVALID
     assert lin(3, p, None, 0, 2, 64, p, p, 32, None, 0, p, 32, None) == INVALID
@@ -198,6 +199,11 @@ def test_the_library_refuses_before_any_launch():
     assert lin(0, p, None, 64, 2, 60, p, p, 32, None, 0, p, 32, None) == misaligned
     assert lin(3, p + 8, p, 0, 2, 64, p, p, 32, None, 0, p, 32, None) == misaligned
     assert lin(3, p, p, 0, 2, 64, p, p, 32, p + 1, 0, p, 32, None) == misaligned
+    assert lib.sf_mx_linear(0, p, None, 64, 17, 64, p, p, 32, None, 0, p, 32, p + 8, None) == misaligned
+    size = lib.sf_mx_linear_workspace
+    assert size(3, 100, 64, 32) == size(0, 16, 64, 32) == size(1, 1, 2048, 16384) == 0
+    assert size(0, 17, 100, 32) == 17 * sum(mx.row_bytes(100)) and size(1, 1, 2048, 16385) == sum(mx.row_bytes(2048))
+    assert size(0, 1, 100, 32) == sum(mx.row_bytes(100)) and size(2, 1, 64, 32) == size(0, 1, 0, 32) == -1
     big = lib.sf_mx_expert_bytes(64, 32)
     g = lib.sf_mx_grouped_swiglu
     assert g(3, p, p, 0, p, p, None, 0, 2, 64, 32, 4, None, p, big, p, p, p, None) == 0
