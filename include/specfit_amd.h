@@ -608,7 +608,7 @@ int sf_logit_rules(int dtype, const void *logits, int64_t logits_stride,
  *           32): 16 bytes of block b and row r of row tile and tile, the first of
  *           two values in the low half; scales [R][quads][4][16][4], the
  *           byte of tile t in t % 4; rows behind the last are zeros
- * Bytes of the last quad's missing tiles are neither written nor read.
+ * Bytes of the last quad's missing tiles count for nothing.
  *   dtype       0 bf16, 1 fp16, 2 fp32
  *   x           [rows, dim], row stride row_stride; batch of them (held 1 only)
  *               at batch_stride elements, the outputs at codes_batch_stride and
@@ -667,7 +667,8 @@ int64_t sf_mx_linear_workspace(int x_dtype, int rows, int dim,
  * e < num_experts that has rows and, with a table, slot_of_expert[e] >= 0.
  *   a       = e4m3(silu(x[t] . gate^T) * (x[t] . up^T))        fp32 up to a
  *   rows[r] = bf16((a . down^T) * route_weights[perm_pos[r]])
- *   x_dtype         as sf_mx_linear (0: at most 16 tokens)
+ *   x_dtype         3: rows in e4m3; 0: at most 16 rows in bf16, hidden_size and
+ *                   x_stride multiples of 8
  *   slots           records of sf_mx_expert_bytes at slot_stride bytes: the codes
  *                   of gate [I, H], up [I, H], down [H, I] and then their
  *                   scales (held 1), at the byte offsets that

@@ -18,7 +18,7 @@
 //            the pieces of two row tiles are that of the 32x32x64 form.
 //            Scales [row tiles][quads][64 lanes][4], the byte of tile t in
 //            t % 4.  Row tiles come in pairs, rows behind the last are zeros.
-// Bytes of tiles that a row does not have (the last quad's) are never read.
+// Bytes of tiles that a row does not have (the last quad's) count for nothing.
 #pragma once
 
 #include "sf_common.h"
@@ -79,6 +79,7 @@ __device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b) {
 
 // Pieces of 16 bytes that start at any element: one load or store all the same.
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+typedef u32x2 __attribute__((aligned(2))) u32x2_any;
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 
 // 8 neighbours at p as fp32.

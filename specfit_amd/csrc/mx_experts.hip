@@ -205,6 +205,18 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p,
                                chunk.begin + c < chunk.end, part);
 }
 
+// Eight columns from h on, two to a word.
+__device__ __forceinline__ void store_row8(const Experts& p, int row, int h, u32x4 w) {
+  uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
+  if (h + 8 <= p.hidden) {
+    *reinterpret_cast<u32x4_any*>(o) = w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (h + i < p.hidden) o[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+}
+
 __device__ __forceinline__ void store_row4(const Experts& p, int row, int h, f32x4 v) {
   uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
   if (p.hidden % 4 == 0) {
@@ -281,12 +293,16 @@ __device__ __forceinline__ void gate_up_tile(const Experts& p, const Chunk& chun
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
       const uint32_t byte = scale_byte<kE4m3>(top);
       const float s = byte == 255 ? 0.f : inverse_scale(byte);
-      if (row < chunk.end && block < tiles(p.inner) * 4) {
-        uint8_t* o = act_row(p, row) + block * kBlock + 4 * g;
+      uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint32_t*>(o + 8 * i) =
-              byte == 255 ? 0u : e4m3x4(a[4 * i] * s, a[4 * i + 1] * s, a[4 * i + 2] * s, a[4 * i + 3] * s);
+      for (int i = 0; i < 4; ++i)
+        w[i] = byte == 255 ? 0u : e4m3x4(a[4 * i] * s, a[4 * i + 1] * s, a[4 * i + 2] * s, a[4 * i + 3] * s);
+      join(w[0], w[1]);
+      join(w[2], w[3]);
+      if (row < chunk.end && block < tiles(p.inner) * 4) {
+        uint8_t* o = act_row(p, row) + block * kBlock + 8 * g;
+        *reinterpret_cast<u32x2*>(o) = u32x2{w[0], w[1]};
+        *reinterpret_cast<u32x2*>(o + 16) = u32x2{w[2], w[3]};
         if (g == 0) *act_scale(p, row, block) = static_cast<uint8_t>(byte);
       }
     }
@@ -306,14 +322,20 @@ __device__ __forceinline__ void down_tile(const Experts& p, const Chunk& chunk, 
 #pragma unroll
   for (int m = 0; m < T::FM; ++m) {
     const int row = chunk.begin + (wm * T::FM + m) * 32 + (lane & 31);
-    if (row >= chunk.end) continue;
-    const float route = route_weight(p, row);
+    const bool live = row < chunk.end;
+    const float route = live ? route_weight(p, row) : 0.f;
 #pragma unroll
     for (int n = 0; n < T::FN; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        store_row4(p, row, tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 4 * (lane >> 5),
-                   f32x4{acc[n][m][4 * i], acc[n][m][4 * i + 1], acc[n][m][4 * i + 2], acc[n][m][4 * i + 3]} * route);
+      for (int i = 0; i < 4; i += 2) {
+        const f32x16 v = acc[n][m] * route;
+        uint32_t w[4] = {narrow2<kBf16>(v[4 * i], v[4 * i + 1]), narrow2<kBf16>(v[4 * i + 2], v[4 * i + 3]),
+                         narrow2<kBf16>(v[4 * i + 4], v[4 * i + 5]), narrow2<kBf16>(v[4 * i + 6], v[4 * i + 7])};
+        join(w[0], w[2]);
+        join(w[1], w[3]);
+        const int h = tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 8 * (lane >> 5);
+        if (live) store_row8(p, row, h, u32x4{w[0], w[1], w[2], w[3]});
+      }
   }
 }
 

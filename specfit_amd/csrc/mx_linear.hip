@@ -26,26 +26,35 @@ struct Linear {
   int out_dtype;
   char* out;
   int64_t out_stride;
-  bool wide;  // 4 outputs at a time fit the output's alignment
 };
 
-__device__ __forceinline__ void store4(const Linear& p, int row, int n, f32x4 v) {
-  if (row >= p.rows || n >= p.out_features) return;
-  const int left = min(4, p.out_features - n);
+// Four outputs from column n on, with the bias, in the output's type.
+__device__ __forceinline__ u32x2 rounded4(const Linear& p, int n, f32x4 v) {
   if (p.bias) {
-    for (int i = 0; i < left; ++i)
+    for (int i = 0; i < min(4, p.out_features - n); ++i)
       v[i] += p.out_dtype == kFp16 ? element<kFp16>(static_cast<const char*>(p.bias) + 2 * (n + i))
                                    : element<kBf16>(static_cast<const char*>(p.bias) + 2 * (n + i));
   }
+  return p.out_dtype == kFp16 ? u32x2{narrow2<kFp16>(v[0], v[1]), narrow2<kFp16>(v[2], v[3])}
+                              : u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
+}
+
+// N outputs of 16 bits, two to a word; past the last column nothing.
+template <int N, class Words, class Any>
+__device__ __forceinline__ void store(const Linear& p, int row, int n, Words w) {
+  if (row >= p.rows || n >= p.out_features) return;
   char* o = p.out + (row * p.out_stride + n) * 2;
-  const u32x2 w = p.out_dtype == kFp16 ? u32x2{narrow2<kFp16>(v[0], v[1]), narrow2<kFp16>(v[2], v[3])}
-                                       : u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
-  if (p.wide && left == 4) {
-    *reinterpret_cast<u32x2*>(o) = w;
+  if (n + N <= p.out_features) {
+    *reinterpret_cast<Any*>(o) = w;
     return;
   }
-  for (int i = 0; i < left; ++i)
-    reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (n + i < p.out_features) reinterpret_cast<uint16_t*>(o)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+}
+
+__device__ __forceinline__ void store4(const Linear& p, int row, int n, f32x4 v) {
+  store<4, u32x2, u32x2_any>(p, row, n, rounded4(p, n, v));
 }
 
 // Few rows: a wavefront takes NT row tiles of the weight and one of KS parts of
@@ -124,9 +133,16 @@ __global__ __launch_bounds__(T::kThreads, 2) void linear_tiled_kernel(Linear p, 
 #pragma unroll
     for (int n = 0; n < T::FN; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        store4(p, row, tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 4 * (lane >> 5),
-               f32x4{acc[n][m][4 * i], acc[n][m][4 * i + 1], acc[n][m][4 * i + 2], acc[n][m][4 * i + 3]});
+      for (int i = 0; i < 4; i += 2) {
+        const int n0 = tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i, g = lane >> 5;
+        const f32x16& v = acc[n][m];
+        u32x2 a = rounded4(p, n0 + 4 * g, f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]});
+        u32x2 b = rounded4(p, n0 + 8 + 4 * g, f32x4{v[4 * i + 4], v[4 * i + 5], v[4 * i + 6], v[4 * i + 7]});
+        uint32_t w[4] = {a[0], a[1], b[0], b[1]};
+        join(w[0], w[2]);
+        join(w[1], w[3]);
+        store<8, u32x4, u32x4_any>(p, row, n0 + 8 * g, u32x4{w[0], w[1], w[2], w[3]});
+      }
   }
 }
 
@@ -246,8 +262,7 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
   }
   const Linear p = {x, static_cast<const uint8_t*>(x_scales), x_stride, rows, dim, out_features,
                     static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), bias,
-                    out_dtype, static_cast<char*>(out), out_stride,
-                    aligned(out, 8) && out_stride % 4 == 0};
+                    out_dtype, static_cast<char*>(out), out_stride};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (x_dtype == kBf16) return launch_few<kBf16>(p, s);
   if (x_dtype == kFp16) return launch_few<kFp16>(p, s);

@@ -395,4 +395,13 @@ __device__ __forceinline__ void multiply(f32x16 (&acc)[T::FN][T::FM], const uint
   __builtin_amdgcn_s_waitcnt(loads_left(0));  // nothing on its way into LDS that is given back
 }
 
+// The 32 x 32 form leaves a lane four neighbours in every eight columns, the other
+// four in lane + 32.  Of two such pieces (in turn) lanes 0 to 31 get the first eight
+// columns' whole, lanes 32 to 63 the second's.
+__device__ __forceinline__ void join(uint32_t& first, uint32_t& second) {
+  const u32x2 both = __builtin_amdgcn_permlane32_swap(first, second, false, false);
+  first = both[0];
+  second = both[1];
+}
+
 }  // namespace sf_mx
