@@ -11,8 +11,8 @@
 //
 // 128 experts of 2,048 x 768, 8 to a token, one MI355X; gate and up, then down:
 //   1 token (no dispatch)        7.6 + 5.6 us   latency of two dependent launches
-//   61 tokens, favourites         36 + 20 us    4.2 and 3.7 TB/s of weights
-//   2,048 tokens                  74 + 59 us    1.4 and 0.9 PFLOP/s, the weights' 214
+//   61 tokens, favourites         36 + 21 us    4.2 and 3.7 TB/s of weights
+//   2,048 tokens                  74 + 54 us    1.4 and 1.0 PFLOP/s, the weights' 214
 //                                               and 107 MB arriving meanwhile
 #include <cmath>
 

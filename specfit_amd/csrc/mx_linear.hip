@@ -7,8 +7,9 @@
 // One MI355X (a large copy moves 5.0 TB/s, an 8,192^3 library product in e4m3 runs
 // at 2,650 TFLOP/s):
 //   1 x 2,048 x 5,120            5.5 us   latency: eight wavefronts cut the sum
-//   61 x 2,048 x 151,936        41 us   the weight's 165 MB at 4.5 TB/s with the output
-//   4,096 x 4,096 x 9,216      133 us   2,330 TFLOP/s, the chip's power: zeros take 115
+//   61 x 2,048 x 151,936        40 us   184 MB, the output among them, at 4.6 TB/s
+//   4,096 x 4,096 x 9,216      126 us   2,450 TFLOP/s, near the chip's power
+//   8,192^3                    415 us   2,650 TFLOP/s, the library product's rate
 #include "mx_product.h"
 
 namespace {
