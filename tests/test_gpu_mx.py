@@ -142,9 +142,9 @@ def test_add_rms_norm(rows, dim, residual, dtype):
     w = (1 + 0.3 * _normal(9, dim)).to(dtype)
     total, y, q = ops.add_rms_norm(x, res, w, 1e-6, quantized=True)
     s, want = _norm_reference(x, res, w, 1e-6)
-    # fp32 adds two 16-bit values exactly enough: they round alike but where
-    # the sum in 64 bits has a longer tail than fp32 holds.
-    assert torch.equal(total, s if dtype == torch.float32 and residual is False else total)
+    # The sum in fp32, rounded to the type: half a step, and half a fp32 step where
+    # it has a longer tail than fp32 holds.
+    assert residual or total is x
     assert (total.double() - (x.double() + (0 if res is None else res.double()))).abs().le(
         ref.half_step(s.double(), dtype) * 1.001).all()
     s, want = _norm_reference(total, None, w, 1e-6)
@@ -344,6 +344,19 @@ def test_far_rows_and_outputs():
     out = ops.mx_linear(q, weight)                  # 2.3e9 outputs
     # Whatever the tile, the same products are added in the same order.
     assert torch.equal(out[-600:], ops.mx_linear(x[-600:], weight))
+
+
+def test_as_many_rows_as_a_product_takes():
+    x = _normal(0, 1 << 20, 32).to(torch.bfloat16)
+    w = ops.mx_quantize_weight(_normal(1, 24, 32))
+    out = ops.mx_linear(x, w)
+    assert torch.equal(out, ops.mx_linear(ops.mx_quantize(x), w))
+    for part in (slice(0, 20000), slice(-20000, None)):
+        assert torch.equal(out[part], ops.mx_linear(x[part], w))
+    more = torch.cat([x, x[:1]])
+    for rows in (more, ops.mx_quantize(more)):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.mx_linear(rows, w)
 
 
 def test_captured_chains_replay_each_their_own():

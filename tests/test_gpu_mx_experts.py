@@ -56,7 +56,7 @@ def test_a_favourite_takes_every_token(tokens):
 
 def test_the_same_expert_twice_and_experts_that_are_not_there():
     h, packed, index, weights = _case(30, 96, 64, 5, 4, distinct=False)
-    index[3, 1], index[7] = 99, -1
+    index[3, 1], index[7], index[9, 2], index[11, 0] = 99, -1, 2 ** 40, 2 ** 32 + 1
     module = Qwen3MXExperts.from_packed(packed, hidden_size=96, intermediate_size=64)
     got = module(h, index, weights)
     _check(got, h, index, weights, packed, 96, 64)
@@ -232,6 +232,19 @@ def test_one_call_takes_any_rows(tokens):
     got = ops.mx_experts(columns, index, weights, records, H, I, stream=side)
     side.synchronize()
     assert torch.equal(got, ops.mx_experts(ops.mx_quantize(h), index, weights, records, H, I))
+
+
+def test_far_rows():
+    """Offsets of rows past 32 bits: the last tokens' outputs are what they are by
+    themselves (as many routes to an expert as make the same tiles)."""
+    H, I, E, K, T = 2048, 32, 8, 8, 140_000
+    h, packed, index, weights = _case(400, H, I, E, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    want = ops.mx_experts(h, index, weights, records, H, I)
+    many = torch.zeros((T, H), dtype=torch.bfloat16, device=DEV)
+    many[-400:] = h
+    many_index, many_weights = index.repeat(T // 400, 1), weights.repeat(T // 400, 1)
+    assert torch.equal(ops.mx_experts(many, many_index, many_weights, records, H, I)[-400:], want)
 
 
 def test_two_calls_at_once():
