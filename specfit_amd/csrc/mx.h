@@ -182,6 +182,30 @@ __device__ __forceinline__ void store_rows_chunk(const float (&f)[8], int c, uin
   }
 }
 
+// Rows to e4m3, chunk `at` of all rows'.  A lane takes 8 neighbours, so a block is
+// four lanes of one DPP quad, and loads and stores of a wavefront lie in a piece.
+template <int DT>
+__device__ __forceinline__ void quantize_rows_chunk(int64_t at, const char* __restrict__ x, int64_t row_stride,
+                                                    int dim, int chunks, int64_t total, uint8_t* __restrict__ codes,
+                                                    uint8_t* __restrict__ scales) {
+  if (at >= total) return;  // a row's chunks are a multiple of 16: quads end together
+  const int64_t row = total <= 0x7fffffff
+                          ? static_cast<int64_t>(static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks))
+                          : at / chunks;
+  const int c = static_cast<int>(at - row * chunks);
+  const char* p = x + (row * row_stride + 8 * c) * size_of<DT>();
+  float f[8] = {};
+  if (8 * c + 8 <= dim) {
+    load8<DT>(p, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (8 * c + i < dim) f[i] = element<DT>(p + i * size_of<DT>());
+  }
+  store_rows_chunk(f, c, codes + row * chunks * 8,
+                   scales + row * (static_cast<int64_t>((chunks + 63) / 64) * 16));
+}
+
 // A grid's work-items are counted in 32 bits.
 inline bool grid_fits(int64_t groups, int threads) { return groups <= 0xffffffffll / threads; }
 

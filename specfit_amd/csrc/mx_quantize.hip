@@ -21,31 +21,15 @@ using namespace sf_mx;
 constexpr int kThreads = 256;
 
 // ------------------------------------------------------------------ K13 ----
-// Rows to e4m3.  A lane takes 8 neighbours, so a block is four lanes of one
-// DPP quad, and loads and stores of a wavefront lie in a piece.
+// Rows to e4m3.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const char* __restrict__ x,
                                                                  int64_t row_stride, int dim,
                                                                  int chunks, int64_t total,
                                                                  uint8_t* __restrict__ codes,
                                                                  uint8_t* __restrict__ scales) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (at >= total) return;  // a row's chunks are a multiple of 16: quads end together
-  const int64_t row = total <= 0x7fffffff
-                          ? static_cast<int64_t>(static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks))
-                          : at / chunks;
-  const int c = static_cast<int>(at - row * chunks);
-  const char* p = x + (row * row_stride + 8 * c) * size_of<DT>();
-  float f[8] = {};
-  if (8 * c + 8 <= dim) {
-    load8<DT>(p, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (8 * c + i < dim) f[i] = element<DT>(p + i * size_of<DT>());
-  }
-  store_rows_chunk(f, c, codes + row * chunks * 8,
-                   scales + row * (static_cast<int64_t>((chunks + 63) / 64) * 16));
+  quantize_rows_chunk<DT>(static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, x, row_stride, dim, chunks, total,
+                          codes, scales);
 }
 
 // A weight to e2m1 tiles: a wavefront takes 16 rows by 512 columns, a lane one
