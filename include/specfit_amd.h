@@ -709,8 +709,10 @@ int sf_mx_routed_swiglu(int x_dtype, const void *x, const void *x_scales,
 
 /*
  * A layer's routed experts in one call: sf_mx_routed_swiglu, or sf_dispatch
- * (with the rows' rounding in the same launch), sf_mx_grouped_swiglu and
- * sf_combine (fp32 sums of the routes' bf16 rows), expert e in slot e.
+ * (with the rows' rounding in the same launch), sf_mx_grouped_swiglu's products
+ * and the sum over a token's routes, in their order, in fp32.  The routes' rows
+ * are kept in fp16 with a power of two for each 32 columns, and the output is
+ * rounded once.  Expert e is in slot e.
  *   x_dtype     0 bf16 rows of row stride x_stride, any number and alignment of
  *               them; 3 rows in e4m3 as above
  *   workspace   sf_mx_experts_workspace bytes (-1: an unsupported shape),

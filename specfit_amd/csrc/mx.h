@@ -106,6 +106,10 @@ __device__ __forceinline__ uint32_t narrow(float f) {
 
 template <int DT>
 __device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if (DT == kFp16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+  }
   return narrow<DT>(a) | (narrow<DT>(b) << 16);
 }
 

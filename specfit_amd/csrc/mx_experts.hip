@@ -5,15 +5,18 @@
 //   rows[r] = bf16((a . down^T) * route_weight)
 // with fp32 sums and one rounding between them: the activation is what the
 // second product reads, so it is rounded once, from fp32, to that product's
-// type.  A route's row is rounded to bf16 for the combine, which halves what the
-// two exchange (8 routes of a token: 0.0024 of the outputs' norm against 64 bits,
-// 0.0016 without); the form without a dispatch adds in fp32 and rounds once.
+// type.  The rows are bf16 as K3's are, for K4.  A layer's experts in one call keep
+// them in 16 bits of their own kind, with three bits more, and round to bf16 once,
+// behind the sum over a token's routes (0.0017 to 0.0019 of the outputs' norm
+// against 64 bits; 0.0024 to 0.0026 with bf16 rows); without a dispatch that sum
+// is in fp32 throughout.
 //
 // 128 experts of 2,048 x 768, 8 to a token, one MI355X; gate and up, then down:
 //   1 token (no dispatch)        7.6 + 5.6 us   latency of two dependent launches
-//   61 tokens, favourites         36 + 21 us    4.2 and 3.7 TB/s of weights
-//   2,048 tokens                  74 + 54 us    1.4 and 1.0 PFLOP/s, the weights' 214
+//   61 tokens, favourites         35 + 21 us    4.2 and 3.7 TB/s of weights
+//   2,048 tokens                  75 + 55 us    1.4 and 0.9 PFLOP/s, the weights' 214
 //                                               and 107 MB arriving meanwhile
+// and the sum over the routes 4.6 and 13.4 us (69 MB at 5.7 TB/s).
 #include <cmath>
 
 #include "dispatch.h"
@@ -54,7 +57,8 @@ struct Experts {
   Record record;
   uint8_t* act;         // e4m3 rows [tokens * top_k, inner]
   uint8_t* act_scales;
-  uint16_t* rows;       // bf16 [tokens * top_k, hidden]
+  uint16_t* rows;       // [tokens * top_k, hidden], bf16 or held in blocks (below)
+  uint8_t* row_scales;  // of rows held in blocks: [tokens * top_k, ceil(hidden / 32)]
 };
 
 // The rows of one workgroup: up to PER of one expert's.  The chunks of more than
@@ -206,57 +210,118 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p,
                                chunk.begin + c < chunk.end, part);
 }
 
-// Eight columns from h on, two to a word.
-__device__ __forceinline__ void store_row8(const Experts& p, int row, int h, u32x4 w) {
-  uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
-  if (h + 8 <= p.hidden) {
-    *reinterpret_cast<u32x4_any*>(o) = w;
+// A route's row on its way to the sum over a token's routes: bf16 for callers, and
+// for this file's own sum fp16 in blocks of 32 columns with a power of two, E - 141
+// its exponent: as many bytes, and three bits more.  E is the biased exponent of
+// the block's largest finite value, at least 15, so that that value becomes 2^14 to
+// 2^15, nothing is lost down to 2^-28 of it, and both factors are normal.
+// Infinities and NaN stay what they are.  2,048 tokens: down 53 us with bf16 rows,
+// 55 so (60 with E by the lanes' exchange through LDS and byte stores).
+constexpr int kHeldRows = 4;
+
+__device__ __forceinline__ uint32_t row_exponent(uint32_t top) { return max(top >> 23, 15u); }
+__device__ __forceinline__ float to_row(uint32_t e) { return __uint_as_float((268u - e) << 23); }
+__device__ __forceinline__ float from_row(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
+
+// The larger of this lane's and the lane's that differs in bit 4 or 5 of its number.
+__device__ __forceinline__ float max16(float x) {
+  const u32x2 both = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float max32(float x) {
+  const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
+// The largest magnitude of N values; NaN are passed over, with FINITE infinities too.
+template <int N, bool FINITE, class Values>
+__device__ __forceinline__ float largest(const Values& v) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    top = fmaxf(top, FINITE && magnitude(v[i]) >= 0x7f800000u ? 0.f : fabsf(v[i]));
+  return top;
+}
+
+__device__ __forceinline__ uint8_t* row_scale(const Experts& p, int row, int h) {
+  return p.row_scales + row * static_cast<int64_t>((p.hidden + kBlock - 1) / kBlock) + h / kBlock;
+}
+
+// The bytes of N blocks from column h on.
+typedef uint32_t __attribute__((aligned(1))) u32_any;
+typedef uint16_t __attribute__((aligned(1))) u16_any;
+
+template <int N>
+__device__ __forceinline__ void store_scales(const Experts& p, int row, int h, uint32_t bytes) {
+  static_assert(N == 4 || N == 2, "a word or half of one");
+  uint8_t* o = row_scale(p, row, h);
+  if (h + 32 * (N - 1) < p.hidden) {
+    if (N == 4)
+      *reinterpret_cast<u32_any*>(o) = bytes;
+    else
+      *reinterpret_cast<u16_any*>(o) = static_cast<uint16_t>(bytes);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (h + i < p.hidden) o[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+  for (int i = 0; i < N; ++i)
+    if (h + 32 * i < p.hidden) o[i] = static_cast<uint8_t>(bytes >> (8 * i));
 }
 
-__device__ __forceinline__ void store_row4(const Experts& p, int row, int h, f32x4 v) {
+// Columns from h on, two to a word.
+template <int N, class Words, class Any>
+__device__ __forceinline__ void store_row(const Experts& p, int row, int h, Words w) {
   uint16_t* o = p.rows + static_cast<int64_t>(row) * p.hidden + h;
-  if (p.hidden % 4 == 0) {
-    if (h < p.hidden)
-      *reinterpret_cast<u32x2*>(o) = u32x2{narrow2<kBf16>(v[0], v[1]), narrow2<kBf16>(v[2], v[3])};
-  } else {
-    for (int i = 0; i < 4; ++i)
-      if (h + i < p.hidden) o[i] = sf_f32_to_bf16(v[i]);
+  if (h + N <= p.hidden) {
+    *reinterpret_cast<Any*>(o) = w;
+    return;
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (h + i < p.hidden) o[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
 }
 
 __device__ __forceinline__ float route_weight(const Experts& p, int row) {
   return p.route_weights ? sf_bf16_to_f32(p.route_weights[p.perm_pos[row]]) : 1.0f;
 }
 
-// A wavefront: NT row tiles of down for 16 rows, over the whole inner size.
-template <int WAVES, int NT>
+// A wavefront: 32 columns of down for 16 rows, over the whole inner size.
+template <int WAVES, int HELD>
 __global__ __launch_bounds__(WAVES * SF_WAVE) void down_few_kernel(Experts p, int blocks) {
-  constexpr int kAhead = NT == 1 ? 4 : NT == 2 ? 3 : 2;
   const Chunk chunk = chunk_of<16, 0>(p, blockIdx.x / blocks);
   if (!chunk.weights) return;
   const int lane = threadIdx.x & (SF_WAVE - 1), wave = threadIdx.x / SF_WAVE;
   const int g = lane >> 4, c = lane & 15;
-  const int group = blockIdx.x % blocks * WAVES + wave, last = row_tiles(p.hidden) - 1;
-  if (group * NT > last) return;
-  WeightSource w[NT];
+  const int pair = blockIdx.x % blocks * WAVES + wave;  // of row tiles, which come in pairs
+  if (2 * pair >= row_tiles(p.hidden)) return;
+  WeightSource w[2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-    w[n].set(chunk.weights + p.record.down_codes, chunk.weights + p.record.down_scales, min(group * NT + n, last),
-             p.inner, lane);
+  for (int n = 0; n < 2; ++n)
+    w[n].set(chunk.weights + p.record.down_codes, chunk.weights + p.record.down_scales, 2 * pair + n, p.inner, lane);
   const int row = min(chunk.begin + c, chunk.end - 1);
   RowSource<kRows> x[1];
   x[0].set(p.act, p.act_scales, row, 0, p.inner, g);
   const float route = route_weight(p, row);
-  f32x4 acc[NT][1] = {};
-  accumulate<1, NT, kRows, kAhead>(acc, w, x, 0, tiles(p.inner), p.inner, g);
+  f32x4 acc[2][1] = {};
+  accumulate<1, 2, kRows, 3>(acc, w, x, 0, tiles(p.inner), p.inner, g);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) acc[n][0] *= route;
+  uint32_t e = 0;
+  if (HELD == kHeldRows) {
+    const float v[8] = {acc[0][0][0], acc[0][0][1], acc[0][0][2], acc[0][0][3],
+                        acc[1][0][0], acc[1][0][1], acc[1][0][2], acc[1][0][3]};
+    float top = max32(max16(largest<8, false>(v)));
+    if (__any(magnitude(top) == 0x7f800000u)) top = max32(max16(largest<8, true>(v)));
+    e = row_exponent(__float_as_uint(top));
+  }
   if (chunk.begin + c >= chunk.end) return;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) store_row4(p, row, (group * NT + n) * 16 + 4 * g, acc[n][0] * route);
+  for (int n = 0; n < 2; ++n) {
+    const f32x4 v = HELD == kHeldRows ? acc[n][0] * to_row(e) : acc[n][0];
+    constexpr int DT = HELD == kHeldRows ? kFp16 : kBf16;
+    store_row<4, u32x2, u32x2_any>(p, row, 32 * pair + 16 * n + 4 * g,
+                                   u32x2{narrow2<DT>(v[0], v[1]), narrow2<DT>(v[2], v[3])});
+  }
+  if (HELD == kHeldRows && g == 0) *row_scale(p, row, 32 * pair) = static_cast<uint8_t>(e);
 }
 
 // Many rows by tiles.  Half of a wavefront's weight rows are gate's, the other
@@ -310,7 +375,7 @@ __device__ __forceinline__ void gate_up_tile(const Experts& p, const Chunk& chun
   }
 }
 
-template <class T>
+template <int HELD, class T>
 __device__ __forceinline__ void down_tile(const Experts& p, const Chunk& chunk, int tile0, typename T::Stage& stage0,
                                           typename T::Stage& stage1, typename T::Scales (&scales)[2]) {
   const int last = row_tiles(p.hidden) - 1;
@@ -325,18 +390,43 @@ __device__ __forceinline__ void down_tile(const Experts& p, const Chunk& chunk, 
     const int row = chunk.begin + (wm * T::FM + m) * 32 + (lane & 31);
     const bool live = row < chunk.end;
     const float route = live ? route_weight(p, row) : 0.f;
+    const int first = tile0 * 16 + wn * T::FN * 32;
+    float top[T::FN];
+    uint32_t scales_word = 0;
+    if (HELD == kHeldRows) {
+      bool infinite = false;
 #pragma unroll
-    for (int n = 0; n < T::FN; ++n)
+      for (int n = 0; n < T::FN; ++n) {
+        top[n] = max32(largest<16, false>(acc[n][m])) * fabsf(route);  // products round monotonically
+        infinite |= !(top[n] < __builtin_inff());
+      }
+      if (__any(infinite)) {
+#pragma unroll
+        for (int n = 0; n < T::FN; ++n) top[n] = max32(largest<16, true>(acc[n][m] * route));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < T::FN; ++n) {
+      const int h0 = first + n * 32;
+      float factor = route;
+      if (HELD == kHeldRows) {
+        const uint32_t e = row_exponent(__float_as_uint(top[n]));
+        factor *= to_row(e);
+        scales_word |= e << (8 * n);
+      }
+      const f32x16 v = acc[n][m] * factor;
+      constexpr int DT = HELD == kHeldRows ? kFp16 : kBf16;
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const f32x16 v = acc[n][m] * route;
-        uint32_t w[4] = {narrow2<kBf16>(v[4 * i], v[4 * i + 1]), narrow2<kBf16>(v[4 * i + 2], v[4 * i + 3]),
-                         narrow2<kBf16>(v[4 * i + 4], v[4 * i + 5]), narrow2<kBf16>(v[4 * i + 6], v[4 * i + 7])};
+        uint32_t w[4] = {narrow2<DT>(v[4 * i], v[4 * i + 1]), narrow2<DT>(v[4 * i + 2], v[4 * i + 3]),
+                         narrow2<DT>(v[4 * i + 4], v[4 * i + 5]), narrow2<DT>(v[4 * i + 6], v[4 * i + 7])};
         join(w[0], w[2]);
         join(w[1], w[3]);
-        const int h = tile0 * 16 + (wn * T::FN + n) * 32 + 8 * i + 8 * (lane >> 5);
-        if (live) store_row8(p, row, h, u32x4{w[0], w[1], w[2], w[3]});
+        if (live)
+          store_row<8, u32x4, u32x4_any>(p, row, h0 + 8 * i + 8 * (lane >> 5), u32x4{w[0], w[1], w[2], w[3]});
       }
+    }
+    if (HELD == kHeldRows && live && lane < 32) store_scales<T::FN>(p, row, first, scales_word);
   }
 }
 
@@ -348,22 +438,24 @@ struct First {
   using type = T;
 };
 
-template <bool GATE_UP, class T, class... Lower>
+constexpr int kGateUp = -1;  // a product: gate and up, or down with rows of this type
+
+template <int PART, class T, class... Lower>
 __device__ __forceinline__ void fitting_tile(const Experts& p, const Chunk& chunk, int out0, void* stage0, void* stage1,
                                              void* scales) {
   if constexpr (sizeof...(Lower) > 0) {
     if (chunk.end - chunk.begin <= First<Lower...>::type::kRows) {
-      fitting_tile<GATE_UP, Lower...>(p, chunk, out0, stage0, stage1, scales);
+      fitting_tile<PART, Lower...>(p, chunk, out0, stage0, stage1, scales);
       return;
     }
   }
   auto& s0 = *static_cast<typename T::Stage*>(stage0);
   auto& s1 = *static_cast<typename T::Stage*>(stage1);
   auto& sc = *static_cast<typename T::Scales(*)[2]>(scales);
-  if constexpr (GATE_UP)
+  if constexpr (PART == kGateUp)
     gate_up_tile<T>(p, chunk, out0, s0, s1, sc);
   else
-    down_tile<T>(p, chunk, out0, s0, s1, sc);
+    down_tile<PART, T>(p, chunk, out0, s0, s1, sc);
 }
 
 // What counts as a short chunk: rows that a lower tiling holds (us, chunks in turn
@@ -376,7 +468,7 @@ constexpr int light_rows() {
     return 0;
 }
 
-template <bool GATE_UP, class T, class... Lower>
+template <int PART, class T, class... Lower>
 __global__ __launch_bounds__(T::kThreads, 2) void experts_tiled_kernel(Experts p, int blocks) {
   static_assert(((Lower::kThreads == T::kThreads && Lower::kOut == T::kOut && Lower::kRows < T::kRows) && ...), "");
   __shared__ __attribute__((aligned(16))) typename T::Stage stage0;
@@ -387,8 +479,8 @@ __global__ __launch_bounds__(T::kThreads, 2) void experts_tiled_kernel(Experts p
   const int id = blockIdx.x / kXcds;
   const Chunk chunk = chunk_of<T::kRows, light_rows<Lower...>()>(p, id / blocks * kXcds + blockIdx.x % kXcds);
   if (!chunk.weights) return;
-  const int out0 = id % blocks * (GATE_UP ? T::kOut / 2 : T::kOut / 16);
-  fitting_tile<GATE_UP, T, Lower...>(p, chunk, out0, &stage0, &stage1, &scales);
+  const int out0 = id % blocks * (PART == kGateUp ? T::kOut / 2 : T::kOut / 16);
+  fitting_tile<PART, T, Lower...>(p, chunk, out0, &stage0, &stage1, &scales);
 }
 
 // ------------------------------------------------ a token's own few routes --
@@ -462,22 +554,22 @@ int gate_up_few(const Experts& p, int64_t routes, hipStream_t s) {
   return SF_OK;
 }
 
-template <int WAVES, int NT>
+template <int WAVES, int HELD>
 int down_few(const Experts& p, int64_t routes, hipStream_t s) {
-  const int blocks = groups(groups(row_tiles(p.hidden), NT), WAVES);
+  const int blocks = groups(row_tiles(p.hidden) / 2, WAVES);
   const int64_t grid = most_chunks(routes, p.num_experts, 16) * blocks;
   if (!grid_fits(grid, WAVES * SF_WAVE)) return SF_ERR_UNSUPPORTED_SHAPE;
-  down_few_kernel<WAVES, NT><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
+  down_few_kernel<WAVES, HELD><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
 
-template <bool GATE_UP, class T, class... Lower>
+template <int PART, class T, class... Lower>
 int tiled(const Experts& p, int64_t routes, hipStream_t s) {
-  const int blocks = GATE_UP ? groups(tiles(p.inner) * 4, T::kOut / 64) : groups(p.hidden, T::kOut);
+  const int blocks = PART == kGateUp ? groups(tiles(p.inner) * 4, T::kOut / 64) : groups(p.hidden, T::kOut);
   const int64_t chunks = (most_chunks(routes, p.num_experts, T::kRows) + kXcds - 1) / kXcds * kXcds;
   if (!grid_fits(chunks * blocks, T::kThreads)) return SF_ERR_UNSUPPORTED_SHAPE;
-  experts_tiled_kernel<GATE_UP, T, Lower...>
+  experts_tiled_kernel<PART, T, Lower...>
       <<<dim3(static_cast<unsigned>(chunks * blocks)), dim3(T::kThreads), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
   return SF_OK;
@@ -500,6 +592,30 @@ int routed(const Experts& p, const Routes& r, int64_t routes, hipStream_t s) {
       <<<dim3(static_cast<unsigned>(down)), dim3(WAVES * SF_WAVE), 0, s>>>(p, r, max(1, WAVES / p.top_k));
   SF_LAUNCH_CHECK();
   return SF_OK;
+}
+
+// Both products over dispatched rows.
+template <int HELD>
+int grouped(const Experts& p, bool raw, int64_t routes, hipStream_t s) {
+  // By the routes to an expert on average: how many rows share its weights.  us
+  // of both products; experts of 2,048 x 768, 4,096 x 1,536 and 1,000 x 424:
+  //   gate and up by tiles of at most 32 and of 128 rows
+  //     16 routes an expert    70.9 / 76.5    67.7 / 68.3    21.7 / 22.8
+  //     32                     90.5 / 87.5    91.0 / 78.5    32.1 / 30.4
+  //   down by wavefronts and by tiles of at most 128 rows
+  //     4                      63.9 / 66.1    67.3 / 64.8    21.1 / 21.5
+  //     8                      67.5 / 67.3    68.5 / 65.6    22.0 / 21.7
+  //     16                     77.2 / 70.7    78.0 / 68.1    23.9 / 22.0
+  int rc;
+  if (raw)
+    rc = gate_up_few<4, kBf16>(p, routes, s);
+  else if (routes <= 16 * p.num_experts)
+    rc = tiled<kGateUp, Tiles32>(p, routes, s);
+  else
+    rc = tiled<kGateUp, Tiles128, Tiles64, Tiles32>(p, routes, s);
+  if (rc) return rc;
+  if (routes <= 8 * p.num_experts) return down_few<1, HELD>(p, routes, s);
+  return tiled<HELD, Tiles128, Tiles64, Tiles32>(p, routes, s);
 }
 
 // What both entry points ask of their arguments.
@@ -525,6 +641,65 @@ int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, in
   return SF_OK;
 }
 
+// out[t] = bf16(sum of token t's rows, in the order of its routes, in fp32).  A
+// thread: eight columns of a token.
+constexpr int kSumThreads = 256, kAhead = 8;
+
+template <bool EIGHTS>  // columns come in whole eights
+__global__ __launch_bounds__(kSumThreads) void sum_rows_kernel(const uint16_t* __restrict__ rows,
+                                                               const uint8_t* __restrict__ scales,
+                                                               const int32_t* __restrict__ inv, int top_k, int hidden,
+                                                               int blocks, uint16_t* __restrict__ out) {
+  const int token = blockIdx.x / blocks;
+  const int h = (blockIdx.x % blocks * kSumThreads + threadIdx.x) * 8;
+  if (h >= hidden) return;
+  const int scale_blocks = (hidden + kBlock - 1) / kBlock;
+  inv += static_cast<int64_t>(token) * top_k;
+  const bool whole = EIGHTS || h + 8 <= hidden;
+  float sum[8] = {};
+  for (int k0 = 0; k0 < top_k; k0 += kAhead) {  // their loads together
+    int row[kAhead];
+    u32x4 words[kAhead];
+    uint32_t e[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) row[j] = inv[min(k0 + j, top_k - 1)];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t at = max(row[j], 0);  // of an expert that is not there: any row, not added
+      const uint16_t* from = rows + at * hidden + h;
+      if (whole) {
+        words[j] = ld<u32x4_any>(from);
+      } else {
+        words[j] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (h + i < hidden) words[j][i / 2] |= static_cast<uint32_t>(ld<uint16_t>(from + i)) << (16 * (i % 2));
+      }
+      e[j] = ld<uint8_t>(scales + at * scale_blocks + h / kBlock);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (k0 + j >= top_k || row[j] < 0) continue;  // wave-uniform
+      const float s = from_row(e[j]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack2<kFp16>(words[j][i], a, b);
+        sum[2 * i] += a * s;
+        sum[2 * i + 1] += b * s;
+      }
+    }
+  }
+  uint16_t* o = out + static_cast<int64_t>(token) * hidden + h;
+  if (whole) {
+    *reinterpret_cast<u32x4_any*>(o) = u32x4{narrow2<kBf16>(sum[0], sum[1]), narrow2<kBf16>(sum[2], sum[3]),
+                                             narrow2<kBf16>(sum[4], sum[5]), narrow2<kBf16>(sum[6], sum[7])};
+    return;
+  }
+  for (int i = 0; i < 8; ++i)
+    if (h + i < hidden) o[i] = sf_f32_to_bf16(sum[i]);
+}
+
 // The dispatch and the rows' rounding need nothing of each other: the first
 // workgroups sort the routes (K2), the others round rows (K13).  61 tokens: two
 // launches 4.4 + 3.9 us, one 4.8; 2,048 tokens 11.4 + 5.2 and 12.6.
@@ -543,7 +718,7 @@ __global__ __launch_bounds__(THREADS) void prepare_kernel(const int64_t* __restr
                                chunks, total, codes, scales);
 }
 
-// Routes that read their experts for themselves save a dispatch, a combine and the
+// Routes that read their experts for themselves save a dispatch, a sum over rows and the
 // launches of both: about 10 us on the device and 10 on the host.  They read an
 // expert again for each further route to it, with even routing routes - E (1 -
 // (1 - 1 / E)^routes) times; 10 us are 40 MB of such reads.  us a call on the
@@ -560,7 +735,7 @@ bool without_dispatch(int64_t routes, int experts, int64_t expert_bytes) {
 
 // sf_mx_experts' workspace: what each part starts at, in bytes.
 struct Workspace {
-  int64_t act, act_scales, x, x_scales, meta, perm, inv, rows, bytes;
+  int64_t act, act_scales, x, x_scales, meta, perm, inv, rows, row_scales, bytes;
 };
 
 Workspace workspace_of(int tokens, int top_k, int hidden, int inner, int experts, bool dispatched) {
@@ -581,9 +756,33 @@ Workspace workspace_of(int tokens, int top_k, int hidden, int inner, int experts
     w.perm = take(4 * routes);
     w.inv = take(4 * routes);
     w.rows = take(2 * routes * hidden);
+    w.row_scales = take(routes * ((hidden + kBlock - 1) / kBlock));
   }
   w.bytes = at;
   return w;
+}
+
+// sf_mx_grouped_swiglu, with its rows as HELD says.
+template <int HELD>
+int grouped_swiglu(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, const int32_t* perm_pos,
+                   const int32_t* offsets, const void* route_weights, int tokens, int top_k, int hidden_size,
+                   int intermediate_size, int num_experts, const int32_t* slot_of_expert, const void* slots,
+                   int64_t slot_stride, void* act, void* act_scales, void* out_rows, void* row_scales,
+                   sf_stream_t stream) {
+  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
+                           slots, slot_stride, act, act_scales))
+    return rc;
+  if (tokens == 0) return SF_OK;
+  if (!perm_pos || !offsets || !out_rows) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(out_rows, 8)) return SF_ERR_MISALIGNED;
+  const Experts p = {x, static_cast<const uint8_t*>(x_scales), x_stride, perm_pos, offsets,
+                     static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size, num_experts,
+                     slot_of_expert, static_cast<const uint8_t*>(slots), slot_stride,
+                     record_of(hidden_size, intermediate_size), static_cast<uint8_t*>(act),
+                     static_cast<uint8_t*>(act_scales), static_cast<uint16_t*>(out_rows),
+                     static_cast<uint8_t*>(row_scales)};
+  return grouped<HELD>(p, x_dtype == kBf16, static_cast<int64_t>(tokens) * top_k,
+                       reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // namespace
@@ -607,38 +806,9 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
                                     int intermediate_size, int num_experts, const int32_t* slot_of_expert,
                                     const void* slots, int64_t slot_stride, void* act, void* act_scales,
                                     void* out_rows, sf_stream_t stream) {
-  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
-                           slots, slot_stride, act, act_scales))
-    return rc;
-  if (tokens == 0) return SF_OK;
-  if (!perm_pos || !offsets || !out_rows) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(out_rows, 8)) return SF_ERR_MISALIGNED;
-  const Experts p = {x, static_cast<const uint8_t*>(x_scales), x_stride, perm_pos, offsets,
-                     static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size, num_experts,
-                     slot_of_expert, static_cast<const uint8_t*>(slots), slot_stride,
-                     record_of(hidden_size, intermediate_size), static_cast<uint8_t*>(act),
-                     static_cast<uint8_t*>(act_scales), static_cast<uint16_t*>(out_rows)};
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
-  // By the routes to an expert on average: how many rows share its weights.  us
-  // of both products; experts of 2,048 x 768, 4,096 x 1,536 and 1,000 x 424:
-  //   gate and up by tiles of at most 32 and of 128 rows
-  //     16 routes an expert    70.9 / 76.5    67.7 / 68.3    21.7 / 22.8
-  //     32                     90.5 / 87.5    91.0 / 78.5    32.1 / 30.4
-  //   down by wavefronts and by tiles of at most 128 rows
-  //     4                      63.9 / 66.1    67.3 / 64.8    21.1 / 21.5
-  //     8                      67.5 / 67.3    68.5 / 65.6    22.0 / 21.7
-  //     16                     77.2 / 70.7    78.0 / 68.1    23.9 / 22.0
-  int rc;
-  if (x_dtype == kBf16)
-    rc = gate_up_few<4, kBf16>(p, routes, s);
-  else if (routes <= 16 * num_experts)
-    rc = tiled<true, Tiles32>(p, routes, s);
-  else
-    rc = tiled<true, Tiles128, Tiles64, Tiles32>(p, routes, s);
-  if (rc) return rc;
-  if (routes <= 8 * num_experts) return down_few<1, 2>(p, routes, s);
-  return tiled<false, Tiles128, Tiles64, Tiles32>(p, routes, s);
+  return grouped_swiglu<kBf16>(x_dtype, x, x_scales, x_stride, perm_pos, offsets, route_weights, tokens, top_k,
+                               hidden_size, intermediate_size, num_experts, slot_of_expert, slots, slot_stride, act,
+                               act_scales, out_rows, nullptr, stream);
 }
 
 extern "C" int sf_mx_routed_swiglu(int x_dtype, const void* x, const void* x_scales, int64_t x_stride,
@@ -737,9 +907,17 @@ extern "C" int sf_mx_experts(int x_dtype, const void* x, const void* x_scales, i
     if (const int rc = sf_dispatch(index, tokens, top_k, num_experts, counts, offsets, perm, inv, nullptr, stream))
       return rc;
   }
-  if (const int rc = sf_mx_grouped_swiglu(x_dtype, x, x_scales, x_stride, perm, offsets, route_weights, tokens, top_k,
-                                          hidden_size, intermediate_size, num_experts, nullptr, slots, slot_stride,
-                                          base + w.act, base + w.act_scales, base + w.rows, stream))
+  if (const int rc = grouped_swiglu<kHeldRows>(x_dtype, x, x_scales, x_stride, perm, offsets, route_weights, tokens,
+                                               top_k, hidden_size, intermediate_size, num_experts, nullptr, slots,
+                                               slot_stride, base + w.act, base + w.act_scales, base + w.rows,
+                                               base + w.row_scales, stream))
     return rc;
-  return sf_combine(base + w.rows, index, inv, nullptr, tokens, top_k, num_experts, hidden_size, 1, out, stream);
+  const int blocks = groups(hidden_size, 8 * kSumThreads);
+  if (!grid_fits(static_cast<int64_t>(tokens) * blocks, kSumThreads)) return SF_ERR_UNSUPPORTED_SHAPE;
+  const auto sum = hidden_size % 8 ? sum_rows_kernel<false> : sum_rows_kernel<true>;
+  sum<<<dim3(static_cast<unsigned>(tokens * blocks)), dim3(kSumThreads), 0, reinterpret_cast<hipStream_t>(stream)>>>(
+      reinterpret_cast<const uint16_t*>(base + w.rows), base + w.row_scales, inv, top_k, hidden_size, blocks,
+      static_cast<uint16_t*>(out));
+  SF_LAUNCH_CHECK();
+  return SF_OK;
 }

@@ -1756,9 +1756,9 @@ def mx_experts(hidden: torch.Tensor | MXRows, index: torch.Tensor, route_weights
 
     hidden [tokens, H] bf16 or its MXRows, ``index`` int64 and ``route_weights``
     bf16 [tokens, top_k], ``records`` uint8 [experts, mx_expert_bytes(H, I)].
-    Few routes run as ``mx_routed_swiglu``, others as ``dispatch``,
-    ``mx_grouped_swiglu`` and ``combine`` with fp32 sums.  Routes to experts that
-    are not there count for nothing.  Nothing is read back to the host.  With
+    Few routes run as ``mx_routed_swiglu``, others through a dispatch; a token's
+    routes are added in fp32 and rounded once.  Routes to experts that are not
+    there count for nothing.  Nothing is read back to the host.  With
     ``stream``, the inputs and the output (memory of the current stream) are the
     caller's to order between the two streams.  No gradients."""
     H, I = hidden_size, intermediate_size

@@ -72,10 +72,11 @@ def half_step(y, dtype):
     return y.abs().clamp_min(tiny) * torch.finfo(dtype).eps / 2
 
 
-def experts(hidden, index, weights, packed, hidden_size, intermediate_size, table=None):
+def experts(hidden, index, weights, packed, hidden_size, intermediate_size, rows=torch.float16):
     """Outputs of K16's chain with its roundings, and what they may be off by
-    beyond it: the product's slack, and where the activation lies so near a
-    border that it may fall on the other side, a step of it."""
+    beyond it: the product's slack, where the activation lies so near a border
+    that it may fall on the other side a step of it, and a route's row rounded to
+    ``rows`` (fp16: in blocks, so down to 2^-39 of the block's largest)."""
     H, I = hidden_size, intermediate_size
     x = quantize(hidden, "e4m3")[0]
     out = torch.zeros((hidden.shape[0], H), dtype=torch.float64, device=hidden.device)
@@ -104,5 +105,8 @@ def experts(hidden, index, weights, packed, hidden_size, intermediate_size, tabl
         r = weights[token, slot].double()[:, None]
         row = y * r
         out.index_add_(0, token, row)
-        slack.index_add_(0, token, dy * r.abs() + half_step(row, torch.bfloat16) * 1.01)
+        step = row.abs() * torch.finfo(rows).eps / 2 * 1.01
+        if rows == torch.float16:
+            step += row.abs().amax(1, keepdim=True) * 2.0 ** -39
+        slack.index_add_(0, token, dy * r.abs() + step)
     return out, slack + half_step(out, torch.bfloat16) + slack * 2.0 ** -8

@@ -25,8 +25,8 @@ def _case(tokens, hidden, inner, experts, top_k, seed=0, favourite=None, distinc
     return h, packed, index, weights.to(torch.bfloat16)
 
 
-def _check(got, h, index, weights, packed, hidden, inner):
-    want, slack = ref.experts(h, index, weights, packed, hidden, inner)
+def _check(got, h, index, weights, packed, hidden, inner, **more):
+    want, slack = ref.experts(h, index, weights, packed, hidden, inner, **more)
     assert (got.double() - want).abs().le(slack).all()
     if want.norm() > 0:
         # Roundings to 8 bits fall on the other side for a few values only.
@@ -245,6 +245,57 @@ def test_far_rows():
     many[-400:] = h
     many_index, many_weights = index.repeat(T // 400, 1), weights.repeat(T // 400, 1)
     assert torch.equal(ops.mx_experts(many, many_index, many_weights, records, H, I)[-400:], want)
+
+
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(9, 64, 32, 8, 3), (40, 100, 424, 20, 2),
+                                                             (200, 256, 160, 8, 4), (300, 512, 256, 2, 2)])
+def test_the_parts_in_turn(tokens, hidden, inner, experts, top_k):
+    """dispatch, the products with bf16 rows, and combine."""
+    h, packed, index, weights = _case(tokens, hidden, inner, experts, top_k)
+    records = ops.mx_quantize_experts(packed, hidden, inner)
+    plan = ops.dispatch(index, experts)
+    rows = torch.empty((tokens * top_k, hidden), dtype=torch.bfloat16, device=DEV)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), records, hidden, inner, rows)
+    got = ops.combine(rows, index, plan, hidden, accumulate_fp32=True)
+    _check(got, h, index, weights, packed, hidden, inner, rows=torch.bfloat16)
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("power", [90, -100])
+def test_outputs_of_any_size(tokens, power):
+    """A power of two in the last weight is one in the outputs."""
+    H, I, E, K = 100, 64, 4, 2
+    h, packed, index, weights = _case(tokens, H, I, E, K)
+    want = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    packed[:, 2 * H * I:] *= 2.0 ** power
+    got = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    assert torch.equal(got.double(), want.double() * 2.0 ** power)
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+def test_a_column_that_is_not_finite_stays_alone(tokens):
+    H, I, E, K = 96, 64, 4, 2
+    h, packed, index, weights = _case(tokens, H, I, E, K)
+    want = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    packed[2, 2 * H * I + 37 * I + 5] = float("inf")       # of expert 2's down, output 37
+    got = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    bad = torch.zeros((tokens, H), dtype=torch.bool, device=DEV)
+    bad[(index == 2).any(1), 37] = True
+    assert bad.any() and torch.equal(torch.isnan(got), bad)
+    assert torch.equal(got[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 300])
+def test_a_route_weight_that_is_not_finite_stays_in_its_token(tokens):
+    H, I, E, K = 96, 64, 4, 2
+    h, packed, index, weights = _case(tokens, H, I, E, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    want = ops.mx_experts(h, index, weights, records, H, I)
+    weights[1, 0], weights[2, 1] = float("inf"), float("nan")
+    got = ops.mx_experts(h, index, weights, records, H, I)
+    assert not torch.isfinite(got[1:3]).any()
+    there = [t for t in range(tokens) if t not in (1, 2)]
+    assert torch.equal(got[there], want[there])
 
 
 def test_two_calls_at_once():
