@@ -391,30 +391,33 @@ __device__ __forceinline__ void down_tile(const Experts& p, const Chunk& chunk, 
     const bool live = row < chunk.end;
     const float route = live ? route_weight(p, row) : 0.f;
     const int first = tile0 * 16 + wn * T::FN * 32;
+    // The weight by itself, not with the block's power of two: of a block of zeros
+    // that is 2^126, and the two factors' product infinite from a weight of 4 on.
+#pragma unroll
+    for (int n = 0; n < T::FN; ++n) acc[n][m] *= route;
     float top[T::FN];
     uint32_t scales_word = 0;
     if (HELD == kHeldRows) {
       bool infinite = false;
 #pragma unroll
       for (int n = 0; n < T::FN; ++n) {
-        top[n] = max32(largest<16, false>(acc[n][m])) * fabsf(route);  // products round monotonically
-        infinite |= !(top[n] < __builtin_inff());
+        top[n] = max32(largest<16, false>(acc[n][m]));
+        infinite |= magnitude(top[n]) == 0x7f800000u;
       }
       if (__any(infinite)) {
 #pragma unroll
-        for (int n = 0; n < T::FN; ++n) top[n] = max32(largest<16, true>(acc[n][m] * route));
+        for (int n = 0; n < T::FN; ++n) top[n] = max32(largest<16, true>(acc[n][m]));
       }
     }
 #pragma unroll
     for (int n = 0; n < T::FN; ++n) {
       const int h0 = first + n * 32;
-      float factor = route;
+      f32x16 v = acc[n][m];
       if (HELD == kHeldRows) {
         const uint32_t e = row_exponent(__float_as_uint(top[n]));
-        factor *= to_row(e);
+        v *= to_row(e);
         scales_word |= e << (8 * n);
       }
-      const f32x16 v = acc[n][m] * factor;
       constexpr int DT = HELD == kHeldRows ? kFp16 : kBf16;
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {

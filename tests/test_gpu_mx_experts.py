@@ -348,3 +348,56 @@ def test_a_model_with_mx_experts_prompt_and_decoding():
     assert len(seen) == 8 and {s[1].shape[0] for s in seen} == {300, 1}
     for i, hidden, index, weights, got in seen:
         _check(got, hidden, index, weights.to(torch.bfloat16), packed[i], 64, 32)
+
+
+def _even(tokens, experts, top_k):
+    """Routes in turn: as many rows for one expert as for another."""
+    t = torch.arange(tokens, device=DEV)[:, None]
+    return (t * top_k + torch.arange(top_k, device=DEV)) % experts
+
+
+# Two routes a token: without a dispatch; then 5 rows an expert (wavefronts), 20, 50,
+# 100 and 150 (tiles of 32, 64 and 128 rows, and of 128 with one of 32).
+FORMS = [(3, 4), (100, 40), (100, 10), (100, 4), (200, 4), (300, 4)]
+
+
+@pytest.mark.parametrize("tokens,experts", FORMS)
+def test_zeros_stay_zeros_under_large_route_weights(tokens, experts):
+    """A token of zeros and outputs that no weight reaches are 0 whatever finite
+    weight their routes have, and the others what they are."""
+    H, I, K = 160, 64, 2
+    h, packed, _, weights = _case(tokens, H, I, experts, K)
+    index = _even(tokens, experts, K)
+    packed.view(experts, 3, -1)[:, 2].view(experts, H, I)[:, 32:64] = 0
+    sizes = torch.tensor([3.984375, 4.0, -8.0, 100.0, -2.0 ** 40], device=DEV, dtype=torch.bfloat16)
+    weights = sizes[torch.arange(tokens * K, device=DEV) % 5].view(tokens, K).clone()
+    empty = [1, tokens // 2, tokens - 1]
+    h[empty] = 0
+    weights[1] = torch.tensor([3e38, -3e38], device=DEV)
+    records = ops.mx_quantize_experts(packed, H, I)
+    got = ops.mx_experts(h, index, weights, records, H, I)
+    assert torch.isfinite(got).all()
+    assert not got[empty].any() and not got[:, 32:64].any()
+    want, slack = ref.experts(h, index, weights, packed, H, I)
+    assert (got.double() - want).abs().le(slack).all()
+    rows = torch.full((tokens * K, H), 7.0, dtype=torch.bfloat16, device=DEV)
+    plan = ops.dispatch(index, experts)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), records, H, I, rows)
+    assert not rows[:, 32:64].any()
+    token = plan.perm_pos.long() // K
+    assert not rows[torch.isin(token, torch.tensor(empty, device=DEV))].any()
+
+
+@pytest.mark.parametrize("tokens,experts", FORMS)
+def test_tiny_sums_under_large_route_weights(tokens, experts):
+    """Sums near 2^-116 and weights of 2^30: neither has to be taken past fp32's
+    range on the way to their product."""
+    H, I, K = 160, 64, 2
+    h, packed, _, weights = _case(tokens, H, I, experts, K)
+    index, weights = _even(tokens, experts, K), weights * 2.0 ** 30
+    packed[:, 2 * H * I:] *= 2.0 ** -116
+    got = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    want, slack = ref.experts(h, index, weights, packed, H, I)
+    # A sum's terms and parts below 2^-126 may count as 0: 64 terms of a route, K routes.
+    slack = slack + I * 2.0 ** -126 * weights.double().abs().sum(1, keepdim=True)
+    assert (got.double() - want).abs().le(slack).all()
