@@ -547,31 +547,38 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void routed_down_kernel(Experts p,
 
 int groups(int n, int per) { return (n - 1) / per + 1; }
 
+// What a launcher does: kCheck only asks whether its grids fit, so that an entry
+// point refuses a call before the first of its launches.
+enum Do { kCheck, kLaunch };
+
 template <int WAVES, int XDT>
-int gate_up_few(const Experts& p, int64_t routes, hipStream_t s) {
+int gate_up_few(const Experts& p, int64_t routes, Do what, hipStream_t s) {
   const int blocks = tiles(p.inner) * 4;
   const int64_t grid = most_chunks(routes, p.num_experts, 16) * blocks;
   if (!grid_fits(grid, WAVES * SF_WAVE)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (what == kCheck) return SF_OK;
   gate_up_few_kernel<WAVES, XDT><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
 
 template <int WAVES, int HELD>
-int down_few(const Experts& p, int64_t routes, hipStream_t s) {
+int down_few(const Experts& p, int64_t routes, Do what, hipStream_t s) {
   const int blocks = groups(row_tiles(p.hidden) / 2, WAVES);
   const int64_t grid = most_chunks(routes, p.num_experts, 16) * blocks;
   if (!grid_fits(grid, WAVES * SF_WAVE)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (what == kCheck) return SF_OK;
   down_few_kernel<WAVES, HELD><<<dim3(static_cast<unsigned>(grid)), dim3(WAVES * SF_WAVE), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
   return SF_OK;
 }
 
 template <int PART, class T, class... Lower>
-int tiled(const Experts& p, int64_t routes, hipStream_t s) {
+int tiled(const Experts& p, int64_t routes, Do what, hipStream_t s) {
   const int blocks = PART == kGateUp ? groups(tiles(p.inner) * 4, T::kOut / 64) : groups(p.hidden, T::kOut);
   const int64_t chunks = (most_chunks(routes, p.num_experts, T::kRows) + kXcds - 1) / kXcds * kXcds;
   if (!grid_fits(chunks * blocks, T::kThreads)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (what == kCheck) return SF_OK;
   experts_tiled_kernel<PART, T, Lower...>
       <<<dim3(static_cast<unsigned>(chunks * blocks)), dim3(T::kThreads), 0, s>>>(p, blocks);
   SF_LAUNCH_CHECK();
@@ -583,11 +590,12 @@ using Tiles64 = Tiling<4, 1, 2, 2>;
 using Tiles128 = Tiling<2, 2, 4, 2>;
 
 template <int WAVES, int XDT>
-int routed(const Experts& p, const Routes& r, int64_t routes, hipStream_t s) {
+int routed(const Experts& p, const Routes& r, int64_t routes, Do what, hipStream_t s) {
   const int blocks = tiles(p.inner) * 4;
   const int64_t down = routes / p.top_k * row_tiles(p.hidden);
   if (!grid_fits(routes * blocks, WAVES * SF_WAVE) || !grid_fits(down, WAVES * SF_WAVE))
     return SF_ERR_UNSUPPORTED_SHAPE;
+  if (what == kCheck) return SF_OK;
   routed_gate_up_kernel<WAVES, XDT>
       <<<dim3(static_cast<unsigned>(routes * blocks)), dim3(WAVES * SF_WAVE), 0, s>>>(p, r, blocks);
   SF_LAUNCH_CHECK();
@@ -599,7 +607,7 @@ int routed(const Experts& p, const Routes& r, int64_t routes, hipStream_t s) {
 
 // Both products over dispatched rows.
 template <int HELD>
-int grouped(const Experts& p, bool raw, int64_t routes, hipStream_t s) {
+int grouped(const Experts& p, bool raw, int64_t routes, Do what, hipStream_t s) {
   // By the routes to an expert on average: how many rows share its weights.  us
   // of both products; experts of 2,048 x 768, 4,096 x 1,536 and 1,000 x 424:
   //   gate and up by tiles of at most 32 and of 128 rows
@@ -611,17 +619,17 @@ int grouped(const Experts& p, bool raw, int64_t routes, hipStream_t s) {
   //     16                     77.2 / 70.7    78.0 / 68.1    23.9 / 22.0
   int rc;
   if (raw)
-    rc = gate_up_few<4, kBf16>(p, routes, s);
+    rc = gate_up_few<4, kBf16>(p, routes, what, s);
   else if (routes <= 16 * p.num_experts)
-    rc = tiled<kGateUp, Tiles32>(p, routes, s);
+    rc = tiled<kGateUp, Tiles32>(p, routes, what, s);
   else
-    rc = tiled<kGateUp, Tiles128, Tiles64, Tiles32>(p, routes, s);
+    rc = tiled<kGateUp, Tiles128, Tiles64, Tiles32>(p, routes, what, s);
   if (rc) return rc;
-  if (routes <= 8 * p.num_experts) return down_few<1, HELD>(p, routes, s);
-  return tiled<HELD, Tiles128, Tiles64, Tiles32>(p, routes, s);
+  if (routes <= 8 * p.num_experts) return down_few<1, HELD>(p, routes, what, s);
+  return tiled<HELD, Tiles128, Tiles64, Tiles32>(p, routes, what, s);
 }
 
-// What both entry points ask of their arguments.
+// What the entry points ask of their arguments.
 int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, int tokens, int top_k, int hidden_size,
           int intermediate_size, int num_experts, const void* slots, int64_t slot_stride, const void* act,
           const void* act_scales) {
@@ -765,27 +773,29 @@ Workspace workspace_of(int tokens, int top_k, int hidden, int inner, int experts
   return w;
 }
 
-// sf_mx_grouped_swiglu, with its rows as HELD says.
-template <int HELD>
-int grouped_swiglu(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, const int32_t* perm_pos,
-                   const int32_t* offsets, const void* route_weights, int tokens, int top_k, int hidden_size,
-                   int intermediate_size, int num_experts, const int32_t* slot_of_expert, const void* slots,
-                   int64_t slot_stride, void* act, void* act_scales, void* out_rows, void* row_scales,
-                   sf_stream_t stream) {
-  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
-                           slots, slot_stride, act, act_scales))
-    return rc;
-  if (tokens == 0) return SF_OK;
-  if (!perm_pos || !offsets || !out_rows) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(out_rows, 8)) return SF_ERR_MISALIGNED;
-  const Experts p = {x, static_cast<const uint8_t*>(x_scales), x_stride, perm_pos, offsets,
-                     static_cast<const uint16_t*>(route_weights), top_k, hidden_size, intermediate_size, num_experts,
-                     slot_of_expert, static_cast<const uint8_t*>(slots), slot_stride,
-                     record_of(hidden_size, intermediate_size), static_cast<uint8_t*>(act),
-                     static_cast<uint8_t*>(act_scales), static_cast<uint16_t*>(out_rows),
-                     static_cast<uint8_t*>(row_scales)};
-  return grouped<HELD>(p, x_dtype == kBf16, static_cast<int64_t>(tokens) * top_k,
-                       reinterpret_cast<hipStream_t>(stream));
+Experts experts_of(const void* x, const void* x_scales, int64_t x_stride, const void* route_weights, int top_k,
+                   int hidden_size, int intermediate_size, int num_experts, const int32_t* slot_of_expert,
+                   const void* slots, int64_t slot_stride, void* act, void* act_scales) {
+  Experts p = {};
+  p.x = x;
+  p.x_scales = static_cast<const uint8_t*>(x_scales);
+  p.x_stride = x_stride;
+  p.route_weights = static_cast<const uint16_t*>(route_weights);
+  p.top_k = top_k;
+  p.hidden = hidden_size;
+  p.inner = intermediate_size;
+  p.num_experts = num_experts;
+  p.slot_of_expert = slot_of_expert;
+  p.slots = static_cast<const uint8_t*>(slots);
+  p.slot_stride = slot_stride;
+  p.record = record_of(hidden_size, intermediate_size);
+  p.act = static_cast<uint8_t*>(act);
+  p.act_scales = static_cast<uint8_t*>(act_scales);
+  return p;
+}
+
+int routed(int x_dtype, const Experts& p, const Routes& r, int64_t routes, Do what, hipStream_t s) {
+  return x_dtype == kBf16 ? routed<8, kBf16>(p, r, routes, what, s) : routed<8, kRows>(p, r, routes, what, s);
 }
 
 }  // namespace
@@ -809,9 +819,21 @@ extern "C" int sf_mx_grouped_swiglu(int x_dtype, const void* x, const void* x_sc
                                     int intermediate_size, int num_experts, const int32_t* slot_of_expert,
                                     const void* slots, int64_t slot_stride, void* act, void* act_scales,
                                     void* out_rows, sf_stream_t stream) {
-  return grouped_swiglu<kBf16>(x_dtype, x, x_scales, x_stride, perm_pos, offsets, route_weights, tokens, top_k,
-                               hidden_size, intermediate_size, num_experts, slot_of_expert, slots, slot_stride, act,
-                               act_scales, out_rows, nullptr, stream);
+  if (const int rc = check(x_dtype, x, x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
+                           slots, slot_stride, act, act_scales))
+    return rc;
+  if (tokens == 0) return SF_OK;
+  if (!perm_pos || !offsets || !out_rows) return SF_ERR_INVALID_ARGUMENT;
+  if (!aligned(out_rows, 8)) return SF_ERR_MISALIGNED;
+  Experts p = experts_of(x, x_scales, x_stride, route_weights, top_k, hidden_size, intermediate_size, num_experts,
+                         slot_of_expert, slots, slot_stride, act, act_scales);
+  p.perm_pos = perm_pos;
+  p.offsets = offsets;
+  p.rows = static_cast<uint16_t*>(out_rows);
+  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (const int rc = grouped<kBf16>(p, x_dtype == kBf16, routes, kCheck, s)) return rc;
+  return grouped<kBf16>(p, x_dtype == kBf16, routes, kLaunch, s);
 }
 
 extern "C" int sf_mx_routed_swiglu(int x_dtype, const void* x, const void* x_scales, int64_t x_stride,
@@ -825,24 +847,10 @@ extern "C" int sf_mx_routed_swiglu(int x_dtype, const void* x, const void* x_sca
   if (tokens == 0) return SF_OK;
   if (!index || !route_weights || !out) return SF_ERR_INVALID_ARGUMENT;
   if (!aligned(index, 8) || !aligned(route_weights, 2) || !aligned(out, 2)) return SF_ERR_MISALIGNED;
-  Experts p = {};
-  p.x = x;
-  p.x_scales = static_cast<const uint8_t*>(x_scales);
-  p.x_stride = x_stride;
-  p.top_k = top_k;
-  p.hidden = hidden_size;
-  p.inner = intermediate_size;
-  p.num_experts = num_experts;
-  p.slot_of_expert = slot_of_expert;
-  p.slots = static_cast<const uint8_t*>(slots);
-  p.slot_stride = slot_stride;
-  p.record = record_of(hidden_size, intermediate_size);
-  p.act = static_cast<uint8_t*>(act);
-  p.act_scales = static_cast<uint8_t*>(act_scales);
+  const Experts p = experts_of(x, x_scales, x_stride, route_weights, top_k, hidden_size, intermediate_size, num_experts,
+                               slot_of_expert, slots, slot_stride, act, act_scales);
   const Routes r = {index, static_cast<const uint16_t*>(route_weights), static_cast<uint16_t*>(out)};
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
-  return x_dtype == kBf16 ? routed<8, kBf16>(p, r, routes, s) : routed<8, kRows>(p, r, routes, s);
+  return routed(x_dtype, p, r, static_cast<int64_t>(tokens) * top_k, kLaunch, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int sf_mx_experts_form(int tokens, int top_k, int hidden_size, int intermediate_size, int num_experts) {
@@ -866,61 +874,63 @@ extern "C" int sf_mx_experts(int x_dtype, const void* x, const void* x_scales, i
   if (bytes < 0) return SF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return SF_OK;
   if (!x || !index || !route_weights || !slots || !workspace || !out) return SF_ERR_INVALID_ARGUMENT;
-  if (!aligned(workspace, 16) || !aligned(out, 2)) return SF_ERR_MISALIGNED;
+  if (!aligned(workspace, 16) || !aligned(out, 2) || !aligned(index, 8) || !aligned(route_weights, 2))
+    return SF_ERR_MISALIGNED;
+  const int64_t routes = static_cast<int64_t>(tokens) * top_k;
   const bool dispatched = !sf_mx_experts_form(tokens, top_k, hidden_size, intermediate_size, num_experts);
   const Workspace w = workspace_of(tokens, top_k, hidden_size, intermediate_size, num_experts, dispatched);
   uint8_t* base = static_cast<uint8_t*>(workspace);
+  // Few rows are rounded by the wavefronts that read them.
+  const bool rounds = x_dtype == kBf16 && (tokens > 16 || hidden_size % 8 || x_stride % 8 || !aligned(x, 16));
+  const int held = rounds ? kRows : x_dtype;  // what the products read
+  if (rounds && !aligned(x, 2)) return SF_ERR_MISALIGNED;
+  Experts p = experts_of(rounds ? base + w.x : x, rounds ? base + w.x_scales : x_scales, x_stride, route_weights, top_k,
+                         hidden_size, intermediate_size, num_experts, nullptr, slots, slot_stride, base + w.act,
+                         base + w.act_scales);
+  if (const int rc = check(held, p.x, p.x_scales, x_stride, tokens, top_k, hidden_size, intermediate_size, num_experts,
+                           slots, slot_stride, p.act, p.act_scales))
+    return rc;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const Routes r = {index, p.route_weights, static_cast<uint16_t*>(out)};
+  if (!dispatched) {
+    if (const int rc = routed(held, p, r, routes, kCheck, s)) return rc;
+    if (rounds) {
+      if (const int rc = sf_mx_quantize(kBf16, x, x_stride, 0, tokens, hidden_size, 1, kE4m3, base + w.x, 0,
+                                        base + w.x_scales, 0, stream))
+        return rc;
+    }
+    return routed(held, p, r, routes, kLaunch, s);
+  }
   int32_t* counts = reinterpret_cast<int32_t*>(base + w.meta);
   int32_t* offsets = counts + num_experts + 1;
   int32_t* perm = reinterpret_cast<int32_t*>(base + w.perm);
   int32_t* inv = reinterpret_cast<int32_t*>(base + w.inv);
-  // Few rows are rounded by the wavefronts that read them.
-  const bool rounds = x_dtype == kBf16 && (tokens > 16 || hidden_size % 8 || x_stride % 8 || !aligned(x, 16));
-  if (rounds && dispatched) {
-    if (x_stride < 0) return SF_ERR_INVALID_ARGUMENT;
-    if (!aligned(x, 2) || !aligned(index, 8)) return SF_ERR_MISALIGNED;
-    const int64_t routes = static_cast<int64_t>(tokens) * top_k;
-    if (routes > 1 << 28) return SF_ERR_UNSUPPORTED_SHAPE;
-    const sf_dispatch_impl::Cut cut = sf_dispatch_impl::cut_of(static_cast<int>(routes));
-    const int chunks = tiles(hidden_size) * 16;
-    const int64_t total = static_cast<int64_t>(tokens) * chunks;
-    const int64_t grid = cut.spans + (total - 1) / cut.threads + 1;
-    if (!grid_fits(grid, cut.threads)) return SF_ERR_UNSUPPORTED_SHAPE;
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  p.perm_pos = perm;
+  p.offsets = offsets;
+  p.rows = reinterpret_cast<uint16_t*>(base + w.rows);
+  p.row_scales = base + w.row_scales;
+  const sf_dispatch_impl::Cut cut = sf_dispatch_impl::cut_of(static_cast<int>(routes));
+  const int chunks = tiles(hidden_size) * 16;
+  const int64_t total = static_cast<int64_t>(tokens) * chunks;
+  const int64_t grid = cut.spans + (total - 1) / cut.threads + 1;
+  const int blocks = groups(hidden_size, 8 * kSumThreads);
+  if (const int rc = grouped<kHeldRows>(p, held == kBf16, routes, kCheck, s)) return rc;
+  if ((rounds && !grid_fits(grid, cut.threads)) || !grid_fits(static_cast<int64_t>(tokens) * blocks, kSumThreads))
+    return SF_ERR_UNSUPPORTED_SHAPE;
+  if (rounds) {
     const auto prepare = cut.threads == 256 ? prepare_kernel<256> : prepare_kernel<1024>;
     prepare<<<dim3(static_cast<unsigned>(grid)), dim3(cut.threads), 0, s>>>(
         index, static_cast<int>(routes), num_experts, cut.span, cut.spans, counts, perm, inv,
         static_cast<const char*>(x), x_stride, hidden_size, chunks, total, base + w.x, base + w.x_scales);
     SF_LAUNCH_CHECK();
-  } else if (rounds) {
-    if (const int rc = sf_mx_quantize(kBf16, x, x_stride, 0, tokens, hidden_size, 1, kE4m3, base + w.x, 0,
-                                      base + w.x_scales, 0, stream))
-      return rc;
-  }
-  if (rounds) {
-    x_dtype = kRows;
-    x = base + w.x;
-    x_scales = base + w.x_scales;
-  }
-  if (!dispatched)
-    return sf_mx_routed_swiglu(x_dtype, x, x_scales, x_stride, index, route_weights, tokens, top_k, hidden_size,
-                               intermediate_size, num_experts, nullptr, slots, slot_stride, base + w.act,
-                               base + w.act_scales, out, stream);
-  if (!rounds) {
+  } else {
     if (const int rc = sf_dispatch(index, tokens, top_k, num_experts, counts, offsets, perm, inv, nullptr, stream))
       return rc;
   }
-  if (const int rc = grouped_swiglu<kHeldRows>(x_dtype, x, x_scales, x_stride, perm, offsets, route_weights, tokens,
-                                               top_k, hidden_size, intermediate_size, num_experts, nullptr, slots,
-                                               slot_stride, base + w.act, base + w.act_scales, base + w.rows,
-                                               base + w.row_scales, stream))
-    return rc;
-  const int blocks = groups(hidden_size, 8 * kSumThreads);
-  if (!grid_fits(static_cast<int64_t>(tokens) * blocks, kSumThreads)) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (const int rc = grouped<kHeldRows>(p, held == kBf16, routes, kLaunch, s)) return rc;
   const auto sum = hidden_size % 8 ? sum_rows_kernel<false> : sum_rows_kernel<true>;
-  sum<<<dim3(static_cast<unsigned>(tokens * blocks)), dim3(kSumThreads), 0, reinterpret_cast<hipStream_t>(stream)>>>(
-      reinterpret_cast<const uint16_t*>(base + w.rows), base + w.row_scales, inv, top_k, hidden_size, blocks,
-      static_cast<uint16_t*>(out));
+  sum<<<dim3(static_cast<unsigned>(tokens * blocks)), dim3(kSumThreads), 0, s>>>(
+      p.rows, p.row_scales, inv, top_k, hidden_size, blocks, static_cast<uint16_t*>(out));
   SF_LAUNCH_CHECK();
   return SF_OK;
 }

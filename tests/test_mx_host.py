@@ -244,3 +244,30 @@ def test_the_workspace_holds_every_part():
         assert sum(parts) <= size(tokens, top_k, hidden, inner, experts) <= sum(parts) + 9 * 256
     assert size(1, 8, 64, 32, 257) == size(1, 8, 0, 32, 4) == size(1, 0, 64, 32, 4) == -1
     assert size(0, 2, 64, 32, 4) >= 0
+
+
+def test_experts_are_refused_before_any_launch():
+    """Calls whose rows are rounded first, with a dispatch and without, and calls
+    whose routes are sorted first: without a GPU a launch would be an error of
+    its own."""
+    lib = _native.lib()
+    a = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(a) + 63 & ~63
+    big = lib.sf_mx_expert_bytes(64, 32)
+    e = lib.sf_mx_experts
+    for dtype, scales, stride, tokens, top_k, hidden, experts, dispatched in [
+            (0, None, 64, 100, 2, 64, 4, True), (0, None, 63, 40, 2, 64, 4, False), (3, p, 0, 100, 2, 64, 4, True),
+            (0, None, 64, 16, 16, 64, 4, True)]:
+        assert lib.sf_mx_experts_form(tokens, top_k, hidden, 32, experts) == (not dispatched)
+        def call(slots=p, slot=big, x=p, index=p, weights=p, stride=stride, workspace=p, out=p):
+            return e(dtype, x, scales, stride, index, weights, tokens, top_k, hidden, 32, experts, slots, slot,
+                     workspace, out, None)
+        assert call(slot=big - 16) == INVALID and call(stride=-8) == INVALID
+        for bad in [dict(slot=big + 8), dict(slots=p + 8), dict(index=p + 4), dict(weights=p + 1), dict(x=p + 1),
+                    dict(workspace=p + 8), dict(out=p + 1)]:
+            assert call(**bad) == MISALIGNED, bad
+    # A grid of the second product or of the sum that does not fit.
+    g = lib.sf_mx_grouped_swiglu
+    wide = lib.sf_mx_expert_bytes(1 << 20, 32)
+    assert g(3, p, p, 0, p, p, None, 1 << 23, 32, 1 << 20, 32, 4, None, p, wide, p, p, p, None) == UNSUPPORTED
+    assert e(0, p, None, 1 << 20, p, p, 1 << 23, 32, 1 << 20, 32, 4, p, wide, p, p, None) == UNSUPPORTED
