@@ -652,7 +652,9 @@ int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
  *   codes, scales   a weight in e2m1 [out_features, dim]
  *   bias      [out_features] of out_dtype, or NULL
  *   out_dtype 0 bf16, 1 fp16; out has row stride out_stride
- * codes, scales and, for x_dtype 3, x and x_scales 16-byte aligned; rows <= 2^20.
+ * codes, scales and, for x_dtype 3, x and x_scales 16-byte aligned; rows <= 2^20,
+ * dim <= 2^24, out_features <= 2^28, and fewer than 2^24 blocks of 128 rows by 256
+ * outputs.
  */
 int sf_mx_linear(int x_dtype, const void *x, const void *x_scales,
                  int64_t x_stride, int rows, int dim, const void *codes,
@@ -715,8 +717,9 @@ int sf_mx_routed_swiglu(int x_dtype, const void *x, const void *x_scales,
  * rounded once.  Expert e is in slot e.
  *   x_dtype     0 bf16 rows of row stride x_stride, any number and alignment of
  *               them; 3 rows in e4m3 as above
- *   workspace   sf_mx_experts_workspace bytes (-1: an unsupported shape),
- *               16-byte aligned; calls that may overlap need one each
+ *   workspace   sf_mx_experts_workspace bytes (-1: an unsupported shape, such as
+ *               more than 2^28 routes), 16-byte aligned; calls that may overlap
+ *               need one each
  * sf_mx_experts_form says which it is: 1 without a dispatch, 0 with one (-1: an
  * unsupported shape).
  */

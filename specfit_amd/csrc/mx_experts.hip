@@ -629,6 +629,8 @@ int grouped(const Experts& p, bool raw, int64_t routes, Do what, hipStream_t s) 
   return tiled<HELD, Tiles128, Tiles64, Tiles32>(p, routes, what, s);
 }
 
+constexpr int64_t kMostRoutes = 1 << 28;
+
 // What the entry points ask of their arguments.
 int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, int tokens, int top_k, int hidden_size,
           int intermediate_size, int num_experts, const void* slots, int64_t slot_stride, const void* act,
@@ -638,7 +640,7 @@ int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, in
   const int64_t bytes = sf_mx_expert_bytes(hidden_size, intermediate_size);
   if (bytes < 0) return SF_ERR_INVALID_ARGUMENT;
   if (num_experts > SF_MAX_EXPERTS || top_k > SF_MAX_TOPK) return SF_ERR_TOO_MANY_EXPERTS;
-  if (static_cast<int64_t>(tokens) * top_k > 1 << 28) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (static_cast<int64_t>(tokens) * top_k > kMostRoutes) return SF_ERR_UNSUPPORTED_SHAPE;
   if (tokens == 0) return SF_OK;
   if (!x || (x_dtype == kRows && !x_scales) || !slots || !act || !act_scales || slot_stride < bytes)
     return SF_ERR_INVALID_ARGUMENT;
@@ -862,7 +864,9 @@ extern "C" int sf_mx_experts_form(int tokens, int top_k, int hidden_size, int in
 extern "C" int64_t sf_mx_experts_workspace(int tokens, int top_k, int hidden_size, int intermediate_size,
                                            int num_experts) {
   const int form = sf_mx_experts_form(tokens, top_k, hidden_size, intermediate_size, num_experts);
-  if (form < 0 || top_k > SF_MAX_TOPK || num_experts > SF_MAX_EXPERTS) return -1;
+  if (form < 0 || top_k > SF_MAX_TOPK || num_experts > SF_MAX_EXPERTS ||
+      static_cast<int64_t>(tokens) * top_k > kMostRoutes)
+    return -1;
   return workspace_of(tokens, top_k, hidden_size, intermediate_size, num_experts, form == 0).bytes;
 }
 

@@ -220,11 +220,18 @@ int launch_rows(const Linear& p, hipStream_t s) {
   return launch_few<kRows>(p, s);
 }
 
+// 32-bit element and tile numbers within a row, and the largest tiles' grid: that
+// of the smaller ones, which run where few of these would, is far within its limit.
+bool supported(int rows, int dim, int out_features) {
+  return dim <= 1 << 24 && out_features <= 1 << 28 && rows <= 1 << 20 &&
+         grid_fits(groups(rows, 128) * groups(out_features, 256), Tiling<2, 2, 4, 2>::kThreads);
+}
+
 }  // namespace
 
 extern "C" int64_t sf_mx_linear_workspace(int x_dtype, int rows, int dim, int out_features) {
-  if (rows < 0 || dim < 1 || out_features < 1 || dim > 1 << 24 || rows > 1 << 20 ||
-      (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows))
+  if (rows < 0 || dim < 1 || out_features < 1 || (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows) ||
+      !supported(rows, dim, out_features))
     return -1;
   if (x_dtype == kRows || as_they_are(rows, dim, out_features)) return 0;
   return rows * (static_cast<int64_t>(tiles(dim)) * kTile + static_cast<int64_t>(quads(dim)) * 16);
@@ -238,8 +245,7 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
       (out_dtype != kBf16 && out_dtype != kFp16) ||
       (x_dtype != kBf16 && x_dtype != kFp16 && x_dtype != kRows))
     return SF_ERR_INVALID_ARGUMENT;
-  // 32-bit element and tile numbers within a row, grids within their limits.
-  if (dim > 1 << 24 || out_features > 1 << 28 || rows > 1 << 20) return SF_ERR_UNSUPPORTED_SHAPE;
+  if (!supported(rows, dim, out_features)) return SF_ERR_UNSUPPORTED_SHAPE;
   if (rows == 0) return SF_OK;
   if (!x || !codes || !scales || !out || (x_dtype == kRows && !x_scales)) return SF_ERR_INVALID_ARGUMENT;
   if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(out, 2) || !aligned(bias, 2) || !aligned(workspace, 16) ||

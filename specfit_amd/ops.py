@@ -1505,7 +1505,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
 def _mx_linear_workspace(kind: int, rows: int, dim: int, out_features: int) -> int:
     n = _native.lib().sf_mx_linear_workspace(kind, rows, dim, out_features)
     if n < 0:
-        raise ValueError("a product takes at most 2^20 rows of 2^24 columns")
+        raise ValueError("a product takes at most 2^20 rows, 2^24 columns and 2^28 outputs of a row")
     return n
 
 
@@ -1743,7 +1743,7 @@ def _mx_experts_workspace(tokens: int, top_k: int, hidden_size: int, intermediat
     n = _native.lib().sf_mx_experts_workspace(tokens, top_k, hidden_size, intermediate_size,
                                               num_experts)
     if n < 0:
-        raise ValueError("unsupported number of experts, or of experts to a token")
+        raise ValueError("unsupported number of experts, of experts to a token, or of routes")
     return n
 
 

@@ -271,3 +271,24 @@ def test_experts_are_refused_before_any_launch():
     wide = lib.sf_mx_expert_bytes(1 << 20, 32)
     assert g(3, p, p, 0, p, p, None, 1 << 23, 32, 1 << 20, 32, 4, None, p, wide, p, p, p, None) == UNSUPPORTED
     assert e(0, p, None, 1 << 20, p, p, 1 << 23, 32, 1 << 20, 32, 4, p, wide, p, p, None) == UNSUPPORTED
+
+
+def test_workspaces_are_refused_for_shapes_that_the_calls_refuse():
+    lib = _native.lib()
+    a = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(a) + 63 & ~63
+    size = lib.sf_mx_linear_workspace
+    for rows, dim, out in [(1, 64, (1 << 28) + 1), ((1 << 20) + 1, 64, 64), (1, (1 << 24) + 1, 64),
+                           (1 << 20, 32, 1 << 28)]:
+        assert size(0, rows, dim, out) == size(3, rows, dim, out) == -1
+        for dtype, stride in [(0, dim), (3, 0)]:
+            assert lib.sf_mx_linear(dtype, p, p, stride, rows, dim, p, p, out, None, 0, p, out, p, None) == UNSUPPORTED
+        with pytest.raises(ValueError):
+            ops._mx_linear_workspace(0, rows, dim, out)
+    assert size(0, 1 << 20, 1 << 24, 256) > 0 and size(3, 1, 64, 1 << 28) == 0
+    size, big = lib.sf_mx_experts_workspace, lib.sf_mx_expert_bytes(64, 32)
+    assert size(1 << 25, 8, 64, 32, 4) > 0
+    assert size((1 << 25) + 1, 8, 64, 32, 4) == -1
+    assert lib.sf_mx_experts(0, p, None, 64, p, p, (1 << 25) + 1, 8, 64, 32, 4, p, big, p, p, None) == INVALID
+    with pytest.raises(ValueError):
+        ops._mx_experts_workspace((1 << 25) + 1, 8, 64, 32, 4)
