@@ -44,10 +44,8 @@ class Qwen3MXExperts(nn.Module):
     @classmethod
     def from_module(cls, experts: nn.Module) -> "Qwen3MXExperts":
         """From an HF ``Qwen3MoeExperts`` on a GPU (shares no storage)."""
-        if type(experts.act_fn).__name__ not in ("SiLUActivation", "SiLU"):
-            raise ValueError("the experts' activation must be silu")
+        E, H, I = _checked(experts)
         gate_up, down = experts.gate_up_proj.detach(), experts.down_proj.detach()
-        E, H, I = down.shape
         records = torch.empty((E, ops.mx_expert_bytes(H, I)), dtype=torch.uint8, device=down.device)
         for e in range(E):  # one expert's copy at a time, not the layer's
             packed = torch.cat([gate_up[e].reshape(-1), down[e].reshape(-1)])[None]
@@ -64,16 +62,39 @@ class Qwen3MXExperts(nn.Module):
                               self.records, self.hidden_size, self.intermediate_size)
 
 
+def _checked(experts: nn.Module) -> tuple[int, int, int]:
+    """(experts, hidden size, intermediate size) of an HF ``Qwen3MoeExperts``
+    that a ``Qwen3MXExperts`` can be made from."""
+    if type(experts.act_fn).__name__ not in ("SiLUActivation", "SiLU"):
+        raise ValueError("the experts' activation must be silu")
+    gate_up, down = experts.gate_up_proj, experts.down_proj
+    E, H, I = down.shape
+    if gate_up.shape != (E, 2 * I, H) or not 1 <= E <= 256:
+        raise ValueError("experts must be [1 to 256, 2 * intermediate, hidden] beside "
+                         "[experts, hidden, intermediate]")
+    if not (gate_up.is_cuda and down.is_cuda) or gate_up.device != down.device:
+        raise ValueError("the experts' weights must be on a HIP device")
+    if gate_up.dtype != down.dtype or down.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError("the experts' weights must be bf16, fp16 or fp32")
+    ops.mx_expert_bytes(H, I)
+    return E, H, I
+
+
 def install_mx_experts(model: nn.Module) -> int:
     """Replace the experts of every Qwen3-MoE layer of ``model`` that are
     transformers' own, on a GPU, with a ``Qwen3MXExperts`` of their weights in
-    4 bits; returns how many.  Layers whose experts are offloaded stay."""
+    4 bits; returns how many.  Layers whose experts are offloaded stay.  All are
+    looked over before the first is replaced, so a model that is refused is as it
+    was."""
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeExperts
 
     targets = [(name, mod) for name, mod in model.named_modules()
                if isinstance(mod, Qwen3MoeExperts)]
+    for _, mod in targets:
+        if mod is model:
+            raise ValueError("the model is the experts themselves: Qwen3MXExperts.from_module")
+        _checked(mod)
     for name, mod in targets:
-        parent_name, _, attr = name.rpartition(".")
-        parent = model.get_submodule(parent_name) if parent_name else model
-        setattr(parent, attr, Qwen3MXExperts.from_module(mod))
+        parent, _, attr = name.rpartition(".")
+        setattr(model.get_submodule(parent), attr, Qwen3MXExperts.from_module(mod))
     return len(targets)

@@ -401,3 +401,40 @@ def test_tiny_sums_under_large_route_weights(tokens, experts):
     # A sum's terms and parts below 2^-126 may count as 0: 64 terms of a route, K routes.
     slack = slack + I * 2.0 ** -126 * weights.double().abs().sum(1, keepdim=True)
     assert (got.double() - want).abs().le(slack).all()
+
+
+def _moe_model(layers=3):
+    from transformers import Qwen3MoeConfig, Qwen3MoeForCausalLM
+
+    torch.manual_seed(5)
+    config = Qwen3MoeConfig(vocab_size=64, hidden_size=64, intermediate_size=48, moe_intermediate_size=32,
+                            num_hidden_layers=layers, num_attention_heads=2, num_key_value_heads=1, head_dim=32,
+                            num_experts=4, num_experts_per_tok=2)
+    return Qwen3MoeForCausalLM(config).to(torch.bfloat16).eval().to(DEV)
+
+
+def test_a_model_that_is_refused_stays_as_it_was():
+    from specfit_amd.runtime import install_mx_experts
+
+    model = _moe_model()
+    before = [layer.mlp.experts for layer in model.model.layers]
+    last = before[-1]
+    good = last.act_fn
+    last.act_fn = torch.nn.GELU()
+    with pytest.raises(ValueError, match="silu"):
+        install_mx_experts(model)
+    last.act_fn = good
+    last.to("cpu")
+    with pytest.raises(ValueError, match="device"):
+        install_mx_experts(model)
+    last.to(DEV)
+    kept, last.gate_up_proj = last.gate_up_proj, torch.nn.Parameter(last.gate_up_proj[:, 2:].contiguous())
+    with pytest.raises(ValueError, match="intermediate"):
+        install_mx_experts(model)
+    last.gate_up_proj = kept
+    assert all(layer.mlp.experts is b for layer, b in zip(model.model.layers, before))
+    with pytest.raises(ValueError, match="from_module"):
+        install_mx_experts(last)
+    assert "" not in last._modules
+    assert install_mx_experts(model) == 3
+    assert all(isinstance(layer.mlp.experts, Qwen3MXExperts) for layer in model.model.layers)
