@@ -85,16 +85,17 @@ def install_mx_experts(model: nn.Module) -> int:
     transformers' own, on a GPU, with a ``Qwen3MXExperts`` of their weights in
     4 bits; returns how many.  Layers whose experts are offloaded stay.  All are
     looked over before the first is replaced, so a model that is refused is as it
-    was."""
+    was; a layer's own weights go before the next one's are rounded."""
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeExperts
 
-    targets = [(name, mod) for name, mod in model.named_modules()
-               if isinstance(mod, Qwen3MoeExperts)]
-    for _, mod in targets:
-        if mod is model:
-            raise ValueError("the model is the experts themselves: Qwen3MXExperts.from_module")
-        _checked(mod)
-    for name, mod in targets:
+    names = []  # not the modules, which would keep their weights
+    for name, mod in model.named_modules():
+        if isinstance(mod, Qwen3MoeExperts):
+            if mod is model:
+                raise ValueError("the model is the experts themselves: Qwen3MXExperts.from_module")
+            _checked(mod)
+            names.append(name)
+    for name in names:
         parent, _, attr = name.rpartition(".")
-        setattr(model.get_submodule(parent), attr, Qwen3MXExperts.from_module(mod))
-    return len(targets)
+        setattr(model.get_submodule(parent), attr, Qwen3MXExperts.from_module(model.get_submodule(name)))
+    return len(names)

@@ -438,3 +438,23 @@ def test_a_model_that_is_refused_stays_as_it_was():
     assert "" not in last._modules
     assert install_mx_experts(model) == 3
     assert all(isinstance(layer.mlp.experts, Qwen3MXExperts) for layer in model.model.layers)
+
+
+def test_layers_are_released_one_by_one(monkeypatch):
+    import gc
+    import weakref
+
+    from specfit_amd.runtime import install_mx_experts
+
+    model = _moe_model()
+    old = [weakref.ref(layer.mlp.experts.gate_up_proj) for layer in model.model.layers]
+    make, alive = Qwen3MXExperts.from_module.__func__, []
+
+    def from_module(cls, experts):
+        gc.collect()
+        alive.append([r() is not None for r in old])
+        return make(cls, experts)
+
+    monkeypatch.setattr(Qwen3MXExperts, "from_module", classmethod(from_module))
+    assert install_mx_experts(model) == 3
+    assert alive == [[True, True, True], [False, True, True], [False, False, True]]
