@@ -88,14 +88,16 @@ def install_mx_experts(model: nn.Module) -> int:
     was; a layer's own weights go before the next one's are rounded."""
     from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeExperts
 
-    names = []  # not the modules, which would keep their weights
-    for name, mod in model.named_modules():
+    places: dict[int, list[str]] = {}  # by module: layers may share one
+    for name, mod in model.named_modules(remove_duplicate=False):
         if isinstance(mod, Qwen3MoeExperts):
             if mod is model:
                 raise ValueError("the model is the experts themselves: Qwen3MXExperts.from_module")
             _checked(mod)
-            names.append(name)
-    for name in names:
-        parent, _, attr = name.rpartition(".")
-        setattr(model.get_submodule(parent), attr, Qwen3MXExperts.from_module(model.get_submodule(name)))
-    return len(names)
+            places.setdefault(id(mod), []).append(name)
+    for names in places.values():
+        new = Qwen3MXExperts.from_module(model.get_submodule(names[0]))
+        for name in names:
+            parent, _, attr = name.rpartition(".")
+            setattr(model.get_submodule(parent), attr, new)
+    return len(places)

@@ -458,3 +458,14 @@ def test_layers_are_released_one_by_one(monkeypatch):
     monkeypatch.setattr(Qwen3MXExperts, "from_module", classmethod(from_module))
     assert install_mx_experts(model) == 3
     assert alive == [[True, True, True], [False, True, True], [False, False, True]]
+
+
+def test_layers_that_share_their_experts():
+    from specfit_amd.runtime import install_mx_experts
+
+    model = _moe_model()
+    layers = model.model.layers
+    layers[2].mlp.experts = layers[0].mlp.experts
+    assert install_mx_experts(model) == 2
+    assert layers[2].mlp.experts is layers[0].mlp.experts and isinstance(layers[0].mlp.experts, Qwen3MXExperts)
+    assert isinstance(layers[1].mlp.experts, Qwen3MXExperts)
