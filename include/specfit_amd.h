@@ -651,7 +651,7 @@ int sf_add_rms_norm(int dtype, const void *x, int64_t x_stride,
  *             x_dtype 0 and 1, x is 16-byte aligned and x_stride a multiple of 8
  *   codes, scales   a weight in e2m1 [out_features, dim]
  *   bias      [out_features] of out_dtype, or NULL
- *   out_dtype 0 bf16, 1 fp16; out has row stride out_stride
+ *   out_dtype 0 bf16, 1 fp16, whatever x_dtype; out has row stride out_stride
  * codes, scales and, for x_dtype 3, x and x_scales 16-byte aligned; rows <= 2^20,
  * dim <= 2^24, out_features <= 2^28, and fewer than 2^24 blocks of 128 rows by 256
  * outputs.

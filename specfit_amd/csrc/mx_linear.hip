@@ -2,7 +2,7 @@
 //   out[m, n] = T(sum_k x[m, k] w[n, k] + bias[n]),
 // x in e4m3 (rounded here where rows come in 16 bits), w in e2m1.  Products are
 // exact, the matrix unit adds a block's in its own fixed order and width and
-// accumulates in fp32; the output is rounded once, to the type that x came in.
+// accumulates in fp32; the output is rounded once, to bf16 or fp16.
 //
 // One MI355X (a large copy moves 5.0 TB/s, an 8,192^3 library product in e4m3 runs
 // at 2,650 TFLOP/s):

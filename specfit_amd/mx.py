@@ -51,7 +51,7 @@ def _check(name: str, t: torch.Tensor, nbytes: int) -> None:
 
 class MXRows:
     """Activations in e4m3: ``shape`` [..., dim], ``dtype`` the type they came
-    in and a product with them gives."""
+    in, which a product with them gives too (of fp32 the caller names one)."""
 
     __slots__ = ("shape", "dtype", "rows", "dim", "_codes", "_scales", "_both")
 

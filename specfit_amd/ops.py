@@ -1510,12 +1510,14 @@ def _mx_linear_workspace(kind: int, rows: int, dim: int, out_features: int) -> i
 
 
 def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | None = None, *,
+              dtype: torch.dtype | None = None,
               stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """x weight^T + bias with the weight in microscaled 4 bits (K15).
 
-    x [..., dim], bf16 or fp16 (rounded to e4m3 as ``mx_quantize`` does) or the
-    MXRows of such; bias [rows of the weight] of that type.  fp32 sums,
-    rounded once to x's type.  With ``stream``, the inputs and the output
+    x [..., dim], bf16 or fp16 (rounded to e4m3 as ``mx_quantize`` does) or
+    MXRows.  fp32 sums, rounded once to ``dtype``, bf16 or fp16: x's by default,
+    to be given with the MXRows of an fp32 stream.  bias [rows of the weight] of
+    the output's type.  With ``stream``, the inputs and the output
     (memory of the current stream) are the caller's to order between the two
     streams.  No gradients."""
     if not isinstance(weight, MXWeight):
@@ -1528,9 +1530,13 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
     else:
         _refuse_gradients("mx_linear", x, bias)
         _require_cuda("x", x)
-    dtype, device, shape = x.dtype, x.device, x.shape
+        if x.dtype not in (_BF16, torch.float16):
+            raise ValueError("x must be bf16, fp16 or MXRows")
+    device, shape = x.device, x.shape
+    if dtype is None:
+        dtype = x.dtype
     if dtype not in (_BF16, torch.float16):
-        raise ValueError("a product's rows must come from bf16 or fp16")
+        raise ValueError("a product gives bf16 or fp16: rows from fp32 need a dtype")
     if len(shape) < 1 or shape[-1] != weight.dim:
         raise ValueError(f"x must be [..., {weight.dim}]")
     index = device.index
@@ -1548,7 +1554,7 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
         kind, rows, stride, (x_ptr, scale_ptr) = _MX_ROWS, x.rows, 0, x._pointers()
     else:
         x = _as_rows("x", x, stream)
-        kind, rows, stride = _DTYPES[dtype], x.shape[0], x.stride(0)
+        kind, rows, stride = _DTYPES[x.dtype], x.shape[0], x.stride(0)
         x_ptr, scale_ptr = x.data_ptr(), None
         if stride % 8 or x_ptr % 16:
             nbytes = rows * sum(mx.row_bytes(weight.dim))

@@ -406,3 +406,34 @@ def test_each_operator_on_another_stream():
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,dim,out", [(1, 128, 16), (3, 40, 33), (20, 768, 520), (61, 520, 2048), (300, 136, 1030),
+                                          (600, 640, 2500)])
+def test_products_of_an_fp32_streams_rows(rows, dim, out, dtype):
+    """Rows that a norm leaves of an fp32 stream, and rows of one 16-bit type with
+    outputs of the other."""
+    x, w = _exact_case(rows + dim + out, rows, dim, out, torch.float32)
+    weight = ops.mx_quantize_weight(w)
+    bias = _whole(7, 1, out, [0.0, 3.0, -8.0])[0].to(dtype)
+    want = x.double() @ w.double().t()
+    for held in (ops.mx_quantize(x), x.to(torch.bfloat16), x.to(torch.float16)):
+        assert torch.equal(ops.mx_linear(held, weight, dtype=dtype), want.to(dtype))
+        assert torch.equal(ops.mx_linear(held, weight, bias, dtype=dtype), (want + bias.double()).to(dtype))
+    _, _, q = ops.add_rms_norm(x, _normal(1, rows, dim), _normal(2, dim), 1e-6, normed=False, quantized=True)
+    got = ops.mx_linear(q, weight, dtype=dtype)
+    assert got.dtype == dtype
+    assert torch.equal(got, ops.mx_linear(ops.mx_quantize(q.values(dtype)), weight))
+
+
+def test_products_refuse_outputs_in_other_types():
+    x, weight = _normal(0, 4, 64), ops.mx_quantize_weight(_normal(1, 32, 64))
+    rows = ops.mx_quantize(x)
+    bias = torch.zeros(32, dtype=torch.bfloat16, device=DEV)
+    for call in [lambda: ops.mx_linear(rows, weight), lambda: ops.mx_linear(rows, weight, dtype=torch.float32),
+                 lambda: ops.mx_linear(x, weight), lambda: ops.mx_linear(x, weight, dtype=torch.bfloat16),
+                 lambda: ops.mx_linear(rows, weight, bias, dtype=torch.float16),
+                 lambda: ops.mx_linear(x.to(torch.bfloat16), weight, bias, dtype=torch.float16)]:
+        with pytest.raises(ValueError):
+            call()
