@@ -1468,7 +1468,7 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
         raise ValueError("x must have at least one column")
     dim = x.shape[-1]
     _require_cuda("weight", weight, dtype)
-    if weight.shape != (dim,) or weight.stride(0) != 1 or weight.device != device:
+    if weight.shape != (dim,) or not weight.is_contiguous() or weight.device != device:
         raise ValueError(f"weight must be a contiguous [{dim}] tensor on x's device")
     if residual is not None:
         _require_cuda("residual", residual, dtype)
@@ -1544,7 +1544,7 @@ def mx_linear(x: torch.Tensor | MXRows, weight: MXWeight, bias: torch.Tensor | N
         raise ValueError("x and the weight must share a device")
     if bias is not None:
         _require_cuda("bias", bias, dtype)
-        if bias.shape != (weight.rows,) or bias.stride(0) != 1 or bias.device != device:
+        if bias.shape != (weight.rows,) or not bias.is_contiguous() or bias.device != device:
             raise ValueError(f"bias must be a contiguous [{weight.rows}] tensor on x's device")
     out = torch.empty(*shape[:-1], weight.rows, dtype=dtype, device=device)
     if out.numel() == 0:
@@ -1620,12 +1620,16 @@ def mx_quantize_experts(packed: torch.Tensor, hidden_size: int, intermediate_siz
 
 
 def _mx_slots(slot_storage: torch.Tensor, slot_of_expert: torch.Tensor | None, num_experts: int,
-              hidden_size: int, intermediate_size: int, device: torch.device) -> None:
+              hidden_size: int, intermediate_size: int, device: torch.device) -> int:
+    """Bytes from one slot to the next."""
     nbytes = mx_expert_bytes(hidden_size, intermediate_size)
     _require_cuda("slot storage", slot_storage, torch.uint8)
+    stride = 0
+    if slot_storage.dim() == 2:  # of one slot, torch may say anything
+        stride = slot_storage.stride(0) if slot_storage.shape[0] > 1 else nbytes
     if slot_storage.dim() != 2 or slot_storage.shape[1] != nbytes or slot_storage.stride(1) != 1 \
-            or slot_storage.stride(0) < nbytes or slot_storage.device != device \
-            or slot_storage.data_ptr() % 16 or slot_storage.stride(0) % 16:
+            or stride < nbytes or slot_storage.device != device \
+            or slot_storage.data_ptr() % 16 or stride % 16:
         raise ValueError(f"slot storage must be 16-byte aligned uint8 [slots, {nbytes}]")
     if slot_of_expert is None:
         if slot_storage.shape[0] < num_experts:
@@ -1635,6 +1639,7 @@ def _mx_slots(slot_storage: torch.Tensor, slot_of_expert: torch.Tensor | None, n
         if slot_of_expert.numel() != num_experts or not slot_of_expert.is_contiguous() \
                 or slot_of_expert.device != device:
             raise ValueError("slot_of_expert must be contiguous int32 [num_experts]")
+    return stride
 
 
 def _mx_hidden(hidden: torch.Tensor | MXRows, tokens: int, hidden_size: int,
@@ -1676,7 +1681,7 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
     device = hidden.device
     if tuple(hidden.shape) != (T, H) or plan.perm_pos.device != device:
         raise ValueError("hidden_states must be [tokens, hidden] of the dispatch plan")
-    _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
+    slot_stride = _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
     _require_cuda("out_rows", out_rows, _BF16)
     if out_rows.shape != (T * K, H) or not out_rows.is_contiguous() or out_rows.device != device:
         raise ValueError("out_rows must be contiguous bf16 [tokens * top_k, hidden]")
@@ -1692,7 +1697,7 @@ def mx_grouped_swiglu(hidden: torch.Tensor | MXRows, plan: DispatchPlan,
     act, act_scales = scratch._pointers()
     rc = _launch(_native.lib().sf_mx_grouped_swiglu, out_rows.get_device(), kind, x_ptr, scale_ptr,
                  stride, plan.perm_pos.data_ptr(), plan.offsets.data_ptr(), _ptr(route_weights), T,
-                 K, H, I, E, _ptr(slot_of_expert), slot_storage.data_ptr(), slot_storage.stride(0),
+                 K, H, I, E, _ptr(slot_of_expert), slot_storage.data_ptr(), slot_stride,
                  act, act_scales, out_rows.data_ptr(), _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_mx_grouped_swiglu")
@@ -1728,7 +1733,7 @@ def mx_routed_swiglu(hidden: torch.Tensor | MXRows, index: torch.Tensor,
             or route_weights.device != device:
         raise ValueError("route weights must be contiguous bf16 [tokens, top_k]")
     E = slot_storage.shape[0] if slot_of_expert is None else slot_of_expert.numel()
-    _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
+    slot_stride = _mx_slots(slot_storage, slot_of_expert, E, H, I, device)
     if T * K == 0:
         return torch.zeros((T, H), dtype=_BF16, device=device)
     out = torch.empty(T, H, dtype=_BF16, device=device)
@@ -1736,7 +1741,7 @@ def mx_routed_swiglu(hidden: torch.Tensor | MXRows, index: torch.Tensor,
     scratch = _mx_rows((T * K, I), T * K, _BF16, device, stream)
     rc = _launch(_native.lib().sf_mx_routed_swiglu, device.index, kind, x_ptr, scale_ptr, stride,
                  index.data_ptr(), route_weights.data_ptr(), T, K, H, I, E, _ptr(slot_of_expert),
-                 slot_storage.data_ptr(), slot_storage.stride(0), *scratch._pointers(),
+                 slot_storage.data_ptr(), slot_stride, *scratch._pointers(),
                  out.data_ptr(), _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_mx_routed_swiglu")
@@ -1784,7 +1789,7 @@ def mx_experts(hidden: torch.Tensor | MXRows, index: torch.Tensor, route_weights
             or route_weights.device != device:
         raise ValueError("route weights must be contiguous bf16 [tokens, top_k]")
     E = records.shape[0]
-    _mx_slots(records, None, E, H, I, device)
+    slot_stride = _mx_slots(records, None, E, H, I, device)
     if T * K == 0:
         return torch.zeros((T, H), dtype=_BF16, device=device)
     out = torch.empty(T, H, dtype=_BF16, device=device)
@@ -1796,7 +1801,7 @@ def mx_experts(hidden: torch.Tensor | MXRows, index: torch.Tensor, route_weights
         kind, stride, x, scales = 0, hidden.stride(0), hidden.data_ptr(), None
     rc = _launch(_native.lib().sf_mx_experts, device.index, kind, x, scales, stride,
                  index.data_ptr(), route_weights.data_ptr(), T, K, H, I, E, records.data_ptr(),
-                 records.stride(0), workspace.data_ptr(), out.data_ptr(),
+                 slot_stride, workspace.data_ptr(), out.data_ptr(),
                  _stream_handle(stream, device))
     if rc:
         _native.check(rc, "sf_mx_experts")

@@ -437,3 +437,15 @@ def test_products_refuse_outputs_in_other_types():
                  lambda: ops.mx_linear(x.to(torch.bfloat16), weight, bias, dtype=torch.float16)]:
         with pytest.raises(ValueError):
             call()
+
+
+def test_one_column_or_output_may_have_any_stride():
+    """Of a dimension of one element torch gives any stride, and calls it contiguous."""
+    w = _normal(0, 5, 7).to(torch.bfloat16)[:1, 3]
+    b = _normal(1, 6, 9).to(torch.bfloat16)[2:3, 4]
+    assert w.stride(0) != 1 and w.is_contiguous() and b.stride(0) != 1
+    x = _normal(2, 40, 1).to(torch.bfloat16)
+    for a, c in zip(ops.add_rms_norm(x, x, w, 1e-6)[:2], ops.add_rms_norm(x, x, w.clone(), 1e-6)[:2]):
+        assert torch.equal(a, c)
+    x, weight = _normal(3, 20, 64).to(torch.bfloat16), ops.mx_quantize_weight(_normal(4, 1, 64))
+    assert torch.equal(ops.mx_linear(x, weight, b), ops.mx_linear(x, weight, b.clone()))

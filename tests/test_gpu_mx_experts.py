@@ -469,3 +469,19 @@ def test_layers_that_share_their_experts():
     assert install_mx_experts(model) == 2
     assert layers[2].mlp.experts is layers[0].mlp.experts and isinstance(layers[0].mlp.experts, Qwen3MXExperts)
     assert isinstance(layers[1].mlp.experts, Qwen3MXExperts)
+
+
+@pytest.mark.parametrize("tokens", [3, 200])
+def test_one_experts_records_may_have_any_stride(tokens):
+    H, I = 64, 32
+    h, packed, index, weights = _case(tokens, H, I, 1, 1)
+    records = ops.mx_quantize_experts(packed, H, I)
+    other = records.as_strided(records.shape, (1, 1))
+    assert other.stride() == (1, 1) and other.is_contiguous()
+    assert torch.equal(ops.mx_experts(h, index, weights, other, H, I), ops.mx_experts(h, index, weights, records, H, I))
+    assert torch.equal(ops.mx_routed_swiglu(h, index, weights, other, H, I),
+                       ops.mx_routed_swiglu(h, index, weights, records, H, I))
+    plan, rows = ops.dispatch(index, 1), torch.empty((2, tokens, H), dtype=torch.bfloat16, device=DEV)
+    for r, out in zip((other, records), rows):
+        ops.mx_grouped_swiglu(h, plan, weights.view(-1), r, H, I, out)
+    assert torch.equal(rows[0], rows[1])
