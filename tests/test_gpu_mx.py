@@ -449,3 +449,13 @@ def test_one_column_or_output_may_have_any_stride():
         assert torch.equal(a, c)
     x, weight = _normal(3, 20, 64).to(torch.bfloat16), ops.mx_quantize_weight(_normal(4, 1, 64))
     assert torch.equal(ops.mx_linear(x, weight, b), ops.mx_linear(x, weight, b.clone()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,dim,out", [(1, 1, 1), (1, 7, 3), (40, 1, 1), (2, 1, 300), (17, 33, 1), (1000, 3, 2)])
+def test_smallest_products(rows, dim, out, dtype):
+    x, w = _exact_case(rows + dim + out, rows, dim, out, dtype)
+    weight = ops.mx_quantize_weight(w)
+    want = (x.double() @ w.double().t()).to(dtype)
+    assert torch.equal(ops.mx_linear(x, weight), want)
+    assert torch.equal(ops.mx_linear(ops.mx_quantize(x), weight), want)

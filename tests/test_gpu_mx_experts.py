@@ -485,3 +485,103 @@ def test_one_experts_records_may_have_any_stride(tokens):
     for r, out in zip((other, records), rows):
         ops.mx_grouped_swiglu(h, plan, weights.view(-1), r, H, I, out)
     assert torch.equal(rows[0], rows[1])
+
+
+def _integers(experts, H, I, low_bits, powers):
+    """Experts in pairs (2p, 2p + 1) whose outputs for a token that holds 1 in its
+    first place are whole numbers of 11 bits, apart in the last ``low_bits`` of them,
+    times ``powers`` [H].  Gates are 32, where silu is the identity in fp32; the
+    activations are 1, 2, ... 1,024, the numbers' bits lie in down: every product and
+    sum is exact."""
+    g = torch.Generator(device=DEV).manual_seed(experts)
+    first = torch.randint(1024, 2048, (experts // 2, H), generator=g, device=DEV)
+    other = first ^ torch.randint(0, 1 << low_bits, first.shape, generator=g, device=DEV)
+    numbers = torch.stack([first, other], 1).flatten(0, 1)
+    gate, up = (torch.zeros((experts, I, H), device=DEV) for _ in range(2))
+    down = torch.zeros((experts, H, I), device=DEV)
+    gate[:, :, 0] = 32
+    bit = torch.arange(11, device=DEV)
+    up[:, :11, 0] = torch.exp2(bit - 5.0)
+    down[:, :, :11] = (numbers[..., None] >> bit & 1) * powers[:, None]
+    return numbers, torch.cat([w.flatten(1) for w in (gate, up, down)], 1).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("tokens,experts", FORMS)
+@pytest.mark.parametrize("H", [64, 100, 328])
+def test_routes_keep_eleven_bits_until_they_are_added(H, tokens, experts):
+    """The difference of two routes of 11 bits, some of them 2^-24 of the others of
+    their 32 columns: one bit less in a route's row, or an exponent that is off, would
+    show."""
+    I, K = 64, 2
+    powers = torch.where(torch.arange(H, device=DEV) % 3 == 1, 2.0 ** -24, 1.0)
+    numbers, packed = _integers(experts, H, I, 7, powers)
+    h = torch.zeros((tokens, H), dtype=torch.bfloat16, device=DEV)
+    h[:, 0] = 1
+    pair = torch.arange(tokens, device=DEV) % (experts // 2)
+    index = torch.stack([2 * pair, 2 * pair + 1], 1)
+    weights = torch.tensor([1.0, -1.0], device=DEV, dtype=torch.bfloat16).expand(tokens, K).contiguous()
+    got = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, H, I), H, I)
+    want = (numbers[2 * pair] - numbers[2 * pair + 1]) * powers
+    assert torch.equal(got.float(), want)
+
+
+@pytest.mark.parametrize("H,I", [(256, 128), (96, 424)])
+def test_chunks_of_every_height_in_one_launch(H, I):
+    """Experts with as many rows as make full chunks, tall rests, which come first,
+    and the rests of 64 and of 32 rows behind them."""
+    counts = [0, 1, 20, 33, 64, 100, 128, 129, 300, 0, 32, 65]
+    tokens = sum(counts)
+    assert tokens > 16 * len(counts)      # both products by tiles of up to 128 rows
+    rests = [c % 128 for c in counts if c % 128]
+    assert any(c >= 128 for c in counts) and any(r > 64 for r in rests) \
+        and any(32 < r <= 64 for r in rests) and any(r <= 32 for r in rests)
+    h, packed, _, weights = _case(tokens, H, I, len(counts), 1)
+    index = torch.repeat_interleave(torch.arange(len(counts), device=DEV), torch.tensor(counts, device=DEV))
+    index = index[torch.randperm(tokens, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)][:, None]
+    weights = torch.rand((tokens, 1), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(torch.bfloat16)
+    records = ops.mx_quantize_experts(packed, H, I)
+    got = ops.mx_experts(h, index, weights, records, H, I)
+    _check(got, h, index, weights, packed, H, I)
+    # An expert's rows by themselves, in chunks of their own: the same sums.
+    for e in (2, 6, 8):
+        mine = index[:, 0] == e
+        rows = torch.empty((int(mine.sum()), H), dtype=torch.bfloat16, device=DEV)
+        ops.mx_grouped_swiglu(h[mine], ops.dispatch(torch.zeros_like(index[mine]), 1), weights[mine].view(-1),
+                              records[e:e + 1], H, I, rows)
+        # Both round the same fp32 row to bf16, one by way of 11 bits: a step of bf16, and
+        # what a block of 11 bits loses below 2^-28 of its largest.
+        alone, among = rows.float(), got[mine].float()
+        step = 2.0 ** -7 * among.abs() + 2.0 ** -38 * among.abs().amax(1, keepdim=True)
+        assert (alone - among).abs().le(step).all()
+
+
+@pytest.mark.parametrize("tokens,hidden,inner,experts,top_k", [(1, 1, 1, 1, 1), (200, 1, 1, 2, 1), (300, 5, 3, 3, 2),
+                                                             (30, 64, 32, 40, 32), (150, 64, 32, 64, 12),
+                                                             (9, 7, 33, 256, 32)])
+def test_smallest_sizes_and_many_routes(tokens, hidden, inner, experts, top_k):
+    h, packed, index, weights = _case(tokens, hidden, inner, experts, top_k)
+    want, slack = ref.experts(h, index, weights, packed, hidden, inner)
+    got = ops.mx_experts(h, index, weights, ops.mx_quantize_experts(packed, hidden, inner), hidden, inner)
+    assert (got.double() - want).abs().le(slack).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 20, 300])
+def test_far_experts(tokens):
+    """Records past 32 bits of offset."""
+    H, I, E = 4096, 4096, 180
+    h, packed, index, weights = _case(tokens, H, I, 2, 1)
+    near = ops.mx_quantize_experts(packed, H, I)
+    assert (E - 2) * near.shape[1] > 1 << 32
+    far = torch.zeros((E, near.shape[1]), dtype=torch.uint8, device=DEV)
+    far[-2:] = near
+    pad = torch.arange(E - 2, device=DEV)[:, None]       # so that as many rows fall to an expert, in either form
+    index = torch.cat([index, pad % 2]) if tokens > 1 else index
+    h, weights = (torch.cat([t, t[:1].expand(index.shape[0] - tokens, -1)]) for t in (h, weights))
+    out = [torch.empty((index.shape[0], H), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    table = torch.tensor([E - 2, E - 1], dtype=torch.int32, device=DEV)
+    plan = ops.dispatch(index, 2)
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), near, H, I, out[0])
+    ops.mx_grouped_swiglu(h, plan, weights.view(-1), far, H, I, out[1], slot_of_expert=table)
+    assert torch.equal(out[0], out[1])
+    assert torch.equal(ops.mx_routed_swiglu(h[:2], index[:2], weights[:2], near, H, I),
+                       ops.mx_routed_swiglu(h[:2], index[:2] + E - 2, weights[:2], far, H, I))
