@@ -82,6 +82,9 @@ extern "C" {
 #define SF_MAX_EXPERTS 256
 /* Largest top-k. */
 #define SF_MAX_TOPK 32
+/* Most rows that the products with 4-bit weights take in 16 bits and round where
+ * they are read: one tile of the matrix instruction. */
+#define SF_MX_RAW_ROWS 16
 /* Values per chunk of an exponent-coded expert record (sf_expert_decode). */
 #define SF_DECODE_CHUNK 4096
 
@@ -669,7 +672,7 @@ int64_t sf_mx_linear_workspace(int x_dtype, int rows, int dim,
  * e < num_experts that has rows and, with a table, slot_of_expert[e] >= 0.
  *   a       = e4m3(silu(x[t] . gate^T) * (x[t] . up^T))        fp32 up to a
  *   rows[r] = bf16((a . down^T) * route_weights[perm_pos[r]])
- *   x_dtype         3: rows in e4m3; 0: at most 16 rows in bf16, hidden_size and
+ *   x_dtype         3: rows in e4m3; 0: at most SF_MX_RAW_ROWS in bf16, hidden_size and
  *                   x_stride multiples of 8
  *   slots           records of sf_mx_expert_bytes at slot_stride bytes: the codes
  *                   of gate [I, H], up [I, H], down [H, I] and then their

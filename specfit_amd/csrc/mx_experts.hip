@@ -649,7 +649,7 @@ int check(int x_dtype, const void* x, const void* x_scales, int64_t x_stride, in
     return SF_ERR_MISALIGNED;
   if (x_dtype != kRows) {
     if (x_stride % 8 || hidden_size % 8) return SF_ERR_MISALIGNED;
-    if (tokens > 16) return SF_ERR_UNSUPPORTED_SHAPE;
+    if (tokens > SF_MX_RAW_ROWS) return SF_ERR_UNSUPPORTED_SHAPE;
   }
   return SF_OK;
 }
@@ -885,7 +885,8 @@ extern "C" int sf_mx_experts(int x_dtype, const void* x, const void* x_scales, i
   const Workspace w = workspace_of(tokens, top_k, hidden_size, intermediate_size, num_experts, dispatched);
   uint8_t* base = static_cast<uint8_t*>(workspace);
   // Few rows are rounded by the wavefronts that read them.
-  const bool rounds = x_dtype == kBf16 && (tokens > 16 || hidden_size % 8 || x_stride % 8 || !aligned(x, 16));
+  const bool rounds =
+      x_dtype == kBf16 && (tokens > SF_MX_RAW_ROWS || hidden_size % 8 || x_stride % 8 || !aligned(x, 16));
   const int held = rounds ? kRows : x_dtype;  // what the products read
   if (rounds && !aligned(x, 2)) return SF_ERR_MISALIGNED;
   Experts p = experts_of(rounds ? base + w.x : x, rounds ? base + w.x_scales : x_scales, x_stride, route_weights, top_k,

@@ -161,11 +161,10 @@ int launch_tiled(const Linear& p, hipStream_t s) {
 // the device, as they are and with the launch (4 more on the host):
 //   1 row of 2,048 by 5,120   5.4 / 6.0   16,384   9.4 / 7.5   40,000   22 / 13.5   151,936   77 / 36
 //   16 rows                   7.2 / 7.2           12.2 / 8.7            30 / 15.4            103 / 37
-constexpr int kMostRawRows = 16;
 constexpr int64_t kMostRawWeight = 1 << 25;  // values
 
 bool as_they_are(int rows, int dim, int out_features) {
-  return rows <= kMostRawRows && dim % 8 == 0 && static_cast<int64_t>(dim) * out_features <= kMostRawWeight;
+  return rows <= SF_MX_RAW_ROWS && dim % 8 == 0 && static_cast<int64_t>(dim) * out_features <= kMostRawWeight;
 }
 
 int64_t groups(int n, int per) { return (n - 1) / per + 1; }
@@ -262,7 +261,7 @@ extern "C" int sf_mx_linear(int x_dtype, const void* x, const void* x_scales, in
     x_dtype = kRows;
     x = held;
     x_scales = held_scales;
-  } else if (rows > kMostRawRows) {
+  } else if (rows > SF_MX_RAW_ROWS) {
     return SF_ERR_UNSUPPORTED_SHAPE;
   } else if (!fits || dim % 8) {
     return SF_ERR_MISALIGNED;

@@ -1336,7 +1336,7 @@ def greedy_tokens(logits: torch.Tensor, *, counts: torch.Tensor | None = None,
 
 # ------------------------------------------------------- K13: microscaled --
 _MX_E4M3, _MX_E2M1, _MX_ROWS = 0, 1, 3
-_MX_RAW_ROWS = 16   # rows of 16-bit values that the experts take as they are
+_MX_RAW_ROWS = 16   # SF_MX_RAW_ROWS
 
 
 def _new(shape, dtype: torch.dtype, device: torch.device,

@@ -292,3 +292,13 @@ def test_workspaces_are_refused_for_shapes_that_the_calls_refuse():
     assert lib.sf_mx_experts(0, p, None, 64, p, p, (1 << 25) + 1, 8, 64, 32, 4, p, big, p, p, None) == INVALID
     with pytest.raises(ValueError):
         ops._mx_experts_workspace((1 << 25) + 1, 8, 64, 32, 4)
+
+
+def test_the_limit_of_unrounded_rows_is_the_headers():
+    import pathlib
+    import re
+
+    header = (pathlib.Path(ops.__file__).parent.parent / "include" / "specfit_amd.h").read_text()
+    assert int(re.search(r"#define SF_MX_RAW_ROWS (\d+)", header)[1]) == ops._MX_RAW_ROWS
+    size = _native.lib().sf_mx_linear_workspace
+    assert size(0, ops._MX_RAW_ROWS, 64, 32) == 0 and size(0, ops._MX_RAW_ROWS + 1, 64, 32) > 0
