@@ -585,3 +585,27 @@ def test_far_experts(tokens):
     assert torch.equal(out[0], out[1])
     assert torch.equal(ops.mx_routed_swiglu(h[:2], index[:2], weights[:2], near, H, I),
                        ops.mx_routed_swiglu(h[:2], index[:2] + E - 2, weights[:2], far, H, I))
+
+
+@pytest.mark.parametrize("tokens,experts", FORMS)
+def test_absent_experts_and_bad_tokens_in_every_form(tokens, experts):
+    """Routes to experts that the layer does not have count for nothing, alone and
+    beside others; a token that is not finite spoils itself only."""
+    H, I, K = 96, 64, 2
+    h, packed, _, weights = _case(tokens, H, I, experts, K)
+    index = _even(tokens, experts, K)
+    records = ops.mx_quantize_experts(packed, H, I)
+    index[0, 1], index[1] = experts, torch.tensor([-1, 2 ** 40], device=DEV)
+    if tokens > 64:
+        index[tokens // 2:tokens // 2 + 30] = -5
+    got = ops.mx_experts(h, index, weights, records, H, I)
+    _check(got, h, index, weights, packed, H, I)
+    absent = ((index < 0) | (index >= experts)).all(1)
+    assert absent.any() and not got[absent].any()
+    h[2, 40], h[tokens - 1, 0], h[1, 7] = float("inf"), float("nan"), float("nan")
+    bad = torch.zeros(tokens, dtype=torch.bool, device=DEV)
+    bad[2] = bad[tokens - 1] = True          # token 1 has no expert to read it
+    again = ops.mx_experts(h, index, weights, records, H, I)
+    assert torch.isnan(again[bad]).all() and torch.equal(again[~bad], got[~bad])
+    index[:] = -1
+    assert not ops.mx_experts(h, index, weights, records, H, I).any()
