@@ -13,10 +13,10 @@
 //
 // 128 experts of 2,048 x 768, 8 to a token, one MI355X; gate and up, then down:
 //   1 token (no dispatch)        7.6 + 5.6 us   latency of two dependent launches
-//   61 tokens, favourites         35 + 21 us    4.2 and 3.7 TB/s of weights
-//   2,048 tokens                  75 + 55 us    1.4 and 0.9 PFLOP/s, the weights' 214
+//   61 tokens, favourites         36 + 21 us    4.2 and 3.6 TB/s of weights
+//   2,048 tokens                  76 + 57 us    1.4 and 0.9 PFLOP/s, the weights' 214
 //                                               and 107 MB arriving meanwhile
-// and the sum over the routes 4.6 and 13.4 us (69 MB at 5.7 TB/s).
+// and the sum over the routes 4.6 and 13.4 us (77 MB at 5.7 TB/s).
 #include <cmath>
 
 #include "dispatch.h"
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(WAVES * SF_WAVE) void gate_up_few_kernel(Experts p,
 // the block's largest finite value, at least 15, so that that value becomes 2^14 to
 // 2^15, nothing is lost down to 2^-28 of it, and both factors are normal.
 // Infinities and NaN stay what they are.  2,048 tokens: down 53 us with bf16 rows,
-// 55 so (60 with E by the lanes' exchange through LDS and byte stores).
+// 55 to 57 so (60 with E by the lanes' exchange through LDS and byte stores).
 constexpr int kHeldRows = 4;
 
 __device__ __forceinline__ uint32_t row_exponent(uint32_t top) { return max(top >> 23, 15u); }

@@ -8,7 +8,7 @@
 // at 2,650 TFLOP/s):
 //   1 x 2,048 x 5,120            5.5 us   latency: eight wavefronts cut the sum
 //   61 x 2,048 x 151,936        40 us   184 MB, the output among them, at 4.6 TB/s
-//   4,096 x 4,096 x 9,216      126 us   2,450 TFLOP/s, near the chip's power
+//   4,096 x 4,096 x 9,216      127 us   2,440 TFLOP/s, near the chip's power
 //   8,192^3                    415 us   2,650 TFLOP/s, the library product's rate
 #include "mx_product.h"
 

@@ -9,7 +9,8 @@
 //
 // bf16, one MI355X (a large copy moves 5.0 TB/s):
 //   8,192 x 4,096 to e4m3     20.8 us   4.9 TB/s     and back   17.4 us   5.8 TB/s
-//   151,936 x 2,048 to e2m1    150 us   5.3 TB/s     and back    125 us   6.3 TB/s
+//   151,936 x 2,048 to e2m1    155 us   5.1 TB/s     and back    128 us   6.1 TB/s
+//       (178 us in turn with the kernel that reads them back)
 //   8,192 x 4,096 residual, norm, e4m3 output   59 us   5.1 TB/s
 //   1 x 2,048: 1.6 (values) to 3 us, a launch's latency
 #include "mx.h"

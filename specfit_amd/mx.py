@@ -51,7 +51,9 @@ def _check(name: str, t: torch.Tensor, nbytes: int) -> None:
 
 class MXRows:
     """Activations in e4m3: ``shape`` [..., dim], ``dtype`` the type they came
-    in, which a product with them gives too (of fp32 the caller names one)."""
+    in, which a product with them gives too (of fp32 the caller names one).
+    Whoever makes ``codes`` and ``scales`` leaves zeros behind a row's end in its
+    last tile of 128: a product reads them."""
 
     __slots__ = ("shape", "dtype", "rows", "dim", "_codes", "_scales", "_both")
 
@@ -120,7 +122,8 @@ class MXRows:
 
 @dataclass(frozen=True, eq=False)
 class MXWeight:
-    """A weight [rows, dim] in e2m1."""
+    """A weight [rows, dim] in e2m1.  Whoever makes ``codes`` and ``scales``
+    (rather than ``from_blocks``) leaves zeros behind a row's end in its last tile."""
 
     codes: torch.Tensor
     scales: torch.Tensor

@@ -2,10 +2,12 @@
 
 Drop-in for transformers' ``Qwen3MoeExperts`` (tf:215-246): the same forward
 arguments, every expert resident.  An expert of the Qwen3-30B-A3B shape takes
-2.5 MB instead of 9.4, so the 48 layers of that model take 15 GB and the 94 of
-Qwen3-235B-A22B 117 of a GPU's 288 GB; ``Qwen3OffloadedExperts`` is for experts
-that have to stay exact and stream.  A forward reads nothing back to the host
-and can be captured into a graph.
+2.5 MB instead of 9.4, so the 48 layers of that model take 15.5 GB and the 94 of
+Qwen3-235B-A22B 121 of a GPU's 288 GB (whose bf16 experts, 454 GB, do not fit:
+``from_packed`` makes one layer at a time, ``install_mx_experts`` is for models that
+are on the GPU).  ``Qwen3OffloadedExperts`` is for experts that have to stay exact
+and stream.  A forward reads nothing back to the host and can be captured into a
+graph.
 """
 from __future__ import annotations
 
